@@ -21,6 +21,9 @@
  * Layouts (HND, as the reference):
  *   q, out        [batch][num_q_heads][head_dim] fp16
  *   k/v cache     [num_pages][num_kv_heads][page_size][head_dim] fp16 or fp8 e4m3
+ *   kv_scales     [num_pages][num_kv_heads][page_size / B][2] uint8, block-scaled
+ *                 caches only: byte e of a block's K (0) and V (1) stands for the
+ *                 scale 2^(e - 127); a block is B = pa_block_tokens(page_size) tokens
  *   block_table   [num_slots][block_table_stride] int32 physical page ids
  *   segments      [num_segments][4] int32 = (batch row, kv head, tok_begin, tok_end)
  */
@@ -44,7 +47,12 @@ typedef enum pa_status {
 /* decode_types.hpp:8 `enum class KVDtype { FP16, FP8_E4M3 }` */
 typedef enum pa_kv_dtype {
     PA_KV_FP16     = 0,
-    PA_KV_FP8_E4M3 = 1
+    PA_KV_FP8_E4M3 = 1,
+    /* E4M3 with a power-of-two scale for each block of tokens and kv head
+     * (kv_scales above) in place of one per tensor: needs no calibration, and a
+     * token of large values costs its own block's neighbours precision, not the
+     * cache's. No counterpart in the reference. */
+    PA_KV_FP8_E4M3_BLOCK = 2
 } pa_kv_dtype;
 
 /* decode_types.hpp:14-45 `struct DecodeParams`, with plain C types:
@@ -100,6 +108,10 @@ typedef struct pa_decode_params {
                                           decodes (the plan zeroes them at upload; every decode
                                           leaves them at zero). block_merge 3: each item's
                                           first work unit follows them. Set by bind. */
+    const uint8_t*  kv_scales;         /* PA_KV_FP8_E4M3_BLOCK: the block scales (4-byte aligned;
+                                          k_scale and v_scale then multiply on top, 1 for a
+                                          cache that the appends here wrote). Other types
+                                          ignore it. */
 } pa_decode_params;
 
 /* Thread-local message describing the last failed call ("" if none). */
@@ -217,11 +229,106 @@ pa_status pa_decode_static(int dtype, const pa_decode_params* p, int num_segment
 /* paged_kv_cache.cu:15-39 quantize<> + append_kernel, launch at :122-131:
  * scatters n tokens of fp16 K/V ([n][num_kv_heads][head_dim]) into pages
  * resolved through block_table_row, token i going to position start_pos + i.
- * fp16: bit copy; fp8: e4m3(RNE, saturate to +-448)(float(x) * inv_scale). */
+ * fp16: bit copy; fp8: e4m3(RNE, saturate to +-448)(float(x) * inv_scale).
+ * Block-scaled caches are refused: pa_append_rope writes them. */
 pa_status pa_append_quantize(int dtype, const uint16_t* k, const uint16_t* v, void* k_cache,
                              void* v_cache, const int32_t* block_table_row, int start_pos, int n,
                              int num_kv_heads, int head_dim, int page_size, float inv_k_scale,
                              float inv_v_scale, void* stream);
+
+/* ---- new tokens: head norms, rotation, append ------------------------------
+ * No counterparts in the reference, whose caches take finished K and V. Between
+ * a layer's QKV projection and its attention, each head of a new token's q and
+ * k is normed and rotated:
+ *   norm      y = x * w / sqrt(mean(x^2) + eps)        over the head's 128 dims
+ *   rotation  (a, b) -> s (a cos t - b sin t, b cos t + a sin t), t = position * freq
+ * for each pair (a, b) of dims. Everything in between is held in 32 bits (the
+ * angles in 64) and rounded once, to fp16 or to the cache's type. */
+
+/* A model's rotation, copied to the current device (one small allocation and a
+ * copy that is waited for; not to be made during graph capture). Pair i turns by
+ * freqs[i] radians per position (rot_dim / 2 host values, finite). rot_dim, a
+ * multiple of 16 up to 128, is how many leading dims turn; pairs are dims (i, i +
+ * rot_dim / 2), or (2i, 2i + 1) if interleaved. With num_axes > 1 (up to 4) a
+ * token has several positions and pair i turns by that of axes[i]; axes may be
+ * NULL for one. scale multiplies every sine and cosine (1 usually). */
+typedef struct pa_rope pa_rope;
+pa_status pa_rope_create(const double* freqs, const int32_t* axes, int rot_dim, int num_axes, int interleaved,
+                         float scale, pa_rope** out);
+void      pa_rope_destroy(pa_rope* rope);
+int       pa_rope_dim(const pa_rope* rope);
+int       pa_rope_axes(const pa_rope* rope);
+
+/* Some heads of every token: token t's head h starts at in + t * in_stride + h *
+ * 128 (fp16, 16-byte aligned, strides in elements and multiples of 8, so a fused
+ * projection's output is read where it lies). weight: 128 floats (16-byte
+ * aligned) or NULL for no norm. out likewise, where the call has an output; it
+ * may be `in` itself with the same stride, and overlaps nothing else the call
+ * reads or writes. heads = 0: none. */
+typedef struct pa_head_rows {
+    const uint16_t* in;
+    int64_t         in_stride;
+    uint16_t*       out;
+    int64_t         out_stride;
+    const float*    weight;
+    float           eps;
+    int32_t         heads;
+} pa_head_rows;
+
+/* q and k (either may be NULL) of n tokens normed and rotated into their `out`.
+ * (Here and below, PA_ERR_LENGTH: some 2^27 / heads tokens at most.)
+ * positions: device, [n][axes of the rotation] int32 (any value), NULL only where
+ * rope is (norms alone). */
+pa_status pa_norm_rope(const pa_rope* rope, const pa_head_rows* q, const pa_head_rows* k,
+                       const int32_t* positions, int n, void* stream);
+
+/* Tokens per block of a block-scaled cache: 16 where the page size is a multiple
+ * of 16, 8 where it is 8 modulo 16, 0 for page sizes such caches do not take. */
+int pa_block_tokens(int page_size);
+
+/* New tokens of several sequences into a paged cache of any type, in one launch.
+ * Entry e (0 <= e < num_entries) holds the tokens tok_begin[e] .. tok_begin[e + 1]
+ * - 1 of the call, which go to the places start_pos[e], start_pos[e] + 1, ... of
+ * the sequence whose pages row slot_ids[e] of the block table lists (row e where
+ * slot_ids is NULL). Entries, places and table are device arrays that the kernel
+ * reads, so a captured call follows their values from replay to replay; a token
+ * whose place, row or page is out of range (num_table_rows, block_table_stride,
+ * num_pages), or whose entry starts below 0, is left out (its q is not).
+ * Block-scaled caches: one call holds each sequence once.
+ *   k   normed and rotated (positions: [num_tokens][axes]; NULL: the token's place
+ *       turns every pair), then stored; its `out` is not used
+ *   v   stored as it is
+ *   q   normed and rotated into its `out` in the same launch (may be NULL)
+ * rope NULL: no rotation. Stored: fp16 rounded to nearest even; FP8 e4m3(x *
+ * (1 / scale)) with k_scale / v_scale, saturating to +-448; block-scaled: a
+ * block's scale is the smallest 2^k, -32 <= k <= 8, with |x| <= 448 * 2^k for its
+ * tokens, and x is stored as e4m3(x / 2^k), saturating to +-448 (+-240 at k = 8, so
+ * that every stored value is an fp16 value; infinities saturate, NaN stays). The
+ * call that stores a block's first token sets its scale, later ones raise it where
+ * their tokens need that, and then round the block's earlier tokens again (which
+ * loses bits only of values that fall below 2^-6 of the new scale). */
+typedef struct pa_append_args {
+    int32_t         num_tokens;
+    int32_t         num_entries;
+    const int32_t*  tok_begin;      /* [num_entries + 1], rising from 0 to num_tokens */
+    const int32_t*  start_pos;      /* [num_entries] */
+    const int32_t*  slot_ids;       /* [num_entries] or NULL */
+    const int32_t*  positions;
+    const uint16_t* v;              /* like a pa_head_rows' in, num_kv_heads heads */
+    int64_t         v_stride;
+    void*           k_cache;
+    void*           v_cache;
+    uint8_t*        kv_scales;      /* block-scaled caches, 2-byte aligned */
+    const int32_t*  block_table;    /* [num_table_rows][block_table_stride] */
+    int32_t         block_table_stride;
+    int32_t         num_table_rows;
+    int32_t         num_pages;
+    int32_t         page_size;
+    float           k_scale;        /* FP8 only; a value stored as code c is c * scale */
+    float           v_scale;
+} pa_append_args;
+pa_status pa_append_rope(int dtype, const pa_append_args* a, const pa_rope* rope, const pa_head_rows* q,
+                         const pa_head_rows* k, void* stream);
 
 /* Block-table resolution probe (decode_kernels.cuh:175-177's address, with the
  * decode kernel's own device function): copies the raw cache bytes of tokens
@@ -303,14 +410,15 @@ typedef struct pa_cache_config {
     int32_t head_dim;
     int32_t max_slots;
     int32_t max_pages_per_slot;
-    int32_t dtype;      /* pa_kv_dtype */
-    float   k_scale;    /* stored = value * (1/scale), FP8 only */
+    int32_t dtype;      /* pa_kv_dtype; PA_KV_FP8_E4M3_BLOCK: page_size a multiple of 8 */
+    float   k_scale;    /* stored = value * (1/scale), FP8 only (1 where blocks have their own) */
     float   v_scale;
 } pa_cache_config;
 
 typedef struct pa_cache pa_cache;
 
 /* paged_kv_cache.cu:43-45 bytes_per_page; :47-49 pages_for_budget. */
+/* (block scales included) */
 size_t    pa_cache_bytes_per_page(const pa_cache_config* cfg);
 int       pa_cache_pages_for_budget(const pa_cache_config* cfg, size_t budget_bytes);
 /* paged_kv_cache.cu:51-74 constructor (device pools, table, seq_lens). The K
@@ -346,6 +454,18 @@ pa_status pa_cache_append(pa_cache* cache, int slot, const uint16_t* d_k, const 
  * write to it are done (the cache cannot tell), and staging goes with the cache. */
 pa_status pa_cache_append_batch(pa_cache* cache, const int32_t* slots, const int32_t* counts, int n,
                                 const uint16_t* d_k, const uint16_t* d_v, void* stream, int* appended);
+/* append_batch for tokens as the projection leaves them: k is normed and rotated
+ * on its way into the pages (any cache type), v goes as it is, and q, where
+ * given, is normed and rotated into its `out` in the same launch (pa_append_rope
+ * says what is stored; k and v have the cache's kv heads). positions: device, [sum(counts)][axes], NULL:
+ * every token's place in its sequence. Bookkeeping, ordering, capture and refusals are
+ * append_batch's. Block-scaled caches take a slot that repeats in one batch
+ * with a further launch; with rope, weights and q all NULL this is append_batch on
+ * strided tokens. */
+pa_status pa_cache_append_rope(pa_cache* cache, const int32_t* slots, const int32_t* counts, int n,
+                               const pa_rope* rope, const int32_t* positions, const pa_head_rows* q,
+                               const pa_head_rows* k, const uint16_t* v, int64_t v_stride, void* stream,
+                               int* appended);
 /* paged_kv_cache.cu:138-146 release. The slot's length on the device becomes
  * zero in order with the cache's other work: queued on the null stream where
  * every call so far was given that (the call does not wait), else before the

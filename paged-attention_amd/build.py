@@ -40,7 +40,7 @@ COMMON = [
     f"-I{CSRC}",
 ]
 
-SOURCES = ["pa_decode.hip", "pa_cache.hip", "pa_scratch.hip", "pa_plan.cpp", "pa_pool.cpp", "pa_kvcache.cpp"]
+SOURCES = ["pa_decode.hip", "pa_cache.hip", "pa_rope.hip", "pa_scratch.hip", "pa_plan.cpp", "pa_pool.cpp", "pa_kvcache.cpp", "pa_append.cpp"]
 
 # Device code only: the first kernel arguments (up to the first struct passed by
 # value) arrive preloaded in SGPRs when the wave starts, so a kernel's first

@@ -10,13 +10,18 @@
 #include <hip/hip_runtime.h>
 
 #include <cstddef>
+#include <cstdint>
 
 namespace decode {
 
-enum class KVDtype { FP16 = PA_KV_FP16, FP8_E4M3 = PA_KV_FP8_E4M3 };
+// FP8_E4M3_BLOCK (no counterpart in the reference): E4M3 with a power-of-two scale
+// for each block of tokens and kv head.
+enum class KVDtype { FP16 = PA_KV_FP16, FP8_E4M3 = PA_KV_FP8_E4M3, FP8_E4M3_BLOCK = PA_KV_FP8_E4M3_BLOCK };
 
 inline int kv_dtype_bytes(KVDtype t) { return t == KVDtype::FP16 ? 2 : 1; }
-inline const char* kv_dtype_name(KVDtype t) { return t == KVDtype::FP16 ? "fp16" : "fp8_e4m3"; }
+inline const char* kv_dtype_name(KVDtype t) {
+    return t == KVDtype::FP16 ? "fp16" : t == KVDtype::FP8_E4M3 ? "fp8_e4m3" : "fp8_e4m3_block";
+}
 
 // Everything the decode kernels read. All pointers are device pointers.
 struct DecodeParams {
@@ -55,6 +60,7 @@ struct DecodeParams {
     int block_merge       = 0;    // split rows merged inside the split kernel (set by DevicePlan::bind)
     int num_segments      = 0;    // segments of the bound plan (set by DevicePlan::bind; 0 = unknown)
     int* merge_counters   = nullptr;   // per-item arrival counters of block_merge 2 (set by DevicePlan::bind)
+    const uint8_t* kv_scales = nullptr;   // block-scaled caches: [num_pages][num_kv_heads][blocks of a page][2]
 };
 
 static_assert(sizeof(DecodeParams) == sizeof(pa_decode_params), "DecodeParams must match pa_decode_params");
@@ -66,6 +72,7 @@ static_assert(offsetof(DecodeParams, max_item_segments) == offsetof(pa_decode_pa
 static_assert(offsetof(DecodeParams, block_merge) == offsetof(pa_decode_params, block_merge));
 static_assert(offsetof(DecodeParams, num_segments) == offsetof(pa_decode_params, num_segments));
 static_assert(offsetof(DecodeParams, merge_counters) == offsetof(pa_decode_params, merge_counters));
+static_assert(offsetof(DecodeParams, kv_scales) == offsetof(pa_decode_params, kv_scales));
 static_assert(sizeof(int4) == 4 * sizeof(int32_t), "segments are int32 quadruples");
 
 namespace detail {

@@ -5,6 +5,7 @@
 // std::invalid_argument / std::length_error on bad input).
 
 #include "decode.hpp"
+#include "new_tokens.hpp"
 
 #include <hip/hip_runtime.h>
 
@@ -17,7 +18,8 @@ namespace decode {
 // Multi-head paged KV cache in HND layout: [page][kv_head][slot_in_page][head_dim].
 // Pages come from a free list and are mapped per sequence by a device block
 // table that is updated incrementally. FP8 caches quantize on append with
-// per-tensor scales (stored = value * (1 / scale)).
+// per-tensor scales (stored = value * (1 / scale)), or with a scale for each block
+// of tokens and kv head that the appends choose (KVDtype::FP8_E4M3_BLOCK).
 class PagedKVCache {
 public:
     struct Config {
@@ -72,6 +74,21 @@ public:
         detail::check(pa_cache_append_batch(h_, slots.data(), counts.data(), static_cast<int>(slots.size()),
                                             reinterpret_cast<const uint16_t*>(d_k),
                                             reinterpret_cast<const uint16_t*>(d_v), stream, &done));
+        return done != 0;
+    }
+    // append_batch for tokens as the projection leaves them: k (of the cache's kv
+    // heads) normed and rotated on its way into the pages, v (strided like k) as it is,
+    // and q, where given, normed and rotated into its output. positions null: every
+    // token's place in its sequence.
+    bool append_rope(const std::vector<int>& slots, const std::vector<int>& counts, const Rope* rope, const HeadRows* q,
+                     const HeadRows& k, const half* d_v, int64_t v_stride, const int* positions = nullptr,
+                     hipStream_t stream = 0) {
+        if (slots.size() != counts.size()) throw std::invalid_argument("append_rope: slots and counts differ in size");
+        const pa_head_rows qr = q ? detail::abi(*q) : pa_head_rows{}, kr = detail::abi(k);
+        int done = 0;
+        detail::check(pa_cache_append_rope(h_, slots.data(), counts.data(), static_cast<int>(slots.size()),
+                                           rope ? rope->handle() : nullptr, positions, q ? &qr : nullptr, &kr,
+                                           reinterpret_cast<const uint16_t*>(d_v), v_stride, stream, &done));
         return done != 0;
     }
     // Returns a slot's pages to the free list.

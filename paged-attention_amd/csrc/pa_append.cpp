@@ -1,0 +1,221 @@
+// C-ABI host layer, part 4: new tokens of a step (pa_rope.hip): the rotation
+// handle, head norms with rotation, appends with rotation into caller-owned
+// caches. (The paged cache's own append is in pa_kvcache.cpp.)
+
+#include "pa_host.hpp"
+
+#include <climits>
+#include <cmath>
+#include <cstring>
+#include <string>
+#include <vector>
+
+namespace {
+
+using namespace pa::host;
+
+bool aligned(const void* p, size_t n) { return reinterpret_cast<uintptr_t>(p) % n == 0; }
+
+// One pass indexes (token, head, 8-dim chunk) in 32 bits.
+void check_count(const char* what, long long n, long long heads) {
+    if (n * heads * (pa::kHeadDim / 8) > INT_MAX)
+        throw std::length_error(std::string(what) + ": tokens * heads * 16 exceeds INT_MAX");
+}
+
+// First and last byte (exclusive) of n strided rows of `heads` heads.
+struct Span {
+    uintptr_t lo, hi;
+};
+Span span_of(const uint16_t* p, long long stride, int n, int heads) {
+    const auto base = reinterpret_cast<uintptr_t>(p);
+    const long long last = static_cast<long long>(n - 1) * stride * 2;
+    const long long row  = 2ll * heads * pa::kHeadDim;
+    return {base + (last < 0 ? last : 0), base + (last > 0 ? last : 0) + row};
+}
+
+}  // namespace
+
+namespace pa::host {
+
+pa::RopeTable rope_table(const pa_rope* rope) {
+    pa::RopeTable t{};
+    t.scale = 1.0f;
+    if (!rope) return t;
+    int dev = 0;
+    pa::hip_check(hipGetDevice(&dev), "hipGetDevice");
+    if (dev != rope->device) throw std::invalid_argument("rope: made on another device than the current one");
+    t.half_turns  = rope->half_turns;
+    t.axes        = rope->axes;
+    t.pairs       = rope->rot_dim / 2;
+    t.num_axes    = rope->num_axes;
+    t.interleaved = rope->interleaved;
+    t.scale       = rope->scale;
+    return t;
+}
+
+pa::HeadRows head_rows(const char* what, const pa_head_rows* r, int n, bool has_out) {
+    pa::HeadRows h{};
+    if (!r || r->heads == 0) return h;
+    const std::string w = std::string(what) + ": ";
+    if (r->heads < 0) throw std::invalid_argument(w + "negative head count");
+    check_count(what, n, r->heads);
+    if (n > 0) {
+        if (!r->in) throw std::invalid_argument(w + "null rows");
+        if (!aligned(r->in, 16) || r->in_stride % 8 != 0)
+            throw std::invalid_argument(w + "rows must be 16-byte aligned, their stride a multiple of 8 elements");
+        if (r->weight && !aligned(r->weight, 16)) throw std::invalid_argument(w + "the norm weight must be 16-byte aligned");
+        if (r->weight && !(r->eps >= 0.0f)) throw std::invalid_argument(w + "eps must not be negative");
+    }
+    if (n > 0 && has_out) {
+        if (!r->out) throw std::invalid_argument(w + "null output");
+        if (!aligned(r->out, 16) || r->out_stride % 8 != 0)
+            throw std::invalid_argument(w + "outputs must be 16-byte aligned, their stride a multiple of 8 elements");
+        if (n > 1 && std::llabs(r->out_stride) < static_cast<long long>(r->heads) * pa::kHeadDim)
+            throw std::invalid_argument(w + "output rows overlap");
+        const Span in = span_of(r->in, r->in_stride, n, r->heads), out = span_of(r->out, r->out_stride, n, r->heads);
+        if (in.lo < out.hi && out.lo < in.hi && !(r->in == r->out && (n == 1 || r->in_stride == r->out_stride)))
+            throw std::invalid_argument(w + "the output overlaps the rows (it may only be the rows themselves)");
+    }
+    h.in         = r->in;
+    h.in_stride  = static_cast<long>(r->in_stride);
+    h.out        = r->out;
+    h.out_stride = static_cast<long>(r->out_stride);
+    h.weight     = r->weight;
+    h.eps        = r->eps;
+    h.heads      = r->heads;
+    return h;
+}
+
+void check_v_rows(const char* what, const uint16_t* v, int64_t stride, int n) {
+    if (n > 0 && !v) throw std::invalid_argument(std::string(what) + ": v is null");
+    if (n > 0 && (!aligned(v, 16) || stride % 8 != 0))
+        throw std::invalid_argument(std::string(what) + ": v must be 16-byte aligned, its stride a multiple of 8 elements");
+}
+
+}  // namespace pa::host
+
+using namespace pa::host;
+
+extern "C" {
+
+pa_status pa_rope_create(const double* freqs, const int32_t* axes, int rot_dim, int num_axes, int interleaved,
+                         float scale, pa_rope** out) {
+    return guarded([&] {
+        if (!freqs || !out) throw std::invalid_argument("rope: freqs or out is null");
+        if (rot_dim < 16 || rot_dim > pa::kHeadDim || rot_dim % 16 != 0)
+            throw std::invalid_argument("rope: rot_dim must be a multiple of 16 from 16 to 128");
+        if (num_axes < 1 || num_axes > 4) throw std::invalid_argument("rope: 1 to 4 axes");
+        if (num_axes > 1 && !axes) throw std::invalid_argument("rope: several axes need each pair's axis");
+        if (!std::isfinite(scale)) throw std::invalid_argument("rope: scale must be finite");
+        const int pairs = rot_dim / 2;
+        // Half turns per position, then the axes.
+        std::vector<unsigned char> host(static_cast<size_t>(pairs) * (sizeof(double) + sizeof(int32_t)));
+        for (int i = 0; i < pairs; ++i) {
+            if (!std::isfinite(freqs[i])) throw std::invalid_argument("rope: freqs must be finite");
+            const double  half = static_cast<double>(freqs[i] / 3.14159265358979323846264338327950288L);
+            const int32_t axis = axes ? axes[i] : 0;
+            if (axis < 0 || axis >= num_axes) throw std::invalid_argument("rope: a pair's axis is out of range");
+            std::memcpy(&host[static_cast<size_t>(i) * sizeof(double)], &half, sizeof half);
+            std::memcpy(&host[static_cast<size_t>(pairs) * sizeof(double) + static_cast<size_t>(i) * sizeof(int32_t)],
+                        &axis, sizeof axis);
+        }
+        auto* r = new pa_rope;
+        try {
+            r->rot_dim     = rot_dim;
+            r->num_axes    = num_axes;
+            r->interleaved = interleaved != 0;
+            r->scale       = scale;
+            pa::hip_check(hipGetDevice(&r->device), "hipGetDevice");
+            pa::hip_check(hipMalloc(reinterpret_cast<void**>(&r->half_turns), host.size()), "hipMalloc rope");
+            pa::hip_check(hipMemcpy(r->half_turns, host.data(), host.size(), hipMemcpyHostToDevice), "hipMemcpy rope");
+            r->axes = reinterpret_cast<int32_t*>(r->half_turns + pairs);
+        } catch (...) {
+            (void)hipFree(r->half_turns);
+            delete r;
+            throw;
+        }
+        *out = r;
+    });
+}
+
+void pa_rope_destroy(pa_rope* rope) {
+    if (!rope) return;
+    (void)hipFree(rope->half_turns);
+    delete rope;
+}
+int pa_rope_dim(const pa_rope* rope) { return rope ? rope->rot_dim : 0; }
+int pa_rope_axes(const pa_rope* rope) { return rope ? rope->num_axes : 0; }
+
+pa_status pa_norm_rope(const pa_rope* rope, const pa_head_rows* q, const pa_head_rows* k, const int32_t* positions,
+                       int n, void* stream) {
+    return guarded([&] {
+        if (n < 0) throw std::invalid_argument("norm_rope: negative token count");
+        pa::RopeAppend a{};
+        a.q = head_rows("norm_rope q", q, n, true);
+        a.k = head_rows("norm_rope k", k, n, true);
+        if (rope && n > 0 && !positions) throw std::invalid_argument("norm_rope: a rotation needs positions");
+        check_count("norm_rope", n, static_cast<long long>(a.q.heads) + a.k.heads + 8);
+        if (n == 0 || a.q.heads + a.k.heads == 0) return;
+        a.rope      = rope_table(rope);
+        a.positions = positions;
+        a.n_tok     = n;
+        pa::hip_check(pa::launch_norm_rope(a, as_stream(stream)), "norm_rope kernel launch");
+    });
+}
+
+int pa_block_tokens(int page_size) { return pa::block_tokens(page_size); }
+
+pa_status pa_append_rope(int dtype, const pa_append_args* p, const pa_rope* rope, const pa_head_rows* q,
+                         const pa_head_rows* k, void* stream) {
+    return guarded([&] {
+        check_dtype(dtype);
+        if (!p || !k) throw std::invalid_argument("append_rope: args or k is null");
+        if (p->num_tokens < 0 || p->num_entries < 0 || p->page_size <= 0 || p->block_table_stride <= 0 ||
+            p->num_table_rows < 0 || p->num_pages < 0)
+            throw std::invalid_argument("append_rope: bad sizes");
+        if (k->heads <= 0) throw std::invalid_argument("append_rope: k needs heads");
+        const bool block = dtype == PA_KV_FP8_E4M3_BLOCK;
+        if (block && pa::block_tokens(p->page_size) == 0)
+            throw std::invalid_argument("append_rope: block-scaled caches need a page_size that is a multiple of 8");
+        const int n = p->num_tokens;
+        pa::RopeAppend a{};
+        a.q = head_rows("append_rope q", q, n, true);
+        a.k = head_rows("append_rope k", k, n, false);
+        check_v_rows("append_rope", p->v, p->v_stride, n);
+        check_count("append_rope", n, static_cast<long long>(a.q.heads) + 2ll * k->heads + 12);
+        check_count("append_rope", p->num_entries, 64);
+        if (n == 0) return;
+        if (p->num_entries == 0) throw std::invalid_argument("append_rope: tokens of no entry");
+        if (!p->tok_begin || !p->start_pos || !p->block_table || !p->k_cache || !p->v_cache)
+            throw std::invalid_argument("append_rope: null pointer");
+        if (!aligned(p->k_cache, 16) || !aligned(p->v_cache, 16))
+            throw std::invalid_argument("append_rope: caches must be 16-byte aligned");
+        if (block && (!p->kv_scales || !aligned(p->kv_scales, 2)))
+            throw std::invalid_argument("append_rope: a block-scaled cache needs kv_scales (2-byte aligned)");
+        if (rope && rope->num_axes > 1 && !p->positions)
+            throw std::invalid_argument("append_rope: a rotation over several axes needs positions");
+        a.rope         = rope_table(rope);
+        a.v            = p->v;
+        a.v_stride     = static_cast<long>(p->v_stride);
+        a.positions    = p->positions;
+        a.n_tok        = n;
+        a.n_ent        = p->num_entries;
+        a.tok_begin    = p->tok_begin;
+        a.start        = p->start_pos;
+        a.slot_ids     = p->slot_ids;
+        a.table        = p->block_table;
+        a.table_stride = p->block_table_stride;
+        a.table_rows   = p->num_table_rows;
+        a.num_pages    = p->num_pages;
+        a.k_cache      = p->k_cache;
+        a.v_cache      = p->v_cache;
+        a.scales       = p->kv_scales;
+        a.page_size    = p->page_size;
+        const bool fp8 = dtype == PA_KV_FP8_E4M3;
+        a.inv_k        = fp8 ? 1.0f / p->k_scale : 1.0f;
+        a.inv_v        = fp8 ? 1.0f / p->v_scale : 1.0f;
+        pa::hip_check(pa::launch_append_rope(dtype, a, nullptr, 0, as_stream(stream)), "append_rope kernel launch");
+    });
+}
+
+}  // extern "C"

@@ -12,6 +12,7 @@
 //   f32_to_f16_kernel, f16_to_f32_kernel  element conversions for the legacy pool's fp32 device entry
 
 #include "pa_device.hpp"
+#include "pa_fp8.hpp"
 
 #include <algorithm>
 #include <climits>
@@ -25,92 +26,12 @@
 namespace pa {
 namespace {
 
-// ---------------------------------------------------------------------------
-// FP8 E4M3 encoder, written from the OCP OFP8 definition (bias 7, max normal
-// 448 = S.1111.110, NaN = S.1111.111, subnormals m * 2^-9): round to nearest
-// even, finite overflow and infinities saturate to +-448, NaN stays NaN.
-__device__ __forceinline__ uint32_t e4m3_encode(float x) {
-    const uint32_t u    = __builtin_bit_cast(uint32_t, x);
-    const uint32_t sign = (u >> 24) & 0x80u;
-    const uint32_t a    = u & 0x7fffffffu;
-    if (a > 0x7f800000u) return sign | 0x7fu;    // NaN
-    if (a >= 0x43e00000u) return sign | 0x7eu;   // |x| >= 448: saturate
-    if (a < 0x3c800000u) {                       // |x| < 2^-6: subnormal grid
-        const float ax = __builtin_bit_cast(float, a);
-        return sign | static_cast<uint32_t>(rintf(ax * 512.0f));   // 0..8; 8 is the min normal
-    }
-    const uint32_t man = a & 0x7fffffu;
-    uint32_t q = (((a >> 23) - 120u) << 3) | (man >> 20);
-    const uint32_t rem = man & 0xfffffu;
-    if (rem > 0x80000u || (rem == 0x80000u && (q & 1u))) q += 1u;
-    return sign | q;
-}
-
-__device__ __forceinline__ float f16_bits_to_f32(uint32_t h16) {
-    return static_cast<float>(__builtin_bit_cast(_Float16, static_cast<uint16_t>(h16)));
-}
-
 // Streaming (non-temporal) loads of the new tokens and stores into the pages:
 // both are touched once per append.
 #ifndef PA_APPEND_NT
 #define PA_APPEND_NT 1
 #endif
 constexpr bool kAppendNT = PA_APPEND_NT != 0;
-
-// E4M3 encode of eight products float(x) * inv through gfx950's OCP FP8
-// conversion (v_cvt_scalef32_pk_fp8_f32, scale 1): each product is rounded to
-// fp32 first, as e4m3_encode's argument is. Finite values are clamped to
-// +-448 beforehand (saturation, and infinities). The instruction writes every
-// NaN as 0xff; a chunk holding a NaN takes e4m3_encode instead, which keeps
-// the sign (0x7f | sign), as the software path and the oracle do.
-#ifndef PA_APPEND_HWCVT
-#define PA_APPEND_HWCVT 1
-#endif
-constexpr bool kAppendHwCvt = PA_APPEND_HWCVT != 0;
-
-typedef short v2i16 __attribute__((ext_vector_type(2)));
-
-__device__ __forceinline__ float sat448(float x) { return __builtin_fminf(__builtin_fmaxf(x, -448.0f), 448.0f); }
-
-__device__ __forceinline__ u32x2 encode8_hw(const u32x4 in, float inv) {
-    float f[8];
-    bool  nan = false;
-#pragma unroll
-    for (int e = 0; e < 8; ++e) {
-        f[e] = f16_bits_to_f32((in[e >> 1] >> (16 * (e & 1))) & 0xffffu) * inv;
-        nan |= f[e] != f[e];
-    }
-    u32x2 out = {0u, 0u};
-    if (__builtin_expect(nan, 0)) {
-#pragma unroll
-        for (int e = 0; e < 8; ++e) out[e >> 2] |= e4m3_encode(f[e]) << (8 * (e & 3));
-        return out;
-    }
-#pragma unroll
-    for (int e = 0; e < 8; ++e) f[e] = sat448(f[e]);
-#pragma unroll
-    for (int w = 0; w < 2; ++w) {
-        v2i16 r = {0, 0};
-        r = __builtin_amdgcn_cvt_scalef32_pk_fp8_f32(r, f[4 * w + 0], f[4 * w + 1], 1.0f, false);
-        r = __builtin_amdgcn_cvt_scalef32_pk_fp8_f32(r, f[4 * w + 2], f[4 * w + 3], 1.0f, true);
-        out[w] = __builtin_bit_cast(uint32_t, r);
-    }
-    return out;
-}
-
-// E4M3 bytes of eight products float(x) * inv, in software (e4m3_encode).
-[[maybe_unused]] __device__ __forceinline__ u32x2 encode8_sw(const u32x4 in, float inv) {
-    u32x2 out = {0u, 0u};
-#pragma unroll
-    for (int e = 0; e < 8; ++e)
-        out[e >> 2] |= e4m3_encode(f16_bits_to_f32((in[e >> 1] >> (16 * (e & 1))) & 0xffffu) * inv) << (8 * (e & 3));
-    return out;
-}
-
-__device__ __forceinline__ u32x2 encode8(const u32x4 in, float inv) {
-    if constexpr (kAppendHwCvt) return encode8_hw(in, inv);
-    else return encode8_sw(in, inv);
-}
 
 // Dims of one row that one thread appends: 8 for fp16 (one 16-byte load and
 // one 16-byte store per pool), 16 for FP8 (two 16-byte loads of fp16, one

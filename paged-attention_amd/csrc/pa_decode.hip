@@ -277,15 +277,6 @@ __device__ __forceinline__ int cursor_step(Cursor& c, const int4* segs, int seg_
     return 1;
 }
 
-// p[i] for a wave-uniform p and i, as a scalar load: the block table is not
-// written while a decode kernel runs, so it may be read through the constant
-// address space, whose loads the compiler always makes scalar (the table reads
-// then stay out of the vector memory counters that the LDS stage waits on).
-__device__ __forceinline__ int load_uniform(const int32_t* p, int i) {
-    using const_ptr = const __attribute__((address_space(4))) int32_t*;
-    return ((const_ptr)(reinterpret_cast<uintptr_t>(p)))[__builtin_amdgcn_readfirstlane(i)];
-}
-
 // Block-table row of batch row b (decode_kernels.cuh:150-153).
 __device__ __forceinline__ const int* table_row(const pa_decode_params& p, const int32_t* __restrict__ tbl,
                                                 const int32_t* __restrict__ sid, int b) {
@@ -549,7 +540,8 @@ __device__ __forceinline__ void block_merge(const pa_decode_params& p, const Slo
 //   NG    tokens per step (16 or 32)
 //   DEPTH steps of K/V in flight per wave
 //   PATH  page resolution (PagePath)
-template <int EB, int G, int NG, int DEPTH, int PATH>
+//   BS    block scales (EB 1; the page-run and power-of-two paths)
+template <int EB, int G, int NG, int DEPTH, int PATH, bool BS = false>
 __device__ __forceinline__ void decode_split_body(const pa_decode_params& p, const int32_t* __restrict__ cta,
                                                   int num_units, const PageDiv pd,
                                                   const int32_t* __restrict__ tbl, const int32_t* __restrict__ sid,
@@ -577,6 +569,8 @@ __device__ __forceinline__ void decode_split_body(const pa_decode_params& p, con
     // The stage's chunk permutation of row r (XOR with r % CPR).
     auto swz = [](int r) { return kStageSwizzle ? r % CPR : 0; };
     static_assert(!DMA || DEPTH == 1, "the LDS-destination stage holds one step");
+    static_assert(!BS || (EB == 1 && (RUNS || PATH == kPagePow2)), "block scales: FP8, wave-uniform pages");
+    constexpr int  NSC = RUNS ? NPART : 1;          // scale pairs per half: one a part, else one
     using VRaw = std::conditional_t<EB == 2, u32x4, u32x2>;
     using KRaw = std::conditional_t<KL == 16, u32x4, u32x2>;
 
@@ -640,6 +634,7 @@ __device__ __forceinline__ void decode_split_body(const pa_decode_params& p, con
     for (int part = 0; part < NPART; ++part)
         dma_chunk[part] = 16 * ((lane % CPR) ^ swz(RPP * part + lane / CPR));
     u32x4* const stage = stage_lds[STG ? wave : 0];
+    const int sc_shift = PATH == kPagePow2 || P % 16 == 0 ? 4 : 3;   // log2 of a scale block's tokens
 
     // ---- pipeline registers, indexed by ring slot = step index mod DEPTH
     KRaw  kr[DEPTH][NH][NK];   // K: token 16hh + c of each half
@@ -656,6 +651,11 @@ __device__ __forceinline__ void decode_split_body(const pa_decode_params& p, con
     int   pent[LN];                                        // lane path: table entry `first page + lane`
     int   pk[DEPTH][NH], sk[DEPTH][NH];            // per-lane paths: K token's page and slot
     int   pv[DEPTH][NH][NVL], sv[DEPTH][NH][NVL];  // per-lane paths: V tokens' page(s) and slot(s)
+    int   scw[BS ? DEPTH : 1][NH][NSC], scs[BS ? DEPTH : 1][NH][NSC];   // block scales: the word that holds the
+                                                                        // pair of bytes, and where in it
+    float ks[NH], vs[NH];   // the current step's scales of the lane's tokens (4kb .. 4kb + 3 of each half)
+#pragma unroll
+    for (int hh = 0; hh < NH; ++hh) ks[hh] = vs[hh] = 1.0f;
 
     Cursor C, L, T;
     C.seg = seg_begin;
@@ -741,6 +741,16 @@ __device__ __forceinline__ void decode_split_body(const pa_decode_params& p, con
         }
     };
 
+    // The word with the K and V scale bytes of the block that holds slot `slot`
+    // of a page (wave-uniform): a scalar load beside the block's rows, used a
+    // step later. (The pair is 2-byte aligned; the aligned word around it ends
+    // inside the array's last 4 bytes.)
+    auto load_scales = [&](int s, int hh, int n, int page, int slot) {
+        const int idx = (page * hkv + L.h) * (P >> sc_shift) + (slot >> sc_shift);
+        scw[s][hh][n] = load_uniform(reinterpret_cast<const int32_t*>(p.kv_scales), idx >> 1);
+        scs[s][hh][n] = 16 * (idx & 1);
+    };
+
     // K/V loads of step L into slot s (and Q at a segment start), then advance L.
     auto issue = [&](int s) {
         if constexpr (DMA) {
@@ -776,6 +786,7 @@ __device__ __forceinline__ void decode_split_body(const pa_decode_params& p, con
                 const int nv = __builtin_amdgcn_readfirstlane(l_more ? max(0, min(16, L.w - t)) : 0);
                 const size_t row0 = static_cast<size_t>(__builtin_amdgcn_readfirstlane(pg[s][hh])) * page_bytes +
                                     static_cast<uint32_t>((L.h * P + (bt & (P - 1))) * ROW);
+                if constexpr (BS) load_scales(s, hh, 0, pg[s][hh], bt & (P - 1));
                 const __amdgpu_buffer_rsrc_t krs = buffer_rsrc(kbase + row0, nv * ROW);
                 const __amdgpu_buffer_rsrc_t vrs = buffer_rsrc(vbase + row0, nv * ROW);
                 if constexpr (DMA) {
@@ -826,6 +837,7 @@ __device__ __forceinline__ void decode_split_body(const pa_decode_params& p, con
                     const size_t row0 =
                         static_cast<size_t>(__builtin_amdgcn_readfirstlane(pgr[s][hh][part])) * page_bytes +
                         static_cast<uint32_t>((L.h * P + part_slot(bt)) * ROW);
+                    if constexpr (BS) load_scales(s, hh, part, pgr[s][hh][part], part_slot(bt));
                     const __amdgpu_buffer_rsrc_t krs = buffer_rsrc(kbase + row0, nv * ROW);
                     const __amdgpu_buffer_rsrc_t vrs = buffer_rsrc(vbase + row0, nv * ROW);
                     if constexpr (DMA) {
@@ -990,6 +1002,16 @@ __device__ __forceinline__ void decode_split_body(const pa_decode_params& p, con
             item_n  = isb[item + 1] - item_s0;
             whole   = item_n == 1;
         }
+        if constexpr (BS) {
+            // Two parts of 8 tokens, or one block a half: lanes kb 0, 1 and 2, 3.
+#pragma unroll
+            for (int hh = 0; hh < NH; ++hh) {
+                int w = scw[s][hh][0] >> scs[s][hh][0];
+                if constexpr (NSC > 1) w = kb < 2 ? w : scw[s][hh][NSC - 1] >> scs[s][hh][NSC - 1];
+                ks[hh] = __builtin_bit_cast(float, (static_cast<uint32_t>(w) & 0xffu) << 23);
+                vs[hh] = __builtin_bit_cast(float, (static_cast<uint32_t>(w) >> 8 & 0xffu) << 23);
+            }
+        }
         if constexpr (STG) {
             // Coalesced rows -> LDS (16-byte chunk j of row r at chunk j ^ (r % CPR))
             // -> the K / V lane layouts of the direct loads.
@@ -1050,7 +1072,7 @@ __device__ __forceinline__ void decode_split_body(const pa_decode_params& p, con
                 sacc = __builtin_amdgcn_mfma_f32_16x16x32_f16(a, __builtin_bit_cast(f16x8, qf[j]), sacc, 0, 0, 0);
             }
 #pragma unroll
-            for (int i = 0; i < 4; ++i) x[hh][i] = sacc[i] * qk_scale;
+            for (int i = 0; i < 4; ++i) x[hh][i] = sacc[i] * (BS ? qk_scale * ks[hh] : qk_scale);
         }
         const int lim = C.w - C.tok;   // valid tokens of the step
         if (__builtin_expect(lim < NG, 0)) {
@@ -1094,10 +1116,10 @@ __device__ __forceinline__ void decode_split_body(const pa_decode_params& p, con
                     const uint32_t hi01 = __builtin_amdgcn_perm(vr[s][0][1][w], vr[s][0][0][w], 0x07030602u);
                     const uint32_t lo23 = __builtin_amdgcn_perm(vr[s][0][3][w], vr[s][0][2][w], 0x05010400u);
                     const uint32_t hi23 = __builtin_amdgcn_perm(vr[s][0][3][w], vr[s][0][2][w], 0x07030602u);
-                    const u32x2 b0 = {fp8x2_to_f16x2<false>(lo01), fp8x2_to_f16x2<false>(lo23)};
-                    const u32x2 b1 = {fp8x2_to_f16x2<true>(lo01), fp8x2_to_f16x2<true>(lo23)};
-                    const u32x2 b2 = {fp8x2_to_f16x2<false>(hi01), fp8x2_to_f16x2<false>(hi23)};
-                    const u32x2 b3 = {fp8x2_to_f16x2<true>(hi01), fp8x2_to_f16x2<true>(hi23)};
+                    const u32x2 b0 = {fp8x2_to_f16x2<false>(lo01, vs[0]), fp8x2_to_f16x2<false>(lo23, vs[0])};
+                    const u32x2 b1 = {fp8x2_to_f16x2<true>(lo01, vs[0]), fp8x2_to_f16x2<true>(lo23, vs[0])};
+                    const u32x2 b2 = {fp8x2_to_f16x2<false>(hi01, vs[0]), fp8x2_to_f16x2<false>(hi23, vs[0])};
+                    const u32x2 b3 = {fp8x2_to_f16x2<true>(hi01, vs[0]), fp8x2_to_f16x2<true>(hi23, vs[0])};
                     oacc[4 * w + 0] = __builtin_amdgcn_mfma_f32_16x16x16f16(pa, __builtin_bit_cast(f16x4, b0), oacc[4 * w + 0], 0, 0, 0);
                     oacc[4 * w + 1] = __builtin_amdgcn_mfma_f32_16x16x16f16(pa, __builtin_bit_cast(f16x4, b1), oacc[4 * w + 1], 0, 0, 0);
                     oacc[4 * w + 2] = __builtin_amdgcn_mfma_f32_16x16x16f16(pa, __builtin_bit_cast(f16x4, b2), oacc[4 * w + 2], 0, 0, 0);
@@ -1134,14 +1156,14 @@ __device__ __forceinline__ void decode_split_body(const pa_decode_params& p, con
                         lo23[hh] = __builtin_amdgcn_perm(vr[s][hh][3][w], vr[s][hh][2][w], 0x05010400u);
                         hi23[hh] = __builtin_amdgcn_perm(vr[s][hh][3][w], vr[s][hh][2][w], 0x07030602u);
                     }
-                    const u32x4 b0 = {fp8x2_to_f16x2<false>(lo01[0]), fp8x2_to_f16x2<false>(lo23[0]),
-                                      fp8x2_to_f16x2<false>(lo01[1]), fp8x2_to_f16x2<false>(lo23[1])};
-                    const u32x4 b1 = {fp8x2_to_f16x2<true>(lo01[0]), fp8x2_to_f16x2<true>(lo23[0]),
-                                      fp8x2_to_f16x2<true>(lo01[1]), fp8x2_to_f16x2<true>(lo23[1])};
-                    const u32x4 b2 = {fp8x2_to_f16x2<false>(hi01[0]), fp8x2_to_f16x2<false>(hi23[0]),
-                                      fp8x2_to_f16x2<false>(hi01[1]), fp8x2_to_f16x2<false>(hi23[1])};
-                    const u32x4 b3 = {fp8x2_to_f16x2<true>(hi01[0]), fp8x2_to_f16x2<true>(hi23[0]),
-                                      fp8x2_to_f16x2<true>(hi01[1]), fp8x2_to_f16x2<true>(hi23[1])};
+                    const u32x4 b0 = {fp8x2_to_f16x2<false>(lo01[0], vs[0]), fp8x2_to_f16x2<false>(lo23[0], vs[0]),
+                                      fp8x2_to_f16x2<false>(lo01[1], vs[1]), fp8x2_to_f16x2<false>(lo23[1], vs[1])};
+                    const u32x4 b1 = {fp8x2_to_f16x2<true>(lo01[0], vs[0]), fp8x2_to_f16x2<true>(lo23[0], vs[0]),
+                                      fp8x2_to_f16x2<true>(lo01[1], vs[1]), fp8x2_to_f16x2<true>(lo23[1], vs[1])};
+                    const u32x4 b2 = {fp8x2_to_f16x2<false>(hi01[0], vs[0]), fp8x2_to_f16x2<false>(hi23[0], vs[0]),
+                                      fp8x2_to_f16x2<false>(hi01[1], vs[1]), fp8x2_to_f16x2<false>(hi23[1], vs[1])};
+                    const u32x4 b3 = {fp8x2_to_f16x2<true>(hi01[0], vs[0]), fp8x2_to_f16x2<true>(hi23[0], vs[0]),
+                                      fp8x2_to_f16x2<true>(hi01[1], vs[1]), fp8x2_to_f16x2<true>(hi23[1], vs[1])};
                     oacc[4 * w + 0] = __builtin_amdgcn_mfma_f32_16x16x32_f16(pa, __builtin_bit_cast(f16x8, b0), oacc[4 * w + 0], 0, 0, 0);
                     oacc[4 * w + 1] = __builtin_amdgcn_mfma_f32_16x16x32_f16(pa, __builtin_bit_cast(f16x8, b1), oacc[4 * w + 1], 0, 0, 0);
                     oacc[4 * w + 2] = __builtin_amdgcn_mfma_f32_16x16x32_f16(pa, __builtin_bit_cast(f16x8, b2), oacc[4 * w + 2], 0, 0, 0);
@@ -1230,6 +1252,17 @@ void decode_split_kernel_fp8(const int32_t* __restrict__ cta, const int32_t* __r
                              const pa_decode_params p) {
     decode_split_body<1, G, NG, DEPTH, PATH>(p, cta, num_units, PageDiv{page_shift, page_magic}, tbl, sid, segp,
                                               isb);
+}
+
+// The FP8 kernel over a block-scaled cache.
+template <int G, int NG, int DEPTH, int PATH>
+__global__ __launch_bounds__(64 * kWaves) __attribute__((amdgpu_waves_per_eu(PA_FP8_WAVES_PER_EU)))
+void decode_split_kernel_fp8_block(const int32_t* __restrict__ cta, const int32_t* __restrict__ segp,
+                                   const int32_t* __restrict__ tbl, const int32_t* __restrict__ sid, int num_units,
+                                   int page_shift, const int32_t* __restrict__ isb, uint32_t page_magic,
+                                   const pa_decode_params p) {
+    decode_split_body<1, G, NG, DEPTH, PATH, true>(p, cta, num_units, PageDiv{page_shift, page_magic}, tbl, sid,
+                                                    segp, isb);
 }
 
 // ---------------------------------------------------------------------------
@@ -1396,10 +1429,14 @@ template <int EB> constexpr int kLaneDepth = kLdsDma ? 1 : EB == 2 ? PA_FP16_LAN
 template <int EB> constexpr int kPow2Depth = kLdsDma && Tune<EB>::stage ? 1 : Tune<EB>::depth;
 template <int EB> constexpr int kRunsDepth = kLdsDma ? 1 : Tune<EB>::depth;
 
-template <int EB, int G, int NG, int DEPTH, int PATH>
+template <int EB, int G, int NG, int DEPTH, int PATH, bool BS = false>
 hipError_t launch_split_p(const pa_decode_params& p, const PageDiv& pd, hipStream_t s) {
     const int blocks = (p.num_ctas + kWaves - 1) / kWaves;
-    if constexpr (EB == 2)
+    if constexpr (BS)
+        hipLaunchKernelGGL((decode_split_kernel_fp8_block<G, NG, DEPTH, PATH>), dim3(blocks), dim3(64 * kWaves), 0, s,
+                           p.cta_seg_begin, p.segments, p.block_table, p.slot_ids, p.num_ctas, pd.shift,
+                           p.item_seg_begin, pd.magic, p);
+    else if constexpr (EB == 2)
         hipLaunchKernelGGL((decode_split_kernel_f16<G, NG, DEPTH, PATH>), dim3(blocks), dim3(64 * kWaves), 0, s,
                            p.cta_seg_begin, p.segments, p.block_table, p.slot_ids, p.num_ctas, pd.shift,
                            p.item_seg_begin, pd.magic, p);
@@ -1417,7 +1454,7 @@ PageDiv page_div(int page_size) {
     return {~(l - 1), static_cast<uint32_t>((1ull << (31 + l)) / P + 1)};
 }
 
-template <int EB, int G>
+template <int EB, int G, bool BS = false>
 hipError_t launch_split_g(const pa_decode_params& p, hipStream_t s) {
     const int     P     = p.page_size;
     const PageDiv pd    = page_div(P);
@@ -1428,16 +1465,23 @@ hipError_t launch_split_g(const pa_decode_params& p, hipStream_t s) {
     auto need_small = [&] {
         if (!small) throw std::invalid_argument("decode: page_size * num_kv_heads * row bytes must be below 2^31");
     };
+    if constexpr (BS) {
+        // A block (16 tokens, or 8 where pages are 8 modulo 16) is a 16-token
+        // half where pages are powers of two from 16 on; elsewhere each 1 KiB
+        // part (8 tokens) takes the scales of the block it lies in.
+        if (block_tokens(P) == 0) throw std::invalid_argument("decode: block-scaled caches need a page_size that is a multiple of 8");
+        need_small();
+    }
     if (pow2 && P >= 16) {
         need_small();
-        return launch_split_p<EB, G, Tune<EB>::step, kPow2Depth<EB>, kPagePow2>(p, pd, s);
+        return launch_split_p<EB, G, Tune<EB>::step, kPow2Depth<EB>, kPagePow2, BS>(p, pd, s);
     }
     if constexpr (EB == 2 || Tune<EB>::stage) {
         // Pages of whole 1 KiB parts (4 fp16 rows, 8 FP8 rows) through the LDS stage.
         constexpr int RPP = 1024 / kRowBytes<EB>;
         if (P == 8 || (EB == 2 && P == 4)) {
             need_small();
-            return launch_split_p<EB, G, Tune<EB>::step, kRunsDepth<EB>, kPageRuns>(p, pd, s);
+            return launch_split_p<EB, G, Tune<EB>::step, kRunsDepth<EB>, kPageRuns, BS>(p, pd, s);
         }
         // The same for pages that are no powers of two but hold whole parts
         // (pages past the 32-bit offsets stay on the per-lane path): one scalar
@@ -1449,22 +1493,25 @@ hipError_t launch_split_g(const pa_decode_params& p, hipStream_t s) {
         // -> 160.3. Sizes below one part (fp16 1 to 3, FP8 1 to 7) and sizes
         // whose pages cut a part in two have no such resource.
         if (!pow2 && P % RPP == 0 && small)
-            return launch_split_p<EB, G, Tune<EB>::step, kRunsDepth<EB>, kPageRunsDiv>(p, pd, s);
+            return launch_split_p<EB, G, Tune<EB>::step, kRunsDepth<EB>, kPageRunsDiv, BS>(p, pd, s);
+        if constexpr (BS) throw std::invalid_argument("decode: no path for this block-scaled page size");
         // Any other size: per-lane rows through the LDS stage.
-        return launch_split_p<EB, G, Tune<EB>::step, kLaneDepth<EB>, kPageLane>(p, pd, s);
+        else return launch_split_p<EB, G, Tune<EB>::step, kLaneDepth<EB>, kPageLane>(p, pd, s);
+    } else if constexpr (BS) {
+        throw std::invalid_argument("decode: this build has no LDS stage for block-scaled pages of this size");
     } else {
         if (pow2 && P >= 4) return launch_split_p<EB, G, Tune<EB>::step, kLaneDepth<EB>, kPageQuad>(p, pd, s);
         return launch_split_p<EB, G, Tune<EB>::step, kLaneDepth<EB>, kPageAny>(p, pd, s);
     }
 }
 
-template <int EB>
+template <int EB, bool BS = false>
 hipError_t launch_split_e(const pa_decode_params& p, int group, hipStream_t s) {
     switch (group) {
-        case 1: return launch_split_g<EB, 1>(p, s);
-        case 2: return launch_split_g<EB, 2>(p, s);
-        case 4: return launch_split_g<EB, 4>(p, s);
-        case 8: return launch_split_g<EB, 8>(p, s);
+        case 1: return launch_split_g<EB, 1, BS>(p, s);
+        case 2: return launch_split_g<EB, 2, BS>(p, s);
+        case 4: return launch_split_g<EB, 4, BS>(p, s);
+        case 8: return launch_split_g<EB, 8, BS>(p, s);
     }
     throw std::invalid_argument("unsupported GQA group size " + std::to_string(group));
 }
@@ -1509,9 +1556,12 @@ int checked_group(const pa_decode_params& p) {
     return g;
 }
 
-template <int EB, int G>
+template <int EB, int G, bool BS = false>
 const void* split_symbol() {
-    if constexpr (EB == 2)
+    if constexpr (BS)
+        return reinterpret_cast<const void*>(
+            &decode_split_kernel_fp8_block<G, Tune<EB>::step, kPow2Depth<EB>, kPagePow2>);
+    else if constexpr (EB == 2)
         return reinterpret_cast<const void*>(
             &decode_split_kernel_f16<G, Tune<EB>::step, kPow2Depth<EB>, kPagePow2>);
     else
@@ -1531,12 +1581,12 @@ int kernel_tile_tokens(int dtype, int group) {
 int kernel_units_per_cu(int dtype, int group) {
     check_kv_dtype(dtype);
     const void* fn = nullptr;
-    const bool fp16 = dtype == PA_KV_FP16;
+    const bool fp16 = dtype == PA_KV_FP16, bs = dtype == PA_KV_FP8_E4M3_BLOCK;
     switch (group) {
-        case 1: fn = fp16 ? split_symbol<2, 1>() : split_symbol<1, 1>(); break;
-        case 2: fn = fp16 ? split_symbol<2, 2>() : split_symbol<1, 2>(); break;
-        case 4: fn = fp16 ? split_symbol<2, 4>() : split_symbol<1, 4>(); break;
-        case 8: fn = fp16 ? split_symbol<2, 8>() : split_symbol<1, 8>(); break;
+        case 1: fn = fp16 ? split_symbol<2, 1>() : bs ? split_symbol<1, 1, true>() : split_symbol<1, 1>(); break;
+        case 2: fn = fp16 ? split_symbol<2, 2>() : bs ? split_symbol<1, 2, true>() : split_symbol<1, 2>(); break;
+        case 4: fn = fp16 ? split_symbol<2, 4>() : bs ? split_symbol<1, 4, true>() : split_symbol<1, 4>(); break;
+        case 8: fn = fp16 ? split_symbol<2, 8>() : bs ? split_symbol<1, 8, true>() : split_symbol<1, 8>(); break;
         default: throw std::invalid_argument("unsupported GQA group size " + std::to_string(group));
     }
     int blocks = 0;
@@ -1575,6 +1625,11 @@ hipError_t launch_decode_split(int dtype, const pa_decode_params& p, hipStream_t
     if (p.block_merge < 0 || p.block_merge > 4) throw std::invalid_argument("decode: block_merge must be 0 to 4");
     if ((p.block_merge == 2 || p.block_merge == 3) && !p.merge_counters)
         throw std::invalid_argument("decode: block_merge 2 and 3 need the plan's merge counters");
+    if (dtype == PA_KV_FP8_E4M3_BLOCK) {
+        if (!p.kv_scales || reinterpret_cast<uintptr_t>(p.kv_scales) % 4 != 0)
+            throw std::invalid_argument("decode: a block-scaled cache needs kv_scales (4-byte aligned)");
+        return launch_split_e<1, true>(p, g, s);
+    }
     return dtype == PA_KV_FP16 ? launch_split_e<2>(p, g, s) : launch_split_e<1>(p, g, s);
 }
 

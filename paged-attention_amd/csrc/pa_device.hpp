@@ -54,11 +54,21 @@ __device__ __forceinline__ float readlane_f(float v, int lane) {
     return __builtin_bit_cast(float, __builtin_amdgcn_readlane(__builtin_bit_cast(int, v), lane));
 }
 
+// p[i] for a wave-uniform p and i, as a scalar load: what it reads (block
+// tables, block scales, an append's arrays) is not written while the kernel runs,
+// so it may be read through the constant address space, whose loads the compiler
+// always makes scalar (in the decode kernel the reads then stay out of the vector
+// memory counters that the LDS stage waits on).
+__device__ __forceinline__ int load_uniform(const int32_t* p, int i) {
+    using const_ptr = const __attribute__((address_space(4))) int32_t*;
+    return ((const_ptr)(reinterpret_cast<uintptr_t>(p)))[__builtin_amdgcn_readfirstlane(i)];
+}
+
 // Two FP8 E4M3 bytes (byte pair HI of w) -> two fp16, exactly (every E4M3
-// value is an fp16 value; scale 1.0).
+// value is an fp16 value; scale 1.0), or those values times a power of two.
 template <bool HI>
-__device__ __forceinline__ uint32_t fp8x2_to_f16x2(uint32_t w) {
-    const f16x2 h = __builtin_amdgcn_cvt_scalef32_pk_f16_fp8(w, 1.0f, HI);
+__device__ __forceinline__ uint32_t fp8x2_to_f16x2(uint32_t w, float scale = 1.0f) {
+    const f16x2 h = __builtin_amdgcn_cvt_scalef32_pk_f16_fp8(w, scale, HI);
     return __builtin_bit_cast(uint32_t, h);
 }
 

@@ -90,6 +90,18 @@ struct pa_device_plan {
     pa_stage_pool staging;
 };
 
+// A model's rotation: half turns per position of each pair and the pairs' axes, in
+// one device block of the device it was made on.
+struct pa_rope {
+    double*  half_turns  = nullptr;
+    int32_t* axes        = nullptr;
+    int      rot_dim     = 0;
+    int      num_axes    = 1;
+    int      interleaved = 0;
+    float    scale       = 1.0f;
+    int      device      = 0;
+};
+
 // Host page allocator and per-slot block tables (paged_kv_cache.hpp:89-92).
 struct pa_pool {
     int page_size          = 0;
@@ -112,6 +124,7 @@ struct pa_cache {
     pa_pool         pool;
     void*           d_k          = nullptr;
     void*           d_v          = nullptr;
+    uint8_t*        d_scales     = nullptr;   // block-scaled: [num_pages][num_kv_heads][blocks][2]
     int32_t*        d_table      = nullptr;   // [max_slots][max_pages_per_slot]
     int32_t*        d_seq_lens   = nullptr;   // [max_slots]
     pa_plan         plan;
@@ -214,6 +227,13 @@ void decode_impl(int dtype, const pa_decode_params& p, hipStream_t s, bool split
 // outside any graph capture of the decode that follows.
 void scratch_prepare();
 size_t scratch_bytes();   // the array's size
+
+// ---- new tokens (pa_append.cpp)
+// The kernels' form of a rotation (none for null), refused on another device.
+pa::RopeTable rope_table(const pa_rope* rope);
+// The same for head rows (no heads for null), checked for n tokens.
+pa::HeadRows head_rows(const char* what, const pa_head_rows* r, int n, bool has_out);
+void check_v_rows(const char* what, const uint16_t* v, int64_t stride, int n);
 
 // ---- page pool (pa_pool.cpp)
 // Entry i of a batched append: the slot's length before it, and the table

@@ -48,7 +48,7 @@ constexpr int kBlockUnits  = PA_BLOCK_UNITS;   // work units (waves) per block o
 constexpr size_t kPoolStagger = PA_POOL_STAGGER;
 
 inline void check_kv_dtype(int dtype) {
-    if (dtype != PA_KV_FP16 && dtype != PA_KV_FP8_E4M3)
+    if (dtype != PA_KV_FP16 && dtype != PA_KV_FP8_E4M3 && dtype != PA_KV_FP8_E4M3_BLOCK)
         throw std::invalid_argument("unknown kv dtype " + std::to_string(dtype));
 }
 
@@ -99,6 +99,67 @@ hipError_t launch_append_batch(int dtype, const AppendBatch& a, const int32_t* m
 // Whether an append's meta of n ints fits the kernel arguments (4 KiB in all).
 constexpr size_t kAppendInlineInts = 896;
 constexpr bool   append_meta_inline(size_t n) { return n <= kAppendInlineInts; }
+// Block-scaled caches: tokens per block, the exponents that a scale may have, and
+// the largest code at the largest of them (240 * 2^8 = 61440; 448 * 2^8, and even
+// 256 * 2^8, would be past fp16, which the decode kernel widens to).
+constexpr int block_tokens(int page_size) { return page_size <= 0 || page_size % 8 ? 0 : page_size % 16 ? 8 : 16; }
+constexpr int   kBlockExpMin = -32, kBlockExpMax = 8;
+constexpr float kBlockTop    = 240.0f;
+
+// A rotation on the device (pairs 0: none): half turns per position of each pair,
+// and the axis whose position turns it.
+struct RopeTable {
+    const double*  half_turns;
+    const int32_t* axes;
+    int            pairs, num_axes, interleaved;
+    float          scale;
+};
+// pa_head_rows, checked.
+struct HeadRows {
+    const uint16_t* in;
+    long            in_stride;
+    uint16_t*       out;
+    long            out_stride;
+    const float*    weight;
+    float           eps;
+    int             heads;
+};
+// One launch of head rows, with or without an append. Where the tokens go comes
+// from the caller's device arrays (tok_begin, start, slot_ids, table), or is a
+// cache's meta as for AppendBatch (meta, or the list kernels' arguments).
+struct RopeAppend {
+    RopeTable       rope;
+    HeadRows        q, k;
+    const uint16_t* v;
+    long            v_stride;
+    const int32_t*  positions;
+    int             n_tok, n_ent;
+    const int32_t*  tok_begin;
+    const int32_t*  start;
+    const int32_t*  slot_ids;
+    const int32_t*  table;
+    int             table_stride, table_rows, num_pages;
+    const int32_t*  meta;
+    int             n_pl, n_tab, n_len;
+    int32_t*        new_table;
+    int32_t*        new_lens;
+    void*           k_cache;
+    void*           v_cache;
+    uint8_t*        scales;
+    int             page_size;
+    float           inv_k, inv_v;
+    int             block_tokens, units;   // block-scaled caches (set by the launch)
+};
+template <int N>
+struct RopeInline {
+    RopeAppend a;
+    alignas(16) int32_t meta[N];
+};
+// Ints of meta that fit the kernel arguments beside RopeAppend.
+constexpr size_t kRopeInlineInts = 896;
+static_assert(sizeof(RopeInline<kRopeInlineInts>) <= 4096, "kernel arguments are 4 KiB at most");
+hipError_t launch_norm_rope(const RopeAppend& a, hipStream_t s);
+hipError_t launch_append_rope(int dtype, const RopeAppend& a, const int32_t* meta, size_t n_meta, hipStream_t s);
 // Stores one zero.
 hipError_t launch_zero_int(int32_t* p, hipStream_t s);
 // Copies n ints (rounded up to whole 16 bytes) from pinned host memory to the

@@ -14,11 +14,19 @@ namespace {
 
 using namespace pa::host;
 
-size_t bytes_per_page_impl(const pa_cache_config& cfg) {
-    const int eb = cfg.dtype == PA_KV_FP8_E4M3 ? 1 : 2;
+size_t kv_bytes_per_page(const pa_cache_config& cfg) {
+    const int eb = cfg.dtype == PA_KV_FP8_E4M3 || cfg.dtype == PA_KV_FP8_E4M3_BLOCK ? 1 : 2;
     return 2ull * static_cast<size_t>(cfg.num_kv_heads) * static_cast<size_t>(cfg.page_size) *
            static_cast<size_t>(cfg.head_dim) * static_cast<size_t>(eb);
 }
+
+// Block scales of one page: a K and a V byte for each block and kv head.
+size_t scale_bytes_per_page(const pa_cache_config& cfg) {
+    const int b = cfg.dtype == PA_KV_FP8_E4M3_BLOCK ? pa::block_tokens(cfg.page_size) : 0;
+    return b ? 2ull * static_cast<size_t>(cfg.num_kv_heads) * static_cast<size_t>(cfg.page_size / b) : 0;
+}
+
+size_t bytes_per_page_impl(const pa_cache_config& cfg) { return kv_bytes_per_page(cfg) + scale_bytes_per_page(cfg); }
 
 void cache_params(const pa_cache& c, pa_decode_params& p) {
     p = pa_decode_params{};
@@ -34,6 +42,7 @@ void cache_params(const pa_cache& c, pa_decode_params& p) {
     const bool fp8       = c.cfg.dtype == PA_KV_FP8_E4M3;
     p.k_scale            = fp8 ? c.cfg.k_scale : 1.0f;
     p.v_scale            = fp8 ? c.cfg.v_scale : 1.0f;
+    p.kv_scales          = c.d_scales;
 }
 
 // Records that an append was queued on s: one event per stream, moved on by
@@ -58,19 +67,27 @@ void mark_append(pa_cache& c, hipStream_t s) {
     pa::hip_check(hipEventRecord(c.append_marks[i].done, s), "hipEventRecord append");
 }
 
-// Queues one kernel that writes the tokens of reserved entries, the table
-// entries they added and the new lengths. Its meta (layout of
+// What an append kernel finds its tokens' places by: meta on the device, or null
+// where it goes over in the arguments.
+struct append_meta {
+    const int32_t* dev;
+    int n_ent, n_pl, n_tab, n_len, n_tok;
+};
+
+// Queues one kernel (launch(meta, host ints or null, how many)) that writes the
+// tokens of reserved entries, the table entries they added and the new lengths.
+// Its meta (layout of
 // pa::AppendBatch::meta: per entry its first token, old length and page-list
 // start; the page lists; the new table entries; one (slot, length) per distinct
 // slot) goes over in the kernel's arguments when it fits, else through a staging
 // buffer and a copy kernel.
-void queue_append(pa_cache& c, const int32_t* slots, const int32_t* counts, int n,
-                  const std::vector<reserve_entry>& entries, long n_tok, const uint16_t* d_k, const uint16_t* d_v,
-                  hipStream_t s) {
+template <class Launch>
+void queue_meta(pa_cache& c, const int32_t* slots, const int32_t* counts, int n, const reserve_entry* entries,
+                long n_tok, hipStream_t s, Launch&& launch) {
     const int P = c.cfg.page_size;
     long n_tab = 0, n_pl = 0;
     for (int i = 0; i < n; ++i) {
-        const reserve_entry& e = entries[static_cast<size_t>(i)];
+        const reserve_entry& e = entries[i];
         n_tab += e.num_new;
         if (counts[i] > 0) n_pl += (e.old_len + counts[i] - 1) / P - e.old_len / P + 1;
     }
@@ -92,7 +109,7 @@ void queue_append(pa_cache& c, const int32_t* slots, const int32_t* counts, int 
     int32_t  tok = 0, pl = 0;
     for (int i = 0; i < n; ++i) {
         const auto& table = c.pool.tables[static_cast<size_t>(slots[i])];
-        const reserve_entry& e = entries[static_cast<size_t>(i)];
+        const reserve_entry& e = entries[i];
         tok_begin[i] = tok;
         old_len[i]   = e.old_len;
         pl_begin[i]  = pl;
@@ -111,32 +128,110 @@ void queue_append(pa_cache& c, const int32_t* slots, const int32_t* counts, int 
         *lens++ = slots[i];
         *lens++ = c.pool.seq_lens[sl];
     }
-    const bool fp8 = c.cfg.dtype == PA_KV_FP8_E4M3;
-    pa::AppendBatch a{};
-    a.k = d_k;
-    a.v = d_v;
-    a.k_cache = c.d_k;
-    a.v_cache = c.d_v;
-    a.meta = in_args ? nullptr : st->dev;
-    a.table = c.d_table;
-    a.seq_lens = c.d_seq_lens;
-    a.n_ent = n;
-    a.n_pl = static_cast<int>(n_pl);
-    a.n_tab = static_cast<int>(n_tab);
-    a.n_len = static_cast<int>(n_len);
-    a.n_tok = static_cast<int>(n_tok);
-    a.hkv = c.cfg.num_kv_heads;
-    a.page_size = P;
-    a.inv_k = fp8 ? 1.0f / c.cfg.k_scale : 1.0f;
-    a.inv_v = fp8 ? 1.0f / c.cfg.v_scale : 1.0f;
+    const append_meta m{in_args ? nullptr : st->dev,  n, static_cast<int>(n_pl), static_cast<int>(n_tab),
+                        static_cast<int>(n_len), static_cast<int>(n_tok)};
     if (!in_args)
         pa::hip_check(pa::launch_stage_copy(st->host_dev, st->dev, need, nullptr, 0, s), "append staging kernel launch");
-    pa::hip_check(pa::launch_append_batch(c.cfg.dtype, a, in_args ? meta : nullptr, need, s), "append kernel launch");
+    pa::hip_check(launch(m, in_args ? meta : nullptr, need), "append kernel launch");
     // Tells a later use of the buffer, and release, when this append is done
     // (release works on the null stream, which orders itself after its own work;
     // nothing tells of a graph's replays).
     if (!in_args) release_stage(*st, s);
     else if (s && !capturing(s)) mark_append(c, s);
+}
+
+// The same for strided rows of k and v, k (and q) normed and rotated on the way.
+void queue_rows(pa_cache& c, const int32_t* slots, const int32_t* counts, int n, const reserve_entry* entries,
+                long n_tok, const pa::RopeAppend& rows, hipStream_t s) {
+    const bool fp8 = c.cfg.dtype == PA_KV_FP8_E4M3;
+    queue_meta(c, slots, counts, n, entries, n_tok, s,
+               [&](const append_meta& m, const int32_t* host, size_t need) {
+                   pa::RopeAppend a = rows;
+                   a.n_tok     = m.n_tok;
+                   a.n_ent     = m.n_ent;
+                   a.meta      = m.dev;
+                   a.n_pl      = m.n_pl;
+                   a.n_tab     = m.n_tab;
+                   a.n_len     = m.n_len;
+                   a.new_table = c.d_table;
+                   a.new_lens  = c.d_seq_lens;
+                   a.k_cache   = c.d_k;
+                   a.v_cache   = c.d_v;
+                   a.scales    = c.d_scales;
+                   a.page_size = c.cfg.page_size;
+                   a.inv_k     = fp8 ? 1.0f / c.cfg.k_scale : 1.0f;
+                   a.inv_v     = fp8 ? 1.0f / c.cfg.v_scale : 1.0f;
+                   return pa::launch_append_rope(c.cfg.dtype, a, host, need, s);
+               });
+}
+
+// In a block-scaled cache two entries of one slot may share a block, whose scale
+// the later one raises over the earlier one's tokens: they go in launches of
+// their own, one after the other. (Elsewhere entries write places of their own.)
+void queue_rows_in_order(pa_cache& c, const int32_t* slots, const int32_t* counts, int n,
+                         const std::vector<reserve_entry>& entries, long n_tok, const pa::RopeAppend& rows,
+                         hipStream_t s) {
+    if (c.cfg.dtype != PA_KV_FP8_E4M3_BLOCK) return queue_rows(c, slots, counts, n, entries.data(), n_tok, rows, s);
+    std::vector<int> in_run(static_cast<size_t>(c.cfg.max_slots), -1);
+    long tok = 0;
+    for (int i = 0, run = 0; i < n; ++run) {
+        int  j = i;
+        long t = 0;
+        for (; j < n && in_run[static_cast<size_t>(slots[j])] != run; ++j) {
+            in_run[static_cast<size_t>(slots[j])] = run;
+            t += counts[j];
+        }
+        if (t > 0) {
+            pa::RopeAppend a = rows;
+            if (a.q.heads) {
+                a.q.in += tok * a.q.in_stride;
+                a.q.out += tok * a.q.out_stride;
+            }
+            a.k.in += tok * a.k.in_stride;
+            a.v += tok * a.v_stride;
+            if (a.positions) a.positions += tok * (a.rope.pairs ? a.rope.num_axes : 1);
+            queue_rows(c, slots + i, counts + i, j - i, entries.data() + i, t, a, s);
+        }
+        tok += t;
+        i = j;
+    }
+}
+
+// Whole tokens as append and append_batch take them: [n_tok][kv heads][128].
+void queue_append(pa_cache& c, const int32_t* slots, const int32_t* counts, int n,
+                  const std::vector<reserve_entry>& entries, long n_tok, const uint16_t* d_k, const uint16_t* d_v,
+                  hipStream_t s) {
+    if (c.cfg.dtype == PA_KV_FP8_E4M3_BLOCK) {
+        pa::RopeAppend a{};
+        a.k.in        = d_k;
+        a.k.in_stride = static_cast<long>(c.cfg.num_kv_heads) * pa::kHeadDim;
+        a.k.heads     = c.cfg.num_kv_heads;
+        a.v           = d_v;
+        a.v_stride    = a.k.in_stride;
+        return queue_rows_in_order(c, slots, counts, n, entries, n_tok, a, s);
+    }
+    const bool fp8 = c.cfg.dtype == PA_KV_FP8_E4M3;
+    queue_meta(c, slots, counts, n, entries.data(), n_tok, s,
+               [&](const append_meta& m, const int32_t* host, size_t need) {
+                   pa::AppendBatch a{};
+                   a.k         = d_k;
+                   a.v         = d_v;
+                   a.k_cache   = c.d_k;
+                   a.v_cache   = c.d_v;
+                   a.meta      = m.dev;
+                   a.table     = c.d_table;
+                   a.seq_lens  = c.d_seq_lens;
+                   a.n_ent     = m.n_ent;
+                   a.n_pl      = m.n_pl;
+                   a.n_tab     = m.n_tab;
+                   a.n_len     = m.n_len;
+                   a.n_tok     = m.n_tok;
+                   a.hkv       = c.cfg.num_kv_heads;
+                   a.page_size = c.cfg.page_size;
+                   a.inv_k     = fp8 ? 1.0f / c.cfg.k_scale : 1.0f;
+                   a.inv_v     = fp8 ? 1.0f / c.cfg.v_scale : 1.0f;
+                   return pa::launch_append_batch(c.cfg.dtype, a, host, need, s);
+               });
 }
 
 // Notes a stream the cache's work is queued on.
@@ -209,16 +304,26 @@ pa_status pa_cache_create(const pa_cache_config* cfg, pa_cache** out) {
             cfg->max_pages_per_slot <= 0)
             throw std::invalid_argument("PagedKVCache: all sizes must be positive");
         if (cfg->head_dim != pa::kHeadDim) throw std::invalid_argument("PagedKVCache: head_dim must be 128");
+        if (cfg->dtype == PA_KV_FP8_E4M3_BLOCK) {
+            if (pa::block_tokens(cfg->page_size) == 0)
+                throw std::invalid_argument("PagedKVCache: block scales need a page_size that is a multiple of 8");
+            if (cfg->k_scale != 1.0f || cfg->v_scale != 1.0f)
+                throw std::invalid_argument("PagedKVCache: blocks have their own scales; k_scale and v_scale must be 1");
+        }
         auto* c = new pa_cache;
         try {
             c->cfg = *cfg;
             pool_init(c->pool, cfg->num_pages, cfg->page_size, cfg->max_slots, cfg->max_pages_per_slot);
-            const size_t half_bytes = bytes_per_page_impl(*cfg) / 2 * static_cast<size_t>(cfg->num_pages);
+            const size_t half_bytes = kv_bytes_per_page(*cfg) / 2 * static_cast<size_t>(cfg->num_pages);
+            const size_t scale_bytes = scale_bytes_per_page(*cfg) * static_cast<size_t>(cfg->num_pages);
             const size_t table = sizeof(int32_t) * static_cast<size_t>(cfg->max_slots) * cfg->max_pages_per_slot;
             // One allocation for both pools, V starting kPoolStagger bytes after
             // the end of K (the K/V bank-conflict gap).
             pa::hip_check(hipMalloc(&c->d_k, 2 * half_bytes + pa::kPoolStagger), "hipMalloc k/v pools");
             c->d_v = static_cast<unsigned char*>(c->d_k) + half_bytes + pa::kPoolStagger;
+            if (scale_bytes)   // read in whole 4-byte words
+                pa::hip_check(hipMalloc(reinterpret_cast<void**>(&c->d_scales), (scale_bytes + 3) & ~size_t{3}),
+                              "hipMalloc block scales");
             pa::hip_check(hipMalloc(reinterpret_cast<void**>(&c->d_table), table), "hipMalloc block table");
             pa::hip_check(hipMalloc(reinterpret_cast<void**>(&c->d_seq_lens), sizeof(int32_t) * cfg->max_slots),
                           "hipMalloc seq_lens");
@@ -226,6 +331,7 @@ pa_status pa_cache_create(const pa_cache_config* cfg, pa_cache** out) {
             pa::hip_check(hipMemset(c->d_seq_lens, 0, sizeof(int32_t) * cfg->max_slots), "hipMemset");
         } catch (...) {
             (void)hipFree(c->d_k);
+            (void)hipFree(c->d_scales);
             (void)hipFree(c->d_table);
             (void)hipFree(c->d_seq_lens);
             delete c;
@@ -238,6 +344,7 @@ pa_status pa_cache_create(const pa_cache_config* cfg, pa_cache** out) {
 void pa_cache_destroy(pa_cache* c) {
     if (!c) return;
     (void)hipFree(c->d_k);   // both pools
+    (void)hipFree(c->d_scales);
     (void)hipFree(c->d_table);
     (void)hipFree(c->d_seq_lens);
     free_stages(c->append_staging);
@@ -263,7 +370,7 @@ pa_status pa_cache_append(pa_cache* c, int slot, const uint16_t* d_k, const uint
         if (appended) *appended = 1;
         if (n <= 0) return;
         const int P = c->cfg.page_size, pages = (old_len + n - 1) / P - old_len / P + 1;
-        if (pa::append_meta_inline(3 + static_cast<size_t>(pages) + 2 * (static_cast<size_t>(num_new) + 1))) {
+        if (c->cfg.dtype == PA_KV_FP8_E4M3_BLOCK || pa::append_meta_inline(3 + static_cast<size_t>(pages) + 2 * (static_cast<size_t>(num_new) + 1))) {
             const std::vector<reserve_entry> entry{{old_len, first_new, num_new}};
             queue_append(*c, &slot, &n, 1, entry, n, d_k, d_v, s);
         } else {
@@ -307,6 +414,39 @@ pa_status pa_cache_append_batch(pa_cache* c, const int32_t* slots, const int32_t
         if (appended) *appended = 1;
         if (n_tok == 0) return;
         queue_append(*c, slots, counts, n, entries, n_tok, d_k, d_v, s);
+    });
+}
+
+pa_status pa_cache_append_rope(pa_cache* c, const int32_t* slots, const int32_t* counts, int n, const pa_rope* rope,
+                               const int32_t* positions, const pa_head_rows* q, const pa_head_rows* k,
+                               const uint16_t* v, int64_t v_stride, void* stream, int* appended) {
+    return guarded([&] {
+        if (!c) throw std::invalid_argument("cache is null");
+        if (appended) *appended = 0;
+        if (!k || k->heads != c->cfg.num_kv_heads)
+            throw std::invalid_argument("append_rope: k must have the cache's kv heads");
+        long n_tok = 0;
+        for (int i = 0; i < n && counts; ++i) n_tok += counts[i] > 0 ? counts[i] : 0;
+        const long heads = 2l * k->heads + (q && q->heads > 0 ? q->heads : 0) + 12;
+        if (n_tok * heads * (pa::kHeadDim / 8) > INT_MAX || n > INT_MAX / (64 * 16))
+            throw std::length_error("append_rope: too many tokens");
+        const int nt = static_cast<int>(n_tok);
+        pa::RopeAppend a{};
+        a.q = head_rows("append_rope q", q, nt, true);
+        a.k = head_rows("append_rope k", k, nt, false);
+        check_v_rows("append_rope", v, v_stride, nt);
+        if (rope && rope->num_axes > 1 && nt > 0 && !positions)
+            throw std::invalid_argument("append_rope: a rotation over several axes needs positions");
+        if (nt > 0) a.rope = rope_table(rope);
+        a.v         = v;
+        a.v_stride  = static_cast<long>(v_stride);
+        a.positions = rope ? positions : nullptr;
+        const hipStream_t s = n_tok > 0 ? append_stream(*c, stream) : nullptr;
+        std::vector<reserve_entry> entries;
+        if (!pool_reserve_batch(c->pool, slots, counts, n, &entries)) return;   // out of pages: nothing appended
+        if (appended) *appended = 1;
+        if (n_tok == 0) return;
+        queue_rows_in_order(*c, slots, counts, n, entries, n_tok, a, s);
     });
 }
 

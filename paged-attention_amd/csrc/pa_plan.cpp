@@ -136,8 +136,7 @@ namespace pa::host {
 thread_local std::string g_last_error;
 
 void check_dtype(int dtype) {
-    if (dtype != PA_KV_FP16 && dtype != PA_KV_FP8_E4M3)
-        throw std::invalid_argument("unknown kv dtype " + std::to_string(dtype));
+    pa::check_kv_dtype(dtype);
 }
 // The shape of any plan, from its arrays (make_plan's cut fills its own).
 pa_split_shape split_shape(const pa_plan& plan) {
@@ -625,7 +624,9 @@ extern "C" {
 const char* pa_last_error(void) { return g_last_error.c_str(); }
 
 int pa_kv_dtype_bytes(int dtype) { return dtype == PA_KV_FP16 ? 2 : 1; }
-const char* pa_kv_dtype_name(int dtype) { return dtype == PA_KV_FP16 ? "fp16" : "fp8_e4m3"; }
+const char* pa_kv_dtype_name(int dtype) {
+    return dtype == PA_KV_FP16 ? "fp16" : dtype == PA_KV_FP8_E4M3_BLOCK ? "fp8_e4m3_block" : "fp8_e4m3";
+}
 
 pa_status pa_tile_tokens(int dtype, int head_dim, int group, int* out) {
     return guarded([&] {
@@ -807,6 +808,8 @@ pa_status pa_append_quantize(int dtype, const uint16_t* k, const uint16_t* v, vo
                              int page_size, float inv_k_scale, float inv_v_scale, void* stream) {
     return guarded([&] {
         check_dtype(dtype);
+        if (dtype == PA_KV_FP8_E4M3_BLOCK)
+            throw std::invalid_argument("append: block-scaled caches are written by pa_append_rope");
         if (head_dim != pa::kHeadDim) throw std::invalid_argument("unsupported head_dim " + std::to_string(head_dim));
         if (num_kv_heads <= 0 || page_size <= 0 || start_pos < 0 || n < 0)
             throw std::invalid_argument("append: bad sizes");

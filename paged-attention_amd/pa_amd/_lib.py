@@ -26,6 +26,7 @@ PA_ERR_DEVICE = 3
 
 PA_KV_FP16 = 0
 PA_KV_FP8_E4M3 = 1
+PA_KV_FP8_E4M3_BLOCK = 2
 
 
 class PaError(Exception):
@@ -75,6 +76,46 @@ class DecodeParams(ctypes.Structure):
         ("block_merge", ctypes.c_int32),
         ("num_segments", ctypes.c_int32),
         ("merge_counters", ctypes.c_void_p),
+        ("kv_scales", ctypes.c_void_p),
+    ]
+
+
+class HeadRows(ctypes.Structure):
+    """pa_head_rows."""
+
+    _fields_ = [
+        ("in_", ctypes.c_void_p),
+        ("in_stride", ctypes.c_int64),
+        ("out", ctypes.c_void_p),
+        ("out_stride", ctypes.c_int64),
+        ("weight", ctypes.c_void_p),
+        ("eps", ctypes.c_float),
+        ("heads", ctypes.c_int32),
+    ]
+
+
+class AppendArgs(ctypes.Structure):
+    """pa_append_args."""
+
+    _fields_ = [
+        ("num_tokens", ctypes.c_int32),
+        ("num_entries", ctypes.c_int32),
+        ("tok_begin", ctypes.c_void_p),
+        ("start_pos", ctypes.c_void_p),
+        ("slot_ids", ctypes.c_void_p),
+        ("positions", ctypes.c_void_p),
+        ("v", ctypes.c_void_p),
+        ("v_stride", ctypes.c_int64),
+        ("k_cache", ctypes.c_void_p),
+        ("v_cache", ctypes.c_void_p),
+        ("kv_scales", ctypes.c_void_p),
+        ("block_table", ctypes.c_void_p),
+        ("block_table_stride", ctypes.c_int32),
+        ("num_table_rows", ctypes.c_int32),
+        ("num_pages", ctypes.c_int32),
+        ("page_size", ctypes.c_int32),
+        ("k_scale", ctypes.c_float),
+        ("v_scale", ctypes.c_float),
     ]
 
 
@@ -99,6 +140,7 @@ _I = ctypes.c_int
 _U = ctypes.c_uint
 _F = ctypes.c_float
 _S = ctypes.c_size_t
+_L = ctypes.c_int64
 _PI = ctypes.POINTER(ctypes.c_int)
 _PP = ctypes.POINTER(ctypes.c_void_p)
 
@@ -131,6 +173,13 @@ SIGNATURES: dict[str, tuple] = {
     "pa_decode_merge": (_I, [_I, ctypes.POINTER(DecodeParams), _P]),
     "pa_decode_static": (_I, [_I, ctypes.POINTER(DecodeParams), _I, _P]),
     "pa_append_quantize": (_I, [_I, _P, _P, _P, _P, _P, _I, _I, _I, _I, _I, _F, _F, _P]),
+    "pa_rope_create": (_I, [_P, _P, _I, _I, _I, _F, _PP]),
+    "pa_rope_destroy": (None, [_P]),
+    "pa_rope_dim": (_I, [_P]),
+    "pa_rope_axes": (_I, [_P]),
+    "pa_norm_rope": (_I, [_P, ctypes.POINTER(HeadRows), ctypes.POINTER(HeadRows), _P, _I, _P]),
+    "pa_block_tokens": (_I, [_I]),
+    "pa_append_rope": (_I, [_I, ctypes.POINTER(AppendArgs), _P, ctypes.POINTER(HeadRows), ctypes.POINTER(HeadRows), _P]),
     "pa_gather_kv": (_I, [_I, _P, _P, _I, _I, _I, _I, _I, _P, _P]),
     "pa_stream_read": (_I, [_P, _S, _I, _P, _P]),
     "pa_stream_read_ex": (_I, [_P, _S, _I, _I, _I, _I, _P, _P]),
@@ -160,6 +209,8 @@ SIGNATURES: dict[str, tuple] = {
     "pa_cache_admit": (_I, [_P]),
     "pa_cache_append": (_I, [_P, _I, _P, _P, _I, _P, _PI]),
     "pa_cache_append_batch": (_I, [_P, _P, _P, _I, _P, _P, _P, _PI]),
+    "pa_cache_append_rope": (_I, [_P, _P, _P, _I, _P, _P, ctypes.POINTER(HeadRows), ctypes.POINTER(HeadRows), _P, _L, _P,
+                                  _PI]),
     "pa_cache_release": (_I, [_P, _I]),
     "pa_cache_shuffle_free_pages": (None, [_P, _U]),
     "pa_cache_params": (_I, [_P, ctypes.POINTER(DecodeParams)]),

@@ -20,6 +20,7 @@ from ._lib import CacheConfig, DecodeParams, InvalidArgument, call, check, load
 
 FP16 = _lib.PA_KV_FP16
 FP8_E4M3 = _lib.PA_KV_FP8_E4M3
+FP8_E4M3_BLOCK = _lib.PA_KV_FP8_E4M3_BLOCK
 
 
 def _ptr(x) -> int | None:
@@ -357,6 +358,35 @@ class PagedKVCache:
              _ptr(k), _ptr(v), _stream(stream), ctypes.byref(done))
         return bool(done.value)
 
+    def append_rope(self, slots, counts, k, v, rope=None, *, q=None, q_out=None, positions=None, q_weight=None,
+                    k_weight=None, eps: float = 1e-6, stream=None):
+        """append_batch for tokens as the projection leaves them (fp16 tensors [sum(counts)][heads][128],
+        tokens may be strided): k normed (k_weight) and rotated (rope) on its way into the pages,
+        v as it is, and q normed and rotated beside them. The rotation takes the tokens' places, or
+        positions ([tokens] or [tokens, axes]). Returns False when the pool lacks pages (nothing
+        changed), else True, or q_out where q is given."""
+        from . import ops
+        import torch
+        slots = np.ascontiguousarray(slots, dtype=np.int32)
+        counts = np.ascontiguousarray(counts, dtype=np.int32)
+        if slots.shape != counts.shape or slots.ndim != 1:
+            raise ValueError("slots and counts must be 1-D of one length")
+        n = int(np.maximum(counts, 0).sum())
+        if k.dim() != 3 or k.size(0) != n or v.shape != k.shape or (q is not None and (q.dim() != 3 or q.size(0) != n)):
+            raise ValueError("k, v and q must be [sum(counts), heads, 128]")
+        dev = k.get_device()
+        kr, vr = ops.head_rows("k", k, k_weight, eps), ops.head_rows("v", v, None, eps, device=dev)
+        qr = None
+        if q is not None:
+            q_out = torch.empty((n, q.size(1), ops.D), dtype=torch.float16, device=q.device) if q_out is None else q_out
+            qr = ctypes.byref(ops.head_rows("q", q, q_weight, eps, q_out, dev))
+        pos = ops.positions_ptr(positions, rope, n, dev)
+        done = ctypes.c_int(0)
+        call("pa_cache_append_rope", self._h, slots.ctypes.data, counts.ctypes.data, slots.size,
+             None if rope is None else rope.handle, pos, qr, ctypes.byref(kr), vr.in_, vr.in_stride, _stream(stream),
+             ctypes.byref(done))
+        return (q_out if q is not None else True) if done.value else False
+
     def release(self, slot: int) -> None:
         call("pa_cache_release", self._h, slot)
 
@@ -421,7 +451,7 @@ def sm_scale(head_dim: int) -> float:
 
 
 __all__ = [
-    "FP16", "FP8_E4M3", "DecodeParams", "CacheConfig", "DecodePlan", "DevicePlan", "PagePool",
+    "FP16", "FP8_E4M3", "FP8_E4M3_BLOCK", "DecodeParams", "CacheConfig", "DecodePlan", "DevicePlan", "PagePool",
     "PagedKVCache", "make_plan", "make_plan_tiled", "paged_decode", "decode_split", "decode_merge",
     "append_quantize", "gather_kv", "stream_read", "stream_read_chunked", "fill_bytes", "tile_tokens", "wave_ctas", "default_ctas",
     "kv_dtype_bytes", "kv_dtype_name", "sm_scale",

@@ -5,6 +5,10 @@
     out = dec.run(q, k_cache, v_cache, block_table, seq_lens_dev, k_scale, v_scale)
     dec.num_ctas, dec.num_segments
 
+Block-scaled FP8 caches (no counterpart in the reference): Decoder(..., True,
+block_scales=True) and run(..., k_scale, v_scale, kv_scales=scales), where k_scale and
+v_scale multiply on top of the blocks' own scales (1.0 for caches that append_rope wrote).
+
 It runs libpa_decode.so's HIP kernels on the current torch stream. Argument
 checks raise RuntimeError, as TORCH_CHECK does in the reference.
 
@@ -41,12 +45,16 @@ def _require(cond: bool, msg: str = "Expected condition to hold") -> None:
 
 
 class Decoder:
-    def __init__(self, num_q_heads: int, num_kv_heads: int, head_dim: int, page_size: int, fp8: bool):
+    def __init__(self, num_q_heads: int, num_kv_heads: int, head_dim: int, page_size: int, fp8: bool,
+                 block_scales: bool = False):
+        _require(fp8 or not block_scales, "block_scales needs fp8")
+        _require(not block_scales or load().pa_block_tokens(int(page_size)) != 0,
+                 "block_scales needs a page_size that is a multiple of 8")
         self._hq = int(num_q_heads)
         self._hkv = int(num_kv_heads)
         self._dim = int(head_dim)
         self._page = int(page_size)
-        self._dtype = core.FP8_E4M3 if fp8 else core.FP16
+        self._dtype = core.FP8_E4M3_BLOCK if block_scales else core.FP8_E4M3 if fp8 else core.FP16
         self._batch = 0
         self._table_cols = 0   # block-table columns the plan's longest row needs
         self._plan: core.DecodePlan | None = None
@@ -82,7 +90,9 @@ class Decoder:
     # torch_decode.cu:31-59
     def run(self, q: torch.Tensor, k_cache: torch.Tensor, v_cache: torch.Tensor,
             block_table: torch.Tensor, seq_lens_dev: torch.Tensor, k_scale: float,
-            v_scale: float) -> torch.Tensor:
+            v_scale: float, kv_scales: torch.Tensor | None = None) -> torch.Tensor:
+        _require((kv_scales is not None) == (self._dtype == core.FP8_E4M3_BLOCK),
+                 "kv_scales goes with a Decoder of block_scales")
         _require(q.is_cuda and q.dtype == torch.float16 and q.is_contiguous(),
                  "q must be a contiguous CUDA fp16 tensor")
         _require(k_cache.is_contiguous() and v_cache.is_contiguous() and block_table.is_contiguous(),
@@ -101,6 +111,9 @@ class Decoder:
                  and block_table.size(1) >= self._table_cols,
                  "block_table must be a CUDA [batch, >= ceil(max seq_len / page_size)] tensor")
         _require(seq_lens_dev.is_cuda and seq_lens_dev.dtype == torch.int32, "seq_lens must be a CUDA int32 tensor")
+        if kv_scales is not None:
+            from .ops import check_kv_scales
+            check_kv_scales(kv_scales, k_cache)
         out = torch.empty_like(q)
         p = DecodeParams.from_buffer_copy(self._params)
         p.q = q.data_ptr()
@@ -112,6 +125,7 @@ class Decoder:
         p.block_table_stride = block_table.size(1)
         p.k_scale = float(k_scale)
         p.v_scale = float(v_scale)
+        p.kv_scales = None if kv_scales is None else kv_scales.data_ptr()
         check(load().pa_decode(self._dtype, ctypes.byref(p), _current_stream(q.get_device())))
         return out
 
@@ -127,11 +141,10 @@ class Decoder:
 _compiled = None
 
 
-def decoder_class():
-    """The compiled binding's Decoder class if its module was built, else this
-    module's ctypes Decoder. A built module that fails to import raises. With
-    PA_DECODE_LIB naming another library build, the ctypes Decoder (the
-    compiled module is linked against the in-tree library)."""
+def compiled():
+    """The compiled binding's module if it was built, else None. A built module that
+    fails to import raises. With PA_DECODE_LIB naming another library build, None
+    (the compiled module is linked against the in-tree library)."""
     global _compiled
     if _compiled is None:
         import os
@@ -139,7 +152,14 @@ def decoder_class():
         if "PA_DECODE_LIB" not in os.environ and any((PKG_DIR / "pa_amd").glob("_pa_torch*.so")):
             _init_torch_device_state()     # torch's HIP state before the library loads
             from . import _pa_torch
-            _compiled = _pa_torch.Decoder
+            _compiled = _pa_torch
         else:
             _compiled = False
-    return _compiled or Decoder
+    return _compiled or None
+
+
+def decoder_class():
+    """The compiled binding's Decoder class if its module was built, else this
+    module's ctypes Decoder."""
+    module = compiled()
+    return Decoder if module is None else module.Decoder
