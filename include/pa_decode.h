@@ -260,8 +260,8 @@ int       pa_rope_dim(const pa_rope* rope);
 int       pa_rope_axes(const pa_rope* rope);
 
 /* Some heads of every token: token t's head h starts at in + t * in_stride + h *
- * 128 (fp16, 16-byte aligned, strides in elements and multiples of 8, so a fused
- * projection's output is read where it lies). weight: 128 floats (16-byte
+ * 128 (fp16, 16-byte aligned; strides in elements, multiples of 8 from 0 to 2^26, so
+ * a fused projection's output is read where it lies). weight: 128 floats (16-byte
  * aligned) or NULL for no norm. out likewise, where the call has an output; it
  * may be `in` itself with the same stride, and overlaps nothing else the call
  * reads or writes. heads = 0: none. */
@@ -276,7 +276,8 @@ typedef struct pa_head_rows {
 } pa_head_rows;
 
 /* q and k (either may be NULL) of n tokens normed and rotated into their `out`.
- * (Here and below, PA_ERR_LENGTH: some 2^27 / heads tokens at most.)
+ * (Here and below, PA_ERR_LENGTH: some 2^27 / heads tokens at most; a page of one
+ * pool is below 2 GiB.)
  * positions: device, [n][axes of the rotation] int32 (any value), NULL only where
  * rope is (norms alone). */
 pa_status pa_norm_rope(const pa_rope* rope, const pa_head_rows* q, const pa_head_rows* k,

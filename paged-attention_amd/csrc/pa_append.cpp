@@ -22,15 +22,17 @@ void check_count(const char* what, long long n, long long heads) {
         throw std::length_error(std::string(what) + ": tokens * heads * 16 exceeds INT_MAX");
 }
 
+// Elements from one token to the next.
+bool stride_ok(int64_t s) { return s >= 0 && s < (1 << 26) && s % 8 == 0; }
+
 // First and last byte (exclusive) of n strided rows of `heads` heads.
 struct Span {
     uintptr_t lo, hi;
 };
 Span span_of(const uint16_t* p, long long stride, int n, int heads) {
     const auto base = reinterpret_cast<uintptr_t>(p);
-    const long long last = static_cast<long long>(n - 1) * stride * 2;
-    const long long row  = 2ll * heads * pa::kHeadDim;
-    return {base + (last < 0 ? last : 0), base + (last > 0 ? last : 0) + row};
+    return {base, base + 2 * (static_cast<uintptr_t>(n - 1) * static_cast<uintptr_t>(stride) +
+                              static_cast<uintptr_t>(heads) * pa::kHeadDim)};
 }
 
 }  // namespace
@@ -61,16 +63,16 @@ pa::HeadRows head_rows(const char* what, const pa_head_rows* r, int n, bool has_
     check_count(what, n, r->heads);
     if (n > 0) {
         if (!r->in) throw std::invalid_argument(w + "null rows");
-        if (!aligned(r->in, 16) || r->in_stride % 8 != 0)
-            throw std::invalid_argument(w + "rows must be 16-byte aligned, their stride a multiple of 8 elements");
+        if (!aligned(r->in, 16) || !stride_ok(r->in_stride))
+            throw std::invalid_argument(w + "rows must be 16-byte aligned, their stride a multiple of 8 elements below 2^26");
         if (r->weight && !aligned(r->weight, 16)) throw std::invalid_argument(w + "the norm weight must be 16-byte aligned");
         if (r->weight && !(r->eps >= 0.0f)) throw std::invalid_argument(w + "eps must not be negative");
     }
     if (n > 0 && has_out) {
         if (!r->out) throw std::invalid_argument(w + "null output");
-        if (!aligned(r->out, 16) || r->out_stride % 8 != 0)
-            throw std::invalid_argument(w + "outputs must be 16-byte aligned, their stride a multiple of 8 elements");
-        if (n > 1 && std::llabs(r->out_stride) < static_cast<long long>(r->heads) * pa::kHeadDim)
+        if (!aligned(r->out, 16) || !stride_ok(r->out_stride))
+            throw std::invalid_argument(w + "outputs must be 16-byte aligned, their stride a multiple of 8 elements below 2^26");
+        if (n > 1 && r->out_stride < static_cast<long long>(r->heads) * pa::kHeadDim)
             throw std::invalid_argument(w + "output rows overlap");
         const Span in = span_of(r->in, r->in_stride, n, r->heads), out = span_of(r->out, r->out_stride, n, r->heads);
         if (in.lo < out.hi && out.lo < in.hi && !(r->in == r->out && (n == 1 || r->in_stride == r->out_stride)))
@@ -86,10 +88,16 @@ pa::HeadRows head_rows(const char* what, const pa_head_rows* r, int n, bool has_
     return h;
 }
 
+void check_page_bytes(const char* what, int dtype, int page_size, int kv_heads) {
+    if (static_cast<long long>(page_size) * kv_heads * pa::kHeadDim * (dtype == PA_KV_FP16 ? 2 : 1) > INT_MAX)
+        throw std::invalid_argument(std::string(what) + ": page_size * kv heads * row bytes must be below 2^31");
+}
+
 void check_v_rows(const char* what, const uint16_t* v, int64_t stride, int n) {
     if (n > 0 && !v) throw std::invalid_argument(std::string(what) + ": v is null");
-    if (n > 0 && (!aligned(v, 16) || stride % 8 != 0))
-        throw std::invalid_argument(std::string(what) + ": v must be 16-byte aligned, its stride a multiple of 8 elements");
+    if (n > 0 && (!aligned(v, 16) || !stride_ok(stride)))
+        throw std::invalid_argument(std::string(what) +
+                                    ": v must be 16-byte aligned, its stride a multiple of 8 elements below 2^26");
 }
 
 }  // namespace pa::host
@@ -175,6 +183,7 @@ pa_status pa_append_rope(int dtype, const pa_append_args* p, const pa_rope* rope
             throw std::invalid_argument("append_rope: bad sizes");
         if (k->heads <= 0) throw std::invalid_argument("append_rope: k needs heads");
         const bool block = dtype == PA_KV_FP8_E4M3_BLOCK;
+        check_page_bytes("append_rope", dtype, p->page_size, k->heads);
         if (block && pa::block_tokens(p->page_size) == 0)
             throw std::invalid_argument("append_rope: block-scaled caches need a page_size that is a multiple of 8");
         const int n = p->num_tokens;

@@ -234,6 +234,7 @@ pa::RopeTable rope_table(const pa_rope* rope);
 // The same for head rows (no heads for null), checked for n tokens.
 pa::HeadRows head_rows(const char* what, const pa_head_rows* r, int n, bool has_out);
 void check_v_rows(const char* what, const uint16_t* v, int64_t stride, int n);
+void check_page_bytes(const char* what, int dtype, int page_size, int kv_heads);
 
 // ---- page pool (pa_pool.cpp)
 // Entry i of a batched append: the slot's length before it, and the table

@@ -148,7 +148,8 @@ struct RopeAppend {
     uint8_t*        scales;
     int             page_size;
     float           inv_k, inv_v;
-    int             block_tokens, units;   // block-scaled caches (set by the launch)
+    int             block_tokens, units, head_groups;   // block-scaled caches (set by the launch)
+    int             parts, parts_q, parts_k;   // waves of a token, of its q, of its k (set by the launch)
 };
 template <int N>
 struct RopeInline {

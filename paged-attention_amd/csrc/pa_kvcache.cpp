@@ -307,6 +307,7 @@ pa_status pa_cache_create(const pa_cache_config* cfg, pa_cache** out) {
         if (cfg->dtype == PA_KV_FP8_E4M3_BLOCK) {
             if (pa::block_tokens(cfg->page_size) == 0)
                 throw std::invalid_argument("PagedKVCache: block scales need a page_size that is a multiple of 8");
+            check_page_bytes("PagedKVCache", cfg->dtype, cfg->page_size, cfg->num_kv_heads);
             if (cfg->k_scale != 1.0f || cfg->v_scale != 1.0f)
                 throw std::invalid_argument("PagedKVCache: blocks have their own scales; k_scale and v_scale must be 1");
         }
@@ -435,6 +436,7 @@ pa_status pa_cache_append_rope(pa_cache* c, const int32_t* slots, const int32_t*
         a.q = head_rows("append_rope q", q, nt, true);
         a.k = head_rows("append_rope k", k, nt, false);
         check_v_rows("append_rope", v, v_stride, nt);
+        check_page_bytes("append_rope", c->cfg.dtype, c->cfg.page_size, c->cfg.num_kv_heads);
         if (rope && rope->num_axes > 1 && nt > 0 && !positions)
             throw std::invalid_argument("append_rope: a rotation over several axes needs positions");
         if (nt > 0) a.rope = rope_table(rope);

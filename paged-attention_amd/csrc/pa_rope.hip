@@ -37,6 +37,7 @@ static_assert(kPairs == 64, "a wave computes one pair's sine and cosine per lane
 struct Turn {
     float c, s;
 };
+constexpr int kNonTemporal = 2;   // cache policy of buffer loads and stores: touched once
 
 // Sum (or maximum) over the 16 lanes of a row, in every lane.
 template <int CTRL>
@@ -59,7 +60,9 @@ __device__ __forceinline__ float row_max(float x) {
 
 // Pair i's sine and cosine at a token (its `positions` row, or its place).
 __device__ __forceinline__ Turn turn_of(const RopeTable& r, const int32_t* positions, int token, int place, int i) {
-    const int pos = positions ? positions[static_cast<size_t>(token) * r.num_axes + r.axes[i]] : place;
+    int pos = place;
+    if (positions && r.num_axes == 1) pos = positions[token];
+    else if (positions) pos = positions[static_cast<size_t>(token) * r.num_axes + r.axes[i]];
     const double half = static_cast<double>(pos) * r.half_turns[i];
     const float  x    = static_cast<float>(half - 2.0 * rint(half * 0.5));   // [-1, 1]
     Turn t;
@@ -69,64 +72,62 @@ __device__ __forceinline__ Turn turn_of(const RopeTable& r, const int32_t* posit
     return t;
 }
 
-// What lane c of a row needs of a token's turns: interleaved pairs 4c .. 4c + 3
-// (the first four), else pairs 8 (c mod h) .. + 7 with the sine's sign.
-struct LaneTurns {
-    Turn t[kDims];
+// The 8 dims that lane c of a row holds, as two chunks of four: with half-split
+// pairs both halves of pairs 4c .. 4c + 3, so that no lane needs another's values;
+// with interleaved ones, and of dims that do not turn, eight dims in a row.
+struct LaneDims {
+    int  lo, hi;   // the chunks' first dims
+    bool turned;
 };
-__device__ __forceinline__ LaneTurns lane_turns(const RopeTable& r, const Turn* tab, int c) {
-    LaneTurns l;
-    const int  h = r.pairs / kDims;
-    const bool upper = c >= h;
-    if (r.interleaved) {
-#pragma unroll
-        for (int e = 0; e < 4; ++e) l.t[e] = tab[min(4 * c + e, kPairs - 1)];
-    } else {
-        const int c0 = min(upper ? c - h : c, kLanes / 2 - 1);
-#pragma unroll
-        for (int e = 0; e < kDims; ++e) {
-            l.t[e] = tab[kDims * c0 + e];
-            if (!upper) l.t[e].s = -l.t[e].s;
-        }
+template <bool INTER>
+__device__ __forceinline__ LaneDims lane_dims(int pairs, int c) {
+    const int l = pairs / 4;   // lanes that turn
+    if (INTER || c >= l) {
+        const int d = kDims * c;   // 2 * pairs + 8 (c - l)
+        return {d, d + 4, c < l};
     }
-    return l;
+    return {4 * c, pairs + 4 * c, true};
 }
 
-// A row chunk's 8 values normed (weight given) and turned, in 32 bits.
-__device__ __forceinline__ void norm_turn(float (&y)[kDims], const HeadRows& rows, const RopeTable& r,
-                                          const LaneTurns& l, int c) {
-    if (rows.weight) {
-        float sq = 0.f;
+// A lane's dims of the row `off` bytes into a resource (past its end: zeros).
+template <bool INTER>
+__device__ __forceinline__ u32x4 load_dims(__amdgpu_buffer_rsrc_t rs, const LaneDims& d, int off) {
+    if constexpr (INTER)
+        return __builtin_bit_cast(u32x4, __builtin_amdgcn_raw_buffer_load_b128(rs, 2 * d.lo + off, 0, kNonTemporal));
+    const u32x2 x = __builtin_bit_cast(u32x2, __builtin_amdgcn_raw_buffer_load_b64(rs, 2 * d.lo + off, 0, kNonTemporal));
+    const u32x2 y = __builtin_bit_cast(u32x2, __builtin_amdgcn_raw_buffer_load_b64(rs, 2 * d.hi + off, 0, kNonTemporal));
+    return u32x4{x[0], x[1], y[0], y[1]};
+}
+// The same stored, as fp16 or as codes (past the end: dropped).
+template <bool INTER>
+__device__ __forceinline__ void store_dims(__amdgpu_buffer_rsrc_t rs, const LaneDims& d, int off, u32x4 x) {
+    if constexpr (INTER) return __builtin_amdgcn_raw_buffer_store_b128(x, rs, 2 * d.lo + off, 0, kNonTemporal);
+    __builtin_amdgcn_raw_buffer_store_b64(u32x2{x[0], x[1]}, rs, 2 * d.lo + off, 0, kNonTemporal);
+    __builtin_amdgcn_raw_buffer_store_b64(u32x2{x[2], x[3]}, rs, 2 * d.hi + off, 0, kNonTemporal);
+}
+template <bool INTER>
+__device__ __forceinline__ void store_dims(__amdgpu_buffer_rsrc_t rs, const LaneDims& d, int off, u32x2 x) {
+    if constexpr (INTER) return __builtin_amdgcn_raw_buffer_store_b64(x, rs, d.lo + off, 0, kNonTemporal);
+    __builtin_amdgcn_raw_buffer_store_b32(x[0], rs, d.lo + off, 0, kNonTemporal);
+    __builtin_amdgcn_raw_buffer_store_b32(x[1], rs, d.hi + off, 0, kNonTemporal);
+}
+
+// A row's norm weights, and a token's turns, as a lane needs them.
+struct LaneWeights {
+    f32x4 w[2];
+};
+struct LaneTurns {
+    Turn t[4];
+};
+__device__ __forceinline__ LaneWeights lane_weights(const float* weight, const LaneDims& d) {
+    if (!weight) return {};
+    return {{*reinterpret_cast<const f32x4*>(weight + d.lo), *reinterpret_cast<const f32x4*>(weight + d.hi)}};
+}
+__device__ __forceinline__ LaneTurns lane_turns(const Turn* tab, int c) {
+    LaneTurns l;
 #pragma unroll
-        for (int e = 0; e < kDims; ++e) sq = fmaf(y[e], y[e], sq);
-        const float inv = 1.0f / sqrtf(row_sum(sq) * (1.0f / kHeadDim) + rows.eps);
-        const f32x4 w0 = *reinterpret_cast<const f32x4*>(rows.weight + kDims * c);
-        const f32x4 w1 = *reinterpret_cast<const f32x4*>(rows.weight + kDims * c + 4);
-#pragma unroll
-        for (int e = 0; e < kDims; ++e) y[e] = y[e] * inv * (e < 4 ? w0[e & 3] : w1[e & 3]);
-    }
-    if (r.pairs == 0) return;
-    const int  h      = r.pairs / kDims;   // lanes of one half
-    const bool turned = c < 2 * h;
-    if (r.interleaved) {
-        if (turned) {
-#pragma unroll
-            for (int e = 0; e < 4; ++e) {
-                const float a = y[2 * e], b = y[2 * e + 1];
-                y[2 * e]     = a * l.t[e].c - b * l.t[e].s;
-                y[2 * e + 1] = b * l.t[e].c + a * l.t[e].s;
-            }
-        }
-        return;
-    }
-    const int partner = (threadIdx.x & 63 & ~(kLanes - 1)) + (turned ? (c < h ? c + h : c - h) : c);
-    float o[kDims];
-#pragma unroll
-    for (int e = 0; e < kDims; ++e) o[e] = __shfl(y[e], partner);
-    if (turned) {
-#pragma unroll
-        for (int e = 0; e < kDims; ++e) y[e] = y[e] * l.t[e].c + o[e] * l.t[e].s;
-    }
+    for (int e = 0; e < 4; ++e) l.t[e] = tab[4 * c + e];
+    return l;
 }
 
 __device__ __forceinline__ void widen(float (&y)[kDims], const u32x4 x) {
@@ -143,25 +144,57 @@ __device__ __forceinline__ u32x4 narrow(const float (&y)[kDims]) {
     return o;
 }
 
+// 1 / sqrt(mean of a row's squares + eps). (v_rsq_f32 is off by 2^-23 at most. Its
+// input is no fp32 subnormal, which it would flush: the mean of squares of fp16
+// values is 0 or at least 2^-55.)
+__device__ __forceinline__ float inv_norm(const float (&y)[kDims], float eps) {
+    float sq = 0.f;
+#pragma unroll
+    for (int e = 0; e < kDims; ++e) sq = fmaf(y[e], y[e], sq);
+    return __builtin_amdgcn_rsqf(fmaf(row_sum(sq), 1.0f / kHeadDim, eps));
+}
+
+// A lane's 8 values of a row under their norm (inv: the row's inv_norm), and turned.
+__device__ __forceinline__ void apply_norm(float (&y)[kDims], float inv, const LaneWeights& w) {
+#pragma unroll
+    for (int e = 0; e < kDims; ++e) y[e] = y[e] * inv * w.w[e / 4][e % 4];
+}
+template <bool INTER>
+__device__ __forceinline__ void apply_turns(float (&y)[kDims], const LaneTurns& l) {
+#pragma unroll
+    for (int e = 0; e < 4; ++e) {
+        const int i = INTER ? 2 * e : e, j = INTER ? 2 * e + 1 : 4 + e;
+        const float a = y[i], b = y[j];
+        y[i] = a * l.t[e].c - b * l.t[e].s;
+        y[j] = b * l.t[e].c + a * l.t[e].s;
+    }
+}
+
 // Where a token goes. Every field is wave-uniform.
 struct Place {
     bool ok;
     int  pos, page, slot;
 };
 
-// The entry that wave-uniform x belongs to: the last one with first(e) <= x, for
-// first rising over n entries. `guess` is tried first (one round of loads).
-template <class First>
-__device__ __forceinline__ int entry_of(int x, int n, int guess, First first) {
+// The entry that wave-uniform x belongs to: the last one with first(i) <= x, for
+// first rising over n entries. `guess` is tried first (scalar loads, one round);
+// else each round has every lane look at one of 64 evenly spaced entries. (With a
+// binary search's scalar loads, one after the other, 64 sequences' step into a
+// block-scaled cache took 1 us more.)
+template <class First, class FirstOf>
+__device__ __forceinline__ int entry_of(int x, int n, int guess, First first, FirstOf first_of) {
     int lo = min(max(guess, 0), n - 1);
-    if (first(lo) > x || (lo + 1 < n && first(lo + 1) <= x)) {
-        lo = 0;
-        int hi = n;
-        while (hi - lo > 1) {
-            const int mid = (lo + hi) >> 1;
-            if (first(mid) <= x) lo = mid;
-            else hi = mid;
-        }
+    if (first(lo) <= x && (lo + 1 >= n || first(lo + 1) > x)) return lo;
+    lo = 0;
+    for (int span = n; span > 1;) {   // it is one of lo .. lo + span - 1
+        const int step = (span + 63) / 64;
+        const int i    = lo + step * static_cast<int>(threadIdx.x & 63);
+        const bool le  = i < lo + span && first_of(i) <= x;
+        // Rising: the lanes that hold are the first ones (lane 0 among them, unless none is).
+        const int at = max(__builtin_popcountll(__builtin_amdgcn_ballot_w64(le)) - 1, 0);
+        const int end = lo + span;
+        lo += step * at;
+        span = min(step, end - lo);
     }
     return lo;
 }
@@ -187,7 +220,8 @@ __device__ __forceinline__ Place place_of(const RopeAppend& a, const int32_t* me
     const int32_t* tok_begin = META == kMetaList ? meta : a.tok_begin;
     const int32_t* start     = META == kMetaList ? meta + a.n_ent : a.start;
     const int guess = static_cast<int>(static_cast<int64_t>(t) * a.n_ent / a.n_tok);
-    const int e = entry_of(t, a.n_ent, guess, [&](int i) { return load_uniform(tok_begin, i); });
+    const int e = entry_of(
+        t, a.n_ent, guess, [&](int i) { return load_uniform(tok_begin, i); }, [&](int i) { return tok_begin[i]; });
     Place p;
     const int st = load_uniform(start, e);
     p.pos  = static_cast<int>(static_cast<uint32_t>(st) +
@@ -206,86 +240,118 @@ __device__ __forceinline__ void write_tables(const RopeAppend& a, const int32_t*
     for (int i = idx; i < a.n_len; i += threads) a.new_lens[lens[2 * i]] = lens[2 * i + 1];
 }
 
-// U groups of four rows of token t, from group g0 on: q's groups, then k's, then
-// (with a cache) v's. CACHE: 0 none (k has an output), 1 fp16 pages, 2 E4M3 pages.
-template <int CACHE, int META, int U>
-__device__ __forceinline__ void rows_of_token(const RopeAppend& a, const int32_t* meta, int t, int g0, Turn* tab) {
+// What a wave's groups of four rows are.
+enum RowKind { kRowQ = 0, kRowK = 1, kRowV = 2 };
+
+// Up to U groups of four rows of one kind of token t, from group g0 on. CACHE: 0
+// none (k has an output), 1 fp16 pages, 2 E4M3 pages. All loads go out first; the
+// token's place and turns are worked out under them. Loads and stores go through
+// buffer resources that end with the token's heads, so a group with fewer than
+// four rows, or none, takes no branch (branches around the loads had the compiler
+// wait for each group's before the next: 8192 tokens of 32 + 8 heads 32.8 us at 8
+// groups a wave, but 37.1 at 4 and 66.8 at 6).
+template <int CACHE, bool INTER, int META, int U>
+__device__ __forceinline__ void rows_of_token(const RopeAppend& a, const int32_t* meta, int t, int kind, int g0,
+                                              Turn* tab) {
     const int lane = threadIdx.x & 63, c = lane % kLanes, r = lane / kLanes;
-    const int gq = (a.q.heads + kRows - 1) / kRows, gk = (a.k.heads + kRows - 1) / kRows;
-    const int groups = gq + gk + (CACHE ? gk : 0);
+    const bool v = CACHE != 0 && kind == kRowV;
+    const HeadRows& rows = kind == kRowQ ? a.q : a.k;
+    const int heads = rows.heads, h0 = kRows * g0;
+    LaneDims d = lane_dims<INTER>(a.rope.pairs, c);
+    if (v) d = LaneDims{kDims * c, kDims * c + 4, false};
+    const uint16_t* in = (v ? a.v + t * a.v_stride : rows.in + t * rows.in_stride) + h0 * kHeadDim;
+    const __amdgpu_buffer_rsrc_t src = buffer_rsrc(in, 2 * kHeadDim * (heads - h0));
     u32x4 x[U];
 #pragma unroll
-    for (int j = 0; j < U; ++j) {
-        const int g = g0 + j;
-        x[j] = u32x4{0, 0, 0, 0};
-        if (g >= groups) continue;
-        const bool q = g < gq, k = !q && g < gq + gk;
-        const int  h = kRows * (q ? g : k ? g - gq : g - gq - gk) + r;
-        const uint16_t* in = q ? a.q.in + t * a.q.in_stride : k ? a.k.in + t * a.k.in_stride : a.v + t * a.v_stride;
-        if (h < (q ? a.q.heads : a.k.heads)) x[j] = load16<true>(in + h * kHeadDim + kDims * c);
-    }
+    for (int j = 0; j < U; ++j) x[j] = load_dims<INTER>(src, d, 2 * kHeadDim * (kRows * j + r));
     Place p{true, 0, 0, 0};
     if constexpr (META != 0) p = place_of<META>(a, meta, t);
+    const bool norm = !v && rows.weight != nullptr;
+    const LaneWeights w = lane_weights(v ? nullptr : rows.weight, d);
     LaneTurns l{};
-    if (a.rope.pairs && g0 < gq + gk) {
+    if (!v && a.rope.pairs) {
         if (lane < a.rope.pairs) tab[lane] = turn_of(a.rope, a.positions, t, p.pos, lane);
         wave_lds_sync();
-        l = lane_turns(a.rope, tab, c);
+        l = lane_turns(tab, c);
     }
+    auto finish = [&](float (&y)[kDims]) {
+        if (norm) apply_norm(y, inv_norm(y, rows.eps), w);
+        if (d.turned) apply_turns<INTER>(y, l);
+    };
+    if (CACHE == 0 || kind == kRowQ) {
+        uint16_t* out = rows.out + t * rows.out_stride + h0 * kHeadDim;
+        const __amdgpu_buffer_rsrc_t dst = buffer_rsrc(out, 2 * kHeadDim * (heads - h0));
 #pragma unroll
-    for (int j = 0; j < U; ++j) {
-        const int g = g0 + j;
-        if (g >= groups) continue;
-        const bool q = g < gq, k = !q && g < gq + gk;
-        const int  h = kRows * (q ? g : k ? g - gq : g - gq - gk) + r;
-        float y[kDims];
-        widen(y, x[j]);
-        if (q || k) norm_turn(y, q ? a.q : a.k, a.rope, l, c);
-        if (h >= (q ? a.q.heads : a.k.heads)) continue;
-        if (q || CACHE == 0) {
-            const HeadRows& rows = q ? a.q : a.k;
-            __builtin_nontemporal_store(narrow(y), reinterpret_cast<u32x4*>(rows.out + t * rows.out_stride +
-                                                                            h * kHeadDim + kDims * c));
-            continue;
+        for (int j = 0; j < U; ++j) {
+            if (h0 + kRows * j >= heads) break;
+            float y[kDims];
+            widen(y, x[j]);
+            finish(y);
+            store_dims<INTER>(dst, d, 2 * kHeadDim * (kRows * j + r), narrow(y));
         }
-        if constexpr (CACHE != 0) {
-            if (!p.ok) continue;
-            constexpr int EB = CACHE == 1 ? 2 : 1;
-            unsigned char* dst = static_cast<unsigned char*>(k ? a.k_cache : a.v_cache) +
-                                 kv_row_offset<EB>(p.page, h, p.slot, a.page_size, a.k.heads) + kDims * EB * c;
-            if constexpr (CACHE == 1) {
-                __builtin_nontemporal_store(k ? narrow(y) : x[j], reinterpret_cast<u32x4*>(dst));
-            } else {
+        return;
+    }
+    if constexpr (CACHE != 0) {
+        if (!p.ok) return;
+        constexpr int EB = CACHE == 1 ? 2 : 1;
+        const int head_bytes = a.page_size * kRowBytes<EB>;   // a page's bytes fit 31 bits
+        unsigned char* page = static_cast<unsigned char*>(v ? a.v_cache : a.k_cache) +
+                              static_cast<size_t>(p.page) * heads * head_bytes + static_cast<size_t>(h0) * head_bytes;
+        const __amdgpu_buffer_rsrc_t dst = buffer_rsrc(page, (heads - h0) * head_bytes);
+        const int slot = p.slot * kRowBytes<EB>;
 #pragma unroll
-                for (int e = 0; e < kDims; ++e) y[e] *= k ? a.inv_k : a.inv_v;
-                __builtin_nontemporal_store(e4m3_encode8(y), reinterpret_cast<u32x2*>(dst));
+        for (int j = 0; j < U; ++j) {
+            if (h0 + kRows * j >= heads) break;
+            const int off = (kRows * j + r) * head_bytes + slot;
+            float y[kDims];
+            widen(y, x[j]);
+            finish(y);
+            if constexpr (CACHE == 1) {
+                store_dims<INTER>(dst, d, off, v ? x[j] : narrow(y));
+            } else {
+                const float inv = v ? a.inv_v : a.inv_k;
+#pragma unroll
+                for (int e = 0; e < kDims; ++e) y[e] *= inv;
+                store_dims<INTER>(dst, d, off, e4m3_encode8(y));
             }
         }
     }
 }
 
-constexpr int kRowWaves = 4;   // waves of a head_rows_kernel block, a token each
+constexpr int kRowWaves = 4;   // waves of a head_rows_kernel block
 
-template <int CACHE, int META, int U>
+// Wave w takes part w % (pq + pk [+ pk]) of a token: U groups of q, of k, or of v.
+template <int CACHE, bool INTER, int META, int U>
 __device__ __forceinline__ void head_rows_body(const RopeAppend& a, const int32_t* meta) {
-    __shared__ Turn tab[kRowWaves][kPairs];
+    __shared__ __attribute__((aligned(16))) Turn tab[kRowWaves][kPairs];
     const int wave = __builtin_amdgcn_readfirstlane(threadIdx.x >> 6);
-    const int t    = blockIdx.x * kRowWaves + wave;
+    const int w    = blockIdx.x * kRowWaves + wave;
+    const int t    = static_cast<int>(static_cast<unsigned>(w) / static_cast<unsigned>(a.parts));
     if constexpr (META == kMetaList)
-        if (blockIdx.y == 0) write_tables(a, meta, blockIdx.x * blockDim.x + threadIdx.x, gridDim.x * blockDim.x);
+        write_tables(a, meta, blockIdx.x * blockDim.x + threadIdx.x, gridDim.x * blockDim.x);
     if (t >= a.n_tok) return;
-    rows_of_token<CACHE, META, U>(a, meta, t, blockIdx.y * U, tab[wave]);
+    int part = w - t * a.parts, kind = kRowQ;
+    if (part >= a.parts_q) {
+        part -= a.parts_q;
+        kind = kRowK;
+        if (CACHE != 0 && part >= a.parts_k) {
+            part -= a.parts_k;
+            kind = kRowV;
+        }
+    }
+    rows_of_token<CACHE, INTER, META, U>(a, meta, t, kind, part * U, tab[wave]);
 }
 
-template <int CACHE, int META, int U>
+template <int CACHE, bool INTER, int META, int U>
 __global__ __launch_bounds__(64 * kRowWaves) void head_rows_kernel(const RopeAppend a) {
-    head_rows_body<CACHE, META, U>(a, a.meta);
+    head_rows_body<CACHE, INTER, META, U>(a, a.meta);
 }
 // The meta is read where the arguments lie, as in pa_cache.hip.
-template <int CACHE, int U, int N>
+template <int CACHE, bool INTER, int U, int N>
 __global__ __launch_bounds__(64 * kRowWaves) void head_rows_inline_kernel(const RopeInline<N> x) {
     const uintptr_t args = (uintptr_t)__builtin_amdgcn_kernarg_segment_ptr();
-    head_rows_body<CACHE, kMetaList, U>(x.a, reinterpret_cast<const int32_t*>(args + offsetof(RopeInline<N>, meta)));
+    head_rows_body<CACHE, INTER, kMetaList, U>(x.a,
+                                               reinterpret_cast<const int32_t*>(args + offsetof(RopeInline<N>, meta)));
 }
 
 // ---- block-scaled caches ---------------------------------------------------
@@ -304,85 +370,67 @@ __device__ __forceinline__ float wave_max(float x) {
     return fmaxf(x, __shfl_xor(x, 32));
 }
 
-// One pool's part of a block: y holds the rows r + 4 i that lie in [s_lo, s_hi),
-// zeros elsewhere. Returns the block's new exponent. `old`: the byte of the
-// block's earlier rows (s_lo > 0).
-__device__ __forceinline__ int store_block(float (&y)[4][kDims], unsigned char* rows, int old, int s_lo, int s_hi) {
-    const int lane = threadIdx.x & 63, c = lane % kLanes, r = lane / kLanes;
-    float amax = 0.f;
-#pragma unroll
-    for (int i = 0; i < 4; ++i)
-#pragma unroll
-        for (int e = 0; e < kDims; ++e) amax = fmaxf(amax, fabsf(y[i][e]));
-    int k = block_exponent(wave_max(amax));
-    if (s_lo > 0) {
-        const int before = old - 127;
-        if (before >= k) {
-            k = before;
-        } else {
-            // The earlier rows to the new scale. A NaN's byte stays as it is.
-            const float f = exp2i(before - k);
-#pragma unroll
-            for (int i = 0; i < 4; ++i) {
-                if (r + 4 * i >= s_lo) continue;
-                u32x2* at = reinterpret_cast<u32x2*>(rows + (r + 4 * i) * kHeadDim + kDims * c);
-                const u32x2 was = *at;
-                const f16x8 h   = fp8x8_to_f16x8(was[0], was[1]);
-                float z[kDims];
-#pragma unroll
-                for (int e = 0; e < kDims; ++e) z[e] = static_cast<float>(h[e]) * f;
-                u32x2 now = e4m3_encode8(z);
-#pragma unroll
-                for (int e = 0; e < kDims; ++e) {
-                    const uint32_t m = 0xffu << (8 * (e & 3));
-                    if (((was[e >> 2] >> (8 * (e & 3))) & 0x7fu) == 0x7fu)
-                        now[e >> 2] = (now[e >> 2] & ~m) | (was[e >> 2] & m);
-                }
-                *at = now;
-            }
-        }
-    }
-    k = __builtin_amdgcn_readfirstlane(k);
-    const float inv = exp2i(-k), top = k == kBlockExpMax ? kBlockTop : 448.0f;
-#pragma unroll
-    for (int i = 0; i < 4; ++i) {
-        const int s = r + 4 * i;
-#pragma unroll
-        for (int e = 0; e < kDims; ++e) y[i][e] *= inv;
-        const u32x2 codes = e4m3_encode8(y[i], top);
-        if (s >= s_lo && s < s_hi)
-            __builtin_nontemporal_store(codes, reinterpret_cast<u32x2*>(rows + s * kHeadDim + kDims * c));
-    }
-    return k;
-}
-
-// One block of tokens of one entry, all its kv heads (a wave takes every
-// waves-th); unit u counts them as the launch does: entry e's i-th block is unit
-// tok_begin[e] / B + 2 e + i. (An entry of n tokens touches at most n / B + 2 blocks,
-// so units of different entries never meet, whatever its start, which the host
-// need not know.)
-template <int META>
-__device__ __forceinline__ void append_block(const RopeAppend& a, const int32_t* meta, int u, int waves,
+// One block of tokens of one entry in one pool (its keys, or its values), a wave for
+// each of the kv heads from h0 on. Unit u counts blocks as the launch does:
+// entry e's i-th block is unit tok_begin[e] / B + 2 e + i. (An entry of n tokens
+// touches at most n / B + 2 blocks, so units of different entries never meet,
+// whatever its start, which the host need not know.)
+//
+// A wave holds the block's 16 rows of a head as they came (four a load, as in the
+// rows kernel), norms and turns them once for their largest magnitude and, with the
+// scale that it asks for, once more for the codes: 160 more instructions a wave, but
+// half the registers, and so twice the waves, of holding the results. The codes of
+// earlier rows and their scale are loaded beside the new rows, so that a scale that
+// grows costs no further trip to memory. Keys and values go in blocks of their own.
+template <bool INTER, int META, bool V>
+__device__ __forceinline__ void append_block(const RopeAppend& a, const int32_t* meta, int u, int h0, int waves,
                                              Turn (*tab)[kPairs]) {
     const int lane = threadIdx.x & 63, c = lane % kLanes, r = lane / kLanes;
-    const int wave = __builtin_amdgcn_readfirstlane(threadIdx.x >> 6);
+    const int h = h0 + __builtin_amdgcn_readfirstlane(threadIdx.x >> 6);
     const int B = a.block_tokens, P = a.page_size, hkv = a.k.heads;
     const int32_t* tok_begin = META == kMetaList ? meta : a.tok_begin;
     const int32_t* start     = META == kMetaList ? meta + a.n_ent : a.start;
-    const int e = entry_of(u, a.n_ent, static_cast<int>(static_cast<int64_t>(u) * a.n_ent / a.units),
-                           [&](int i) { return load_uniform(tok_begin, i) / B + 2 * i; });
+    const int guess = static_cast<int>((static_cast<int64_t>(u) * a.n_ent + a.units / 2) / a.units);
+    const int e = entry_of(
+        u, a.n_ent, guess, [&](int i) { return load_uniform(tok_begin, i) / B + 2 * i; },
+        [&](int i) { return tok_begin[i] / B + 2 * i; });
     const int t0 = load_uniform(tok_begin, e), st = load_uniform(start, e);
     const int t1 = META == kMetaList && e + 1 == a.n_ent ? a.n_tok : min(load_uniform(tok_begin, e + 1), a.n_tok);
     if (st < 0 || t0 < 0 || t1 <= t0 || st > INT_MAX - (t1 - t0) - B) return;
     const int blk = st / B + (u - (t0 / B + 2 * e));   // block of the sequence
     const int lo = max(st, blk * B), hi = min(st + (t1 - t0), (blk + 1) * B);
     if (lo >= hi) return;
-    const int page = page_of<META>(a, meta, e, lo);
-    if (page < 0) return;
     const int s_lo = lo - blk * B, s_hi = hi - blk * B;
     const int tok  = t0 + (lo - st);          // token at s_lo
-    const int b    = blk * B % P / B;         // block of the page
-    if (a.rope.pairs) {
+    const LaneDims d = lane_dims<INTER || V>(V ? 0 : a.rope.pairs, c);
+    // The new rows, on their way under the page's lookup and the turns. Rows outside
+    // the block's part of the entry read zeros. (Strides are below 2^26.)
+    const long stride = V ? a.v_stride : a.k.in_stride;
+    const __amdgpu_buffer_rsrc_t src = buffer_rsrc((V ? a.v : a.k.in) + tok * stride, h < hkv ? INT_MAX : 0);
+    u32x4 x[4];
+#pragma unroll
+    for (int i = 0; i < 4; ++i) {
+        const int s = r + kRows * i;
+        const int off = s >= s_lo && s < s_hi ? 2 * ((s - s_lo) * static_cast<int>(stride) + h * kHeadDim) : INT_MIN;
+        x[i] = load_dims<INTER || V>(src, d, off);
+    }
+    const int page = page_of<META>(a, meta, e, lo);
+    if (page < 0) return;
+    const bool norm = !V && a.k.weight != nullptr;
+    const LaneWeights w = lane_weights(V ? nullptr : a.k.weight, d);
+    // The head's earlier rows (none past s_lo is read) and their scale.
+    const int b = blk * B % P / B;            // block of the page
+    uint8_t* const sc = a.scales + 2 * ((static_cast<size_t>(page) * hkv + h) * (P / B) + b) + (V ? 1 : 0);
+    unsigned char* const rows = static_cast<unsigned char*>(V ? a.v_cache : a.k_cache) + kv_row_offset<1>(page, h, b * B, P, hkv);
+    const bool earlier = s_lo > 0 && h < hkv;
+    const __amdgpu_buffer_rsrc_t held = buffer_rsrc(rows, earlier ? s_lo * kHeadDim : 0);
+    const int old = earlier ? *sc : 0;
+    u32x2 was[4];
+#pragma unroll
+    for (int i = 0; i < 4; ++i)
+        was[i] = __builtin_bit_cast(
+            u32x2, __builtin_amdgcn_raw_buffer_load_b64(held, (r + kRows * i) * kHeadDim + kDims * c, 0, 0));
+    if (!V && a.rope.pairs) {
         const int threads = 64 * waves;
         for (int i = threadIdx.x; i < (s_hi - s_lo) * kPairs; i += threads) {
             const int s = s_lo + i / kPairs, p = i % kPairs;
@@ -390,116 +438,197 @@ __device__ __forceinline__ void append_block(const RopeAppend& a, const int32_t*
         }
         __syncthreads();
     }
-    for (int h = wave; h < hkv; h += waves) {
-        u32x4 kx[4], vx[4];
+    if (h >= hkv) return;
+    float amax = 0.f, inv_n[4];
+    auto value = [&](float (&y)[kDims], int i) {   // row r + 4 i, its norm known
+        if (norm) apply_norm(y, inv_n[i], w);
+        if (!V && d.turned) apply_turns<INTER>(y, lane_turns(tab[r + kRows * i], c));
+    };
 #pragma unroll
-        for (int i = 0; i < 4; ++i) {
-            const int s = r + 4 * i;
-            kx[i] = vx[i] = u32x4{0, 0, 0, 0};
-            if (s >= s_lo && s < s_hi) {
-                const size_t t = static_cast<size_t>(tok + s - s_lo);
-                kx[i] = load16<true>(a.k.in + t * a.k.in_stride + h * kHeadDim + kDims * c);
-                vx[i] = load16<true>(a.v + t * a.v_stride + h * kHeadDim + kDims * c);
-            }
-        }
-        uint16_t* sc = reinterpret_cast<uint16_t*>(a.scales) + (static_cast<size_t>(page) * hkv + h) * (P / B) + b;
-        const int old = s_lo > 0 ? *sc : 0;
-        const size_t row0 = kv_row_offset<1>(page, h, b * B, P, hkv);
-        float y[4][kDims];
+    for (int i = 0; i < 4; ++i) {
+        float y[kDims];
+        widen(y, x[i]);
+        inv_n[i] = norm ? inv_norm(y, a.k.eps) : 1.0f;
+        value(y, i);
+        float m = 0.f;
 #pragma unroll
-        for (int i = 0; i < 4; ++i) {
-            widen(y[i], kx[i]);
-            LaneTurns l{};
-            if (a.rope.pairs) l = lane_turns(a.rope, tab[min(r + 4 * i, 15)], c);
-            norm_turn(y[i], a.k, a.rope, l, c);
-            const int s = r + 4 * i;
-            if (s < s_lo || s >= s_hi) {
-#pragma unroll
-                for (int e2 = 0; e2 < kDims; ++e2) y[i][e2] = 0.f;
-            }
-        }
-        const int kk = store_block(y, static_cast<unsigned char*>(a.k_cache) + row0, old & 0xff, s_lo, s_hi);
-#pragma unroll
-        for (int i = 0; i < 4; ++i) widen(y[i], vx[i]);
-        const int kv = store_block(y, static_cast<unsigned char*>(a.v_cache) + row0, old >> 8, s_lo, s_hi);
-        if (lane == 0) *sc = static_cast<uint16_t>((kk + 127) | ((kv + 127) << 8));
+        for (int n = 0; n < kDims; ++n) m = fmaxf(m, fabsf(y[n]));
+        const int s = r + kRows * i;
+        if (s >= s_lo && s < s_hi) amax = fmaxf(amax, m);
+        // The second time through starts from the rows again: the compiler would keep y.
+        asm volatile("" : "+v"(x[i]), "+v"(inv_n[i])::"memory");
     }
+    int k = __builtin_amdgcn_readfirstlane(block_exponent(wave_max(amax)));
+    if (s_lo > 0) {
+        const int before = __builtin_amdgcn_readfirstlane(old) - 127;
+        if (before < k) {
+            // The earlier rows to the new scale. A NaN's byte stays as it is.
+            const float f = exp2i(max(before - k, -126));
+#pragma unroll
+            for (int i = 0; i < 4; ++i) {
+                const f16x8 g = fp8x8_to_f16x8(was[i][0], was[i][1]);
+                float z[kDims];
+#pragma unroll
+                for (int n = 0; n < kDims; ++n) z[n] = static_cast<float>(g[n]) * f;
+                u32x2 now = e4m3_encode8(z);
+#pragma unroll
+                for (int n = 0; n < kDims; ++n) {
+                    const uint32_t m = 0xffu << (8 * (n & 3));
+                    if (((was[i][n >> 2] >> (8 * (n & 3))) & 0x7fu) == 0x7fu)
+                        now[n >> 2] = (now[n >> 2] & ~m) | (was[i][n >> 2] & m);
+                }
+                __builtin_amdgcn_raw_buffer_store_b64(now, held, (r + kRows * i) * kHeadDim + kDims * c, 0, 0);
+                asm volatile("" ::: "memory");
+            }
+        }
+        k = max(k, before);
+    }
+    const float inv = exp2i(-k), top = k == kBlockExpMax ? kBlockTop : 448.0f;
+    const __amdgpu_buffer_rsrc_t dst = buffer_rsrc(rows, s_hi * kHeadDim);   // no row past the new ones is written
+#pragma unroll
+    for (int i = 0; i < 4; ++i) {
+        const int s = r + kRows * i;
+        float y[kDims];
+        widen(y, x[i]);
+        value(y, i);
+#pragma unroll
+        for (int n = 0; n < kDims; ++n) y[n] *= inv;
+        const u32x2 codes = e4m3_encode8(y, top);
+        if (s >= s_lo) store_dims<INTER || V>(dst, d, s * kHeadDim, codes);
+        asm volatile("" ::: "memory");
+    }
+    if (lane == 0) *sc = static_cast<uint8_t>(k + 127);
 }
 
-// Blocks of the grid: the units of k and v, then the tokens' q rows.
-template <int META>
+// Groups of a token's q rows that one wave takes beside the blocks.
+constexpr int kBlockQ = 4;
+
+// Blocks of the grid: the units of k, those of v, then the tokens' q rows.
+template <bool INTER, int META>
 __device__ __forceinline__ void block_append_body(const RopeAppend& a, const int32_t* meta) {
-    __shared__ Turn tab[16][kPairs];
+    __shared__ __attribute__((aligned(16))) Turn tab[16][kPairs];
     const int waves = blockDim.x >> 6;
     if constexpr (META == kMetaList)
         write_tables(a, meta, blockIdx.x * blockDim.x + threadIdx.x, gridDim.x * blockDim.x);
-    if (static_cast<int>(blockIdx.x) < a.units) {
-        append_block<META>(a, meta, blockIdx.x, waves, tab);
+    const int blocks = a.units * a.head_groups;   // of k, and of v
+    if (static_cast<int>(blockIdx.x) < 2 * blocks) {
+        const bool v = static_cast<int>(blockIdx.x) >= blocks;
+        const unsigned i = blockIdx.x - (v ? blocks : 0), groups = a.head_groups;
+        const int u = static_cast<int>(i / groups), h0 = static_cast<int>(i % groups) * waves;
+        if (v) append_block<INTER, META, true>(a, meta, u, h0, waves, tab);
+        else append_block<INTER, META, false>(a, meta, u, h0, waves, tab);
         return;
     }
     const int wave = __builtin_amdgcn_readfirstlane(threadIdx.x >> 6);
-    const int gq = (a.q.heads + kRows - 1) / kRows;
-    const int w  = (blockIdx.x - a.units) * waves + wave;
-    const int t  = w / gq;
+    const int w = (blockIdx.x - 2 * blocks) * waves + wave;
+    const int t = static_cast<int>(static_cast<unsigned>(w) / static_cast<unsigned>(a.parts_q));
     if (t >= a.n_tok) return;
-    RopeAppend q = a;
-    q.k.heads = 0;
-    rows_of_token<0, META, 1>(q, meta, t, w - t * gq, tab[wave]);
+    rows_of_token<0, INTER, META, kBlockQ>(a, meta, t, kRowQ, (w - t * a.parts_q) * kBlockQ, tab[wave]);
 }
 
 constexpr int kBlockWaves = 8;
+#ifndef PA_BLOCK_WPE
+#define PA_BLOCK_WPE 4
+#endif
 
-template <int META>
-__global__ __launch_bounds__(64 * kBlockWaves) void block_append_kernel(const RopeAppend a) {
-    block_append_body<META>(a, a.meta);
+template <bool INTER, int META>
+__global__ __launch_bounds__(64 * kBlockWaves) __attribute__((amdgpu_waves_per_eu(PA_BLOCK_WPE))) void block_append_kernel(const RopeAppend a) {
+    block_append_body<INTER, META>(a, a.meta);
 }
-template <int N>
-__global__ __launch_bounds__(64 * kBlockWaves) void block_append_inline_kernel(const RopeInline<N> x) {
+template <bool INTER, int N>
+__global__ __launch_bounds__(64 * kBlockWaves) __attribute__((amdgpu_waves_per_eu(PA_BLOCK_WPE))) void block_append_inline_kernel(const RopeInline<N> x) {
     const uintptr_t args = (uintptr_t)__builtin_amdgcn_kernarg_segment_ptr();
-    block_append_body<kMetaList>(x.a, reinterpret_cast<const int32_t*>(args + offsetof(RopeInline<N>, meta)));
+    block_append_body<INTER, kMetaList>(x.a, reinterpret_cast<const int32_t*>(args + offsetof(RopeInline<N>, meta)));
 }
 
-int groups_of(const RopeAppend& a, bool cache) {
-    const int gq = (a.q.heads + kRows - 1) / kRows, gk = (a.k.heads + kRows - 1) / kRows;
-    return gq + gk + (cache ? gk : 0);
+int groups(int heads) { return (heads + kRows - 1) / kRows; }
+
+#ifndef PA_ROWS_U
+#define PA_ROWS_U 4
+#endif
+// A large call's waves take up to PA_ROWS_U groups, a small one's one each.
+constexpr long kManyGroups = 16384;
+
+// Parts of a token at u groups a wave, and the grid.
+dim3 rows_grid(RopeAppend& a, bool cache, int u) {
+    a.parts_q = (groups(a.q.heads) + u - 1) / u;
+    a.parts_k = (groups(a.k.heads) + u - 1) / u;
+    a.parts   = a.parts_q + (cache ? 2 : 1) * a.parts_k;
+    const long waves = static_cast<long>(a.n_tok) * a.parts;
+    return dim3(static_cast<unsigned>((waves + kRowWaves - 1) / kRowWaves));
+}
+bool many(const RopeAppend& a, bool cache) {
+    return static_cast<long>(a.n_tok) * (groups(a.q.heads) + (cache ? 2 : 1) * groups(a.k.heads)) >= kManyGroups;
 }
 
+template <int CACHE, bool INTER, int META>
+void launch_rows_i(RopeAppend a, hipStream_t s) {
+    const dim3 block(64 * kRowWaves);
+    if (many(a, CACHE != 0)) {
+        const dim3 grid = rows_grid(a, CACHE != 0, PA_ROWS_U);
+        hipLaunchKernelGGL((head_rows_kernel<CACHE, INTER, META, PA_ROWS_U>), grid, block, 0, s, a);
+    } else {
+        const dim3 grid = rows_grid(a, CACHE != 0, 1);
+        hipLaunchKernelGGL((head_rows_kernel<CACHE, INTER, META, 1>), grid, block, 0, s, a);
+    }
+}
 template <int CACHE, int META>
 void launch_rows(const RopeAppend& a, hipStream_t s) {
-    const dim3 grid((a.n_tok + kRowWaves - 1) / kRowWaves, groups_of(a, CACHE != 0));
-    hipLaunchKernelGGL((head_rows_kernel<CACHE, META, 1>), grid, dim3(64 * kRowWaves), 0, s, a);
+    if (a.rope.interleaved) launch_rows_i<CACHE, true, META>(a, s);
+    else launch_rows_i<CACHE, false, META>(a, s);
 }
-template <int CACHE, int N>
-void launch_rows_inline(const RopeAppend& a, const int32_t* meta, size_t n, hipStream_t s) {
+template <int CACHE, bool INTER, int N>
+void launch_rows_inline_i(const RopeAppend& a, const int32_t* meta, size_t n, hipStream_t s) {
     RopeInline<N> x;
     x.a = a;
     std::copy(meta, meta + n, x.meta);
-    const dim3 grid((a.n_tok + kRowWaves - 1) / kRowWaves, groups_of(a, CACHE != 0));
-    hipLaunchKernelGGL((head_rows_inline_kernel<CACHE, 1, N>), grid, dim3(64 * kRowWaves), 0, s, x);
+    const dim3 block(64 * kRowWaves);
+    if (many(a, true)) {
+        const dim3 grid = rows_grid(x.a, true, PA_ROWS_U);
+        hipLaunchKernelGGL((head_rows_inline_kernel<CACHE, INTER, PA_ROWS_U, N>), grid, block, 0, s, x);
+    } else {
+        const dim3 grid = rows_grid(x.a, true, 1);
+        hipLaunchKernelGGL((head_rows_inline_kernel<CACHE, INTER, 1, N>), grid, block, 0, s, x);
+    }
+}
+template <int CACHE, int N>
+void launch_rows_inline(const RopeAppend& a, const int32_t* meta, size_t n, hipStream_t s) {
+    if (a.rope.interleaved) launch_rows_inline_i<CACHE, true, N>(a, meta, n, s);
+    else launch_rows_inline_i<CACHE, false, N>(a, meta, n, s);
 }
 
 // Waves of a block and blocks of a block_append_kernel launch; sets a.units.
 dim3 block_grid(RopeAppend& a, int& waves) {
     waves = std::min(a.k.heads, kBlockWaves);
     a.block_tokens = block_tokens(a.page_size);
-    a.units = a.n_tok / a.block_tokens + 2 * a.n_ent;
-    const long q = static_cast<long>(a.n_tok) * ((a.q.heads + kRows - 1) / kRows);
-    return dim3(static_cast<unsigned>(a.units + (q + waves - 1) / waves));
+    a.units       = a.n_tok / a.block_tokens + 2 * a.n_ent;
+    a.head_groups = (a.k.heads + waves - 1) / waves;
+    a.parts_q = (groups(a.q.heads) + kBlockQ - 1) / kBlockQ;
+    const long q = static_cast<long>(a.n_tok) * a.parts_q;
+    return dim3(static_cast<unsigned>(2l * a.units * a.head_groups + (q + waves - 1) / waves));
+}
+template <int META>
+void launch_block(RopeAppend a, hipStream_t s) {
+    int waves = 0;
+    const dim3 grid = block_grid(a, waves), block(64 * waves);
+    if (a.rope.interleaved) hipLaunchKernelGGL((block_append_kernel<true, META>), grid, block, 0, s, a);
+    else hipLaunchKernelGGL((block_append_kernel<false, META>), grid, block, 0, s, a);
 }
 template <int N>
-void launch_block_inline(RopeAppend a, const int32_t* meta, size_t n, hipStream_t s) {
-    int waves = 0;
-    const dim3 grid = block_grid(a, waves);
+void launch_block_inline(const RopeAppend& a, const int32_t* meta, size_t n, hipStream_t s) {
     RopeInline<N> x;
     x.a = a;
     std::copy(meta, meta + n, x.meta);
-    hipLaunchKernelGGL((block_append_inline_kernel<N>), grid, dim3(64 * waves), 0, s, x);
+    int waves = 0;
+    const dim3 grid = block_grid(x.a, waves), block(64 * waves);
+    if (a.rope.interleaved) hipLaunchKernelGGL((block_append_inline_kernel<true, N>), grid, block, 0, s, x);
+    else hipLaunchKernelGGL((block_append_inline_kernel<false, N>), grid, block, 0, s, x);
 }
 
 }  // namespace
 
 hipError_t launch_norm_rope(const RopeAppend& a, hipStream_t s) {
-    if (a.n_tok <= 0 || groups_of(a, false) == 0) return hipSuccess;
+    if (a.n_tok <= 0 || a.q.heads + a.k.heads == 0) return hipSuccess;
     launch_rows<0, 0>(a, s);
     return hipGetLastError();
 }
@@ -507,33 +636,22 @@ hipError_t launch_norm_rope(const RopeAppend& a, hipStream_t s) {
 hipError_t launch_append_rope(int dtype, const RopeAppend& a, const int32_t* meta, size_t n_meta, hipStream_t s) {
     check_kv_dtype(dtype);
     if (a.n_tok <= 0) return hipSuccess;
-    const bool list = meta || a.meta;   // a cache's append; else the caller's device arrays
+    const bool list  = a.meta != nullptr;   // a cache's append, its meta too long for the arguments
+    const bool small = meta && n_meta <= 256;
     if (dtype == PA_KV_FP8_E4M3_BLOCK) {
-        if (meta && n_meta <= 256) {
-            launch_block_inline<256>(a, meta, n_meta, s);
-        } else if (meta) {
-            launch_block_inline<kRopeInlineInts>(a, meta, n_meta, s);
-        } else {
-            RopeAppend b = a;
-            int waves = 0;
-            const dim3 grid = block_grid(b, waves);
-            if (list) hipLaunchKernelGGL(block_append_kernel<kMetaList>, grid, dim3(64 * waves), 0, s, b);
-            else hipLaunchKernelGGL(block_append_kernel<kMetaTable>, grid, dim3(64 * waves), 0, s, b);
-        }
-        return hipGetLastError();
-    }
-    const bool fp16 = dtype == PA_KV_FP16;
-    if (meta && n_meta <= 256) {
-        if (fp16) launch_rows_inline<1, 256>(a, meta, n_meta, s);
-        else launch_rows_inline<2, 256>(a, meta, n_meta, s);
-    } else if (meta) {
-        if (fp16) launch_rows_inline<1, kRopeInlineInts>(a, meta, n_meta, s);
-        else launch_rows_inline<2, kRopeInlineInts>(a, meta, n_meta, s);
-    } else if (list) {
-        if (fp16) launch_rows<1, kMetaList>(a, s);
-        else launch_rows<2, kMetaList>(a, s);
+        if (small) launch_block_inline<256>(a, meta, n_meta, s);
+        else if (meta) launch_block_inline<kRopeInlineInts>(a, meta, n_meta, s);
+        else if (list) launch_block<kMetaList>(a, s);
+        else launch_block<kMetaTable>(a, s);
+    } else if (dtype == PA_KV_FP16) {
+        if (small) launch_rows_inline<1, 256>(a, meta, n_meta, s);
+        else if (meta) launch_rows_inline<1, kRopeInlineInts>(a, meta, n_meta, s);
+        else if (list) launch_rows<1, kMetaList>(a, s);
+        else launch_rows<1, kMetaTable>(a, s);
     } else {
-        if (fp16) launch_rows<1, kMetaTable>(a, s);
+        if (small) launch_rows_inline<2, 256>(a, meta, n_meta, s);
+        else if (meta) launch_rows_inline<2, kRopeInlineInts>(a, meta, n_meta, s);
+        else if (list) launch_rows<2, kMetaList>(a, s);
         else launch_rows<2, kMetaTable>(a, s);
     }
     return hipGetLastError();

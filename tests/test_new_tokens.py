@@ -51,6 +51,7 @@ def test_bytes_per_page_counts_the_scales():
 
 @pytest.mark.parametrize("change,word", [
     (dict(in_=None), "null rows"), (dict(in_=A + 8), "aligned"), (dict(in_stride=1028), "aligned"),
+    (dict(in_stride=-1024), "aligned"), (dict(in_stride=2**26), "aligned"), (dict(out_stride=-1024), "aligned"),
     (dict(out=None), "null output"), (dict(out=A + (1 << 19) + 4), "aligned"), (dict(out_stride=1020), "aligned"),
     (dict(out_stride=512), "rows overlap"), (dict(out_stride=0), "rows overlap"),
     (dict(weight=A + 4), "weight"), (dict(weight=A, eps=-1.0), "eps"), (dict(weight=A, eps=float("nan")), "eps"),
@@ -116,7 +117,7 @@ def append(dtype=pa_amd.FP8_E4M3_BLOCK, q=None, k=None, **kw):
 @pytest.mark.parametrize("change,word", [
     (dict(num_tokens=-1), "sizes"), (dict(num_entries=-1), "sizes"), (dict(page_size=0), "sizes"),
     (dict(block_table_stride=0), "sizes"), (dict(num_table_rows=-1), "sizes"), (dict(num_pages=-1), "sizes"),
-    (dict(v=None), "v is null"), (dict(v=A + 2), "aligned"), (dict(v_stride=100), "aligned"),
+    (dict(v=None), "v is null"), (dict(v=A + 2), "aligned"), (dict(v_stride=100), "aligned"), (dict(v_stride=-1024), "aligned"),
     (dict(tok_begin=None), "null"), (dict(start_pos=None), "null"), (dict(block_table=None), "null"),
     (dict(k_cache=None), "null"), (dict(v_cache=None), "null"), (dict(k_cache=A + 8), "caches"),
     (dict(kv_scales=None), "kv_scales"), (dict(kv_scales=A + 1), "kv_scales"),
