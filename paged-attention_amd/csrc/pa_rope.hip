@@ -37,7 +37,9 @@ static_assert(kPairs == 64, "a wave computes one pair's sine and cosine per lane
 struct Turn {
     float c, s;
 };
-constexpr int kNonTemporal = 2;   // cache policy of buffer loads and stores: touched once
+constexpr int kStoreAux = 2;   // buffer stores are non-temporal: what is stored is read by later kernels only
+// ... and loads where NT is given: see streams().
+template <bool NT> constexpr int kLoadAux = NT ? 2 : 0;
 
 // Sum (or maximum) over the 16 lanes of a row, in every lane.
 template <int CTRL>
@@ -73,43 +75,42 @@ __device__ __forceinline__ Turn turn_of(const RopeTable& r, const int32_t* posit
 }
 
 // The 8 dims that lane c of a row holds, as two chunks of four: with half-split
-// pairs both halves of pairs 4c .. 4c + 3, so that no lane needs another's values;
-// with interleaved ones, and of dims that do not turn, eight dims in a row.
+// pairs both halves of pairs 4c .. 4c + 3, so that no lane needs another's values
+// (the dims that do not turn are halved likewise: a load then takes runs of whole
+// 64 bytes); with interleaved ones, eight dims in a row.
 struct LaneDims {
     int  lo, hi;   // the chunks' first dims
     bool turned;
 };
 template <bool INTER>
 __device__ __forceinline__ LaneDims lane_dims(int pairs, int c) {
-    const int l = pairs / 4;   // lanes that turn
-    if (INTER || c >= l) {
-        const int d = kDims * c;   // 2 * pairs + 8 (c - l)
-        return {d, d + 4, c < l};
-    }
-    return {4 * c, pairs + 4 * c, true};
+    const bool turned = 4 * c < pairs;
+    if constexpr (INTER) return {kDims * c, kDims * c + 4, turned};
+    const int lo = 4 * c + (turned ? 0 : pairs);   // 2 * pairs + 4 (c - pairs / 4)
+    return {lo, lo + (turned ? pairs : kPairs - pairs), turned};
 }
 
 // A lane's dims of the row `off` bytes into a resource (past its end: zeros).
-template <bool INTER>
+template <bool INTER, bool NT>
 __device__ __forceinline__ u32x4 load_dims(__amdgpu_buffer_rsrc_t rs, const LaneDims& d, int off) {
     if constexpr (INTER)
-        return __builtin_bit_cast(u32x4, __builtin_amdgcn_raw_buffer_load_b128(rs, 2 * d.lo + off, 0, kNonTemporal));
-    const u32x2 x = __builtin_bit_cast(u32x2, __builtin_amdgcn_raw_buffer_load_b64(rs, 2 * d.lo + off, 0, kNonTemporal));
-    const u32x2 y = __builtin_bit_cast(u32x2, __builtin_amdgcn_raw_buffer_load_b64(rs, 2 * d.hi + off, 0, kNonTemporal));
+        return __builtin_bit_cast(u32x4, __builtin_amdgcn_raw_buffer_load_b128(rs, 2 * d.lo + off, 0, kLoadAux<NT>));
+    const u32x2 x = __builtin_bit_cast(u32x2, __builtin_amdgcn_raw_buffer_load_b64(rs, 2 * d.lo + off, 0, kLoadAux<NT>));
+    const u32x2 y = __builtin_bit_cast(u32x2, __builtin_amdgcn_raw_buffer_load_b64(rs, 2 * d.hi + off, 0, kLoadAux<NT>));
     return u32x4{x[0], x[1], y[0], y[1]};
 }
 // The same stored, as fp16 or as codes (past the end: dropped).
 template <bool INTER>
 __device__ __forceinline__ void store_dims(__amdgpu_buffer_rsrc_t rs, const LaneDims& d, int off, u32x4 x) {
-    if constexpr (INTER) return __builtin_amdgcn_raw_buffer_store_b128(x, rs, 2 * d.lo + off, 0, kNonTemporal);
-    __builtin_amdgcn_raw_buffer_store_b64(u32x2{x[0], x[1]}, rs, 2 * d.lo + off, 0, kNonTemporal);
-    __builtin_amdgcn_raw_buffer_store_b64(u32x2{x[2], x[3]}, rs, 2 * d.hi + off, 0, kNonTemporal);
+    if constexpr (INTER) return __builtin_amdgcn_raw_buffer_store_b128(x, rs, 2 * d.lo + off, 0, kStoreAux);
+    __builtin_amdgcn_raw_buffer_store_b64(u32x2{x[0], x[1]}, rs, 2 * d.lo + off, 0, kStoreAux);
+    __builtin_amdgcn_raw_buffer_store_b64(u32x2{x[2], x[3]}, rs, 2 * d.hi + off, 0, kStoreAux);
 }
 template <bool INTER>
 __device__ __forceinline__ void store_dims(__amdgpu_buffer_rsrc_t rs, const LaneDims& d, int off, u32x2 x) {
-    if constexpr (INTER) return __builtin_amdgcn_raw_buffer_store_b64(x, rs, d.lo + off, 0, kNonTemporal);
-    __builtin_amdgcn_raw_buffer_store_b32(x[0], rs, d.lo + off, 0, kNonTemporal);
-    __builtin_amdgcn_raw_buffer_store_b32(x[1], rs, d.hi + off, 0, kNonTemporal);
+    if constexpr (INTER) return __builtin_amdgcn_raw_buffer_store_b64(x, rs, d.lo + off, 0, kStoreAux);
+    __builtin_amdgcn_raw_buffer_store_b32(x[0], rs, d.lo + off, 0, kStoreAux);
+    __builtin_amdgcn_raw_buffer_store_b32(x[1], rs, d.hi + off, 0, kStoreAux);
 }
 
 // A row's norm weights, and a token's turns, as a lane needs them.
@@ -250,20 +251,19 @@ enum RowKind { kRowQ = 0, kRowK = 1, kRowV = 2 };
 // four rows, or none, takes no branch (branches around the loads had the compiler
 // wait for each group's before the next: 8192 tokens of 32 + 8 heads 32.8 us at 8
 // groups a wave, but 37.1 at 4 and 66.8 at 6).
-template <int CACHE, bool INTER, int META, int U>
+template <int CACHE, bool INTER, int META, int U, bool NT>
 __device__ __forceinline__ void rows_of_token(const RopeAppend& a, const int32_t* meta, int t, int kind, int g0,
                                               Turn* tab) {
     const int lane = threadIdx.x & 63, c = lane % kLanes, r = lane / kLanes;
     const bool v = CACHE != 0 && kind == kRowV;
     const HeadRows& rows = kind == kRowQ ? a.q : a.k;
     const int heads = rows.heads, h0 = kRows * g0;
-    LaneDims d = lane_dims<INTER>(a.rope.pairs, c);
-    if (v) d = LaneDims{kDims * c, kDims * c + 4, false};
+    const LaneDims d = lane_dims<INTER>(v ? 0 : a.rope.pairs, c);
     const uint16_t* in = (v ? a.v + t * a.v_stride : rows.in + t * rows.in_stride) + h0 * kHeadDim;
     const __amdgpu_buffer_rsrc_t src = buffer_rsrc(in, 2 * kHeadDim * (heads - h0));
     u32x4 x[U];
 #pragma unroll
-    for (int j = 0; j < U; ++j) x[j] = load_dims<INTER>(src, d, 2 * kHeadDim * (kRows * j + r));
+    for (int j = 0; j < U; ++j) x[j] = load_dims<INTER, NT>(src, d, 2 * kHeadDim * (kRows * j + r));
     Place p{true, 0, 0, 0};
     if constexpr (META != 0) p = place_of<META>(a, meta, t);
     const bool norm = !v && rows.weight != nullptr;
@@ -321,7 +321,7 @@ __device__ __forceinline__ void rows_of_token(const RopeAppend& a, const int32_t
 constexpr int kRowWaves = 4;   // waves of a head_rows_kernel block
 
 // Wave w takes part w % (pq + pk [+ pk]) of a token: U groups of q, of k, or of v.
-template <int CACHE, bool INTER, int META, int U>
+template <int CACHE, bool INTER, int META, int U, bool NT>
 __device__ __forceinline__ void head_rows_body(const RopeAppend& a, const int32_t* meta) {
     __shared__ __attribute__((aligned(16))) Turn tab[kRowWaves][kPairs];
     const int wave = __builtin_amdgcn_readfirstlane(threadIdx.x >> 6);
@@ -339,19 +339,19 @@ __device__ __forceinline__ void head_rows_body(const RopeAppend& a, const int32_
             kind = kRowV;
         }
     }
-    rows_of_token<CACHE, INTER, META, U>(a, meta, t, kind, part * U, tab[wave]);
+    rows_of_token<CACHE, INTER, META, U, NT>(a, meta, t, kind, part * U, tab[wave]);
 }
 
-template <int CACHE, bool INTER, int META, int U>
+template <int CACHE, bool INTER, int META, int U, bool NT>
 __global__ __launch_bounds__(64 * kRowWaves) void head_rows_kernel(const RopeAppend a) {
-    head_rows_body<CACHE, INTER, META, U>(a, a.meta);
+    head_rows_body<CACHE, INTER, META, U, NT>(a, a.meta);
 }
 // The meta is read where the arguments lie, as in pa_cache.hip.
 template <int CACHE, bool INTER, int U, int N>
 __global__ __launch_bounds__(64 * kRowWaves) void head_rows_inline_kernel(const RopeInline<N> x) {
     const uintptr_t args = (uintptr_t)__builtin_amdgcn_kernarg_segment_ptr();
-    head_rows_body<CACHE, INTER, kMetaList, U>(x.a,
-                                               reinterpret_cast<const int32_t*>(args + offsetof(RopeInline<N>, meta)));
+    head_rows_body<CACHE, INTER, kMetaList, U, false>(
+        x.a, reinterpret_cast<const int32_t*>(args + offsetof(RopeInline<N>, meta)));
 }
 
 // ---- block-scaled caches ---------------------------------------------------
@@ -382,7 +382,7 @@ __device__ __forceinline__ float wave_max(float x) {
 // half the registers, and so twice the waves, of holding the results. The codes of
 // earlier rows and their scale are loaded beside the new rows, so that a scale that
 // grows costs no further trip to memory. Keys and values go in blocks of their own.
-template <bool INTER, int META, bool V>
+template <bool INTER, int META, bool V, bool NT>
 __device__ __forceinline__ void append_block(const RopeAppend& a, const int32_t* meta, int u, int h0, int waves,
                                              Turn (*tab)[kPairs]) {
     const int lane = threadIdx.x & 63, c = lane % kLanes, r = lane / kLanes;
@@ -412,7 +412,7 @@ __device__ __forceinline__ void append_block(const RopeAppend& a, const int32_t*
     for (int i = 0; i < 4; ++i) {
         const int s = r + kRows * i;
         const int off = s >= s_lo && s < s_hi ? 2 * ((s - s_lo) * static_cast<int>(stride) + h * kHeadDim) : INT_MIN;
-        x[i] = load_dims<INTER || V>(src, d, off);
+        x[i] = load_dims<INTER || V, NT>(src, d, off);
     }
     const int page = page_of<META>(a, meta, e, lo);
     if (page < 0) return;
@@ -444,8 +444,12 @@ __device__ __forceinline__ void append_block(const RopeAppend& a, const int32_t*
         if (norm) apply_norm(y, inv_n[i], w);
         if (!V && d.turned) apply_turns<INTER>(y, lane_turns(tab[r + kRows * i], c));
     };
+    // Four rows at a time, those that hold none of the new tokens left out.
+    auto live = [&](int i) { return s_lo < kRows * (i + 1) && kRows * i < s_hi; };
 #pragma unroll
     for (int i = 0; i < 4; ++i) {
+        inv_n[i] = 1.0f;
+        if (!live(i)) continue;
         float y[kDims];
         widen(y, x[i]);
         inv_n[i] = norm ? inv_norm(y, a.k.eps) : 1.0f;
@@ -487,6 +491,7 @@ __device__ __forceinline__ void append_block(const RopeAppend& a, const int32_t*
     const __amdgpu_buffer_rsrc_t dst = buffer_rsrc(rows, s_hi * kHeadDim);   // no row past the new ones is written
 #pragma unroll
     for (int i = 0; i < 4; ++i) {
+        if (!live(i)) continue;
         const int s = r + kRows * i;
         float y[kDims];
         widen(y, x[i]);
@@ -504,7 +509,7 @@ __device__ __forceinline__ void append_block(const RopeAppend& a, const int32_t*
 constexpr int kBlockQ = 4;
 
 // Blocks of the grid: the units of k, those of v, then the tokens' q rows.
-template <bool INTER, int META>
+template <bool INTER, int META, bool NT>
 __device__ __forceinline__ void block_append_body(const RopeAppend& a, const int32_t* meta) {
     __shared__ __attribute__((aligned(16))) Turn tab[16][kPairs];
     const int waves = blockDim.x >> 6;
@@ -515,39 +520,47 @@ __device__ __forceinline__ void block_append_body(const RopeAppend& a, const int
         const bool v = static_cast<int>(blockIdx.x) >= blocks;
         const unsigned i = blockIdx.x - (v ? blocks : 0), groups = a.head_groups;
         const int u = static_cast<int>(i / groups), h0 = static_cast<int>(i % groups) * waves;
-        if (v) append_block<INTER, META, true>(a, meta, u, h0, waves, tab);
-        else append_block<INTER, META, false>(a, meta, u, h0, waves, tab);
+        if (v) append_block<INTER, META, true, NT>(a, meta, u, h0, waves, tab);
+        else append_block<INTER, META, false, NT>(a, meta, u, h0, waves, tab);
         return;
     }
     const int wave = __builtin_amdgcn_readfirstlane(threadIdx.x >> 6);
     const int w = (blockIdx.x - 2 * blocks) * waves + wave;
     const int t = static_cast<int>(static_cast<unsigned>(w) / static_cast<unsigned>(a.parts_q));
     if (t >= a.n_tok) return;
-    rows_of_token<0, INTER, META, kBlockQ>(a, meta, t, kRowQ, (w - t * a.parts_q) * kBlockQ, tab[wave]);
+    rows_of_token<0, INTER, META, kBlockQ, NT>(a, meta, t, kRowQ, (w - t * a.parts_q) * kBlockQ, tab[wave]);
 }
 
 constexpr int kBlockWaves = 8;
-#ifndef PA_BLOCK_WPE
-#define PA_BLOCK_WPE 4
-#endif
 
-template <bool INTER, int META>
-__global__ __launch_bounds__(64 * kBlockWaves) __attribute__((amdgpu_waves_per_eu(PA_BLOCK_WPE))) void block_append_kernel(const RopeAppend a) {
-    block_append_body<INTER, META>(a, a.meta);
+template <bool INTER, int META, bool NT>
+__global__ __launch_bounds__(64 * kBlockWaves) void block_append_kernel(const RopeAppend a) {
+    block_append_body<INTER, META, NT>(a, a.meta);
 }
 template <bool INTER, int N>
-__global__ __launch_bounds__(64 * kBlockWaves) __attribute__((amdgpu_waves_per_eu(PA_BLOCK_WPE))) void block_append_inline_kernel(const RopeInline<N> x) {
+__global__ __launch_bounds__(64 * kBlockWaves) void block_append_inline_kernel(const RopeInline<N> x) {
     const uintptr_t args = (uintptr_t)__builtin_amdgcn_kernarg_segment_ptr();
-    block_append_body<INTER, kMetaList>(x.a, reinterpret_cast<const int32_t*>(args + offsetof(RopeInline<N>, meta)));
+    block_append_body<INTER, kMetaList, false>(x.a, reinterpret_cast<const int32_t*>(args + offsetof(RopeInline<N>, meta)));
 }
 
 int groups(int heads) { return (heads + kRows - 1) / kRows; }
 
-#ifndef PA_ROWS_U
-#define PA_ROWS_U 4
-#endif
-// A large call's waves take up to PA_ROWS_U groups, a small one's one each.
+// A large call's waves take up to kManyU groups of four rows (the turns are worked
+// out once a wave), a small one's one each. Same box, us, 8192 tokens of 32 + 8
+// heads at 2, 3, 4, 5, 6, 12 groups: 35.0, 34.6, 32.7, 32.9, 34.2, 38.7; 512 tokens
+// 4.4 at any of them, 1 token 2.5 at one group and 3.4 at two.
+constexpr int  kManyU      = 4;
 constexpr long kManyGroups = 16384;
+
+// Whether a call's loads bypass the caches: from some 100 MB of rows on, which the
+// projection before it cannot have left in the memory-side cache (256 MB, the
+// outputs beside them), and where a load takes whole 128-byte lines, which partial
+// half-split rotations do not. us with cached and with non-temporal loads: 37
+// ragged prompts (64 of 128 dims turn, 11 000 tokens of 16 + 2 x 4 heads) 24.7 /
+// 30.2, 2048 tokens of 32 + 8 heads 7.9 / 9.8, 8192 with 96 dims turned 29.0 / 36.4,
+// 8192 tokens into FP8 pages (126 MB) 35.8 / 34.4, 32768 into block-scaled ones 145
+// / 137.
+constexpr long kStreamBytes = 96l << 20;
 
 // Parts of a token at u groups a wave, and the grid.
 dim3 rows_grid(RopeAppend& a, bool cache, int u) {
@@ -561,15 +574,23 @@ bool many(const RopeAppend& a, bool cache) {
     return static_cast<long>(a.n_tok) * (groups(a.q.heads) + (cache ? 2 : 1) * groups(a.k.heads)) >= kManyGroups;
 }
 
+bool streams(const RopeAppend& a, bool cache) {
+    const bool lines = a.rope.interleaved || a.rope.pairs == 0 || a.rope.pairs == kPairs;
+    const long rows  = static_cast<long>(a.n_tok) * (a.q.heads + (cache ? 2 : 1) * a.k.heads);
+    return lines && rows * kRowBytes<2> >= kStreamBytes;
+}
+
 template <int CACHE, bool INTER, int META>
 void launch_rows_i(RopeAppend a, hipStream_t s) {
     const dim3 block(64 * kRowWaves);
     if (many(a, CACHE != 0)) {
-        const dim3 grid = rows_grid(a, CACHE != 0, PA_ROWS_U);
-        hipLaunchKernelGGL((head_rows_kernel<CACHE, INTER, META, PA_ROWS_U>), grid, block, 0, s, a);
+        const dim3 grid = rows_grid(a, CACHE != 0, kManyU);
+        if (streams(a, CACHE != 0))
+            hipLaunchKernelGGL((head_rows_kernel<CACHE, INTER, META, kManyU, true>), grid, block, 0, s, a);
+        else hipLaunchKernelGGL((head_rows_kernel<CACHE, INTER, META, kManyU, false>), grid, block, 0, s, a);
     } else {
         const dim3 grid = rows_grid(a, CACHE != 0, 1);
-        hipLaunchKernelGGL((head_rows_kernel<CACHE, INTER, META, 1>), grid, block, 0, s, a);
+        hipLaunchKernelGGL((head_rows_kernel<CACHE, INTER, META, 1, false>), grid, block, 0, s, a);
     }
 }
 template <int CACHE, int META>
@@ -584,8 +605,8 @@ void launch_rows_inline_i(const RopeAppend& a, const int32_t* meta, size_t n, hi
     std::copy(meta, meta + n, x.meta);
     const dim3 block(64 * kRowWaves);
     if (many(a, true)) {
-        const dim3 grid = rows_grid(x.a, true, PA_ROWS_U);
-        hipLaunchKernelGGL((head_rows_inline_kernel<CACHE, INTER, PA_ROWS_U, N>), grid, block, 0, s, x);
+        const dim3 grid = rows_grid(x.a, true, kManyU);
+        hipLaunchKernelGGL((head_rows_inline_kernel<CACHE, INTER, kManyU, N>), grid, block, 0, s, x);
     } else {
         const dim3 grid = rows_grid(x.a, true, 1);
         hipLaunchKernelGGL((head_rows_inline_kernel<CACHE, INTER, 1, N>), grid, block, 0, s, x);
@@ -611,8 +632,14 @@ template <int META>
 void launch_block(RopeAppend a, hipStream_t s) {
     int waves = 0;
     const dim3 grid = block_grid(a, waves), block(64 * waves);
-    if (a.rope.interleaved) hipLaunchKernelGGL((block_append_kernel<true, META>), grid, block, 0, s, a);
-    else hipLaunchKernelGGL((block_append_kernel<false, META>), grid, block, 0, s, a);
+    const bool nt = streams(a, true);
+    if (a.rope.interleaved) {
+        if (nt) hipLaunchKernelGGL((block_append_kernel<true, META, true>), grid, block, 0, s, a);
+        else hipLaunchKernelGGL((block_append_kernel<true, META, false>), grid, block, 0, s, a);
+    } else {
+        if (nt) hipLaunchKernelGGL((block_append_kernel<false, META, true>), grid, block, 0, s, a);
+        else hipLaunchKernelGGL((block_append_kernel<false, META, false>), grid, block, 0, s, a);
+    }
 }
 template <int N>
 void launch_block_inline(const RopeAppend& a, const int32_t* meta, size_t n, hipStream_t s) {
