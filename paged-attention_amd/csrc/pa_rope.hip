@@ -374,14 +374,18 @@ __device__ __forceinline__ float wave_max(float x) {
 // each of the kv heads from h0 on. Unit u counts blocks as the launch does:
 // entry e's i-th block is unit tok_begin[e] / B + 2 e + i. (An entry of n tokens
 // touches at most n / B + 2 blocks, so units of different entries never meet,
-// whatever its start, which the host need not know.)
+// whatever its start, which the host need not know.) Where that makes more units
+// than tokens, as in a decode step, a unit is a token, and the first of a block takes it.
 //
 // A wave holds the block's 16 rows of a head as they came (four a load, as in the
 // rows kernel), norms and turns them once for their largest magnitude and, with the
 // scale that it asks for, once more for the codes: 160 more instructions a wave, but
-// half the registers, and so twice the waves, of holding the results. The codes of
-// earlier rows and their scale are loaded beside the new rows, so that a scale that
-// grows costs no further trip to memory. Keys and values go in blocks of their own.
+// half the registers, and so twice the waves, of holding the results (8 x 4096
+// tokens 166 us with keys and values in one wave and 145 registers, 150 with values
+// worked out twice and 112, 138.5 with 89 for one head a wave). The codes of
+// earlier rows and their scale are loaded beside the new rows: a scale grows in some
+// 2% of a decode step's blocks, so in nearly every step, and would cost it a further
+// trip to memory (where none grows the loads cost 0.1 us at 64 sequences, 0.5 at 512).
 template <bool INTER, int META, bool V, bool NT>
 __device__ __forceinline__ void append_block(const RopeAppend& a, const int32_t* meta, int u, int h0, int waves,
                                              Turn (*tab)[kPairs]) {
@@ -390,14 +394,18 @@ __device__ __forceinline__ void append_block(const RopeAppend& a, const int32_t*
     const int B = a.block_tokens, P = a.page_size, hkv = a.k.heads;
     const int32_t* tok_begin = META == kMetaList ? meta : a.tok_begin;
     const int32_t* start     = META == kMetaList ? meta + a.n_ent : a.start;
+    const bool by_token = a.units == a.n_tok;
+    const int  div = by_token ? 1 : B, plus = by_token ? 0 : 2;
     const int guess = static_cast<int>((static_cast<int64_t>(u) * a.n_ent + a.units / 2) / a.units);
     const int e = entry_of(
-        u, a.n_ent, guess, [&](int i) { return load_uniform(tok_begin, i) / B + 2 * i; },
-        [&](int i) { return tok_begin[i] / B + 2 * i; });
+        u, a.n_ent, guess, [&](int i) { return load_uniform(tok_begin, i) / div + plus * i; },
+        [&](int i) { return tok_begin[i] / div + plus * i; });
     const int t0 = load_uniform(tok_begin, e), st = load_uniform(start, e);
     const int t1 = META == kMetaList && e + 1 == a.n_ent ? a.n_tok : min(load_uniform(tok_begin, e + 1), a.n_tok);
     if (st < 0 || t0 < 0 || t1 <= t0 || st > INT_MAX - (t1 - t0) - B) return;
-    const int blk = st / B + (u - (t0 / B + 2 * e));   // block of the sequence
+    // Block of the sequence. (One that an earlier token of the entry lies in has its unit there.)
+    if (by_token && u > t0 && (st + (u - t0)) % B != 0) return;
+    const int blk = by_token ? (st + (u - t0)) / B : st / B + (u - (t0 / B + 2 * e));
     const int lo = max(st, blk * B), hi = min(st + (t1 - t0), (blk + 1) * B);
     if (lo >= hi) return;
     const int s_lo = lo - blk * B, s_hi = hi - blk * B;
@@ -622,7 +630,7 @@ void launch_rows_inline(const RopeAppend& a, const int32_t* meta, size_t n, hipS
 dim3 block_grid(RopeAppend& a, int& waves) {
     waves = std::min(a.k.heads, kBlockWaves);
     a.block_tokens = block_tokens(a.page_size);
-    a.units       = a.n_tok / a.block_tokens + 2 * a.n_ent;
+    a.units       = std::min(a.n_tok / a.block_tokens + 2 * a.n_ent, a.n_tok);
     a.head_groups = (a.k.heads + waves - 1) / waves;
     a.parts_q = (groups(a.q.heads) + kBlockQ - 1) / kBlockQ;
     const long q = static_cast<long>(a.n_tok) * a.parts_q;

@@ -13,6 +13,7 @@
 
 #include <torch/extension.h>
 
+#include <ATen/hip/EmptyTensor.h>
 #include <c10/hip/HIPStream.h>
 
 #include <algorithm>
@@ -189,7 +190,9 @@ pa_head_rows rows_of(const char* name, const torch::Tensor& x, const OptTensor& 
         r.weight = static_cast<const float*>(weight->data_ptr());
     }
     if (out) {
-        if (!out->has_value()) *out = torch::empty({n, x.size(1), 128}, x.options());
+        // (Past the dispatcher: half of torch::empty's 0.45 us, where a small call takes 5.)
+        if (!out->has_value())
+            *out = torch::Tensor(at::detail::empty_cuda({n, x.size(1), 128}, torch::kHalf, x.device(), std::nullopt));
         TORCH_CHECK(heads_ok(**out, n) && (*out)->get_device() == device && (*out)->size(1) == x.size(1), name,
                     "_out must be a CUDA fp16 tensor of the shape of ", name, " whose heads are contiguous");
         r.out        = u16(**out);
