@@ -192,7 +192,7 @@ pa_status pa_append_rope(int dtype, const pa_append_args* p, const pa_rope* rope
         a.k = head_rows("append_rope k", k, n, false);
         check_v_rows("append_rope", p->v, p->v_stride, n);
         check_count("append_rope", n, static_cast<long long>(a.q.heads) + 2ll * k->heads + 12);
-        check_count("append_rope", p->num_entries, 64);
+        check_count("append_rope", p->num_entries, 128);
         if (n == 0) return;
         if (p->num_entries == 0) throw std::invalid_argument("append_rope: tokens of no entry");
         if (!p->tok_begin || !p->start_pos || !p->block_table || !p->k_cache || !p->v_cache)

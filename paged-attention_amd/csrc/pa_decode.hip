@@ -232,19 +232,6 @@ enum PagePath : int {
                         // lies in one page): the page by division, see PageDiv
 };
 
-// tok / page_size and what is left, without a divide: a shift for powers of
-// two (shift >= 0), else floor(tok * magic / 2^(31 + l)) with l = ceil(log2 P)
-// and magic = floor(2^(31 + l) / P) + 1, stored as shift = ~(l - 1). Exact for
-// 0 <= tok < 2^31: with r = tok mod P, tok * magic / 2^(31 + l) = tok / P + e and
-// 0 < e <= tok / 2^(31 + l) < 2^-l <= 1 / P, so adding e to r / P <= (P - 1) / P stays below 1.
-struct PageDiv {
-    int      shift;
-    uint32_t magic;
-    __device__ __forceinline__ int page(int tok) const {
-        return shift >= 0 ? tok >> shift : static_cast<int>(__umulhi(static_cast<uint32_t>(tok), magic) >> ~shift);
-    }
-};
-
 // One position of a wave's schedule: the current step of the current segment.
 // Every field is wave-uniform.
 struct Cursor {
@@ -1445,13 +1432,6 @@ hipError_t launch_split_p(const pa_decode_params& p, const PageDiv& pd, hipStrea
                            p.cta_seg_begin, p.segments, p.block_table, p.slot_ids, p.num_ctas, pd.shift,
                            p.item_seg_begin, pd.magic, p);
     return hipGetLastError();
-}
-
-PageDiv page_div(int page_size) {
-    const uint32_t P = static_cast<uint32_t>(page_size);
-    if ((P & (P - 1)) == 0) return {__builtin_ctz(P), 0u};
-    const int l = 32 - __builtin_clz(P - 1);   // ceil(log2 P), at least 2
-    return {~(l - 1), static_cast<uint32_t>((1ull << (31 + l)) / P + 1)};
 }
 
 template <int EB, int G, bool BS = false>

@@ -99,6 +99,25 @@ hipError_t launch_append_batch(int dtype, const AppendBatch& a, const int32_t* m
 // Whether an append's meta of n ints fits the kernel arguments (4 KiB in all).
 constexpr size_t kAppendInlineInts = 896;
 constexpr bool   append_meta_inline(size_t n) { return n <= kAppendInlineInts; }
+// tok / page_size and what is left, without a divide: a shift for powers of
+// two (shift >= 0), else floor(tok * magic / 2^(31 + l)) with l = ceil(log2 P)
+// and magic = floor(2^(31 + l) / P) + 1, stored as shift = ~(l - 1). Exact for
+// 0 <= tok < 2^31: with r = tok mod P, tok * magic / 2^(31 + l) = tok / P + e and
+// 0 < e <= tok / 2^(31 + l) < 2^-l <= 1 / P, so adding e to r / P <= (P - 1) / P stays below 1.
+struct PageDiv {
+    int      shift;
+    uint32_t magic;
+    __device__ __forceinline__ int page(int tok) const {
+        return shift >= 0 ? tok >> shift : static_cast<int>(__umulhi(static_cast<uint32_t>(tok), magic) >> ~shift);
+    }
+};
+inline PageDiv page_div(int page_size) {
+    const uint32_t P = static_cast<uint32_t>(page_size);
+    if ((P & (P - 1)) == 0) return {__builtin_ctz(P), 0u};
+    const int l = 32 - __builtin_clz(P - 1);   // ceil(log2 P), at least 2
+    return {~(l - 1), static_cast<uint32_t>((1ull << (31 + l)) / P + 1)};
+}
+
 // Block-scaled caches: tokens per block, the exponents that a scale may have, and
 // the largest code at the largest of them (240 * 2^8 = 61440; 448 * 2^8, and even
 // 256 * 2^8, would be past fp16, which the decode kernel widens to).
@@ -148,8 +167,13 @@ struct RopeAppend {
     uint8_t*        scales;
     int             page_size;
     float           inv_k, inv_v;
-    int             block_tokens, units, head_groups;   // block-scaled caches (set by the launch)
-    int             parts, parts_q, parts_k;   // waves of a token, of its q, of its k (set by the launch)
+    // Set by the launch: block-scaled caches' units (of 2^block_shift tokens), by_token
+    // where a unit is a token; waves of a token, of its q, of its k; quotients by
+    // these, and entries per token or unit.
+    int             block_shift, units, by_token, head_groups;
+    int             parts, parts_q, parts_k;
+    PageDiv         by_page, by_parts;
+    float           ent_rate;
 };
 template <int N>
 struct RopeInline {

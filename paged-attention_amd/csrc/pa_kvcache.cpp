@@ -429,7 +429,7 @@ pa_status pa_cache_append_rope(pa_cache* c, const int32_t* slots, const int32_t*
         long n_tok = 0;
         for (int i = 0; i < n && counts; ++i) n_tok += counts[i] > 0 ? counts[i] : 0;
         const long heads = 2l * k->heads + (q && q->heads > 0 ? q->heads : 0) + 12;
-        if (n_tok * heads * (pa::kHeadDim / 8) > INT_MAX || n > INT_MAX / (64 * 16))
+        if (n_tok * heads * (pa::kHeadDim / 8) > INT_MAX || n > INT_MAX / (128 * 16))
             throw std::length_error("append_rope: too many tokens");
         const int nt = static_cast<int>(n_tok);
         pa::RopeAppend a{};

@@ -205,11 +205,11 @@ template <int META>
 __device__ __forceinline__ int page_of(const RopeAppend& a, const int32_t* meta, int e, int pos) {
     if constexpr (META == kMetaList) {
         const int first = load_uniform(meta + a.n_ent, e);
-        return load_uniform(meta + 3 * a.n_ent, load_uniform(meta + 2 * a.n_ent, e) + pos / a.page_size -
-                                                    first / a.page_size);
+        return load_uniform(meta + 3 * a.n_ent, load_uniform(meta + 2 * a.n_ent, e) + a.by_page.page(pos) -
+                                                    a.by_page.page(first));
     } else {
         const int row = a.slot_ids ? load_uniform(a.slot_ids, e) : e;
-        const int i   = pos / a.page_size;
+        const int i   = a.by_page.page(pos);   // below 0: refused with the place
         if (pos < 0 || row < 0 || row >= a.table_rows || i >= a.table_stride) return -1;
         const int page = load_uniform(a.table + static_cast<size_t>(row) * a.table_stride, i);
         return page < a.num_pages ? page : -1;
@@ -220,7 +220,7 @@ template <int META>
 __device__ __forceinline__ Place place_of(const RopeAppend& a, const int32_t* meta, int t) {
     const int32_t* tok_begin = META == kMetaList ? meta : a.tok_begin;
     const int32_t* start     = META == kMetaList ? meta + a.n_ent : a.start;
-    const int guess = static_cast<int>(static_cast<int64_t>(t) * a.n_ent / a.n_tok);
+    const int guess = static_cast<int>(static_cast<float>(t) * a.ent_rate);
     const int e = entry_of(
         t, a.n_ent, guess, [&](int i) { return load_uniform(tok_begin, i); }, [&](int i) { return tok_begin[i]; });
     Place p;
@@ -229,7 +229,7 @@ __device__ __forceinline__ Place place_of(const RopeAppend& a, const int32_t* me
                               static_cast<uint32_t>(t - load_uniform(tok_begin, e)));   // may wrap: then out of range
     p.page = st < 0 ? -1 : page_of<META>(a, meta, e, p.pos);
     p.ok   = p.page >= 0;
-    p.slot = p.ok ? p.pos % a.page_size : 0;
+    p.slot = p.ok ? p.pos - a.by_page.page(p.pos) * a.page_size : 0;
     return p;
 }
 
@@ -326,7 +326,7 @@ __device__ __forceinline__ void head_rows_body(const RopeAppend& a, const int32_
     __shared__ __attribute__((aligned(16))) Turn tab[kRowWaves][kPairs];
     const int wave = __builtin_amdgcn_readfirstlane(threadIdx.x >> 6);
     const int w    = blockIdx.x * kRowWaves + wave;
-    const int t    = static_cast<int>(static_cast<unsigned>(w) / static_cast<unsigned>(a.parts));
+    const int t    = a.by_parts.page(w);
     if constexpr (META == kMetaList)
         write_tables(a, meta, blockIdx.x * blockDim.x + threadIdx.x, gridDim.x * blockDim.x);
     if (t >= a.n_tok) return;
@@ -391,21 +391,21 @@ __device__ __forceinline__ void append_block(const RopeAppend& a, const int32_t*
                                              Turn (*tab)[kPairs]) {
     const int lane = threadIdx.x & 63, c = lane % kLanes, r = lane / kLanes;
     const int h = h0 + __builtin_amdgcn_readfirstlane(threadIdx.x >> 6);
-    const int B = a.block_tokens, P = a.page_size, hkv = a.k.heads;
+    const int sh = a.block_shift, B = 1 << sh, P = a.page_size, hkv = a.k.heads;
     const int32_t* tok_begin = META == kMetaList ? meta : a.tok_begin;
     const int32_t* start     = META == kMetaList ? meta + a.n_ent : a.start;
-    const bool by_token = a.units == a.n_tok;
-    const int  div = by_token ? 1 : B, plus = by_token ? 0 : 2;
-    const int guess = static_cast<int>((static_cast<int64_t>(u) * a.n_ent + a.units / 2) / a.units);
+    const bool by_token = a.by_token != 0;
+    const int  div = by_token ? 0 : sh, plus = by_token ? 0 : 2;
+    const int  guess = static_cast<int>(fmaf(static_cast<float>(u), a.ent_rate, 0.5f));
     const int e = entry_of(
-        u, a.n_ent, guess, [&](int i) { return load_uniform(tok_begin, i) / div + plus * i; },
-        [&](int i) { return tok_begin[i] / div + plus * i; });
+        u, a.n_ent, guess, [&](int i) { return (load_uniform(tok_begin, i) >> div) + plus * i; },
+        [&](int i) { return (tok_begin[i] >> div) + plus * i; });
     const int t0 = load_uniform(tok_begin, e), st = load_uniform(start, e);
     const int t1 = META == kMetaList && e + 1 == a.n_ent ? a.n_tok : min(load_uniform(tok_begin, e + 1), a.n_tok);
     if (st < 0 || t0 < 0 || t1 <= t0 || st > INT_MAX - (t1 - t0) - B) return;
     // Block of the sequence. (One that an earlier token of the entry lies in has its unit there.)
-    if (by_token && u > t0 && (st + (u - t0)) % B != 0) return;
-    const int blk = by_token ? (st + (u - t0)) / B : st / B + (u - (t0 / B + 2 * e));
+    if (by_token && u > t0 && ((st + (u - t0)) & (B - 1)) != 0) return;
+    const int blk = by_token ? (st + (u - t0)) >> sh : (st >> sh) + (u - ((t0 >> sh) + 2 * e));
     const int lo = max(st, blk * B), hi = min(st + (t1 - t0), (blk + 1) * B);
     if (lo >= hi) return;
     const int s_lo = lo - blk * B, s_hi = hi - blk * B;
@@ -427,8 +427,8 @@ __device__ __forceinline__ void append_block(const RopeAppend& a, const int32_t*
     const bool norm = !V && a.k.weight != nullptr;
     const LaneWeights w = lane_weights(V ? nullptr : a.k.weight, d);
     // The head's earlier rows (none past s_lo is read) and their scale.
-    const int b = blk * B % P / B;            // block of the page
-    uint8_t* const sc = a.scales + 2 * ((static_cast<size_t>(page) * hkv + h) * (P / B) + b) + (V ? 1 : 0);
+    const int b = (blk * B - a.by_page.page(blk * B) * P) >> sh;   // block of the page
+    uint8_t* const sc = a.scales + 2 * ((static_cast<size_t>(page) * hkv + h) * (P >> sh) + b) + (V ? 1 : 0);
     unsigned char* const rows = static_cast<unsigned char*>(V ? a.v_cache : a.k_cache) + kv_row_offset<1>(page, h, b * B, P, hkv);
     const bool earlier = s_lo > 0 && h < hkv;
     const __amdgpu_buffer_rsrc_t held = buffer_rsrc(rows, earlier ? s_lo * kHeadDim : 0);
@@ -526,15 +526,15 @@ __device__ __forceinline__ void block_append_body(const RopeAppend& a, const int
     const int blocks = a.units * a.head_groups;   // of k, and of v
     if (static_cast<int>(blockIdx.x) < 2 * blocks) {
         const bool v = static_cast<int>(blockIdx.x) >= blocks;
-        const unsigned i = blockIdx.x - (v ? blocks : 0), groups = a.head_groups;
-        const int u = static_cast<int>(i / groups), h0 = static_cast<int>(i % groups) * waves;
+        const int  i = blockIdx.x - (v ? blocks : 0);
+        const int  u = a.head_groups == 1 ? i : i / a.head_groups, h0 = (i - u * a.head_groups) * waves;
         if (v) append_block<INTER, META, true, NT>(a, meta, u, h0, waves, tab);
         else append_block<INTER, META, false, NT>(a, meta, u, h0, waves, tab);
         return;
     }
     const int wave = __builtin_amdgcn_readfirstlane(threadIdx.x >> 6);
     const int w = (blockIdx.x - 2 * blocks) * waves + wave;
-    const int t = static_cast<int>(static_cast<unsigned>(w) / static_cast<unsigned>(a.parts_q));
+    const int t = a.by_parts.page(w);
     if (t >= a.n_tok) return;
     rows_of_token<0, INTER, META, kBlockQ, NT>(a, meta, t, kRowQ, (w - t * a.parts_q) * kBlockQ, tab[wave]);
 }
@@ -575,6 +575,9 @@ dim3 rows_grid(RopeAppend& a, bool cache, int u) {
     a.parts_q = (groups(a.q.heads) + u - 1) / u;
     a.parts_k = (groups(a.k.heads) + u - 1) / u;
     a.parts   = a.parts_q + (cache ? 2 : 1) * a.parts_k;
+    a.by_page  = page_div(std::max(a.page_size, 1));
+    a.by_parts = page_div(a.parts);
+    a.ent_rate = static_cast<float>(a.n_ent) / static_cast<float>(a.n_tok);
     const long waves = static_cast<long>(a.n_tok) * a.parts;
     return dim3(static_cast<unsigned>((waves + kRowWaves - 1) / kRowWaves));
 }
@@ -629,10 +632,15 @@ void launch_rows_inline(const RopeAppend& a, const int32_t* meta, size_t n, hipS
 // Waves of a block and blocks of a block_append_kernel launch; sets a.units.
 dim3 block_grid(RopeAppend& a, int& waves) {
     waves = std::min(a.k.heads, kBlockWaves);
-    a.block_tokens = block_tokens(a.page_size);
-    a.units       = std::min(a.n_tok / a.block_tokens + 2 * a.n_ent, a.n_tok);
+    const int b   = block_tokens(a.page_size);
+    a.block_shift = b == 16 ? 4 : 3;
+    a.by_token    = a.n_tok <= a.n_tok / b + 2 * a.n_ent;
+    a.units       = a.by_token ? a.n_tok : a.n_tok / b + 2 * a.n_ent;
     a.head_groups = (a.k.heads + waves - 1) / waves;
-    a.parts_q = (groups(a.q.heads) + kBlockQ - 1) / kBlockQ;
+    a.parts_q     = (groups(a.q.heads) + kBlockQ - 1) / kBlockQ;
+    a.by_page     = page_div(a.page_size);
+    a.by_parts    = page_div(std::max(a.parts_q, 1));
+    a.ent_rate    = static_cast<float>(a.n_ent) / static_cast<float>(a.units);
     const long q = static_cast<long>(a.n_tok) * a.parts_q;
     return dim3(static_cast<unsigned>(2l * a.units * a.head_groups + (q + waves - 1) / waves));
 }
