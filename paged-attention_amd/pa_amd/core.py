@@ -375,6 +375,8 @@ class PagedKVCache:
         if k.dim() != 3 or k.size(0) != n or v.shape != k.shape or (q is not None and (q.dim() != 3 or q.size(0) != n)):
             raise ValueError("k, v and q must be [sum(counts), heads, 128]")
         dev = k.get_device()
+        if k.is_cuda and dev != torch.cuda.current_device():
+            raise ValueError("k must be on the current device (the cache's)")
         kr, vr = ops.head_rows("k", k, k_weight, eps), ops.head_rows("v", v, None, eps, device=dev)
         qr = None
         if q is not None:

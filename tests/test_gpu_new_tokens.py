@@ -573,3 +573,105 @@ def test_cache_append_rope_captured(kind):
         assert np.array_equal(bits(out), bits(want))
     cache.close()
     eager.close()
+
+
+@pytest.mark.parametrize("kind", CACHES)
+@pytest.mark.parametrize("entries,empty", [(3, False), (65, True), (200, False), (4500, True)])
+def test_append_rope_many_entries(kind, entries, empty):
+    """Entries are found among many, evenly spread or not (empty ones, one long one among single tokens)."""
+    import torch
+    rng = np.random.default_rng(entries)
+    hkv, P, rows = 1, 16, entries
+    counts = np.ones(entries, int)
+    if empty:
+        counts[rng.random(entries) < 0.5] = 0
+    counts[entries // 3] = 100
+    starts = rng.integers(0, 16, entries)
+    cols = 8
+    table = np.arange(rows * cols, dtype=np.int32)[::-1].reshape(rows, cols).copy()
+    begin = np.concatenate([[0], np.cumsum(counts)])
+    n = int(begin[-1])
+    kb, vb = normal_f16(rng, (n, hkv, D)), normal_f16(rng, (n, hkv, D))
+    eb = torch.float16 if kind == "fp16" else torch.uint8
+    k_cache, v_cache = (torch.zeros((rows * cols, hkv, P, D), dtype=eb, device="cuda") for _ in range(2))
+    scales = pa_amd.alloc_kv_scales(rows * cols, hkv, P) if kind == "block" else None
+    dev = lambda a: torch.tensor(a, dtype=torch.int32, device="cuda")   # noqa: E731
+    pa_amd.append_rope(None, half(kb), half(vb), k_cache, v_cache, to_device(table), dev(begin), dev(starts), kv_scales=scales)
+    torch.cuda.synchronize()
+    e = np.repeat(np.arange(entries), counts)
+    pos = starts[e] + np.arange(n) - begin[e]
+    page, slot = table[e, pos // P], pos % P
+    for t, b in ((k_cache, kb), (v_cache, vb)):
+        got = t.cpu()
+        if kind == "fp16":
+            host = got.view(torch.int16).numpy().view(np.uint16)
+            assert np.array_equal(host[page, :, slot], b)
+        elif kind == "fp8":
+            host = got.numpy()
+            assert np.array_equal(host[page, :, slot], nt.e4m3_encode(nt.f16(b)))
+        else:
+            host = got.numpy()
+            sc = scales.cpu().numpy()[page, :, slot // 16, 0 if t is k_cache else 1].astype(int) - 127
+            val = nt.e4m3(host[page, :, slot]) * 2.0 ** sc[..., None]
+            assert np.all(np.abs(val - nt.f16(b)) <= np.maximum(np.abs(nt.f16(b)) * 2.0 ** -4, 2.0 ** (sc[..., None] - 10.0)))
+        assert int((host != 0).any(axis=(1, 3)).sum()) == n   # one row each, no other
+
+
+@pytest.mark.parametrize("kind", CACHES)
+def test_append_rope_several_axes(binding, kind):
+    """Image tokens: three positions each, in a cache at places of its own."""
+    import torch
+    rng = np.random.default_rng(3)
+    n, hq, hkv, P, pages = 50, 4, 2, 16, 6
+    cache = Paged(rng, kind, pages, hkv, P)
+    cache.begin()
+    axis = np.repeat([0, 1, 2], [16, 24, 24])
+    rope = pa_amd.Rope(nt.freqs(128), axes=axis)
+    assert rope.num_axes == 3
+    pos = rng.integers(0, 4096, (n, 3))
+    table = rng.permutation(pages)[:4].astype(np.int32)
+    (q, k, v), (qb, kb, vb) = make_heads(rng, n, (hq, hkv, hkv), True)
+    dev = lambda a: torch.tensor(a, dtype=torch.int32, device="cuda")   # noqa: E731
+    args = (to_device(table[None]), dev([0, n]), dev([7]), rope)
+    with pytest.raises(ValueError, match="axes"):
+        pa_amd.append_rope(q, k, v, *cache.dev, *args, **cache.args())
+    qo = pa_amd.append_rope(q, k, v, *cache.dev, *args, positions=dev(pos), **cache.args())
+    ref, mag = nt.norm_rotate(nt.f16(kb), None, 0, pos, nt.freqs(128), axis)
+    cache.append(ref, mag, vb, 7, table)
+    cache.check()
+    check_rows(bits(qo), *nt.norm_rotate(nt.f16(qb), None, 0, pos, nt.freqs(128), axis))
+
+
+@pytest.mark.parametrize("kind", CACHES)
+def test_append_rope_past_4_gib(kind):
+    """Pages whose offsets pass 32 bits, in bytes and in elements."""
+    import torch
+    rng = np.random.default_rng(4)
+    hkv, P = 8, 128
+    eb = 2 if kind == "fp16" else 1
+    pages = (5 << 30) // (hkv * P * D * eb)
+    dt = torch.float16 if kind == "fp16" else torch.uint8
+    k_cache, v_cache = (torch.empty((pages, hkv, P, D), dtype=dt, device="cuda") for _ in range(2))
+    scales = pa_amd.alloc_kv_scales(pages, hkv, P) if kind == "block" else None
+    table = torch.tensor([[pages - 1, 0, pages - 2]], dtype=torch.int32, device="cuda")
+    n = 2 * P + 9
+    kb, vb = normal_f16(rng, (n, hkv, D)), normal_f16(rng, (n, hkv, D))
+    dev = lambda a: torch.tensor(a, dtype=torch.int32, device="cuda")   # noqa: E731
+    pa_amd.append_rope(None, half(kb), half(vb), k_cache, v_cache, table, dev([0, n]), dev([0]), kv_scales=scales)
+    d = pa_amd.Decoder(8, hkv, D, P, kind != "fp16", **(dict(block_scales=True) if kind == "block" else {}))
+    lens = torch.tensor([n], dtype=torch.int32)
+    d.plan(lens)
+    qb = normal_f16(rng, (1, 8, D))
+    out = d.run(half(qb), k_cache, v_cache, table, lens.cuda(), 1.0, 1.0, **(dict(kv_scales=scales) if kind == "block" else {}))
+    torch.cuda.synchronize()
+    pg = np.array([pages - 1, 0, pages - 2])
+    held = [t[torch.from_numpy(pg).cuda()].cpu() for t in (k_cache, v_cache)]
+    sc = None if scales is None else scales[torch.from_numpy(pg).cuda()].cpu().numpy()
+    pools = [t.view(torch.int16).numpy().view(np.uint16) if kind == "fp16" else t.numpy() for t in held]
+    k, v = stored(pools, sc, [0, 1, 2], n, P, 1.0)
+    for got, b in ((k, kb), (v, vb)):
+        want = nt.f16(b)
+        tol = 0 if kind == "fp16" else np.abs(want) * 2.0 ** -4 + 2.0 ** -10
+        assert np.all(np.abs(got - want) <= tol)
+    ref, weight, big = nt.attention(nt.f16(qb[0]), k, v)
+    assert np.all(np.abs(out[0].double().cpu().numpy() - ref) <= nt.attention_tol(ref, weight, big))
