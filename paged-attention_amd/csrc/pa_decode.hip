@@ -728,12 +728,13 @@ __device__ __forceinline__ void decode_split_body(const pa_decode_params& p, con
         }
     };
 
-    // The word with the K and V scale bytes of the block that holds slot `slot`
-    // of a page (wave-uniform): a scalar load beside the block's rows, used a
-    // step later. (The pair is 2-byte aligned; the aligned word around it ends
-    // inside the array's last 4 bytes.)
-    auto load_scales = [&](int s, int hh, int n, int page, int slot) {
-        const int idx = (page * hkv + L.h) * (P >> sc_shift) + (slot >> sc_shift);
+    // The word with the K and V scale bytes of the block that holds the row at
+    // byte row0 of a pool (wave-uniform; blocks are counted as their rows are): a
+    // scalar load beside the block's rows, used a step later. (The pair is 2-byte
+    // aligned; the aligned word around it ends inside the array's last 4 bytes.)
+    auto load_scales = [&](int s, int hh, int n, size_t row0) {
+        static_assert(!BS || ROW == 128, "a row's bytes are 2^7");
+        const int idx = static_cast<int>(row0 >> (7 + sc_shift));
         scw[s][hh][n] = load_uniform(reinterpret_cast<const int32_t*>(p.kv_scales), idx >> 1);
         scs[s][hh][n] = 16 * (idx & 1);
     };
@@ -773,7 +774,7 @@ __device__ __forceinline__ void decode_split_body(const pa_decode_params& p, con
                 const int nv = __builtin_amdgcn_readfirstlane(l_more ? max(0, min(16, L.w - t)) : 0);
                 const size_t row0 = static_cast<size_t>(__builtin_amdgcn_readfirstlane(pg[s][hh])) * page_bytes +
                                     static_cast<uint32_t>((L.h * P + (bt & (P - 1))) * ROW);
-                if constexpr (BS) load_scales(s, hh, 0, pg[s][hh], bt & (P - 1));
+                if constexpr (BS) load_scales(s, hh, 0, row0);
                 const __amdgpu_buffer_rsrc_t krs = buffer_rsrc(kbase + row0, nv * ROW);
                 const __amdgpu_buffer_rsrc_t vrs = buffer_rsrc(vbase + row0, nv * ROW);
                 if constexpr (DMA) {
@@ -824,7 +825,7 @@ __device__ __forceinline__ void decode_split_body(const pa_decode_params& p, con
                     const size_t row0 =
                         static_cast<size_t>(__builtin_amdgcn_readfirstlane(pgr[s][hh][part])) * page_bytes +
                         static_cast<uint32_t>((L.h * P + part_slot(bt)) * ROW);
-                    if constexpr (BS) load_scales(s, hh, part, pgr[s][hh][part], part_slot(bt));
+                    if constexpr (BS) load_scales(s, hh, part, row0);
                     const __amdgpu_buffer_rsrc_t krs = buffer_rsrc(kbase + row0, nv * ROW);
                     const __amdgpu_buffer_rsrc_t vrs = buffer_rsrc(vbase + row0, nv * ROW);
                     if constexpr (DMA) {
