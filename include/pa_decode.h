@@ -24,6 +24,8 @@
  *   kv_scales     [num_pages][num_kv_heads][page_size / B][2] uint8, block-scaled
  *                 caches only: byte e of a block's K (0) and V (1) stands for the
  *                 scale 2^(e - 127); a block is B = pa_block_tokens(page_size) tokens
+ *                 (the decode reads whole 4-byte words, and holds V in fp16: a value
+ *                 past that, which appends never store, is infinite there)
  *   block_table   [num_slots][block_table_stride] int32 physical page ids
  *   segments      [num_segments][4] int32 = (batch row, kv head, tok_begin, tok_end)
  */
@@ -307,7 +309,9 @@ int pa_block_tokens(int page_size);
  * that every stored value is an fp16 value; infinities saturate, NaN stays). The
  * call that stores a block's first token sets its scale, later ones raise it where
  * their tokens need that, and then round the block's earlier tokens again (which
- * loses bits only of values that fall below 2^-6 of the new scale). */
+ * loses bits only of values that fall below 2^-6 of the new scale). A place that is
+ * stored again, as by a graph's replay or after a rollback, finds its block's scale
+ * as the earlier call left it unless it is the block's first. */
 typedef struct pa_append_args {
     int32_t         num_tokens;
     int32_t         num_entries;

@@ -554,20 +554,21 @@ __global__ __launch_bounds__(64 * kBlockWaves) void block_append_inline_kernel(c
 int groups(int heads) { return (heads + kRows - 1) / kRows; }
 
 // A large call's waves take up to kManyU groups of four rows (the turns are worked
-// out once a wave), a small one's one each. Same box, us, 8192 tokens of 32 + 8
-// heads at 2, 3, 4, 5, 6, 12 groups: 35.0, 34.6, 32.7, 32.9, 34.2, 38.7; 512 tokens
-// 4.4 at any of them, 1 token 2.5 at one group and 3.4 at two.
+// out once a wave), a small one's one each (more waves, shorter ones). Same box, us,
+// 8192 tokens of 32 + 8 heads at 2, 3, 4, 5, 6, 12 groups: 35.0, 34.6, 32.7, 32.9,
+// 34.2, 38.7. One group and four: 128 tokens (1280 groups) 2.7 / 3.4, 800 4.7 / 5.2,
+// 1200 6.9 / 6.3, 3200 14.8 / 12.2; into fp16 pages 256 tokens (3072 groups) 3.6 /
+// 3.8, 512 4.6 / 4.3, 1024 7.8 / 6.1.
 constexpr int  kManyU      = 4;
-constexpr long kManyGroups = 16384;
+constexpr long kManyGroups = 8192;
 
 // Whether a call's loads bypass the caches: from some 100 MB of rows on, which the
 // projection before it cannot have left in the memory-side cache (256 MB, the
 // outputs beside them), and where a load takes whole 128-byte lines, which partial
-// half-split rotations do not. us with cached and with non-temporal loads: 37
-// ragged prompts (64 of 128 dims turn, 11 000 tokens of 16 + 2 x 4 heads) 24.7 /
-// 30.2, 2048 tokens of 32 + 8 heads 7.9 / 9.8, 8192 with 96 dims turned 29.0 / 36.4,
-// 8192 tokens into FP8 pages (126 MB) 35.8 / 34.4, 32768 into block-scaled ones 145
-// / 137.
+// half-split rotations do not. us with cached and with non-temporal loads: 3200
+// tokens of 32 + 8 heads (33 MB) 12.0 / 14.0, 6400 21.7 / 25.1, 12800 (131 MB) 46.9 /
+// 45.8, 8192 of 64 + 8 (151 MB) 52.7 / 51.1, 32768 into block-scaled pages (403 MB)
+// 145 / 137; with 96 of 128 dims turned 8192 of 32 + 8 29.0 / 36.4.
 constexpr long kStreamBytes = 96l << 20;
 
 // Parts of a token at u groups a wave, and the grid.
