@@ -516,7 +516,11 @@ __device__ __forceinline__ void append_block(const RopeAppend& a, const int32_t*
 // Groups of a token's q rows that one wave takes beside the blocks.
 constexpr int kBlockQ = 4;
 
-// Blocks of the grid: the units of k, those of v, then the tokens' q rows.
+// Blocks of the grid: the units of k and v in turn (a streaming call's, which is long
+// enough to have both at once anyway, k before v), then the tokens' q rows. us with
+// k before v and in turn: 37 ragged prompts 24.1 / 22.8, 4096 tokens 18.5 / 18.3,
+// 64 single tokens 4.3 / 4.3, 8 x 4096 tokens 133.9 / 137.2; q first 24.6, 19.8, 4.5,
+// 133.4.
 template <bool INTER, int META, bool NT>
 __device__ __forceinline__ void block_append_body(const RopeAppend& a, const int32_t* meta) {
     __shared__ __attribute__((aligned(16))) Turn tab[16][kPairs];
@@ -525,8 +529,9 @@ __device__ __forceinline__ void block_append_body(const RopeAppend& a, const int
         write_tables(a, meta, blockIdx.x * blockDim.x + threadIdx.x, gridDim.x * blockDim.x);
     const int blocks = a.units * a.head_groups;   // of k, and of v
     if (static_cast<int>(blockIdx.x) < 2 * blocks) {
-        const bool v = static_cast<int>(blockIdx.x) >= blocks;
-        const int  i = blockIdx.x - (v ? blocks : 0);
+        const int  n = blockIdx.x;
+        const bool v = NT ? n >= blocks : (n & 1) != 0;
+        const int  i = NT ? n - (v ? blocks : 0) : n >> 1;
         const int  u = a.head_groups == 1 ? i : i / a.head_groups, h0 = (i - u * a.head_groups) * waves;
         if (v) append_block<INTER, META, true, NT>(a, meta, u, h0, waves, tab);
         else append_block<INTER, META, false, NT>(a, meta, u, h0, waves, tab);
