@@ -7,13 +7,23 @@
 //
 // (No counterparts in the reference, whose caches take finished K and V.)
 //
-// A head's row is 128 fp16: 16 lanes hold 8 dims each, so a wave holds four rows
-// and every load and store is 16 bytes a lane (8 for E4M3 codes). The norm's sum
-// goes over the 16 lanes by rotations within them. A token's sines and cosines are
+//   y = x w / sqrt(mean(x^2) + eps); (a, b) -> s (a cos t - b sin t, b cos t + a sin t)
+//
+// with t = position * frequency of the pair, in 32 bits, rounded once.
+//
+// A head's row is 128 fp16: 16 lanes hold 8 dims each, a wave four rows. The norm's
+// sum goes over the 16 lanes by rotations within them. A token's sines and cosines are
 // computed once per wave or block, one pair a lane, and handed out through LDS:
 // angles in 64 bits (position * frequency in half turns, less whole turns: the
 // product of a position up to 2^31 is off by 2^-22 of a turn at most), sines of
 // what is left in 32. No table of positions is read, and none limits them.
+//
+// Bound by memory from some thousand tokens on: 8192 tokens of 32 + 8 heads take 30 us
+// (168 MB, 5.6 TB/s; a copy of as many bytes 33), of which the arithmetic is half
+// (SQ_ACTIVE_INST_VALU), 8 x 4096 tokens of 32 + 2 x 8 into block-scaled pages 133
+// us (738 MB, 5.5 TB/s); below by the chain kernel arguments, entry, place, rows,
+// store: 2.4 us for one token, 3.1 for a step of 64 into fp16 pages, 4.2 into
+// block-scaled ones.
 
 #include "pa_device.hpp"
 #include "pa_fp8.hpp"
@@ -60,12 +70,26 @@ __device__ __forceinline__ float row_max(float x) {
     return fmaxf(x, rot16<0x121>(x));
 }
 
-// Pair i's sine and cosine at a token (its `positions` row, or its place).
-__device__ __forceinline__ Turn turn_of(const RopeTable& r, const int32_t* positions, int token, int place, int i) {
-    int pos = place;
-    if (positions && r.num_axes == 1) pos = positions[token];
-    else if (positions) pos = positions[static_cast<size_t>(token) * r.num_axes + r.axes[i]];
-    const double half = static_cast<double>(pos) * r.half_turns[i];
+// What turns pair i, loaded before a wave looks up its token's place: the lookup's
+// loads would otherwise be waited for first. (Into block-scaled pages: a step of 64
+// sequences 4.3 -> 4.2 us, a prompt of 333 tokens 6.7 -> 6.3.)
+struct Pair {
+    double half_turns;   // per position
+    int    axis;
+};
+__device__ __forceinline__ Pair pair_of(const RopeTable& r, int i) {
+    Pair p{0.0, 0};
+    if (i < r.pairs) {
+        p.half_turns = r.half_turns[i];
+        if (r.num_axes > 1) p.axis = r.axes[i];
+    }
+    return p;
+}
+// Its sine and cosine at a token (its `positions` row, or its place).
+__device__ __forceinline__ Turn turn_of(const RopeTable& r, const Pair& p, const int32_t* positions, int token,
+                                        int place) {
+    const int    pos  = positions ? positions[static_cast<size_t>(token) * r.num_axes + p.axis] : place;
+    const double half = static_cast<double>(pos) * p.half_turns;
     const float  x    = static_cast<float>(half - 2.0 * rint(half * 0.5));   // [-1, 1]
     Turn t;
     sincospif(x, &t.s, &t.c);
@@ -259,6 +283,7 @@ __device__ __forceinline__ void rows_of_token(const RopeAppend& a, const int32_t
     const HeadRows& rows = kind == kRowQ ? a.q : a.k;
     const int heads = rows.heads, h0 = kRows * g0;
     const LaneDims d = lane_dims<INTER>(v ? 0 : a.rope.pairs, c);
+    const Pair pair = pair_of(a.rope, v ? kPairs : lane);
     const uint16_t* in = (v ? a.v + t * a.v_stride : rows.in + t * rows.in_stride) + h0 * kHeadDim;
     const __amdgpu_buffer_rsrc_t src = buffer_rsrc(in, 2 * kHeadDim * (heads - h0));
     u32x4 x[U];
@@ -270,7 +295,7 @@ __device__ __forceinline__ void rows_of_token(const RopeAppend& a, const int32_t
     const LaneWeights w = lane_weights(v ? nullptr : rows.weight, d);
     LaneTurns l{};
     if (!v && a.rope.pairs) {
-        if (lane < a.rope.pairs) tab[lane] = turn_of(a.rope, a.positions, t, p.pos, lane);
+        if (lane < a.rope.pairs) tab[lane] = turn_of(a.rope, pair, a.positions, t, p.pos);
         wave_lds_sync();
         l = lane_turns(tab, c);
     }
@@ -394,6 +419,7 @@ __device__ __forceinline__ void append_block(const RopeAppend& a, const int32_t*
     const int sh = a.block_shift, B = 1 << sh, P = a.page_size, hkv = a.k.heads;
     const int32_t* tok_begin = META == kMetaList ? meta : a.tok_begin;
     const int32_t* start     = META == kMetaList ? meta + a.n_ent : a.start;
+    const Pair pair = pair_of(a.rope, V ? kPairs : lane);   // the thread's: it takes every waves-th token's
     const bool by_token = a.by_token != 0;
     const int  div = by_token ? 0 : sh, plus = by_token ? 0 : 2;
     const int  guess = static_cast<int>(fmaf(static_cast<float>(u), a.ent_rate, 0.5f));
@@ -423,6 +449,10 @@ __device__ __forceinline__ void append_block(const RopeAppend& a, const int32_t*
         x[i] = load_dims<INTER || V, NT>(src, d, off);
     }
     const int page = page_of<META>(a, meta, e, lo);
+    if (!V && a.rope.pairs) {
+        for (int s = s_lo + (threadIdx.x >> 6); s < s_hi; s += waves)
+            if (lane < a.rope.pairs) tab[s][lane] = turn_of(a.rope, pair, a.positions, tok + s - s_lo, blk * B + s);
+    }
     if (page < 0) return;
     const bool norm = !V && a.k.weight != nullptr;
     const LaneWeights w = lane_weights(V ? nullptr : a.k.weight, d);
@@ -438,14 +468,7 @@ __device__ __forceinline__ void append_block(const RopeAppend& a, const int32_t*
     for (int i = 0; i < 4; ++i)
         was[i] = __builtin_bit_cast(
             u32x2, __builtin_amdgcn_raw_buffer_load_b64(held, (r + kRows * i) * kHeadDim + kDims * c, 0, 0));
-    if (!V && a.rope.pairs) {
-        const int threads = 64 * waves;
-        for (int i = threadIdx.x; i < (s_hi - s_lo) * kPairs; i += threads) {
-            const int s = s_lo + i / kPairs, p = i % kPairs;
-            if (p < a.rope.pairs) tab[s][p] = turn_of(a.rope, a.positions, tok + s - s_lo, blk * B + s, p);
-        }
-        __syncthreads();
-    }
+    if (!V && a.rope.pairs) __syncthreads();
     if (h >= hkv) return;
     float amax = 0.f, inv_n[4];
     auto value = [&](float (&y)[kDims], int i) {   // row r + 4 i, its norm known
