@@ -264,7 +264,7 @@ int       pa_rope_axes(const pa_rope* rope);
 /* Some heads of every token: token t's head h starts at in + t * in_stride + h *
  * 128 (fp16, 16-byte aligned; strides in elements, multiples of 8 from 0 to 2^26, so
  * a fused projection's output is read where it lies). weight: 128 floats (16-byte
- * aligned) or NULL for no norm. out likewise, where the call has an output; it
+ * aligned) or NULL for no norm; eps 0 or at least 2^-126. out likewise, where the call has an output; it
  * may be `in` itself with the same stride, and overlaps nothing else the call
  * reads or writes. heads = 0: none. */
 typedef struct pa_head_rows {
@@ -296,7 +296,8 @@ int pa_block_tokens(int page_size);
  * slot_ids is NULL). Entries, places and table are device arrays that the kernel
  * reads, so a captured call follows their values from replay to replay; a token
  * whose place, row or page is out of range (num_table_rows, block_table_stride,
- * num_pages), or whose entry starts below 0, is left out (its q is not).
+ * num_pages), whose entry starts below 0, or that is in no entry (a padded batch's
+ * last ones, past tok_begin[num_entries]) is left out (its q is not).
  * Block-scaled caches: one call holds each sequence once.
  *   k   normed and rotated (positions: [num_tokens][axes]; NULL: the token's place
  *       turns every pair), then stored; its `out` is not used
@@ -315,7 +316,7 @@ int pa_block_tokens(int page_size);
 typedef struct pa_append_args {
     int32_t         num_tokens;
     int32_t         num_entries;
-    const int32_t*  tok_begin;      /* [num_entries + 1], rising from 0 to num_tokens */
+    const int32_t*  tok_begin;      /* [num_entries + 1], rising within 0 .. num_tokens */
     const int32_t*  start_pos;      /* [num_entries] */
     const int32_t*  slot_ids;       /* [num_entries] or NULL */
     const int32_t*  positions;

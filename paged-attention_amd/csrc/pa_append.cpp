@@ -4,6 +4,7 @@
 
 #include "pa_host.hpp"
 
+#include <cfloat>
 #include <climits>
 #include <cmath>
 #include <cstring>
@@ -66,7 +67,8 @@ pa::HeadRows head_rows(const char* what, const pa_head_rows* r, int n, bool has_
         if (!aligned(r->in, 16) || !stride_ok(r->in_stride))
             throw std::invalid_argument(w + "rows must be 16-byte aligned, their stride a multiple of 8 elements below 2^26");
         if (r->weight && !aligned(r->weight, 16)) throw std::invalid_argument(w + "the norm weight must be 16-byte aligned");
-        if (r->weight && !(r->eps >= 0.0f)) throw std::invalid_argument(w + "eps must not be negative");
+        if (r->weight && r->eps != 0.0f && !(r->eps >= FLT_MIN))   // (v_rsq_f32 takes subnormals for 0)
+            throw std::invalid_argument(w + "eps must be 0 or a positive normal number");
     }
     if (n > 0 && has_out) {
         if (!r->out) throw std::invalid_argument(w + "null output");
@@ -203,6 +205,11 @@ pa_status pa_append_rope(int dtype, const pa_append_args* p, const pa_rope* rope
             throw std::invalid_argument("append_rope: a block-scaled cache needs kv_scales (2-byte aligned)");
         if (rope && rope->num_axes > 1 && !p->positions)
             throw std::invalid_argument("append_rope: a rotation over several axes needs positions");
+        const bool fp8 = dtype == PA_KV_FP8_E4M3;
+        a.inv_k        = fp8 ? 1.0f / p->k_scale : 1.0f;
+        a.inv_v        = fp8 ? 1.0f / p->v_scale : 1.0f;
+        if (!std::isfinite(a.inv_k) || !std::isfinite(a.inv_v) || a.inv_k == 0.0f || a.inv_v == 0.0f)
+            throw std::invalid_argument("append_rope: k_scale and v_scale must have finite reciprocals");
         a.rope         = rope_table(rope);
         a.v            = p->v;
         a.v_stride     = static_cast<long>(p->v_stride);
@@ -220,9 +227,6 @@ pa_status pa_append_rope(int dtype, const pa_append_args* p, const pa_rope* rope
         a.v_cache      = p->v_cache;
         a.scales       = p->kv_scales;
         a.page_size    = p->page_size;
-        const bool fp8 = dtype == PA_KV_FP8_E4M3;
-        a.inv_k        = fp8 ? 1.0f / p->k_scale : 1.0f;
-        a.inv_v        = fp8 ? 1.0f / p->v_scale : 1.0f;
         pa::hip_check(pa::launch_append_rope(dtype, a, nullptr, 0, as_stream(stream)), "append_rope kernel launch");
     });
 }

@@ -248,10 +248,11 @@ __device__ __forceinline__ Place place_of(const RopeAppend& a, const int32_t* me
     const int e = entry_of(
         t, a.n_ent, guess, [&](int i) { return load_uniform(tok_begin, i); }, [&](int i) { return tok_begin[i]; });
     Place p;
-    const int st = load_uniform(start, e);
-    p.pos  = static_cast<int>(static_cast<uint32_t>(st) +
-                              static_cast<uint32_t>(t - load_uniform(tok_begin, e)));   // may wrap: then out of range
-    p.page = st < 0 ? -1 : page_of<META>(a, meta, e, p.pos);
+    const int st = load_uniform(start, e), t0 = load_uniform(tok_begin, e);
+    p.pos = static_cast<int>(static_cast<uint32_t>(st) + static_cast<uint32_t>(t - t0));   // may wrap: then out of range
+    // A caller's arrays may leave tokens out on both sides (a padded batch's).
+    const bool none = META == kMetaTable && (st < 0 || t < t0 || t >= load_uniform(tok_begin, e + 1));
+    p.page = none ? -1 : page_of<META>(a, meta, e, p.pos);
     p.ok   = p.page >= 0;
     p.slot = p.ok ? p.pos - a.by_page.page(p.pos) * a.page_size : 0;
     return p;
@@ -429,6 +430,7 @@ __device__ __forceinline__ void append_block(const RopeAppend& a, const int32_t*
     const int t0 = load_uniform(tok_begin, e), st = load_uniform(start, e);
     const int t1 = META == kMetaList && e + 1 == a.n_ent ? a.n_tok : min(load_uniform(tok_begin, e + 1), a.n_tok);
     if (st < 0 || t0 < 0 || t1 <= t0 || st > INT_MAX - (t1 - t0) - B) return;
+    if (u < (t0 >> div) + plus * e) return;   // a token before the first entry
     // Block of the sequence. (One that an earlier token of the entry lies in has its unit there.)
     if (by_token && u > t0 && ((st + (u - t0)) & (B - 1)) != 0) return;
     const int blk = by_token ? (st + (u - t0)) >> sh : (st >> sh) + (u - ((t0 >> sh) + 2 * e));
@@ -585,8 +587,8 @@ int groups(int heads) { return (heads + kRows - 1) / kRows; }
 // out once a wave), a small one's one each (more waves, shorter ones). Same box, us,
 // 8192 tokens of 32 + 8 heads at 2, 3, 4, 5, 6, 12 groups: 35.0, 34.6, 32.7, 32.9,
 // 34.2, 38.7. One group and four: 128 tokens (1280 groups) 2.7 / 3.4, 800 4.7 / 5.2,
-// 1200 6.9 / 6.3, 3200 14.8 / 12.2; into fp16 pages 256 tokens (3072 groups) 3.6 /
-// 3.8, 512 4.6 / 4.3, 1024 7.8 / 6.1.
+// 1200 6.9 / 6.3, 3200 14.8 / 12.2; into fp16 pages 256 tokens 3.6 / 3.8, 512
+// (6144 groups) 4.6 / 4.3, 1024 7.8 / 6.1.
 constexpr int  kManyU      = 4;
 constexpr long kManyGroups = 8192;
 

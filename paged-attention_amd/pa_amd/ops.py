@@ -129,6 +129,7 @@ def norm_rope(q, k, positions, rope: Rope | None = None, *, q_weight=None, k_wei
     x = q if q is not None else k
     _require(x.is_cuda and x.dim() == 3, "q and k must be CUDA fp16 [tokens, heads, 128] tensors")
     n, dev = x.size(0), x.get_device()
+    _require(n < 2**31, "too many tokens")
     rows = []
     for name, t, w, out in (("q", q, q_weight, q_out), ("k", k, k_weight, k_out)):
         if t is None:
@@ -156,7 +157,7 @@ def append_rope(q, k, v, k_cache, v_cache, block_table, tok_begin, start_pos, ro
     what the rotation takes in place of the tokens' places ([n] or [n, axes]). Caches: fp16, or
     one-byte FP8 with k_scale / v_scale (a code c stands for c * scale), or with kv_scales (alloc_kv_scales)
     block-scaled, where one call holds each sequence once. Tokens whose place, row or page is
-    out of range are left out. Returns q_out (None without q)."""
+    out of range, or that are in no entry (padding), are left out. Returns q_out (None without q)."""
     c = compiled()
     if c is not None:
         return c.append_rope(q, k, v, k_cache, v_cache, block_table, tok_begin, start_pos,
@@ -164,6 +165,7 @@ def append_rope(q, k, v, k_cache, v_cache, block_table, tok_begin, start_pos, ro
                              kv_scales, slot_ids, q_out)
     _require(k.is_cuda and k.dim() == 3, "k must be a CUDA fp16 [tokens, heads, 128] tensor")
     n, dev, hkv = k.size(0), k.get_device(), k.size(1)
+    _require(n < 2**31, "too many tokens")
     qr = None
     if q is not None:
         _require(q.dim() == 3 and q.size(0) == n, "q must be a CUDA fp16 [tokens, heads, 128] tensor whose heads are contiguous")

@@ -302,3 +302,52 @@ def test_block_cache_on_another_stream():
         assert np.abs(rows[0][0] - ref).max() < np.abs(ref).max() * 2.0 ** -4
         cache.release(s)
     cache.close()
+
+
+def test_step_replayed_over_a_caller_s_cache():
+    """Append and attention of one step in a graph, over pools of the caller's: every replay stores the tokens then in
+    k and v and attends with the q then there; eager steps on a cache of their own between the replays."""
+    import torch
+    rng = np.random.default_rng(51)
+    hq, hkv, P, pages, m = 8, 2, 16, 12, 3
+    lens = [17, 5, 40]                                 # with the step's token
+    table = rng.permutation(pages).astype(np.int32).reshape(m, 4)[:, :3].copy()
+    rope = pa_amd.Rope(nt.freqs(128))
+    dt = to_device(table)
+    begin, starts = dev(list(range(m + 1))), dev([n - 1 for n in lens])
+    lt = torch.tensor(lens, dtype=torch.int32)
+    lens_dev = lt.cuda()
+
+    def fresh():
+        k_cache, v_cache = (torch.zeros((pages, hkv, P, D), dtype=torch.uint8, device="cuda") for _ in range(2))
+        return k_cache, v_cache, pa_amd.alloc_kv_scales(pages, hkv, P)
+
+    (pk, pv), _ = make_heads(rng, sum(lens) - m, (hkv, hkv), False)
+    caches = [fresh(), fresh()]
+    for c in caches:
+        pa_amd.append_rope(None, pk, pv, c[0], c[1], dt, dev(np.concatenate([[0], np.cumsum([n - 1 for n in lens])])),
+                           dev([0] * m), rope, kv_scales=c[2])
+    d = pa_amd.Decoder(hq, hkv, D, P, True, block_scales=True)
+    d.plan(lt)
+    (q, k, v), _ = make_heads(rng, m, (hq, hkv, hkv), False)
+
+    def step(c, q, k, v):
+        qo = pa_amd.append_rope(q, k, v, c[0], c[1], dt, begin, starts, rope, kv_scales=c[2])
+        return d.run(qo, c[0], c[1], dt, lens_dev, 1.0, 1.0, kv_scales=c[2])
+
+    step(caches[1], q, k, v)
+    torch.cuda.synchronize()
+    graph = torch.cuda.CUDAGraph()
+    with torch.cuda.graph(graph):
+        out = step(caches[0], q, k, v)
+    step(caches[0], q, k, v)   # what the eager cache has seen
+    for _ in range(4):
+        (q2, k2, v2), _ = make_heads(rng, m, (hq, hkv, hkv), False)
+        q.copy_(q2), k.copy_(k2), v.copy_(v2)
+        graph.replay()
+        torch.cuda.synchronize()
+        want = step(caches[1], q2, k2, v2)
+        torch.cuda.synchronize()
+        assert torch.equal(out, want) and torch.isfinite(out).all()
+        for a, b in zip(*caches):
+            assert torch.equal(a, b)

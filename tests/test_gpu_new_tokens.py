@@ -675,3 +675,51 @@ def test_append_rope_past_4_gib(kind):
         assert np.all(np.abs(got - want) <= tol)
     ref, weight, big = nt.attention(nt.f16(qb[0]), k, v)
     assert np.all(np.abs(out[0].double().cpu().numpy() - ref) <= nt.attention_tol(ref, weight, big))
+
+
+@pytest.mark.parametrize("kind", CACHES)
+@pytest.mark.parametrize("lead,tail", [(0, 7), (5, 0), (3, 40)])
+def test_append_rope_padded(kind, lead, tail):
+    """Tokens before the first entry and after the last are in none: left out, their q is not."""
+    import torch
+    rng = np.random.default_rng(lead + tail)
+    hq, hkv, P, pages = 4, 2, 16, 8
+    cache = Paged(rng, kind, pages, hkv, P)
+    cache.begin()
+    counts, starts = [1, 20, 1], [13, 15, 0]
+    begin = lead + np.concatenate([[0], np.cumsum(counts)])
+    n = int(begin[-1]) + tail
+    table = np.array([[0, 1, 2], [3, 4, 5], [6, 7, 7]], np.int32)
+    (q, k, v), (qb, kb, vb) = make_heads(rng, n, (hq, hkv, hkv), True)
+    dev = lambda a: torch.tensor(a, dtype=torch.int32, device="cuda")   # noqa: E731
+    qo = pa_amd.append_rope(q, k, v, *cache.dev, to_device(table), dev(begin), dev(starts), **cache.args())
+    for e, (c, s) in enumerate(zip(counts, starts)):
+        part = slice(begin[e], begin[e] + c)
+        cache.append(nt.f16(kb[part]), np.abs(nt.f16(kb[part])), vb[part], s, table[e])
+    cache.check()
+    assert np.array_equal(bits(qo), qb)
+
+
+def test_norm_rope_replayed():
+    """Captured, every replay turns what is then in q, k and positions, beside eager calls on the same Rope."""
+    import torch
+    rng = np.random.default_rng(6)
+    rope = pa_amd.Rope(nt.freqs(128))
+    (q, k), _ = make_heads(rng, 9, (8, 2), False)
+    pos = torch.zeros(9, dtype=torch.int32, device="cuda")
+    w, wf = weights(rng, True)
+    pa_amd.norm_rope(q, k, pos, rope)
+    torch.cuda.synchronize()
+    graph = torch.cuda.CUDAGraph()
+    with torch.cuda.graph(graph):
+        qo, ko = pa_amd.norm_rope(q, k, pos, rope, q_weight=w, k_weight=w)
+    for step in range(4):
+        (q2, k2), (qb, kb) = make_heads(rng, 9, (8, 2), False)
+        p = rng.integers(0, 9999, 9)
+        q.copy_(q2), k.copy_(k2), pos.copy_(torch.from_numpy(p.astype(np.int32)))
+        graph.replay()
+        eager = pa_amd.norm_rope(q2, k2, pos, rope, q_weight=w, k_weight=w)
+        torch.cuda.synchronize()
+        for got, same, b in ((qo, eager[0], qb), (ko, eager[1], kb)):
+            assert np.array_equal(bits(got), bits(same))
+            check_rows(bits(got), *nt.norm_rotate(nt.f16(b), wf, float(np.float32(1e-6)), p, nt.freqs(128)))

@@ -55,6 +55,7 @@ def test_bytes_per_page_counts_the_scales():
     (dict(out=None), "null output"), (dict(out=A + (1 << 19) + 4), "aligned"), (dict(out_stride=1020), "aligned"),
     (dict(out_stride=512), "rows overlap"), (dict(out_stride=0), "rows overlap"),
     (dict(weight=A + 4), "weight"), (dict(weight=A, eps=-1.0), "eps"), (dict(weight=A, eps=float("nan")), "eps"),
+    (dict(weight=A, eps=1e-39), "eps"),
     (dict(heads=-1), "negative"), (dict(out=A + 1024), "overlaps"), (dict(out=A - 2048), "overlaps"),
     (dict(out=A, out_stride=2048), "overlaps"),
 ])
@@ -132,6 +133,8 @@ def test_append_rope_refuses_rows_and_types():
     assert append(k=rows(in_=A + 2)) == BAD and append(q=rows(out=None)) == BAD
     assert append(num_tokens=2**31 // (16 * 24)) == LONG
     assert append(num_tokens=0) == _lib.PA_OK and append(num_entries=0) == BAD
+    for bad in (dict(k_scale=0.0), dict(v_scale=float("nan")), dict(k_scale=float("inf"))):
+        assert append(dtype=pa_amd.FP8_E4M3, **bad) == BAD and "scale" in message()
     lib, k = _lib.load(), rows()
     assert lib.pa_append_rope(0, None, None, None, ctypes.byref(k), None) == BAD
     assert lib.pa_cache_append_rope(None, None, None, 0, None, None, None, ctypes.byref(k), A, 1024, None, None) == BAD
