@@ -328,7 +328,9 @@ __device__ __forceinline__ void rows_of_token(const RopeAppend& a, const int32_t
 #pragma unroll
         for (int j = 0; j < U; ++j) {
             if (h0 + kRows * j >= heads) break;
-            const int off = (kRows * j + r) * head_bytes + slot;
+            // (A row without a head goes past the end by name: its offset may reach 2^32.)
+            const int row = kRows * j + r;
+            const int off = h0 + row < heads ? row * head_bytes + slot : INT_MIN;
             float y[kDims];
             widen(y, x[j]);
             finish(y);
