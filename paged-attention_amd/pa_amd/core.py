@@ -10,6 +10,7 @@ runs the HIP kernels of libpa_decode.so on the given (default: current) stream.
 
 from __future__ import annotations
 
+import contextlib
 import ctypes
 from dataclasses import dataclass
 
@@ -48,6 +49,15 @@ def _stream(stream) -> int | None:
     if isinstance(stream, int):
         return stream
     return stream.cuda_stream
+
+
+def _allocating_on(raw: int | None):
+    """What torch allocates in this context belongs to the stream of this handle: a block that an earlier tensor of
+    another stream left is not handed out while that stream may still use it."""
+    import torch
+    if raw == _stream(None):
+        return contextlib.nullcontext()
+    return torch.cuda.stream(torch.cuda.ExternalStream(raw) if raw else torch.cuda.default_stream())
 
 
 def kv_dtype_bytes(dtype: int) -> int:
@@ -364,7 +374,7 @@ class PagedKVCache:
         tokens may be strided): k normed (k_weight) and rotated (rope) on its way into the pages,
         v as it is, and q normed and rotated beside them. The rotation takes the tokens' places, or
         positions ([tokens] or [tokens, axes]). Returns False when the pool lacks pages (nothing
-        changed), else True, or q_out where q is given."""
+        changed), else True, or q_out where q is given (a new one is allocated on `stream`)."""
         from . import ops
         import torch
         slots = np.ascontiguousarray(slots, dtype=np.int32)
@@ -378,14 +388,16 @@ class PagedKVCache:
         if k.is_cuda and dev != torch.cuda.current_device():
             raise ValueError("k must be on the current device (the cache's)")
         kr, vr = ops.head_rows("k", k, k_weight, eps), ops.head_rows("v", v, None, eps, device=dev)
-        qr = None
+        qr, raw = None, _stream(stream)
         if q is not None:
-            q_out = torch.empty((n, q.size(1), ops.D), dtype=torch.float16, device=q.device) if q_out is None else q_out
+            if q_out is None:
+                with _allocating_on(raw):
+                    q_out = torch.empty((n, q.size(1), ops.D), dtype=torch.float16, device=q.device)
             qr = ctypes.byref(ops.head_rows("q", q, q_weight, eps, q_out, dev))
         pos = ops.positions_ptr(positions, rope, n, dev)
         done = ctypes.c_int(0)
         call("pa_cache_append_rope", self._h, slots.ctypes.data, counts.ctypes.data, slots.size,
-             None if rope is None else rope.handle, pos, qr, ctypes.byref(kr), vr.in_, vr.in_stride, _stream(stream),
+             None if rope is None else rope.handle, pos, qr, ctypes.byref(kr), vr.in_, vr.in_stride, raw,
              ctypes.byref(done))
         return (q_out if q is not None else True) if done.value else False
 
