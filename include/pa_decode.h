@@ -266,7 +266,8 @@ int       pa_rope_axes(const pa_rope* rope);
  * a fused projection's output is read where it lies). weight: 128 floats (16-byte
  * aligned) or NULL for no norm; eps 0 or at least 2^-126. out likewise, where the call has an output; it
  * may be `in` itself with the same stride, and overlaps nothing else the call
- * reads or writes. heads = 0: none. */
+ * reads or writes (other rows are refused; rows that lie between each other, as
+ * the columns of one buffer do, do not overlap). heads = 0: none. */
 typedef struct pa_head_rows {
     const uint16_t* in;
     int64_t         in_stride;

@@ -4,6 +4,7 @@
 
 #include "pa_host.hpp"
 
+#include <algorithm>
 #include <cfloat>
 #include <climits>
 #include <cmath>
@@ -26,14 +27,37 @@ void check_count(const char* what, long long n, long long heads) {
 // Elements from one token to the next.
 bool stride_ok(int64_t s) { return s >= 0 && s < (1 << 26) && s % 8 == 0; }
 
-// First and last byte (exclusive) of n strided rows of `heads` heads.
-struct Span {
-    uintptr_t lo, hi;
+// n rows of some heads, `step` bytes apart.
+struct Rows {
+    int64_t base, step, bytes;
 };
-Span span_of(const uint16_t* p, long long stride, int n, int heads) {
-    const auto base = reinterpret_cast<uintptr_t>(p);
-    return {base, base + 2 * (static_cast<uintptr_t>(n - 1) * static_cast<uintptr_t>(stride) +
-                              static_cast<uintptr_t>(heads) * pa::kHeadDim)};
+Rows rows_at(const uint16_t* p, long long stride, int heads) {
+    return {static_cast<int64_t>(reinterpret_cast<uintptr_t>(p)), 2 * stride, 2ll * heads * pa::kHeadDim};
+}
+int64_t floor_div(int64_t a, int64_t b) { return a / b - (a % b < 0); }   // b > 0
+
+// Whether any of a's n rows shares a byte with any of b's. (Columns of one buffer
+// lie between each other and do not.) Rows of one stride: whether a row's distance
+// from some row of the other, which moves by that stride, falls inside it; else
+// row by row, which only rows of different strides that lie among each other need.
+bool meet(const Rows& a, const Rows& b, int n) {
+    const int64_t last = n - 1;
+    if (a.base >= b.base + last * b.step + b.bytes || b.base >= a.base + last * a.step + a.bytes) return false;
+    auto hits = [&](int64_t from, int64_t bytes, int64_t first, int64_t steps) {   // of b's rows first .. steps
+        if (b.step == 0) return from < b.base + b.bytes && b.base < from + bytes;
+        const int64_t lo = std::max(first, floor_div(from - b.base - b.bytes, b.step) + 1);
+        return lo <= steps && b.base + lo * b.step < from + bytes;
+    };
+    if (a.step == b.step) return hits(a.base, a.bytes, -last, last);
+    for (int64_t i = 0; i <= last; ++i)
+        if (hits(a.base + i * a.step, a.bytes, 0, last)) return true;
+    return false;
+}
+
+// r's output against other rows (none where p is null) that the call reads or writes.
+bool meets_output(const pa::HeadRows& r, const uint16_t* p, long long stride, int heads, int n) {
+    return n > 0 && r.heads > 0 && heads > 0 && p &&
+           meet(rows_at(r.out, r.out_stride, r.heads), rows_at(p, stride, heads), n);
 }
 
 }  // namespace
@@ -76,8 +100,8 @@ pa::HeadRows head_rows(const char* what, const pa_head_rows* r, int n, bool has_
             throw std::invalid_argument(w + "outputs must be 16-byte aligned, their stride a multiple of 8 elements below 2^26");
         if (n > 1 && r->out_stride < static_cast<long long>(r->heads) * pa::kHeadDim)
             throw std::invalid_argument(w + "output rows overlap");
-        const Span in = span_of(r->in, r->in_stride, n, r->heads), out = span_of(r->out, r->out_stride, n, r->heads);
-        if (in.lo < out.hi && out.lo < in.hi && !(r->in == r->out && (n == 1 || r->in_stride == r->out_stride)))
+        if (!(r->in == r->out && (n == 1 || r->in_stride == r->out_stride)) &&
+            meet(rows_at(r->in, r->in_stride, r->heads), rows_at(r->out, r->out_stride, r->heads), n))
             throw std::invalid_argument(w + "the output overlaps the rows (it may only be the rows themselves)");
     }
     h.in         = r->in;
@@ -100,6 +124,16 @@ void check_v_rows(const char* what, const uint16_t* v, int64_t stride, int n) {
     if (n > 0 && (!aligned(v, 16) || !stride_ok(stride)))
         throw std::invalid_argument(std::string(what) +
                                     ": v must be 16-byte aligned, its stride a multiple of 8 elements below 2^26");
+}
+
+void check_outputs(const char* what, const pa::HeadRows& q, const pa::HeadRows& k, bool k_out, const uint16_t* v,
+                   int64_t v_stride, int n) {
+    const char* met = meets_output(q, k.in, k.in_stride, k.heads, n)                              ? "q's output overlaps k"
+                      : meets_output(q, v, v_stride, k.heads, n)                                  ? "q's output overlaps v"
+                      : k_out && meets_output(q, k.out, k.out_stride, k.heads, n)                 ? "the outputs overlap"
+                      : k_out && meets_output(k, q.in, q.in_stride, q.heads, n)                   ? "k's output overlaps q"
+                                                                                                  : nullptr;
+    if (met) throw std::invalid_argument(std::string(what) + ": " + met);
 }
 
 }  // namespace pa::host
@@ -163,6 +197,7 @@ pa_status pa_norm_rope(const pa_rope* rope, const pa_head_rows* q, const pa_head
         pa::RopeAppend a{};
         a.q = head_rows("norm_rope q", q, n, true);
         a.k = head_rows("norm_rope k", k, n, true);
+        check_outputs("norm_rope", a.q, a.k, true, nullptr, 0, n);
         if (rope && n > 0 && !positions) throw std::invalid_argument("norm_rope: a rotation needs positions");
         check_count("norm_rope", n, static_cast<long long>(a.q.heads) + a.k.heads + 8);
         if (n == 0 || a.q.heads + a.k.heads == 0) return;
@@ -193,6 +228,7 @@ pa_status pa_append_rope(int dtype, const pa_append_args* p, const pa_rope* rope
         a.q = head_rows("append_rope q", q, n, true);
         a.k = head_rows("append_rope k", k, n, false);
         check_v_rows("append_rope", p->v, p->v_stride, n);
+        check_outputs("append_rope", a.q, a.k, false, p->v, p->v_stride, n);
         check_count("append_rope", n, static_cast<long long>(a.q.heads) + 2ll * k->heads + 12);
         check_count("append_rope", p->num_entries, 128);
         if (n == 0) return;

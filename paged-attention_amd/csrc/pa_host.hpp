@@ -234,6 +234,10 @@ pa::RopeTable rope_table(const pa_rope* rope);
 // The same for head rows (no heads for null), checked for n tokens.
 pa::HeadRows head_rows(const char* what, const pa_head_rows* r, int n, bool has_out);
 void check_v_rows(const char* what, const uint16_t* v, int64_t stride, int n);
+// Refuses outputs that share memory with other rows of the call (their own rows:
+// head_rows). k_out: k has an output, too; v null: none (k's heads).
+void check_outputs(const char* what, const pa::HeadRows& q, const pa::HeadRows& k, bool k_out, const uint16_t* v,
+                   int64_t v_stride, int n);
 void check_page_bytes(const char* what, int dtype, int page_size, int kv_heads);
 
 // ---- page pool (pa_pool.cpp)

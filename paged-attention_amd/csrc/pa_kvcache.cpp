@@ -436,6 +436,7 @@ pa_status pa_cache_append_rope(pa_cache* c, const int32_t* slots, const int32_t*
         a.q = head_rows("append_rope q", q, nt, true);
         a.k = head_rows("append_rope k", k, nt, false);
         check_v_rows("append_rope", v, v_stride, nt);
+        check_outputs("append_rope", a.q, a.k, false, v, v_stride, nt);
         check_page_bytes("append_rope", c->cfg.dtype, c->cfg.page_size, c->cfg.num_kv_heads);
         if (rope && rope->num_axes > 1 && nt > 0 && !positions)
             throw std::invalid_argument("append_rope: a rotation over several axes needs positions");
