@@ -444,7 +444,8 @@ void      pa_cache_destroy(pa_cache* cache);
 /* Host bookkeeping view (seq_len, free_pages, block tables, ...). */
 pa_pool*  pa_cache_pool(pa_cache* cache);
 int       pa_cache_admit(pa_cache* cache);
-/* paged_kv_cache.cu:95-136 append (synchronizes `stream`, as the reference). */
+/* paged_kv_cache.cu:95-136 append (synchronizes `stream`, as the reference). Here and
+ * in append_batch k and v of a block-scaled cache are 16-byte aligned. */
 pa_status pa_cache_append(pa_cache* cache, int slot, const uint16_t* d_k, const uint16_t* d_v,
                           int n, void* stream, int* appended);
 /* paged_kv_cache.cu:95-136 append, batched across sequences: appends counts[i]

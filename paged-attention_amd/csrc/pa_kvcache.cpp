@@ -234,6 +234,15 @@ void queue_append(pa_cache& c, const int32_t* slots, const int32_t* counts, int 
                });
 }
 
+// k and v of append and append_batch. Into block-scaled caches they go as head rows
+// do (queue_append), which are read in aligned pieces.
+void check_tokens(const char* what, const pa_cache& c, const uint16_t* d_k, const uint16_t* d_v) {
+    if (!d_k || !d_v) throw std::invalid_argument(std::string(what) + ": k or v is null");
+    const uintptr_t bits = reinterpret_cast<uintptr_t>(d_k) | reinterpret_cast<uintptr_t>(d_v);
+    if (c.cfg.dtype == PA_KV_FP8_E4M3_BLOCK && bits % 16 != 0)
+        throw std::invalid_argument(std::string(what) + ": k and v must be 16-byte aligned (block-scaled caches)");
+}
+
 // Notes a stream the cache's work is queued on.
 hipStream_t use_stream(pa_cache& c, void* stream) {
     if (stream) c.null_stream_only = false;
@@ -364,6 +373,7 @@ pa_status pa_cache_append(pa_cache* c, int slot, const uint16_t* d_k, const uint
         if (appended) *appended = 0;
         if (static_cast<long long>(n) * c->cfg.num_kv_heads * (pa::kHeadDim / 8) > INT_MAX)
             throw std::length_error("append: n * num_kv_heads * 16 exceeds INT_MAX");
+        if (n > 0) check_tokens("append", *c, d_k, d_v);
         const int old_len = slot_ok(c->pool, slot) ? c->pool.seq_lens[static_cast<size_t>(slot)] : 0;
         const hipStream_t s = n > 0 ? append_stream(*c, stream) : nullptr;
         int first_new = 0, num_new = 0;
@@ -408,7 +418,7 @@ pa_status pa_cache_append_batch(pa_cache* c, const int32_t* slots, const int32_t
         for (int i = 0; i < n && counts; ++i) n_tok += counts[i] > 0 ? counts[i] : 0;
         const int hkv = c->cfg.num_kv_heads;
         if (n_tok * hkv * (pa::kHeadDim / 8) > INT_MAX) throw std::length_error("append_batch: too many tokens");
-        if (n_tok > 0 && (!d_k || !d_v)) throw std::invalid_argument("append_batch: k or v is null");
+        if (n_tok > 0) check_tokens("append_batch", *c, d_k, d_v);
         const hipStream_t s = n_tok > 0 ? append_stream(*c, stream) : nullptr;
         std::vector<reserve_entry> entries;
         if (!pool_reserve_batch(c->pool, slots, counts, n, &entries)) return;   // out of pages: nothing appended
