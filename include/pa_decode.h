@@ -279,8 +279,8 @@ typedef struct pa_head_rows {
 } pa_head_rows;
 
 /* q and k (either may be NULL) of n tokens normed and rotated into their `out`.
- * (Here and below, PA_ERR_LENGTH: some 2^27 / heads tokens and 2^20 entries at most; a
- * page of one pool is below 2 GiB.)
+ * (Here and below, PA_ERR_LENGTH: some 2^27 / heads tokens, 2^19 heads and 2^20 entries
+ * at most; a page of one pool is below 2 GiB.)
  * positions: device, [n][axes of the rotation] int32 (any value), NULL only where
  * rope is (norms alone). */
 pa_status pa_norm_rope(const pa_rope* rope, const pa_head_rows* q, const pa_head_rows* k,

@@ -24,6 +24,10 @@ void check_count(const char* what, long long n, long long heads) {
         throw std::length_error(std::string(what) + ": tokens * heads * 16 exceeds INT_MAX");
 }
 
+// Heads of one operand: a wave's resource over a token's heads, and in a block
+// 15 strides and the heads, stay below 2^31 bytes.
+constexpr int kMaxHeads = 1 << 19;
+
 // Elements from one token to the next.
 bool stride_ok(int64_t s) { return s >= 0 && s < (1 << 26) && s % 8 == 0; }
 
@@ -85,6 +89,7 @@ pa::HeadRows head_rows(const char* what, const pa_head_rows* r, int n, bool has_
     if (!r || r->heads == 0) return h;
     const std::string w = std::string(what) + ": ";
     if (r->heads < 0) throw std::invalid_argument(w + "negative head count");
+    if (r->heads > kMaxHeads) throw std::length_error(w + "more than 2^19 heads");
     check_count(what, n, r->heads);
     if (n > 0) {
         if (!r->in) throw std::invalid_argument(w + "null rows");

@@ -1,0 +1,46 @@
+"""CPU tests of the largest sizes that the new-token entry points take: refused before anything is launched."""
+
+from __future__ import annotations
+
+import ctypes
+
+import pytest
+
+from pa_amd import _lib
+
+A = 1 << 40   # an address that nothing reads
+
+
+def rows(heads, **kw):
+    r = _lib.HeadRows()
+    r.in_, r.heads, r.in_stride, r.eps = A, heads, 8, 1e-6
+    r.out, r.out_stride = A << 2, (1 << 26) - 8
+    for k, v in kw.items():
+        setattr(r, k, v)
+    return r
+
+
+@pytest.mark.parametrize("heads", [2**19 + 1, 2**23, 2**26])
+def test_heads_whose_rows_pass_32_bits(heads):
+    """A token of more heads would lie 2^31 bytes and more past its first (2^23), or, in a block, past its first token's
+    (15 strides of 2^26 elements before it)."""
+    lib, r = _lib.load(), rows(heads)
+    one = rows(1)
+    for q, k in ((r, None), (None, r), (one, r)):
+        ref = [None if x is None else ctypes.byref(x) for x in (q, k)]
+        assert lib.pa_norm_rope(None, *ref, None, 1, None) == _lib.PA_ERR_LENGTH and b"heads" in lib.pa_last_error()
+    a = _lib.AppendArgs()
+    a.num_tokens, a.num_entries, a.tok_begin, a.start_pos = 1, 1, A, A
+    a.v, a.v_stride, a.k_cache, a.v_cache, a.kv_scales = A, 8, A, A, A
+    a.block_table, a.block_table_stride, a.num_table_rows, a.num_pages = A, 4, 2, 8
+    a.page_size, a.k_scale, a.v_scale = 8, 1.0, 1.0
+    got = lib.pa_append_rope(2, ctypes.byref(a), None, None, ctypes.byref(r), None)
+    assert got == (_lib.PA_ERR_LENGTH if heads < 2**21 else _lib.PA_ERR_INVALID_ARGUMENT)   # (its page passes 2 GiB first)
+    got = lib.pa_append_rope(2, ctypes.byref(a), None, ctypes.byref(r), ctypes.byref(one), None)
+    assert got == _lib.PA_ERR_LENGTH
+
+
+def test_largest_head_count_fits_the_kernels_offsets():
+    """2^19 heads of 256 bytes, and the last of a block's 16 rows at the largest stride (2^26 - 8 elements)."""
+    heads, stride = 2**19, 2**26 - 8
+    assert 2 * 128 * heads < 2**31 and 2 * (15 * stride + heads * 128) <= 2**31 - 1
