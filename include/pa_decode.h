@@ -467,7 +467,8 @@ pa_status pa_cache_append_batch(pa_cache* cache, const int32_t* slots, const int
  * given, is normed and rotated into its `out` in the same launch (pa_append_rope
  * says what is stored; k and v have the cache's kv heads). positions: device, [sum(counts)][axes], NULL:
  * every token's place in its sequence. Bookkeeping, ordering, capture and refusals are
- * append_batch's. Block-scaled caches take a slot that repeats in one batch
+ * append_batch's; rows are pa_append_rope's, and so is the refusal of FP8 scales without
+ * a finite reciprocal. Block-scaled caches take a slot that repeats in one batch
  * with a further launch; with rope, weights and q all NULL this is append_batch on
  * strided tokens. */
 pa_status pa_cache_append_rope(pa_cache* cache, const int32_t* slots, const int32_t* counts, int n,

@@ -131,6 +131,14 @@ void check_v_rows(const char* what, const uint16_t* v, int64_t stride, int n) {
                                     ": v must be 16-byte aligned, its stride a multiple of 8 elements below 2^26");
 }
 
+float inverse_scale(const char* what, int dtype, float scale) {
+    if (dtype != PA_KV_FP8_E4M3) return 1.0f;
+    const float inv = 1.0f / scale;
+    if (!std::isfinite(inv) || inv == 0.0f)
+        throw std::invalid_argument(std::string(what) + ": k_scale and v_scale must have finite reciprocals");
+    return inv;
+}
+
 void check_outputs(const char* what, const pa::HeadRows& q, const pa::HeadRows& k, bool k_out, const uint16_t* v,
                    int64_t v_stride, int n) {
     const char* met = meets_output(q, k.in, k.in_stride, k.heads, n)                              ? "q's output overlaps k"
@@ -246,11 +254,8 @@ pa_status pa_append_rope(int dtype, const pa_append_args* p, const pa_rope* rope
             throw std::invalid_argument("append_rope: a block-scaled cache needs kv_scales (2-byte aligned)");
         if (rope && rope->num_axes > 1 && !p->positions)
             throw std::invalid_argument("append_rope: a rotation over several axes needs positions");
-        const bool fp8 = dtype == PA_KV_FP8_E4M3;
-        a.inv_k        = fp8 ? 1.0f / p->k_scale : 1.0f;
-        a.inv_v        = fp8 ? 1.0f / p->v_scale : 1.0f;
-        if (!std::isfinite(a.inv_k) || !std::isfinite(a.inv_v) || a.inv_k == 0.0f || a.inv_v == 0.0f)
-            throw std::invalid_argument("append_rope: k_scale and v_scale must have finite reciprocals");
+        a.inv_k        = inverse_scale("append_rope", dtype, p->k_scale);
+        a.inv_v        = inverse_scale("append_rope", dtype, p->v_scale);
         a.rope         = rope_table(rope);
         a.v            = p->v;
         a.v_stride     = static_cast<long>(p->v_stride);

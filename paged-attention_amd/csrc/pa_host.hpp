@@ -234,6 +234,8 @@ pa::RopeTable rope_table(const pa_rope* rope);
 // The same for head rows (no heads for null), checked for n tokens.
 pa::HeadRows head_rows(const char* what, const pa_head_rows* r, int n, bool has_out);
 void check_v_rows(const char* what, const uint16_t* v, int64_t stride, int n);
+// What FP8 values are multiplied by, refused where there is no such number; 1 for other types.
+float inverse_scale(const char* what, int dtype, float scale);
 // Refuses outputs that share memory with other rows of the call (their own rows:
 // head_rows). k_out: k has an output, too; v null: none (k's heads).
 void check_outputs(const char* what, const pa::HeadRows& q, const pa::HeadRows& k, bool k_out, const uint16_t* v,

@@ -143,7 +143,6 @@ void queue_meta(pa_cache& c, const int32_t* slots, const int32_t* counts, int n,
 // The same for strided rows of k and v, k (and q) normed and rotated on the way.
 void queue_rows(pa_cache& c, const int32_t* slots, const int32_t* counts, int n, const reserve_entry* entries,
                 long n_tok, const pa::RopeAppend& rows, hipStream_t s) {
-    const bool fp8 = c.cfg.dtype == PA_KV_FP8_E4M3;
     queue_meta(c, slots, counts, n, entries, n_tok, s,
                [&](const append_meta& m, const int32_t* host, size_t need) {
                    pa::RopeAppend a = rows;
@@ -159,8 +158,6 @@ void queue_rows(pa_cache& c, const int32_t* slots, const int32_t* counts, int n,
                    a.v_cache   = c.d_v;
                    a.scales    = c.d_scales;
                    a.page_size = c.cfg.page_size;
-                   a.inv_k     = fp8 ? 1.0f / c.cfg.k_scale : 1.0f;
-                   a.inv_v     = fp8 ? 1.0f / c.cfg.v_scale : 1.0f;
                    return pa::launch_append_rope(c.cfg.dtype, a, host, need, s);
                });
 }
@@ -450,7 +447,11 @@ pa_status pa_cache_append_rope(pa_cache* c, const int32_t* slots, const int32_t*
         check_page_bytes("append_rope", c->cfg.dtype, c->cfg.page_size, c->cfg.num_kv_heads);
         if (rope && rope->num_axes > 1 && nt > 0 && !positions)
             throw std::invalid_argument("append_rope: a rotation over several axes needs positions");
-        if (nt > 0) a.rope = rope_table(rope);
+        if (nt > 0) {
+            a.inv_k = inverse_scale("append_rope", c->cfg.dtype, c->cfg.k_scale);
+            a.inv_v = inverse_scale("append_rope", c->cfg.dtype, c->cfg.v_scale);
+            a.rope  = rope_table(rope);
+        }
         a.v         = v;
         a.v_stride  = static_cast<long>(v_stride);
         a.positions = rope ? positions : nullptr;

@@ -29,3 +29,16 @@ def test_appends_refuse_null_and_unaligned_tokens(kind):
     assert cache.append(s, good, good, 5) and cache.append_batch([s], [5], good, good)
     assert cache.seq_len(s) == 10
     cache.close()
+
+
+@pytest.mark.parametrize("scale", [0.0, 1e-39, float("inf"), float("nan")])
+def test_append_rope_refuses_a_cache_without_reciprocals(scale):
+    """A per-tensor FP8 cache whose scale no value can be divided by (the raw append refuses such scales, too)."""
+    x = torch.zeros((3, 2, D), dtype=torch.float16, device="cuda")
+    for k_scale, v_scale in ((scale, 1.0), (1.0, scale)):
+        cache = pa_amd.PagedKVCache(4, 16, 2, D, 2, 4, pa_amd.FP8_E4M3, k_scale, v_scale)
+        s = cache.admit()
+        with pytest.raises(pa_amd.InvalidArgument, match="reciprocals"):
+            cache.append_rope([s], [3], x, x)
+        assert cache.seq_len(s) == 0 and cache.free_pages() == 4
+        cache.close()
