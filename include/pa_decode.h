@@ -24,8 +24,10 @@
  *   kv_scales     [num_pages][num_kv_heads][page_size / B][2] uint8, block-scaled
  *                 caches only: byte e of a block's K (0) and V (1) stands for the
  *                 scale 2^(e - 127); a block is B = pa_block_tokens(page_size) tokens
- *                 (the decode reads whole 4-byte words, and holds V in fp16: a value
- *                 past that, which appends never store, is infinite there)
+ *                 (the decode holds V in fp16: a value past that, which appends
+ *                 never store, is infinite there). The decode reads whole 4-byte words:
+ *                 the array's memory is rounded up to a multiple of 4 bytes, where the
+ *                 number of its pairs is odd (what is in the last 2 does not matter)
  *   block_table   [num_slots][block_table_stride] int32 physical page ids
  *   segments      [num_segments][4] int32 = (batch row, kv head, tok_begin, tok_end)
  */

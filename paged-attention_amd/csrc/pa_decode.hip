@@ -731,7 +731,8 @@ __device__ __forceinline__ void decode_split_body(const pa_decode_params& p, con
     // The word with the K and V scale bytes of the block that holds the row at
     // byte row0 of a pool (wave-uniform; blocks are counted as their rows are): a
     // scalar load beside the block's rows, used a step later. (The pair is 2-byte
-    // aligned; the aligned word around it ends inside the array's last 4 bytes.)
+    // aligned. The aligned word around the last of an odd number of pairs ends 2
+    // bytes behind the array, which callers therefore round up to whole words.)
     auto load_scales = [&](int s, int hh, int n, size_t row0) {
         static_assert(!BS || ROW == 128, "a row's bytes are 2^7");
         const int idx = static_cast<int>(row0 >> (7 + sc_shift));

@@ -13,6 +13,7 @@ RuntimeError (as Decoder's do) or the library's errors; nothing is differentiate
 from __future__ import annotations
 
 import ctypes
+import math
 
 import numpy as np
 import torch
@@ -31,12 +32,15 @@ def block_tokens(page_size: int) -> int:
 
 def alloc_kv_scales(num_pages: int, num_kv_heads: int, page_size: int, device=None) -> torch.Tensor:
     """Scale bytes of a block-scaled cache ([pages][kv heads][blocks of a page][2]; byte e
-    stands for 2^(e - 127)). What is in them before a block's first token does not matter."""
+    stands for 2^(e - 127)). What is in them before a block's first token does not matter.
+    The memory is rounded up to whole 4-byte words, which the decode reads."""
     b = block_tokens(page_size)
     if b == 0:
         raise InvalidArgument("block-scaled caches need a page_size that is a multiple of 8")
-    return torch.full((num_pages, num_kv_heads, page_size // b, 2), 127, dtype=torch.uint8,
-                      device=device if device is not None else "cuda")
+    shape = (num_pages, num_kv_heads, page_size // b, 2)
+    n = math.prod(shape)
+    flat = torch.full(((n + 3) // 4 * 4,), 127, dtype=torch.uint8, device=device if device is not None else "cuda")
+    return flat[:n].view(shape)
 
 
 class Rope:

@@ -44,3 +44,12 @@ def test_largest_head_count_fits_the_kernels_offsets():
     """2^19 heads of 256 bytes, and the last of a block's 16 rows at the largest stride (2^26 - 8 elements)."""
     heads, stride = 2**19, 2**26 - 8
     assert 2 * 128 * heads < 2**31 and 2 * (15 * stride + heads * 128) <= 2**31 - 1
+
+
+@pytest.mark.parametrize("pages,hkv,page", [(3, 1, 16), (1, 1, 8), (5, 3, 24), (4, 2, 16), (0, 1, 16)])
+def test_scale_bytes_come_in_whole_words(pages, hkv, page):
+    """The decode reads the word around a block's pair of bytes: behind an odd number of pairs that is memory, too."""
+    import pa_amd
+    s = pa_amd.alloc_kv_scales(pages, hkv, page, device="cpu")
+    assert s.shape == (pages, hkv, page // pa_amd.block_tokens(page), 2) and s.is_contiguous() and bool((s == 127).all())
+    assert s.untyped_storage().nbytes() % 4 == 0 and s.storage_offset() == 0
