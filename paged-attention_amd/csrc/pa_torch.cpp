@@ -40,10 +40,11 @@ void check_status(pa_status s) {
 void check_kv_scales(const torch::Tensor& s, const torch::Tensor& cache) {
     const int b = pa_block_tokens(static_cast<int>(cache.size(2)));
     TORCH_CHECK(b != 0, "block-scaled caches need a page_size that is a multiple of 8");
-    TORCH_CHECK(s.is_cuda() && s.is_contiguous() && s.element_size() == 1 && s.dim() == 4 &&
-                    s.size(0) == cache.size(0) && s.size(1) == cache.size(1) && s.size(2) == cache.size(2) / b &&
-                    s.size(3) == 2,
-                "kv_scales must be a contiguous CUDA uint8 [pages, num_kv_heads, page_size / ", b, ", 2] tensor");
+    TORCH_CHECK(s.is_cuda() && s.get_device() == cache.get_device() && s.is_contiguous() && s.element_size() == 1 &&
+                    s.dim() == 4 && s.size(0) == cache.size(0) && s.size(1) == cache.size(1) &&
+                    s.size(2) == cache.size(2) / b && s.size(3) == 2,
+                "kv_scales must be a contiguous CUDA uint8 [pages, num_kv_heads, page_size / ", b,
+                ", 2] tensor on the cache's device");
 }
 
 class Decoder {
@@ -256,10 +257,7 @@ OptTensor append_rope(const OptTensor& q, const torch::Tensor& k, const torch::T
                     "or both one-byte FP8");
     const bool fp16 = k_cache.scalar_type() == torch::kHalf;
     TORCH_CHECK(!kv_scales || !fp16, "kv_scales goes with one-byte FP8 caches");
-    if (kv_scales) {
-        check_kv_scales(*kv_scales, k_cache);
-        TORCH_CHECK(kv_scales->get_device() == device, "kv_scales must be on k's device");
-    }
+    if (kv_scales) check_kv_scales(*kv_scales, k_cache);
     auto ints = [&](const torch::Tensor& t, int64_t size, const char* what) {
         TORCH_CHECK(t.is_cuda() && t.get_device() == device && t.scalar_type() == torch::kInt32 && t.is_contiguous() &&
                         t.dim() == 1 && (size < 0 || t.size(0) == size) && t.size(0) <= INT_MAX,

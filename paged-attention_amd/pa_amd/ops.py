@@ -188,7 +188,6 @@ def append_rope(q, k, v, k_cache, v_cache, block_table, tok_begin, start_pos, ro
     _require(kv_scales is None or not fp16, "kv_scales goes with one-byte FP8 caches")
     if kv_scales is not None:
         check_kv_scales(kv_scales, k_cache)
-        _require(kv_scales.get_device() == dev, "kv_scales must be on k's device")
 
     def ints(t, size, what):
         _require(t.is_cuda and t.get_device() == dev and t.dtype == torch.int32 and t.is_contiguous() and t.dim() == 1
@@ -220,6 +219,7 @@ def append_rope(q, k, v, k_cache, v_cache, block_table, tok_begin, start_pos, ro
 def check_kv_scales(s, cache) -> None:
     b = block_tokens(cache.size(2))
     _require(b != 0, "block-scaled caches need a page_size that is a multiple of 8")
-    _require(s.is_cuda and s.is_contiguous() and s.element_size() == 1
+    _require(s.is_cuda and s.get_device() == cache.get_device() and s.is_contiguous() and s.element_size() == 1
              and tuple(s.shape) == (cache.size(0), cache.size(1), cache.size(2) // b, 2),
-             f"kv_scales must be a contiguous CUDA uint8 [pages, num_kv_heads, page_size / {b}, 2] tensor")
+             f"kv_scales must be a contiguous CUDA uint8 [pages, num_kv_heads, page_size / {b}, 2] tensor on the "
+             "cache's device")

@@ -53,3 +53,32 @@ def test_scale_bytes_come_in_whole_words(pages, hkv, page):
     s = pa_amd.alloc_kv_scales(pages, hkv, page, device="cpu")
     assert s.shape == (pages, hkv, page // pa_amd.block_tokens(page), 2) and s.is_contiguous() and bool((s == 127).all())
     assert s.untyped_storage().nbytes() % 4 == 0 and s.storage_offset() == 0
+
+
+class _OnDevice:
+    """What the checks ask of a CUDA tensor."""
+
+    def __init__(self, shape, device):
+        self.shape, self.device_index, self.is_cuda = shape, device, True
+
+    def get_device(self):
+        return self.device_index
+
+    def is_contiguous(self):
+        return True
+
+    def element_size(self):
+        return 1
+
+    def size(self, i):
+        return self.shape[i]
+
+
+def test_scales_of_another_device_are_refused():
+    """The decode's caches and scales lie on one device. (The compiled binding makes the same check; two devices are not
+    at hand.)"""
+    from pa_amd import ops
+    cache = _OnDevice((6, 2, 16, 128), 1)
+    ops.check_kv_scales(_OnDevice((6, 2, 1, 2), 1), cache)
+    with pytest.raises(RuntimeError, match="device"):
+        ops.check_kv_scales(_OnDevice((6, 2, 1, 2), 0), cache)
