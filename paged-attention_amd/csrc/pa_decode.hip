@@ -630,8 +630,10 @@ __device__ __forceinline__ void decode_split_body(const pa_decode_params& p, con
     // 16 (lane % 8) .. +15 of each half), moved into kr / vr by the stage.
     u32x4 kc[STG && !DMA ? DEPTH : 1][NH][NPART], vc[STG && !DMA ? DEPTH : 1][NH][NPART];
     u32x4 qc[DMA ? 1 : DEPTH][NQ];   // compact Q, loaded with a segment's first step (direct paths)
-    int   pg[DEPTH][NH];       // power-of-two path: page of each half (wave-uniform)
-    int   pgr[RUNS ? DEPTH : 1][NH][NPART];   // page of each part
+    // (Zero before a slot's first lookup: a unit of fewer steps than slots issues the
+    // rest empty, and their block scales are read all the same.)
+    int   pg[DEPTH][NH] = {};  // power-of-two path: page of each half (wave-uniform)
+    int   pgr[RUNS ? DEPTH : 1][NH][NPART] = {};   // page of each part
     constexpr int LN = PATH == kPageLane ? DEPTH : 1;
     int   plk[LN][NH][NPART], psl[LN][NH][NPART];          // lane path: byte address of the lane holding
                                                            // the row's page entry, slot in the page
