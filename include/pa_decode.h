@@ -27,7 +27,9 @@
  *                 (the decode holds V in fp16: a value past that, which appends
  *                 never store, is infinite there). The decode reads whole 4-byte words:
  *                 the array's memory is rounded up to a multiple of 4 bytes, where the
- *                 number of its pairs is odd (what is in the last 2 does not matter)
+ *                 number of its pairs is odd (what is in the last 2 does not matter).
+ *                 A caller's own bytes: 1 to 254, and 95 to 135 (what appends choose)
+ *                 in blocks that an append goes on to fill
  *   block_table   [num_slots][block_table_stride] int32 physical page ids
  *   segments      [num_segments][4] int32 = (batch row, kv head, tok_begin, tok_end)
  */
@@ -300,7 +302,8 @@ int pa_block_tokens(int page_size);
  * reads, so a captured call follows their values from replay to replay; a token
  * whose place, row or page is out of range (num_table_rows, block_table_stride,
  * num_pages), whose entry starts below 0, or that is in no entry (a padded batch's
- * last ones, past tok_begin[num_entries]) is left out (its q is not).
+ * last ones, past tok_begin[num_entries]) is left out (its q is not). Tokens need
+ * an entry, an empty one at least.
  * Block-scaled caches: one call holds each sequence once.
  *   k   normed and rotated (positions: [num_tokens][axes]; NULL: the token's place
  *       turns every pair), then stored; its `out` is not used

@@ -46,9 +46,16 @@
 //     reference max per head that only moves (with the exact O/l rescale) when
 //     a score exceeds it by more than 2^8, so the cross-lane max reduction is
 //     paid at a segment's first step and then almost never. P <= 256 stays far
-//     inside fp16 range and l in fp32.
+//     inside fp16 range. Scores, maxima, l and O are fp32; P is rounded to fp16
+//     for its MFMA, 2^-11 of each probability, as much as the result's own
+//     rounding (64 x 8192 tokens: off by 2.4e-4 of the exact result (r.m.s.),
+//     2.1e-4 from rounding the result alone): P in two fp16 terms would double
+//     the P V products.
 //   * FP8 E4M3 is widened to fp16 in registers (exact); k_scale folds into the
-//     softmax scale and v_scale into the output normalization.
+//     softmax scale and v_scale into the output normalization. A block's scale
+//     multiplies K's scores in fp32 and goes into V's widening: V is fp16 under
+//     it, exact for what appends store (values that came as fp16, rounded to
+//     coarser steps).
 //   * Q of each segment is fetched compactly (G x 256 B across the wave) with
 //     the segment's first K/V loads and expanded to the B-operand layout
 //     through a per-wave LDS slot once per segment; on the LDS-stage paths it

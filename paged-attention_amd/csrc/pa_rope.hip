@@ -374,7 +374,9 @@ template <int CACHE, bool INTER, int META, int U, bool NT>
 __global__ __launch_bounds__(64 * kRowWaves) void head_rows_kernel(const RopeAppend a) {
     head_rows_body<CACHE, INTER, META, U, NT>(a, a.meta);
 }
-// The meta is read where the arguments lie, as in pa_cache.hip.
+// The meta is read where the arguments lie, as in pa_cache.hip. (Calls that fit there
+// are short, but for prompts into pages of 64 tokens and more: those never take the
+// streaming loads, which would save them 2 to 5%.)
 template <int CACHE, bool INTER, int U, int N>
 __global__ __launch_bounds__(64 * kRowWaves) void head_rows_inline_kernel(const RopeInline<N> x) {
     const uintptr_t args = (uintptr_t)__builtin_amdgcn_kernarg_segment_ptr();
@@ -588,9 +590,11 @@ int groups(int heads) { return (heads + kRows - 1) / kRows; }
 // A large call's waves take up to kManyU groups of four rows (the turns are worked
 // out once a wave), a small one's one each (more waves, shorter ones). Same box, us,
 // 8192 tokens of 32 + 8 heads at 2, 3, 4, 5, 6, 12 groups: 35.0, 34.6, 32.7, 32.9,
-// 34.2, 38.7. One group and four: 128 tokens (1280 groups) 2.7 / 3.4, 800 4.7 / 5.2,
-// 1200 6.9 / 6.3, 3200 14.8 / 12.2; into fp16 pages 256 tokens 3.6 / 3.8, 512
-// (6144 groups) 4.6 / 4.3, 1024 7.8 / 6.1.
+// 34.2, 38.7. One group and four: 128 tokens (1280 groups) 2.7 / 3.4, 800 (8000) 4.7 /
+// 5.2, 1200 (12000) 6.9 / 6.3, 3200 14.8 / 12.2; into fp16 pages 256 tokens (3072) 3.6 /
+// 3.8, 512 (6144) 4.6 / 4.3, 1024 7.8 / 6.1. So calls without a cache cross near 8192
+// groups, appends between 3072 and 6144: one border for both costs appends of 6144
+// groups 0.3 us.
 constexpr int  kManyU      = 4;
 constexpr long kManyGroups = 8192;
 
@@ -598,9 +602,12 @@ constexpr long kManyGroups = 8192;
 // projection before it cannot have left in the memory-side cache (256 MB, the
 // outputs beside them), and where a load takes whole 128-byte lines, which partial
 // half-split rotations do not. us with cached and with non-temporal loads: 3200
-// tokens of 32 + 8 heads (33 MB) 12.0 / 14.0, 6400 21.7 / 25.1, 12800 (131 MB) 46.9 /
-// 45.8, 8192 of 64 + 8 (151 MB) 52.7 / 51.1, 32768 into block-scaled pages (403 MB)
-// 145 / 137; with 96 of 128 dims turned 8192 of 32 + 8 29.0 / 36.4.
+// tokens of 32 + 8 heads (33 MB) 12.0 / 14.0, 6400 (66) 21.8 / 24.7, 8600 (88) 31.5 /
+// 31.2, 9830 (101, the border) 34.1 / 35.5, 11000 (113) 39.1 / 38.8, 12800 (131) 45.6 /
+// 44.8; with 8 more heads of values into FP8 pages 7200 (88) 29.0 / 30.4, 8192 (101)
+// 34.0 / 34.3, 9400 (116) 39.8 / 38.7, 10700 (131) 44.7 / 43.8; into block-scaled ones
+// 6200 (76) 25.7 / 29.3, 8192 38.2 / 37.0, 10700 48.6 / 45.9, 32768 (403) 145 / 137; with
+// 96 of 128 dims turned 8192 of 32 + 8 29.0 / 36.4.
 constexpr long kStreamBytes = 96l << 20;
 
 // Parts of a token at u groups a wave, and the grid.
