@@ -591,10 +591,10 @@ int groups(int heads) { return (heads + kRows - 1) / kRows; }
 // out once a wave), a small one's one each (more waves, shorter ones). Same box, us,
 // 8192 tokens of 32 + 8 heads at 2, 3, 4, 5, 6, 12 groups: 35.0, 34.6, 32.7, 32.9,
 // 34.2, 38.7. One group and four: 128 tokens (1280 groups) 2.7 / 3.4, 800 (8000) 4.7 /
-// 5.2, 1200 (12000) 6.9 / 6.3, 3200 14.8 / 12.2; into fp16 pages 256 tokens (3072) 3.6 /
-// 3.8, 512 (6144) 4.6 / 4.3, 1024 7.8 / 6.1. So calls without a cache cross near 8192
-// groups, appends between 3072 and 6144: one border for both costs appends of 6144
-// groups 0.3 us.
+// 5.2, 1200 (12000) 6.9 / 6.3, 3200 14.8 / 12.2; into fp16 pages 256 tokens (12 groups
+// each) 3.6 / 3.8, 512 4.6 / 4.3, 1024 7.8 / 6.1. So calls without a cache cross near
+// 8192 groups, appends of these heads between 256 and 512 tokens, 4000 groups or so:
+// one border for both costs 512 of them 0.3 us.
 constexpr int  kManyU      = 4;
 constexpr long kManyGroups = 8192;
 
