@@ -342,6 +342,89 @@ typedef struct pa_append_args {
 pa_status pa_append_rope(int dtype, const pa_append_args* a, const pa_rope* rope, const pa_head_rows* q,
                          const pa_head_rows* k, void* stream);
 
+/* ---- drafted tokens: attention over a cache, accepted rows, rows read back ----
+ * No counterparts in the reference. Several new tokens of a sequence (a tree that a
+ * draft model proposed, a chain, a piece of a prompt) are appended, attend over the
+ * cache at once, and those that turn out right stay:
+ *   pa_append_rope      their keys and values behind the sequence, token i at place start + i
+ *   pa_tree_attention   each sees the earlier places and, of the new ones, its own branch
+ *   pa_keep_rows        the accepted tokens' rows move up to start, start + 1, ...
+ *   pa_read_cache       any places read back as fp16, bf16 or fp32 */
+
+/* Tokens of several sequences in a paged cache of any type. Entry e (0 <= e <
+ * num_entries) holds the tokens tok_begin[e] .. tok_begin[e + 1] - 1 of the call,
+ * which lie at the places start_pos[e], start_pos[e] + 1, ... of the sequence whose
+ * pages row slot_ids[e] of the block table lists (row e where slot_ids is NULL).
+ * Entries, places and table are device arrays that the kernels read, so a captured
+ * call follows their values from replay to replay. */
+typedef struct pa_cached_tokens {
+    int32_t         num_tokens;
+    int32_t         num_entries;
+    const int32_t*  tok_begin;      /* [num_entries + 1], rising within 0 .. num_tokens */
+    const int32_t*  start_pos;      /* [num_entries] */
+    const int32_t*  slot_ids;       /* [num_entries] or NULL */
+    void*           k_cache;        /* 16-byte aligned */
+    void*           v_cache;
+    uint8_t*        kv_scales;      /* block-scaled caches, 2-byte aligned */
+    const int32_t*  block_table;    /* [num_table_rows][block_table_stride] */
+    int32_t         block_table_stride;
+    int32_t         num_table_rows;
+    int32_t         num_pages;
+    int32_t         page_size;
+    int32_t         num_kv_heads;
+    float           k_scale;        /* FP8: a stored code c stands for c * scale (times its block's, */
+    float           v_scale;        /* where blocks have one: 1 for a cache that the appends here wrote) */
+} pa_cached_tokens;
+
+/* Attention of the call's tokens, all of them in the cache already, over their
+ * sequences: token i of entry e (counted from the entry's first) attends to the places
+ * 0 .. start_pos[e] - 1 and to the entry's token j where
+ *   tree   [num_tokens][tree_words], bit j of token i's row (bit j % 64 of word j / 64) is
+ *          set (its own bit and its ancestors', usually; tokens past the row's bits are not seen)
+ *   tree NULL: j <= i
+ * out = sum_p softmax_p(sm_scale q k_p) v_p, in one pass: products of fp16 values in
+ * matrix instructions, sums and the softmax in 32 bits, probabilities rounded to fp16 for
+ * the second product, one rounding at the end. A token that sees nothing (no earlier
+ * place, no bit) gets zeros. What lies in a place reaches only the tokens that see it,
+ * infinities and NaN among the entry's own tokens included.
+ * q: head rows (no weight) of num_kv_heads * (1 to 32) heads, query heads h * group ..
+ * (h + 1) * group - 1 reading kv head h; out may be the rows themselves. Tokens of no entry,
+ * and of one whose start is below 0, whose row is out of range or whose places pass the
+ * table's row or 2^31 - 130, are left out: their `out` stays as it was. Pages out of range (num_pages) read as
+ * rows of zeros.
+ * workspace: pa_tree_attention_workspace bytes (may be 0) for these sizes on this device,
+ * 16-byte aligned, of any content and without meaning after the call; calls that may run at
+ * the same time have one each. */
+pa_status pa_tree_attention_workspace(int dtype, const pa_cached_tokens* c, int num_q_heads, size_t* bytes);
+pa_status pa_tree_attention(int dtype, const pa_cached_tokens* c, const pa_head_rows* q, const uint64_t* tree,
+                            int tree_words, float sm_scale, void* workspace, size_t workspace_bytes, void* stream);
+
+/* Rows as numbers: token t's kv head h to k_out + t * k_stride + h * 128 (elements of
+ * `type`), its value row to v_out likewise (either may be NULL; 16-byte aligned, strides
+ * multiples of 8 below 2^26, rows that do not overlap). code * scale in 32 bits, rounded once. Tokens of no entry
+ * and those whose place, row or page is out of range keep what their output held. */
+typedef enum pa_value_type {
+    PA_VALUE_FP16 = 0,
+    PA_VALUE_BF16 = 1,
+    PA_VALUE_FP32 = 2
+} pa_value_type;
+pa_status pa_read_cache(int dtype, const pa_cached_tokens* c, int type, void* k_out, int64_t k_stride, void* v_out,
+                        int64_t v_stride, void* stream);
+
+/* Of the tokens at the places start_pos[e], start_pos[e] + 1, ... of a sequence those
+ * with the numbers kept[e][0] < kept[e][1] < ... < kept[e][counts[e] - 1] move to the
+ * places start_pos[e], start_pos[e] + 1, ... (token kept[e][j] to start_pos[e] + j), in place. kept:
+ * device, [num_entries][width] int32; counts: device, [num_entries] (at most width are
+ * taken, none if negative). Each sequence once a call; num_tokens and tok_begin are not used. Rows past
+ * the last kept one keep their bytes. A row whose number is below its index, or whose
+ * places or pages are out of range, is left out.
+ * Block-scaled caches: a block (of places) that no row moves into keeps its bytes and scale.
+ * Any other gets the smallest scale that holds its kept rows, as an append would choose; if it
+ * begins before start_pos[e], not below the scale that it has, and its earlier rows are
+ * rounded again where it grows. Kept rows are rounded again to their new block's scale. */
+pa_status pa_keep_rows(int dtype, const pa_cached_tokens* c, const int32_t* kept, int width, const int32_t* counts,
+                       void* stream);
+
 /* Block-table resolution probe (decode_kernels.cuh:175-177's address, with the
  * decode kernel's own device function): copies the raw cache bytes of tokens
  * [0, len) of one kv head into out ([len][head_dim] elements of the cache type). */

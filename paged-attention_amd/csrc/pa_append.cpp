@@ -119,6 +119,12 @@ pa::HeadRows head_rows(const char* what, const pa_head_rows* r, int n, bool has_
     return h;
 }
 
+bool rows_overlap(const void* a, int64_t a_stride, const void* b, int64_t b_stride, int64_t row, int elem, int n) {
+    const Rows x{static_cast<int64_t>(reinterpret_cast<uintptr_t>(a)), elem * a_stride, elem * row};
+    const Rows y{static_cast<int64_t>(reinterpret_cast<uintptr_t>(b)), elem * b_stride, elem * row};
+    return meet(x, y, n);
+}
+
 void check_page_bytes(const char* what, int dtype, int page_size, int kv_heads) {
     if (static_cast<long long>(page_size) * kv_heads * pa::kHeadDim * (dtype == PA_KV_FP16 ? 2 : 1) > INT_MAX)
         throw std::invalid_argument(std::string(what) + ": page_size * kv heads * row bytes must be below 2^31");

@@ -240,6 +240,8 @@ float inverse_scale(const char* what, int dtype, float scale);
 // head_rows). k_out: k has an output, too; v null: none (k's heads).
 void check_outputs(const char* what, const pa::HeadRows& q, const pa::HeadRows& k, bool k_out, const uint16_t* v,
                    int64_t v_stride, int n);
+// Whether any of n rows of `row` elements of `elem` bytes at a shares a byte with one at b.
+bool rows_overlap(const void* a, int64_t a_stride, const void* b, int64_t b_stride, int64_t row, int elem, int n);
 void check_page_bytes(const char* what, int dtype, int page_size, int kv_heads);
 
 // ---- page pool (pa_pool.cpp)

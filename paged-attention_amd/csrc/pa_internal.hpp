@@ -185,6 +185,60 @@ constexpr size_t kRopeInlineInts = 896;
 static_assert(sizeof(RopeInline<kRopeInlineInts>) <= 4096, "kernel arguments are 4 KiB at most");
 hipError_t launch_norm_rope(const RopeAppend& a, hipStream_t s);
 hipError_t launch_append_rope(int dtype, const RopeAppend& a, const int32_t* meta, size_t n_meta, hipStream_t s);
+// Tokens of several sequences in a paged cache (pa_cached_tokens, checked).
+struct CachedTokens {
+    const int32_t* tok_begin;
+    const int32_t* start;
+    const int32_t* slot_ids;
+    const int32_t* table;
+    void*          k_cache;
+    void*          v_cache;
+    uint8_t*       scales;
+    int            n_tok, n_ent;
+    int            table_stride, table_rows, num_pages, page_size, hkv;
+    float          k_scale, v_scale;
+    PageDiv        by_page;
+};
+// Attention of those tokens over their sequences.
+struct TreeAttention {
+    CachedTokens    c;
+    const uint16_t* q;
+    long            q_stride;
+    uint16_t*       out;
+    long            out_stride;
+    const uint64_t* tree;      // [n_tok][words], or null: a chain
+    int             words;
+    int             group;     // query heads of a kv head
+    PageDiv         by_group;
+    float           score_scale;   // of q k into base-2 exponents
+    // Set by tree_shape, with the workspace.
+    int             rows, tile_tokens, split, grid;
+    float*          part_out;  // [2 grid][rows][128]
+    float*          part_ml;   // [2 grid][rows][2]
+    int32_t*        desc;      // [n_tok][hkv][2]
+};
+// Chooses the launch from the call's sizes (host only, but for the device's CU count).
+void   tree_shape(int dtype, TreeAttention& a);
+size_t tree_workspace(const TreeAttention& a);
+void   tree_place(TreeAttention& a, void* workspace);
+hipError_t launch_tree_attention(int dtype, const TreeAttention& a, hipStream_t s);
+// Rows of the caches into k_out / v_out (one may be null); out_type: pa_value_type.
+struct ReadCache {
+    CachedTokens c;
+    void*        k_out;
+    long         k_stride;
+    void*        v_out;
+    long         v_stride;
+};
+hipError_t launch_read_cache(int dtype, int out_type, const ReadCache& a, hipStream_t s);
+// Accepted rows up in their sequences: kept [n_ent][width], counts [n_ent].
+struct KeepRows {
+    CachedTokens   c;
+    const int32_t* kept;
+    int            width;
+    const int32_t* counts;
+};
+hipError_t launch_keep_rows(int dtype, const KeepRows& a, hipStream_t s);
 // Stores one zero.
 hipError_t launch_zero_int(int32_t* p, hipStream_t s);
 // Copies n ints (rounded up to whole 16 bytes) from pinned host memory to the

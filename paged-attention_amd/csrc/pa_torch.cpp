@@ -294,6 +294,127 @@ OptTensor append_rope(const OptTensor& q, const torch::Tensor& k, const torch::T
     return q ? q_out : OptTensor();
 }
 
+// Caches, table and places of a call over cached tokens (n of them; tok_begin null: none).
+int cached_tokens_of(pa_cached_tokens& c, const torch::Tensor& k_cache, const torch::Tensor& v_cache,
+                     const torch::Tensor& block_table, const torch::Tensor* tok_begin, const torch::Tensor& start_pos,
+                     double k_scale, double v_scale, const OptTensor& kv_scales, const OptTensor& slot_ids, int64_t n) {
+    const int device = k_cache.is_cuda() ? static_cast<int>(k_cache.get_device()) : -1;
+    for (const torch::Tensor* x : {&k_cache, &v_cache})
+        TORCH_CHECK(x->is_cuda() && x->get_device() == device && x->is_contiguous() && x->dim() == 4 &&
+                        x->size(0) <= INT_MAX && x->size(1) > 0 && x->size(1) <= INT_MAX && x->size(2) > 0 &&
+                        x->size(2) <= INT_MAX && x->size(3) == 128 && x->sizes() == k_cache.sizes() &&
+                        (x->scalar_type() == torch::kHalf || x->element_size() == 1) &&
+                        x->scalar_type() == k_cache.scalar_type(),
+                    "k_cache and v_cache must be contiguous CUDA [pages, kv heads, page_size, 128] tensors, both fp16 "
+                    "or both one-byte FP8");
+    const bool fp16 = k_cache.scalar_type() == torch::kHalf;
+    TORCH_CHECK(!kv_scales || !fp16, "kv_scales goes with one-byte FP8 caches");
+    if (kv_scales) check_kv_scales(*kv_scales, k_cache);
+    auto ints = [&](const torch::Tensor& t, int64_t size, const char* what) {
+        TORCH_CHECK(t.is_cuda() && t.get_device() == device && t.scalar_type() == torch::kInt32 && t.is_contiguous() &&
+                        t.dim() == 1 && (size < 0 || t.size(0) == size) && t.size(0) <= INT_MAX,
+                    what);
+        return t.data_ptr<int32_t>();
+    };
+    TORCH_CHECK(n >= 0 && n <= INT_MAX, "too many tokens");
+    c.num_tokens = static_cast<int32_t>(n);
+    c.start_pos  = ints(start_pos, -1, "start_pos must be a contiguous CUDA int32 [entries] tensor");
+    const int64_t m = start_pos.size(0);
+    c.num_entries = static_cast<int32_t>(m);
+    if (tok_begin) c.tok_begin = ints(*tok_begin, m + 1, "tok_begin must be a contiguous CUDA int32 [entries + 1] tensor");
+    if (slot_ids) c.slot_ids = ints(*slot_ids, m, "slot_ids must be a contiguous CUDA int32 [entries] tensor");
+    TORCH_CHECK(block_table.is_cuda() && block_table.get_device() == device && block_table.scalar_type() == torch::kInt32 &&
+                    block_table.is_contiguous() && block_table.dim() == 2 && block_table.size(1) > 0 &&
+                    block_table.size(0) <= INT_MAX && block_table.size(1) <= INT_MAX,
+                "block_table must be a contiguous CUDA int32 [rows, columns] tensor");
+    c.k_cache            = k_cache.data_ptr();
+    c.v_cache            = v_cache.data_ptr();
+    c.kv_scales          = kv_scales ? static_cast<uint8_t*>(kv_scales->data_ptr()) : nullptr;
+    c.block_table        = block_table.data_ptr<int32_t>();
+    c.block_table_stride = static_cast<int32_t>(block_table.size(1));
+    c.num_table_rows     = static_cast<int32_t>(block_table.size(0));
+    c.num_pages          = static_cast<int32_t>(k_cache.size(0));
+    c.page_size          = static_cast<int32_t>(k_cache.size(2));
+    c.num_kv_heads       = static_cast<int32_t>(k_cache.size(1));
+    c.k_scale            = static_cast<float>(k_scale);
+    c.v_scale            = static_cast<float>(v_scale);
+    return kv_scales ? PA_KV_FP8_E4M3_BLOCK : fp16 ? PA_KV_FP16 : PA_KV_FP8_E4M3;
+}
+
+torch::Tensor tree_attention(const torch::Tensor& q, const torch::Tensor& k_cache, const torch::Tensor& v_cache,
+                             const torch::Tensor& block_table, const torch::Tensor& tok_begin,
+                             const torch::Tensor& start_pos, const OptTensor& tree, double k_scale, double v_scale,
+                             const OptTensor& kv_scales, const OptTensor& slot_ids, double sm_scale, OptTensor out) {
+    TORCH_CHECK(q.is_cuda() && q.dim() == 3, "q must be a CUDA fp16 [tokens, heads, 128] tensor");
+    const int64_t n = q.size(0);
+    const int device = q.get_device();
+    pa_cached_tokens c{};
+    const int dtype = cached_tokens_of(c, k_cache, v_cache, block_table, &tok_begin, start_pos, k_scale, v_scale,
+                                       kv_scales, slot_ids, n);
+    TORCH_CHECK(k_cache.get_device() == device, "q and the caches must be on one device");
+    const pa_head_rows r = rows_of("q", q, OptTensor(), 0.0, &out, n, device);
+    int words = 0;
+    if (tree) {
+        TORCH_CHECK(tree->is_cuda() && tree->get_device() == device && tree->scalar_type() == torch::kLong &&
+                        tree->is_contiguous() && tree->dim() == 2 && tree->size(0) == n && tree->size(1) > 0 &&
+                        tree->size(1) <= INT_MAX,
+                    "tree must be a contiguous CUDA int64 [tokens, words] tensor");
+        words = static_cast<int>(tree->size(1));
+    }
+    const OnDevice on(device);
+    size_t bytes = 0;
+    check_status(pa_tree_attention_workspace(dtype, &c, r.heads, &bytes));
+    torch::Tensor ws;
+    if (bytes) ws = torch::Tensor(at::detail::empty_cuda({static_cast<int64_t>(bytes)}, torch::kByte, q.device(), std::nullopt));
+    check_status(pa_tree_attention(dtype, &c, &r, tree ? reinterpret_cast<const uint64_t*>(tree->data_ptr()) : nullptr,
+                                   words, static_cast<float>(sm_scale), bytes ? ws.data_ptr() : nullptr, bytes,
+                                   c10::hip::getCurrentHIPStream(device).stream()));
+    return *out;
+}
+
+std::tuple<torch::Tensor, torch::Tensor> read_cache(const torch::Tensor& k_cache, const torch::Tensor& v_cache,
+                                                    const torch::Tensor& block_table, const torch::Tensor& tok_begin,
+                                                    const torch::Tensor& start_pos, int64_t n, int type,
+                                                    double k_scale, double v_scale, const OptTensor& kv_scales,
+                                                    const OptTensor& slot_ids, OptTensor k_out, OptTensor v_out) {
+    pa_cached_tokens c{};
+    const int dtype = cached_tokens_of(c, k_cache, v_cache, block_table, &tok_begin, start_pos, k_scale, v_scale,
+                                       kv_scales, slot_ids, n);
+    const int device = k_cache.get_device();
+    const auto want = type == PA_VALUE_FP32 ? torch::kFloat : type == PA_VALUE_BF16 ? torch::kBFloat16 : torch::kHalf;
+    for (OptTensor* o : {&k_out, &v_out}) {
+        if (!o->has_value())
+            *o = torch::Tensor(at::detail::empty_cuda({n, k_cache.size(1), 128}, want, k_cache.device(), std::nullopt));
+        const torch::Tensor& x = **o;
+        TORCH_CHECK(x.is_cuda() && x.get_device() == device && x.scalar_type() == want && x.dim() == 3 && x.size(0) == n &&
+                        x.size(1) == k_cache.size(1) && x.size(2) == 128 && x.stride(2) == 1 &&
+                        (x.size(1) == 1 || x.stride(1) == 128),
+                    "k_out and v_out must be CUDA [tokens, kv heads, 128] tensors of the dtype asked for, their heads contiguous");
+    }
+    const OnDevice on(device);
+    check_status(pa_read_cache(dtype, &c, type, k_out->data_ptr(), row_stride(*k_out), v_out->data_ptr(),
+                               row_stride(*v_out), c10::hip::getCurrentHIPStream(device).stream()));
+    return {*k_out, *v_out};
+}
+
+void keep_rows(const torch::Tensor& k_cache, const torch::Tensor& v_cache, const torch::Tensor& block_table,
+               const torch::Tensor& kept, const torch::Tensor& counts, const torch::Tensor& start_pos,
+               const OptTensor& kv_scales, const OptTensor& slot_ids) {
+    pa_cached_tokens c{};
+    const int dtype = cached_tokens_of(c, k_cache, v_cache, block_table, nullptr, start_pos, 1.0, 1.0, kv_scales,
+                                       slot_ids, 0);
+    const int device = k_cache.get_device();
+    TORCH_CHECK(kept.is_cuda() && kept.get_device() == device && kept.scalar_type() == torch::kInt32 &&
+                    kept.is_contiguous() && kept.dim() == 2 && kept.size(0) == c.num_entries && kept.size(1) <= INT_MAX,
+                "kept must be a contiguous CUDA int32 [entries, width] tensor");
+    TORCH_CHECK(counts.is_cuda() && counts.get_device() == device && counts.scalar_type() == torch::kInt32 &&
+                    counts.is_contiguous() && counts.dim() == 1 && counts.size(0) == c.num_entries,
+                "counts must be a contiguous CUDA int32 [entries] tensor");
+    const OnDevice on(device);
+    check_status(pa_keep_rows(dtype, &c, kept.data_ptr<int32_t>(), static_cast<int>(kept.size(1)),
+                              counts.data_ptr<int32_t>(), c10::hip::getCurrentHIPStream(device).stream()));
+}
+
 }  // namespace
 
 PYBIND11_MODULE(TORCH_EXTENSION_NAME, m) {
@@ -311,4 +432,7 @@ PYBIND11_MODULE(TORCH_EXTENSION_NAME, m) {
     // pa_amd.ops gives these their defaults and takes the rotation's handle.
     m.def("norm_rope", &norm_rope);
     m.def("append_rope", &append_rope);
+    m.def("tree_attention", &tree_attention);
+    m.def("read_cache", &read_cache);
+    m.def("keep_rows", &keep_rows);
 }

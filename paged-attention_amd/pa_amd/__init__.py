@@ -14,7 +14,8 @@ from .core import (FP16, FP8_E4M3, FP8_E4M3_BLOCK, DecodePlan, DevicePlan, PageP
                    kv_dtype_name, sm_scale, kv_pool_stagger, alloc_kv_pools)
 
 
-_OPS = ("Rope", "norm_rope", "append_rope", "block_tokens", "alloc_kv_scales")
+_OPS = ("Rope", "norm_rope", "append_rope", "block_tokens", "alloc_kv_scales", "tree_attention",
+        "tree_rows", "keep_rows", "read_cache")
 
 
 def __getattr__(name: str):

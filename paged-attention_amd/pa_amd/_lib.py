@@ -28,6 +28,10 @@ PA_KV_FP16 = 0
 PA_KV_FP8_E4M3 = 1
 PA_KV_FP8_E4M3_BLOCK = 2
 
+PA_VALUE_FP16 = 0
+PA_VALUE_BF16 = 1
+PA_VALUE_FP32 = 2
+
 
 class PaError(Exception):
     """Base class of every error the library reports."""
@@ -119,6 +123,29 @@ class AppendArgs(ctypes.Structure):
     ]
 
 
+class CachedTokens(ctypes.Structure):
+    """pa_cached_tokens."""
+
+    _fields_ = [
+        ("num_tokens", ctypes.c_int32),
+        ("num_entries", ctypes.c_int32),
+        ("tok_begin", ctypes.c_void_p),
+        ("start_pos", ctypes.c_void_p),
+        ("slot_ids", ctypes.c_void_p),
+        ("k_cache", ctypes.c_void_p),
+        ("v_cache", ctypes.c_void_p),
+        ("kv_scales", ctypes.c_void_p),
+        ("block_table", ctypes.c_void_p),
+        ("block_table_stride", ctypes.c_int32),
+        ("num_table_rows", ctypes.c_int32),
+        ("num_pages", ctypes.c_int32),
+        ("page_size", ctypes.c_int32),
+        ("num_kv_heads", ctypes.c_int32),
+        ("k_scale", ctypes.c_float),
+        ("v_scale", ctypes.c_float),
+    ]
+
+
 class CacheConfig(ctypes.Structure):
     """pa_cache_config (paged_kv_cache.hpp:19-29 PagedKVCache::Config)."""
 
@@ -180,6 +207,10 @@ SIGNATURES: dict[str, tuple] = {
     "pa_norm_rope": (_I, [_P, ctypes.POINTER(HeadRows), ctypes.POINTER(HeadRows), _P, _I, _P]),
     "pa_block_tokens": (_I, [_I]),
     "pa_append_rope": (_I, [_I, ctypes.POINTER(AppendArgs), _P, ctypes.POINTER(HeadRows), ctypes.POINTER(HeadRows), _P]),
+    "pa_tree_attention_workspace": (_I, [_I, ctypes.POINTER(CachedTokens), _I, ctypes.POINTER(_S)]),
+    "pa_tree_attention": (_I, [_I, ctypes.POINTER(CachedTokens), ctypes.POINTER(HeadRows), _P, _I, _F, _P, _S, _P]),
+    "pa_read_cache": (_I, [_I, ctypes.POINTER(CachedTokens), _I, _P, _L, _P, _L, _P]),
+    "pa_keep_rows": (_I, [_I, ctypes.POINTER(CachedTokens), _P, _I, _P, _P]),
     "pa_gather_kv": (_I, [_I, _P, _P, _I, _I, _I, _I, _I, _P, _P]),
     "pa_stream_read": (_I, [_P, _S, _I, _P, _P]),
     "pa_stream_read_ex": (_I, [_P, _S, _I, _I, _I, _I, _P, _P]),

@@ -1,9 +1,14 @@
-"""New tokens of a step on torch tensors: head norms with rotation, and appends
-with rotation into caller-owned paged caches (pa_norm_rope, pa_append_rope).
+"""New tokens of a step on torch tensors: head norms with rotation, appends with
+rotation into caller-owned paged caches (pa_norm_rope, pa_append_rope), and what
+drafted tokens need there: attention of several tokens per sequence (pa_tree_attention),
+accepted rows kept (pa_keep_rows), rows read back (pa_read_cache).
 
     rope = Rope(freqs)                                   # a model's rotation, made once
     q, k = norm_rope(q, k, positions, rope, q_weight=wq, k_weight=wk)
     q = append_rope(q, k, v, k_cache, v_cache, block_table, tok_begin, start_pos, rope, ...)
+    out = tree_attention(q, k_cache, v_cache, block_table, tok_begin, start_pos, tree, ...)
+    keep_rows(k_cache, v_cache, block_table, kept, counts, start_pos, ...)
+    k, v = read_cache(k_cache, v_cache, block_table, tok_begin, start_pos, num_tokens, ...)
 
 They run on the current torch stream of the tensors' device, through the compiled
 binding where it was built, else through ctypes. Argument errors raise
@@ -19,7 +24,7 @@ import numpy as np
 import torch
 
 from . import _lib
-from ._lib import AppendArgs, HeadRows, InvalidArgument, call, check, load
+from ._lib import AppendArgs, CachedTokens, HeadRows, InvalidArgument, call, check, load
 from .decoder import _current_stream, _require, compiled
 
 D = 128
@@ -214,6 +219,149 @@ def append_rope(q, k, v, k_cache, v_cache, block_table, tok_begin, start_pos, ro
         check(load().pa_append_rope(dtype, ctypes.byref(a), None if rope is None else rope.handle,
                                     None if qr is None else ctypes.byref(qr), ctypes.byref(kr), _current_stream(dev)))
     return q_out
+
+
+def _cached_tokens(k_cache, v_cache, block_table, tok_begin, start_pos, k_scale, v_scale, kv_scales, slot_ids, n: int):
+    """pa_cached_tokens of n tokens (tok_begin None: none), checked as the compiled binding does, and the cache's type."""
+    dev = k_cache.get_device() if k_cache.is_cuda else -1
+    for x in (k_cache, v_cache):
+        _require(x.is_cuda and x.get_device() == dev and x.is_contiguous() and x.dim() == 4 and x.size(1) > 0
+                 and x.size(2) > 0 and x.size(3) == D and x.shape == k_cache.shape and x.dtype == k_cache.dtype
+                 and (x.dtype == torch.float16 or x.element_size() == 1),
+                 "k_cache and v_cache must be contiguous CUDA [pages, kv heads, page_size, 128] tensors, both fp16 "
+                 "or both one-byte FP8")
+    fp16 = k_cache.dtype == torch.float16
+    _require(kv_scales is None or not fp16, "kv_scales goes with one-byte FP8 caches")
+    if kv_scales is not None:
+        check_kv_scales(kv_scales, k_cache)
+
+    def ints(t, size, what):
+        _require(t.is_cuda and t.get_device() == dev and t.dtype == torch.int32 and t.is_contiguous() and t.dim() == 1
+                 and (size is None or t.size(0) == size), what)
+        return t.data_ptr()
+    _require(0 <= n < 2**31, "too many tokens")
+    c = CachedTokens()
+    c.num_tokens = n
+    c.start_pos = ints(start_pos, None, "start_pos must be a contiguous CUDA int32 [entries] tensor")
+    m = c.num_entries = start_pos.size(0)
+    if tok_begin is not None:
+        c.tok_begin = ints(tok_begin, m + 1, "tok_begin must be a contiguous CUDA int32 [entries + 1] tensor")
+    if slot_ids is not None:
+        c.slot_ids = ints(slot_ids, m, "slot_ids must be a contiguous CUDA int32 [entries] tensor")
+    _require(block_table.is_cuda and block_table.get_device() == dev and block_table.dtype == torch.int32
+             and block_table.is_contiguous() and block_table.dim() == 2 and block_table.size(1) > 0,
+             "block_table must be a contiguous CUDA int32 [rows, columns] tensor")
+    c.k_cache, c.v_cache = k_cache.data_ptr(), v_cache.data_ptr()
+    c.kv_scales = None if kv_scales is None else kv_scales.data_ptr()
+    c.block_table, c.block_table_stride, c.num_table_rows = block_table.data_ptr(), block_table.size(1), block_table.size(0)
+    c.num_pages, c.num_kv_heads, c.page_size = k_cache.size(0), k_cache.size(1), k_cache.size(2)
+    c.k_scale, c.v_scale = float(k_scale), float(v_scale)
+    return c, _lib.PA_KV_FP16 if fp16 else _lib.PA_KV_FP8_E4M3 if kv_scales is None else _lib.PA_KV_FP8_E4M3_BLOCK
+
+
+def tree_rows(parents, device=None) -> torch.Tensor:
+    """tree_attention's `tree` for drafted trees given by their tokens' parents: parents[e][i] is the number within
+    entry e of the token that its token i continues, below i, or -1 where it continues the sequence itself. Returns
+    int64 [tokens of all entries, words of the largest], a token's bits being its own and its ancestors'."""
+    words = max([1] + [(len(p) + 63) // 64 for p in parents])
+    out = np.zeros((sum(len(p) for p in parents), words), dtype=np.uint64)
+    at = 0
+    for p in parents:
+        for i, up in enumerate(p):
+            up = int(up)
+            if not -1 <= up < i:
+                raise InvalidArgument("tree_rows: a token's parent comes before it (-1: the sequence itself)")
+            if up >= 0:
+                out[at + i] = out[at + up]
+            out[at + i, i // 64] |= np.uint64(1 << (i % 64))
+        at += len(p)
+    return torch.from_numpy(out.view(np.int64)).to(device if device is not None else "cuda")
+
+
+def tree_attention(q, k_cache, v_cache, block_table, tok_begin, start_pos, tree=None, *, k_scale: float = 1.0,
+                   v_scale: float = 1.0, kv_scales=None, slot_ids=None, sm_scale: float | None = None, out=None):
+    """Attention of several new tokens per sequence, all of them in the paged cache already, over their sequences:
+    q [n, Hq, 128] fp16 -> out [n, Hq, 128] (Hq up to 32 times the cache's heads; tokens may be strided). Entry e holds tokens
+    tok_begin[e] .. tok_begin[e + 1] - 1 (device int32 [entries + 1]), whose keys and values lie at places start_pos[e],
+    start_pos[e] + 1, ... of the sequence whose pages block_table[slot_ids[e]] lists (row e without slot_ids). Token i
+    of an entry sees every place before start_pos[e] and, of the entry's tokens, those whose bits its row of tree
+    (int64 [n, words]; tree_rows makes it) has, or without tree itself and those before it: a chain, a piece of a
+    prompt. Caches as append_rope's. sm_scale: 1 / sqrt(128) unless given. A token that sees nothing gets zeros;
+    tokens of no entry (padding), or of one out of range, keep what out held; out may be q. Returns out."""
+    scale = 1.0 / math.sqrt(D) if sm_scale is None else float(sm_scale)
+    c = compiled()
+    if c is not None:
+        return c.tree_attention(q, k_cache, v_cache, block_table, tok_begin, start_pos, tree, k_scale, v_scale,
+                                kv_scales, slot_ids, scale, out)
+    _require(q.is_cuda and q.dim() == 3, "q must be a CUDA fp16 [tokens, heads, 128] tensor")
+    n, dev = q.size(0), q.get_device()
+    a, dtype = _cached_tokens(k_cache, v_cache, block_table, tok_begin, start_pos, k_scale, v_scale, kv_scales, slot_ids, n)
+    _require(k_cache.get_device() == dev, "q and the caches must be on one device")
+    out = torch.empty((n, q.size(1), D), dtype=torch.float16, device=q.device) if out is None else out
+    r = head_rows("q", q, None, 0.0, out, dev)
+    if tree is not None:
+        _require(tree.is_cuda and tree.get_device() == dev and tree.dtype == torch.int64 and tree.is_contiguous()
+                 and tree.dim() == 2 and tree.size(0) == n and tree.size(1) > 0,
+                 "tree must be a contiguous CUDA int64 [tokens, words] tensor")
+    with torch.cuda.device(dev):
+        need = ctypes.c_size_t()
+        check(load().pa_tree_attention_workspace(dtype, ctypes.byref(a), q.size(1), ctypes.byref(need)))
+        ws = torch.empty(need.value, dtype=torch.uint8, device=q.device) if need.value else None
+        check(load().pa_tree_attention(dtype, ctypes.byref(a), ctypes.byref(r), None if tree is None else tree.data_ptr(),
+                                       0 if tree is None else tree.size(1), scale, None if ws is None else ws.data_ptr(),
+                                       need.value, _current_stream(dev)))
+    return out
+
+
+_VALUE_TYPES = {torch.float16: _lib.PA_VALUE_FP16, torch.bfloat16: _lib.PA_VALUE_BF16, torch.float32: _lib.PA_VALUE_FP32}
+
+
+def read_cache(k_cache, v_cache, block_table, tok_begin, start_pos, num_tokens: int, *, dtype=torch.float16,
+               k_scale: float = 1.0, v_scale: float = 1.0, kv_scales=None, slot_ids=None, k_out=None, v_out=None):
+    """Rows of a paged cache as numbers: token t of num_tokens (those of the last entry and any padding behind) of
+    entry e, the place start_pos[e] + t - tok_begin[e] of its sequence, to k_out[t] and v_out[t] ([n, Hkv, 128] of
+    dtype: float16, bfloat16 or float32; tokens may be strided). Entries, tables and caches as tree_attention's. Tokens
+    of no entry, and those whose place, row or page is out of range, keep what the outputs held. Returns (k_out, v_out)."""
+    _require(dtype in _VALUE_TYPES, "dtype must be float16, bfloat16 or float32")
+    c = compiled()
+    if c is not None:
+        return c.read_cache(k_cache, v_cache, block_table, tok_begin, start_pos, num_tokens, _VALUE_TYPES[dtype], k_scale,
+                            v_scale, kv_scales, slot_ids, k_out, v_out)
+    a, cache = _cached_tokens(k_cache, v_cache, block_table, tok_begin, start_pos, k_scale, v_scale, kv_scales, slot_ids,
+                              num_tokens)
+    dev = k_cache.get_device()
+    outs = []
+    for x in (k_out, v_out):
+        x = torch.empty((num_tokens, k_cache.size(1), D), dtype=dtype, device=k_cache.device) if x is None else x
+        _require(x.is_cuda and x.get_device() == dev and x.dtype == dtype and x.dim() == 3 and x.size(0) == num_tokens
+                 and x.size(1) == k_cache.size(1) and x.size(2) == D and x.stride(2) == 1
+                 and (x.size(1) == 1 or x.stride(1) == D),
+                 "k_out and v_out must be CUDA [tokens, kv heads, 128] tensors of the dtype asked for, their heads contiguous")
+        outs.append(x)
+    with torch.cuda.device(dev):
+        check(load().pa_read_cache(cache, ctypes.byref(a), _VALUE_TYPES[dtype], outs[0].data_ptr(), _row_stride(outs[0]),
+                                   outs[1].data_ptr(), _row_stride(outs[1]), _current_stream(dev)))
+    return outs[0], outs[1]
+
+
+def keep_rows(k_cache, v_cache, block_table, kept, counts, start_pos, *, kv_scales=None, slot_ids=None) -> None:
+    """Accepted drafted tokens up in their sequences, in place: of the rows at places start_pos[e], start_pos[e] + 1,
+    ... those with the numbers kept[e][0] < ... < kept[e][counts[e] - 1] (device int32 [entries, width] and [entries])
+    go to places start_pos[e], start_pos[e] + 1, ... of their sequence. Each sequence once a call. Rows past the last
+    kept one keep their bytes. In block-scaled caches the blocks that a row moves into get the scale that their kept
+    rows ask for, as an append chooses it."""
+    c = compiled()
+    if c is not None:
+        return c.keep_rows(k_cache, v_cache, block_table, kept, counts, start_pos, kv_scales, slot_ids)
+    a, cache = _cached_tokens(k_cache, v_cache, block_table, None, start_pos, 1.0, 1.0, kv_scales, slot_ids, 0)
+    dev = k_cache.get_device()
+    _require(kept.is_cuda and kept.get_device() == dev and kept.dtype == torch.int32 and kept.is_contiguous()
+             and kept.dim() == 2 and kept.size(0) == a.num_entries, "kept must be a contiguous CUDA int32 [entries, width] tensor")
+    _require(counts.is_cuda and counts.get_device() == dev and counts.dtype == torch.int32 and counts.is_contiguous()
+             and counts.dim() == 1 and counts.size(0) == a.num_entries, "counts must be a contiguous CUDA int32 [entries] tensor")
+    with torch.cuda.device(dev):
+        check(load().pa_keep_rows(cache, ctypes.byref(a), kept.data_ptr(), kept.size(1), counts.data_ptr(),
+                                  _current_stream(dev)))
 
 
 def check_kv_scales(s, cache) -> None:
