@@ -9,6 +9,7 @@
 #include <cstdint>
 #include <stdexcept>
 #include <string>
+#include <type_traits>
 
 namespace pa {
 namespace {
@@ -18,8 +19,8 @@ typedef float    f32x2  __attribute__((ext_vector_type(2)));
 typedef short    s16x4  __attribute__((ext_vector_type(4)));
 
 constexpr int kSub     = 32;              // places of one MFMA step
-constexpr int kWavesT  = 4;
-constexpr int kThreads = 64 * kWavesT;
+constexpr int kScan    = 256;             // entries that a block looks at together
+constexpr int kMergeWaves = 4;
 constexpr int kOutLd   = kHeadDim + 4;    // floats of a row in the joining of waves
 
 // A probability is kept as 2^(score - reference + kShift) in fp16, where the reference
@@ -40,7 +41,7 @@ __device__ __forceinline__ Entry entry_at(const CachedTokens& c, int e) {
     x.start = load_uniform(c.start, e);
     x.row   = c.slot_ids ? load_uniform(c.slot_ids, e) : e;
     const bool ok = x.t0 >= 0 && x.n > 0 && x.start >= 0 && x.row >= 0 && x.row < c.table_rows &&
-                    static_cast<long>(x.start) + x.n <= min(static_cast<long>(c.table_stride) * c.page_size, static_cast<long>(INT_MAX - kSub * kWavesT));
+                    static_cast<long>(x.start) + x.n <= min(static_cast<long>(c.table_stride) * c.page_size, static_cast<long>(INT_MAX - 256));
     if (!ok) x.n = 0;
     return x;
 }
@@ -52,7 +53,7 @@ __device__ __forceinline__ Entry entry_of_lane(const CachedTokens& c, int e) {
     x.start = c.start[e];
     x.row   = c.slot_ids ? c.slot_ids[e] : e;
     const bool ok = x.t0 >= 0 && x.n > 0 && x.start >= 0 && x.row >= 0 && x.row < c.table_rows &&
-                    static_cast<long>(x.start) + x.n <= min(static_cast<long>(c.table_stride) * c.page_size, static_cast<long>(INT_MAX - kSub * kWavesT));
+                    static_cast<long>(x.start) + x.n <= min(static_cast<long>(c.table_stride) * c.page_size, static_cast<long>(INT_MAX - 256));
     if (!ok) x.n = 0;
     return x;
 }
@@ -66,38 +67,40 @@ __device__ __forceinline__ long entry_cost(const TreeAttention& a, const Entry& 
 }
 
 struct Schedule {
-    long pre[kThreads + 1];   // units before each entry of the chunk
-    long wave_sum[kWavesT];
+    long pre[kScan + 1];   // units before each entry of the chunk
+    long wave_sum[kScan / 64];
     int  hit;
 };
 
-// The units of entries c0 .. c0 + 255 as a running sum in s.pre.
-__device__ long scan_chunk(const TreeAttention& a, Schedule& s, int c0, int step) {
+// The units of entries c0 .. c0 + 255 as a running sum in s.pre (by the block's first 256 threads).
+__device__ __forceinline__ long scan_chunk(const TreeAttention& a, Schedule& s, int c0, int step) {
     const int tid = threadIdx.x, lane = tid & 63, wave = tid >> 6;
     if (a.c.n_ent == 1) {
         const long one = entry_cost(a, entry_at(a.c, 0), step);
-        __syncthreads();
-        s.pre[tid + 1] = one;
-        if (tid == 0) s.pre[0] = 0;
+        if (tid == 0) {
+            s.pre[0] = 0;
+            s.pre[1] = one;
+        }
         __syncthreads();
         return one;
     }
-    long x = c0 + tid < a.c.n_ent ? entry_cost(a, entry_of_lane(a.c, c0 + tid), step) : 0;
+    const bool mine = tid < kScan;
+    long x = mine && c0 + tid < a.c.n_ent ? entry_cost(a, entry_of_lane(a.c, c0 + tid), step) : 0;
 #pragma unroll
     for (int o = 1; o < 64; o <<= 1) {
         const long y = __shfl_up(x, o);
         if (lane >= o) x += y;
     }
     __syncthreads();
-    if (lane == 63) s.wave_sum[wave] = x;
+    if (mine && lane == 63) s.wave_sum[wave] = x;
     __syncthreads();
     long before = 0, total = 0;
 #pragma unroll
-    for (int w = 0; w < kWavesT; ++w) {
+    for (int w = 0; w < kScan / 64; ++w) {
         if (w < wave) before += s.wave_sum[w];
         total += s.wave_sum[w];
     }
-    s.pre[tid + 1] = before + x;
+    if (mine) s.pre[tid + 1] = before + x;
     if (tid == 0) s.pre[0] = 0;
     __syncthreads();
     return total;
@@ -147,18 +150,27 @@ __device__ __forceinline__ uint32_t visible(const TreeAttention& a, const Entry&
     return bits & ones(x.n - j0);
 }
 
-// EB: bytes of a cached value; BS: block scales. 32 RQ rows a wave, WQ waves of rows,
-// WK waves along the places.
-template <int EB, bool BS, int RQ, int WQ, int WK>
+// EB: bytes of a cached value; BS: block scales. A wave holds 32 rows of queries; WQ
+// waves of rows share a stream of places, WK streams are joined at the end. UNI: pages
+// hold whole runs of 4 places, so a load of 4 rows lies in one page.
+template <int EB, bool BS, int WQ, int WK, bool UNI>
 struct TreeKernel {
-    static constexpr int kRowsM = 32 * RQ * WQ;
-    static constexpr int kStep  = kSub * WK;
-    static constexpr int NJ     = 8 / WQ;              // 8-dim chunks of K (and of V) per thread and step
-    static constexpr int kBufs  = WQ > 1 ? 2 : 1;
-    static constexpr int kTile  = kSub * 256;          // bytes of 32 rows in fp16
-    static constexpr int kStage = WK * kBufs * (2 * kTile + (BS ? 128 : 0));
-    static constexpr int kJoin  = kWavesT * 32 * kOutLd * 4 + kWavesT * 32 * 8;
-    static constexpr int kLds   = kStage > kJoin ? kStage : kJoin;
+    static constexpr int kWaves  = WQ * WK;
+    static constexpr int kBlock  = 64 * kWaves;
+    static constexpr int kRowsM  = 32 * WQ;
+    static constexpr int SUBS    = WQ >= 4 ? 2 : 1;            // 32-place parts of a stream's step
+    static constexpr int kPart   = kSub * SUBS;                // places of a stream's step
+    static constexpr int kStep   = kPart * WK;
+    static constexpr int NJ      = kPart / (4 * WQ);           // loads of 4 rows per wave, of K and of V
+    static constexpr int kBufs   = WQ > 1 ? 2 : 1;
+    static constexpr int kTile   = kPart * 256;                // bytes of a step's rows in fp16
+    static constexpr int kBuf    = 2 * kTile + (BS ? 4 * kPart / 4 : 0);
+    static constexpr int kStage  = WK * kBufs * kBuf;
+    static constexpr int kJoin   = kWaves * 32 * (kOutLd * 4 + 8);
+    static constexpr int kJoinOf = WK > 1 ? kJoin : 0;
+    static constexpr int kLds    = kStage > kJoinOf ? kStage : kJoinOf;
+    static constexpr int RG      = UNI ? 4 : 1;                // rows that a lane looks up
+    static_assert(kPart / RG <= 64 && NJ >= 1);
 
     typedef uint32_t Raw __attribute__((ext_vector_type(EB == 2 ? 4 : 2)));
 
@@ -168,22 +180,23 @@ struct TreeKernel {
         const int nb = gridDim.x;
         const int lb = nb % 8 == 0 ? (blockIdx.x % 8) * (nb / 8) + blockIdx.x / 8 : blockIdx.x;
         long total = 0, chunk = 0;
-        for (int c0 = 0; c0 < a.c.n_ent; c0 += kThreads) total += chunk = scan_chunk(a, sch, c0, kStep);
+        for (int c0 = 0; c0 < a.c.n_ent; c0 += kScan) total += chunk = scan_chunk(a, sch, c0, kStep);
         const long per = a.split ? max((total + nb - 1) / nb, 1l) : 1;
         long w = lb * per;
         const long w_end = min(w + per, total);
         if (w >= w_end) return;
         int  c0 = 0;
         long before = 0;
-        if (a.c.n_ent > kThreads) chunk = scan_chunk(a, sch, 0, kStep);
+        if (a.c.n_ent > kScan) chunk = scan_chunk(a, sch, 0, kStep);
         const long w_first = w;
         while (w < w_end) {
             while (w >= before + chunk) {
                 before += chunk;
-                c0 += kThreads;
+                c0 += kScan;
                 chunk = scan_chunk(a, sch, c0, kStep);
             }
-            if (sch.pre[threadIdx.x] <= w - before && w - before < sch.pre[threadIdx.x + 1]) sch.hit = threadIdx.x;
+            const int tid = threadIdx.x;
+            if (tid < kScan && sch.pre[tid] <= w - before && w - before < sch.pre[tid + 1]) sch.hit = tid;
             __syncthreads();
             const int  hit = a.c.n_ent == 1 ? 0 : __builtin_amdgcn_readfirstlane(sch.hit);
             const long at  = before + sch.pre[hit];
@@ -203,7 +216,7 @@ struct TreeKernel {
                 // For the merge: where the item's parts lie.
                 const long b0 = w / per, b1 = (at + (item + 1) * units - 1) / per;
                 const int  n  = min(a.tile_tokens, x.n - rt * a.tile_tokens);
-                for (int i = threadIdx.x; i < n; i += kThreads) {
+                for (int i = threadIdx.x; i < n; i += kBlock) {
                     int32_t* d = a.desc + 2 * (static_cast<size_t>(x.t0 + rt * a.tile_tokens + i) * a.c.hkv + h);
                     d[0] = static_cast<int>(2 * b0 + (w == w_first ? 0 : 1));
                     d[1] = static_cast<int>(b1 - b0 + 1);
@@ -227,64 +240,75 @@ struct TreeKernel {
         const int end = x.start + (a.tree ? x.n : tok0 + tile_n);   // places from here on are not seen
         k1 = min(k1, (end + kStep - 1) / kStep);
 
-        // Query fragments, and each lane's token.
-        f16x8 q[RQ][8];
-        int   tok[RQ];
+        // Query fragments, and the lane's token.
+        f16x8 q[8];
+        const int my_row = 32 * wq + ql, my_i = a.by_group.page(my_row), my_g = my_row - my_i * G;
+        const bool row_ok = my_i < tile_n;
+        const int  tok = row_ok ? tok0 + my_i : INT_MAX;
+        {
+            const uint16_t* p = a.q + (x.t0 + tok0 + (row_ok ? my_i : 0)) * a.q_stride + (h * G + (row_ok ? my_g : 0)) * kHeadDim + 8 * hl;
 #pragma unroll
-        for (int r = 0; r < RQ; ++r) {
-            const int row = 32 * (RQ * wq + r) + ql;
-            const int i = a.by_group.page(row), g = row - i * G;
-            const bool ok = i < tile_n;
-            tok[r] = ok ? tok0 + i : INT_MAX;
-            const uint16_t* p = a.q + (x.t0 + tok0 + (ok ? i : 0)) * a.q_stride + (h * G + (ok ? g : 0)) * kHeadDim + 8 * hl;
-#pragma unroll
-            for (int s = 0; s < 8; ++s) q[r][s] = __builtin_bit_cast(f16x8, *reinterpret_cast<const u32x4*>(p + 16 * s));
+            for (int s = 0; s < 8; ++s) q[s] = __builtin_bit_cast(f16x8, *reinterpret_cast<const u32x4*>(p + 16 * s));
         }
-        // First token of the wave's rows: what it sees all of them see, in a chain.
-        const int first_tok = tok0 + a.by_group.page(32 * RQ * wq);
+        // Places before this one are seen by every row of the wave.
+        const int open_end = x.start + (a.tree ? 0 : tok0 + a.by_group.page(32 * wq) + 1);
 
-        f32x16 o[RQ][4];
-        float  m[RQ], l[RQ];
+        f32x16 o[4];
+        float  m = -INFINITY, l = 0.f;
 #pragma unroll
-        for (int r = 0; r < RQ; ++r) {
-            m[r] = -INFINITY;
-            l[r] = 0.f;
+        for (int d = 0; d < 4; ++d)
 #pragma unroll
-            for (int d = 0; d < 4; ++d)
-#pragma unroll
-                for (int i = 0; i < 16; ++i) o[r][d][i] = 0.f;
-        }
+            for (int i = 0; i < 16; ++i) o[d][i] = 0.f;
 
-        // Staging: this thread's rows row0 + 4 WQ j of a step's 32, chunk ch of each.
-        const int gt = 64 * wq + lane, row0 = gt >> 4, ch = gt & 15;
+        // Staging. Lane i looks up rows RG i .. of a step; load j of a wave takes the 4 rows
+        // from 4 (wq + WQ j) on, 16 lanes a row, 8 dims each.
+        const int row0 = lane >> 4, ch = lane & 15;
         const int32_t* table = c.table + static_cast<size_t>(x.row) * c.table_stride;
         const size_t page_bytes = static_cast<size_t>(c.hkv) * P * kRowBytes<EB>;
-        const size_t head_off   = static_cast<size_t>(h) * P * kRowBytes<EB> + ch * 8 * EB;
+        const size_t head_off   = static_cast<size_t>(h) * P * kRowBytes<EB>;
         const int    bsh = BS ? (P % 16 == 0 ? 4 : 3) : 0, nblk = BS ? P >> bsh : 0;
-        int      pg[NJ];
+        int      pg = -1;
         Raw      kr[NJ], vr[NJ];
-        uint32_t sc[NJ];
-        uint32_t live = 0;   // rows of kr / vr that hold a place
+        uint32_t sc = 0;       // the lane's rows' scale pair
+        uint32_t live = 0;     // general pages: loads whose row holds a place
         auto lookup = [&](int k) {
-#pragma unroll
-            for (int j = 0; j < NJ; ++j) {
-                const int t = k * kStep + kSub * wk + row0 + 4 * WQ * j;
-                pg[j] = t < end ? table[c.by_page.page(t)] : -1;
-            }
+            const int t = k * kStep + kPart * wk + RG * lane;
+            pg = lane < kPart / RG && t < end ? table[c.by_page.page(t)] : -1;
         };
         auto issue = [&](int k) {
+            const int  t  = k * kStep + kPart * wk + RG * lane;
+            const bool ok = pg >= 0 && pg < c.num_pages;
+            const int  s  = t - c.by_page.page(t) * P;
+            const size_t off = ok ? pg * page_bytes + head_off + static_cast<size_t>(s) * kRowBytes<EB> : 0;
+            const uint32_t lo = static_cast<uint32_t>(off), hi = static_cast<uint32_t>(off >> 32);
+            const int rows = ok ? min(RG, end - t) : 0;
+            if constexpr (BS)
+                sc = rows > 0 ? *reinterpret_cast<const uint16_t*>(c.scales + 2 * ((static_cast<size_t>(pg) * c.hkv + h) * nblk + (s >> bsh))) : 0;
             live = 0;
 #pragma unroll
             for (int j = 0; j < NJ; ++j) {
-                const int t = k * kStep + kSub * wk + row0 + 4 * WQ * j;
-                const bool ok = pg[j] >= 0 && pg[j] < c.num_pages;
-                live |= ok ? 1u << j : 0u;
-                const int page = ok ? pg[j] : 0, s = ok ? t - c.by_page.page(t) * P : 0;
-                const size_t off = page * page_bytes + head_off + static_cast<size_t>(s) * kRowBytes<EB>;
-                kr[j] = *reinterpret_cast<const Raw*>(static_cast<const unsigned char*>(c.k_cache) + off);
-                vr[j] = *reinterpret_cast<const Raw*>(static_cast<const unsigned char*>(c.v_cache) + off);
-                if constexpr (BS)
-                    sc[j] = *reinterpret_cast<const uint16_t*>(c.scales + 2 * ((static_cast<size_t>(page) * c.hkv + h) * nblk + (s >> bsh)));
+                const int r4 = wq + WQ * j;   // run of 4 rows
+                if constexpr (UNI) {
+                    const size_t at = static_cast<size_t>(static_cast<uint32_t>(__builtin_amdgcn_readlane(hi, r4))) << 32 |
+                                      static_cast<uint32_t>(__builtin_amdgcn_readlane(lo, r4));
+                    const int bytes = __builtin_amdgcn_readlane(rows, r4) * kRowBytes<EB>;
+                    const __amdgpu_buffer_rsrc_t kb = buffer_rsrc(static_cast<const unsigned char*>(c.k_cache) + at, bytes);
+                    const __amdgpu_buffer_rsrc_t vb = buffer_rsrc(static_cast<const unsigned char*>(c.v_cache) + at, bytes);
+                    if constexpr (EB == 2) {
+                        kr[j] = __builtin_bit_cast(Raw, __builtin_amdgcn_raw_buffer_load_b128(kb, 16 * lane, 0, 0));
+                        vr[j] = __builtin_bit_cast(Raw, __builtin_amdgcn_raw_buffer_load_b128(vb, 16 * lane, 0, 0));
+                    } else {
+                        kr[j] = __builtin_bit_cast(Raw, __builtin_amdgcn_raw_buffer_load_b64(kb, 8 * lane, 0, 0));
+                        vr[j] = __builtin_bit_cast(Raw, __builtin_amdgcn_raw_buffer_load_b64(vb, 8 * lane, 0, 0));
+                    }
+                } else {
+                    const int from = 4 * r4 + row0;
+                    const size_t at = (static_cast<size_t>(static_cast<uint32_t>(__shfl(static_cast<int>(hi), from))) << 32 |
+                                       static_cast<uint32_t>(__shfl(static_cast<int>(lo), from))) + ch * 8 * EB;
+                    live |= __shfl(rows, from) > 0 ? 1u << j : 0u;
+                    kr[j] = *reinterpret_cast<const Raw*>(static_cast<const unsigned char*>(c.k_cache) + at);
+                    vr[j] = *reinterpret_cast<const Raw*>(static_cast<const unsigned char*>(c.v_cache) + at);
+                }
             }
         };
         auto widen = [](Raw x, float scale) {
@@ -292,22 +316,24 @@ struct TreeKernel {
             else return u32x4{fp8x2_to_f16x2<false>(x[0], scale), fp8x2_to_f16x2<true>(x[0], scale),
                               fp8x2_to_f16x2<false>(x[1], scale), fp8x2_to_f16x2<true>(x[1], scale)};
         };
-        auto stage_at = [&](int buf) { return lds + (wk * kBufs + buf) * (2 * kTile + (BS ? 128 : 0)); };
+        auto stage_at = [&](int buf) { return lds + (wk * kBufs + buf) * kBuf; };
         auto store = [&](int buf) {
             unsigned char* k = stage_at(buf);
 #pragma unroll
             for (int j = 0; j < NJ; ++j) {
-                const int row = row0 + 4 * WQ * j;
-                const bool ok = live >> j & 1;
-                const float vs = BS ? __builtin_bit_cast(float, (sc[j] >> 8) << 23) : 1.0f;
+                const int r4 = wq + WQ * j, row = 4 * r4 + row0;
+                float vs = 1.0f;
+                if constexpr (BS) {
+                    const uint32_t pair = __builtin_amdgcn_readlane(sc, r4 * 4 / RG);
+                    vs = __builtin_bit_cast(float, (pair >> 8) << 23);
+                    if (lane == 0)
+                        *reinterpret_cast<float*>(k + 2 * kTile + 4 * r4) = a.score_scale * __builtin_bit_cast(float, (pair & 0xff) << 23);
+                }
                 u32x4 kx = widen(kr[j], 1.0f), vx = widen(vr[j], vs);
-                if (!ok) kx = vx = u32x4{0, 0, 0, 0};
+                if (!UNI && !(live >> j & 1)) kx = vx = u32x4{0, 0, 0, 0};
                 const int at = row * 256 + ((ch ^ swizzle(row)) << 4);
                 *reinterpret_cast<u32x4*>(k + at) = kx;
                 *reinterpret_cast<u32x4*>(k + kTile + at) = vx;
-                if constexpr (BS)
-                    if (ch == 0)
-                        *reinterpret_cast<float*>(k + 2 * kTile + 4 * row) = __builtin_bit_cast(float, (sc[j] & 0xff) << 23);
             }
         };
 
@@ -316,135 +342,138 @@ struct TreeKernel {
         const int vi = lane & 15, vg = (lane >> 4) & 1;
         const int va = (4 * hl + (vi >> 2)) * 256 + ((((vi >> 2) << 2) | ((2 * vg + ((vi >> 1) & 1)) ^ hl)) << 4) + 8 * (vi & 1);
 
-        auto compute = [&](int k, int buf) {
-            const int base = k * kStep + kSub * wk;
-            if (base >= end) return;
-            const unsigned char* ks = stage_at(buf);
+        auto step_of = [&](auto masked_c, int base, const unsigned char* ks) {
+            constexpr bool MASK = decltype(masked_c)::value;
             const unsigned char* vs = ks + kTile;
-            f32x16 s[RQ];
+            f32x16 s[SUBS];
 #pragma unroll
-            for (int r = 0; r < RQ; ++r)
+            for (int b = 0; b < SUBS; ++b) {
 #pragma unroll
-                for (int i = 0; i < 16; ++i) s[r][i] = 0.f;
+                for (int i = 0; i < 16; ++i) s[b][i] = 0.f;
 #pragma unroll
-            for (int t = 0; t < 8; ++t) {
-                const f16x8 kf = *reinterpret_cast<const f16x8*>(ks + (ka ^ (t << 5)));
-#pragma unroll
-                for (int r = 0; r < RQ; ++r) s[r] = __builtin_amdgcn_mfma_f32_32x32x16_f16(kf, q[r][t], s[r], 0, 0, 0);
-            }
-            float cs[4];   // base-2 scores of a raw product, per eight places
-#pragma unroll
-            for (int i = 0; i < 4; ++i)
-                cs[i] = BS ? a.score_scale * *reinterpret_cast<const float*>(ks + 2 * kTile + 32 * i) : a.score_scale;
-            const bool masked = base + kSub > x.start + (a.tree ? 0 : first_tok + 1);
-            uint32_t seen[RQ];
-            f16x8    p[RQ][2];
-#pragma unroll
-            for (int r = 0; r < RQ; ++r) {
-                seen[r] = ~0u;
-                if (masked) {
-                    seen[r] = visible(a, x, tok[r], base - x.start);
-                    const uint32_t mine = seen[r] >> (4 * hl);
-#pragma unroll
-                    for (int i = 0; i < 16; ++i) s[r][i] = mine >> (8 * (i / 4) + i % 4) & 1 ? s[r][i] * cs[i / 4] : -INFINITY;
-                } else {
-#pragma unroll
-                    for (int i = 0; i < 16; ++i) s[r][i] *= cs[i / 4];
-                }
-                float top = s[r][0];
-#pragma unroll
-                for (int i = 1; i < 16; ++i) top = fmaxf(top, s[r][i]);
-                top = max_halves(top);
-                if (__builtin_amdgcn_ballot_w64(top > m[r] + kLag) != 0) {
-                    const float now = fmaxf(m[r], top), ref = now == -INFINITY ? 0.f : now;
-                    const float f = exp2_fast(m[r] - ref);
-                    l[r] *= f;
-#pragma unroll
-                    for (int d = 0; d < 4; ++d)
-#pragma unroll
-                        for (int i = 0; i < 16; ++i) o[r][d][i] *= f;
-                    m[r] = now;
-                }
-                const float ref = (m[r] == -INFINITY ? 0.f : m[r]) - kShift;
-#pragma unroll
-                for (int i = 0; i < 16; ++i) {
-                    const float e = exp2_fast(s[r][i] - ref);
-                    l[r] += e;
-                    p[r][i / 8][i % 8] = static_cast<_Float16>(e);
+                for (int t = 0; t < 8; ++t) {
+                    const f16x8 kf = *reinterpret_cast<const f16x8*>(ks + (ka ^ (t << 5)) + b * kSub * 256);
+                    s[b] = __builtin_amdgcn_mfma_f32_32x32x16_f16(kf, q[t], s[b], 0, 0, 0);
                 }
             }
-            auto v_part = [&](int d, int u, int w) {
-                const int at = (va ^ (d << 6) ^ (w << 5)) + (16 * u + 8 * w) * 256;
-                return __builtin_amdgcn_ds_read_tr16_b64_v4i16((__attribute__((address_space(3))) s16x4*)(vs + at));
-            };
-            auto v_frag = [&](int d, int u) {
-                const s16x4 lo = v_part(d, u, 0), hi = v_part(d, u, 1);
-                return __builtin_bit_cast(f16x8, __builtin_shufflevector(lo, hi, 0, 1, 2, 3, 4, 5, 6, 7));
-            };
-            if (!masked) {
+            uint32_t seen[SUBS];
+            float top = -INFINITY;
+            const float one = a.score_scale;
+#pragma unroll
+            for (int b = 0; b < SUBS; ++b) {
+                if constexpr (BS) {
+                    // Scores in base 2 (elsewhere the one scale goes into the exponent's argument).
+#pragma unroll
+                    for (int i = 0; i < 4; ++i) {
+                        const float cs = *reinterpret_cast<const float*>(ks + 2 * kTile + 4 * (8 * b + 2 * i + hl));
+#pragma unroll
+                        for (int e = 0; e < 4; ++e) s[b][4 * i + e] *= cs;
+                    }
+                }
+                if constexpr (MASK) {
+                    seen[b] = visible(a, x, tok, base + kSub * b - x.start);
+                    const uint32_t mine = seen[b] >> (4 * hl);
+#pragma unroll
+                    for (int i = 0; i < 16; ++i)
+                        s[b][i] = mine >> (8 * (i / 4) + i % 4) & 1 ? (BS ? s[b][i] : s[b][i] * one) : -INFINITY;
+                } else if constexpr (!BS) {
+#pragma unroll
+                    for (int i = 0; i < 16; ++i) s[b][i] *= one;
+                }
+#pragma unroll
+                for (int i = 0; i < 16; ++i) top = fmaxf(top, s[b][i]);
+            }
+            top = max_halves(top);
+            if (__builtin_amdgcn_ballot_w64(top > m + kLag) != 0) {
+                const float now = fmaxf(m, top), ref = now == -INFINITY ? 0.f : now;
+                const float f = exp2_fast(m - ref);
+                l *= f;
 #pragma unroll
                 for (int d = 0; d < 4; ++d)
 #pragma unroll
-                    for (int u = 0; u < 2; ++u) {
-                        const f16x8 v = v_frag(d, u);
-#pragma unroll
-                        for (int r = 0; r < RQ; ++r)
-                            o[r][d] = __builtin_amdgcn_mfma_f32_32x32x16_f16(v, p[r][u], o[r][d], 0, 0, 0);
-                    }
-                return;
+                    for (int i = 0; i < 16; ++i) o[d][i] *= f;
+                m = now;
             }
-            // A place that a row does not see must not reach it, whatever its value: 0 * infinity
-            // is NaN. Values that are not finite are taken as zeros, and then added as such to the
-            // rows that see them: how many of each sign a row sees comes from two more products.
-            uint32_t odd = 0;
+            const float ref = (m == -INFINITY ? 0.f : m) - kShift;
+            f16x8 p[SUBS][2];
 #pragma unroll
-            for (int d = 0; d < 4; ++d)
+            for (int b = 0; b < SUBS; ++b)
 #pragma unroll
-                for (int u = 0; u < 2; ++u) {
-                    f16x8 v = v_frag(d, u);
-                    u32x4 b = __builtin_bit_cast(u32x4, v);
-                    bool bad = false;
-#pragma unroll
-                    for (int e = 0; e < 8; ++e) bad |= (b[e / 2] >> (16 * (e & 1)) & 0x7c00u) == 0x7c00u;
-                    if (__builtin_amdgcn_ballot_w64(bad) != 0) {
-                        odd |= 1u << d;
-#pragma unroll
-                        for (int e = 0; e < 8; ++e)
-                            if ((b[e / 2] >> (16 * (e & 1)) & 0x7c00u) == 0x7c00u) v[e] = static_cast<_Float16>(0.f);
-                    }
-#pragma unroll
-                    for (int r = 0; r < RQ; ++r)
-                        o[r][d] = __builtin_amdgcn_mfma_f32_32x32x16_f16(v, p[r][u], o[r][d], 0, 0, 0);
+                for (int i = 0; i < 16; ++i) {
+                    const float e = exp2_fast(s[b][i] - ref);
+                    l += e;
+                    p[b][i / 8][i % 8] = static_cast<_Float16>(e);
                 }
-            if (odd == 0) return;
+            auto v_part = [&](int b, int d, int u, int w) {
+                const int at = (va ^ (d << 6) ^ (w << 5)) + (kSub * b + 16 * u + 8 * w) * 256;
+                return __builtin_amdgcn_ds_read_tr16_b64_v4i16((__attribute__((address_space(3))) s16x4*)(vs + at));
+            };
+            auto v_frag = [&](int b, int d, int u) {
+                const s16x4 lo = v_part(b, d, u, 0), hi = v_part(b, d, u, 1);
+                return __builtin_bit_cast(f16x8, __builtin_shufflevector(lo, hi, 0, 1, 2, 3, 4, 5, 6, 7));
+            };
+            if constexpr (!MASK) {
 #pragma unroll
-            for (int d = 0; d < 4; ++d) {
-                if (!(odd >> d & 1)) continue;
+                for (int b = 0; b < SUBS; ++b)
 #pragma unroll
-                for (int r = 0; r < RQ; ++r) {
-                    const uint32_t mine = seen[r] >> (4 * hl);
+                    for (int u = 0; u < 2; ++u)
 #pragma unroll
-                    for (int sign = 0; sign < 2; ++sign) {
-                        f32x16 n = {};
+                        for (int d = 0; d < 4; ++d)
+                            o[d] = __builtin_amdgcn_mfma_f32_32x32x16_f16(v_frag(b, d, u), p[b][u], o[d], 0, 0, 0);
+                return;
+            } else {
+                // A place that a row does not see must not reach it, whatever its value: 0 * infinity
+                // is NaN. Values that are not finite are taken as zeros, and then added as such to the
+                // rows that see them: how many of each sign a row sees comes from two more products.
+                uint32_t odd = 0;
 #pragma unroll
-                        for (int u = 0; u < 2; ++u) {
-                            const u32x4 b = __builtin_bit_cast(u32x4, v_frag(d, u));
-                            f16x8 is, sees;
+                for (int b = 0; b < SUBS; ++b)
 #pragma unroll
-                            for (int e = 0; e < 8; ++e) {
-                                const uint32_t y = b[e / 2] >> (16 * (e & 1)) & 0xffffu;
-                                const bool hit = (y & 0x7fffu) > 0x7c00u || y == (sign ? 0xfc00u : 0x7c00u);
-                                const int  i = 8 * u + e;
-                                is[e]   = static_cast<_Float16>(hit ? 1.f : 0.f);
-                                sees[e] = static_cast<_Float16>(mine >> (8 * (i / 4) + i % 4) & 1 ? 1.f : 0.f);
+                    for (int u = 0; u < 2; ++u)
+#pragma unroll
+                        for (int d = 0; d < 4; ++d) {
+                            f16x8 v = v_frag(b, d, u);
+                            const u32x4 w = __builtin_bit_cast(u32x4, v);
+                            bool bad = false;
+#pragma unroll
+                            for (int e = 0; e < 8; ++e) bad |= (w[e / 2] >> (16 * (e & 1)) & 0x7c00u) == 0x7c00u;
+                            if (__builtin_amdgcn_ballot_w64(bad) != 0) {
+                                odd |= 1u << (4 * b + d);
+#pragma unroll
+                                for (int e = 0; e < 8; ++e)
+                                    if ((w[e / 2] >> (16 * (e & 1)) & 0x7c00u) == 0x7c00u) v[e] = static_cast<_Float16>(0.f);
                             }
-                            n = __builtin_amdgcn_mfma_f32_32x32x16_f16(is, sees, n, 0, 0, 0);
+                            o[d] = __builtin_amdgcn_mfma_f32_32x32x16_f16(v, p[b][u], o[d], 0, 0, 0);
                         }
+                if (odd == 0) return;
 #pragma unroll
-                        for (int i = 0; i < 16; ++i)
-                            if (n[i] > 0.f) o[r][d][i] += sign ? -INFINITY : INFINITY;
+                for (int b = 0; b < SUBS; ++b)
+#pragma unroll
+                    for (int d = 0; d < 4; ++d) {
+                        if (!(odd >> (4 * b + d) & 1)) continue;
+                        const uint32_t mine = seen[b] >> (4 * hl);
+#pragma unroll 1
+                        for (int sign = 0; sign < 2; ++sign) {
+                            f32x16 n = {};
+#pragma unroll
+                            for (int u = 0; u < 2; ++u) {
+                                const u32x4 w = __builtin_bit_cast(u32x4, v_frag(b, d, u));
+                                f16x8 is, sees;
+#pragma unroll
+                                for (int e = 0; e < 8; ++e) {
+                                    const uint32_t y = w[e / 2] >> (16 * (e & 1)) & 0xffffu;
+                                    const bool hit = (y & 0x7fffu) > 0x7c00u || y == (sign ? 0xfc00u : 0x7c00u);
+                                    const int  i = 8 * u + e;
+                                    is[e]   = static_cast<_Float16>(hit ? 1.f : 0.f);
+                                    sees[e] = static_cast<_Float16>(mine >> (8 * (i / 4) + i % 4) & 1 ? 1.f : 0.f);
+                                }
+                                n = __builtin_amdgcn_mfma_f32_32x32x16_f16(is, sees, n, 0, 0, 0);
+                            }
+#pragma unroll
+                            for (int i = 0; i < 16; ++i)
+                                if (n[i] > 0.f) o[d][i] += sign ? -INFINITY : INFINITY;
+                        }
                     }
-                }
             }
         };
 
@@ -462,87 +491,111 @@ struct TreeKernel {
             }
             if constexpr (WQ > 1) block_sync();
             else wave_lds_sync();
-            compute(k, buf);
+            const int base = k * kStep + kPart * wk;
+            if (base + kPart <= open_end) step_of(std::false_type{}, base, stage_at(buf));
+            else if (base < end) step_of(std::true_type{}, base, stage_at(buf));
             if constexpr (WQ == 1) wave_lds_sync();
         }
 
-        // The waves along the places joined, through LDS, 32 rows of each wave at a time.
-        float* const ol = reinterpret_cast<float*>(lds);
-        float* const ml = ol + kWavesT * 32 * kOutLd;
+        const float sum = add_halves(l);
+        if constexpr (WK == 1) {
+            // The wave has its rows' whole sums: from the registers.
+            if (slot >= 0) {
+                const size_t at = static_cast<size_t>(slot) * kRowsM + my_row;
+                float* po = a.part_out + at * kHeadDim + 4 * hl;
 #pragma unroll
-        for (int r = 0; r < RQ; ++r) {
-            const float sum = add_halves(l[r]);
-            __syncthreads();
-            float* mine = ol + (32 * wave + ql) * kOutLd;
+                for (int d = 0; d < 4; ++d)
 #pragma unroll
-            for (int d = 0; d < 4; ++d)
+                    for (int i = 0; i < 4; ++i)
+                        *reinterpret_cast<f32x4*>(po + 32 * d + 8 * i) =
+                            f32x4{o[d][4 * i], o[d][4 * i + 1], o[d][4 * i + 2], o[d][4 * i + 3]};
+                if (hl == 0) *reinterpret_cast<f32x2*>(a.part_ml + 2 * at) = f32x2{m, sum};
+            } else if (row_ok) {
+                const float scale = sum == 0.f ? 0.f : c.v_scale / sum;
+                uint16_t* out = a.out + (x.t0 + tok) * a.out_stride + (h * G + my_g) * kHeadDim + 4 * hl;
 #pragma unroll
-                for (int i = 0; i < 4; ++i)
-                    *reinterpret_cast<f32x4*>(mine + 32 * d + 8 * i + 4 * hl) =
-                        f32x4{o[r][d][4 * i], o[r][d][4 * i + 1], o[r][d][4 * i + 2], o[r][d][4 * i + 3]};
-            if (hl == 0) *reinterpret_cast<f32x2*>(ml + 2 * (32 * wave + ql)) = f32x2{m[r], sum};
-            __syncthreads();
-            constexpr int TR = kThreads / (32 * WQ);   // threads of a row
-            const int jr = tid / TR, part = tid % TR;  // row among 32 WQ; a quarter-dims of it
-            const int w0 = jr / 32, row = 32 * (RQ * w0 + r) + jr % 32;
-            float top = -INFINITY, den = 0.f;
-            float f[WK];
+                for (int d = 0; d < 4; ++d)
 #pragma unroll
-            for (int g = 0; g < WK; ++g) top = fmaxf(top, ml[2 * (32 * (g * WQ + w0) + jr % 32)]);
-            const float ref = top == -INFINITY ? 0.f : top;
-#pragma unroll
-            for (int g = 0; g < WK; ++g) {
-                const float* e = ml + 2 * (32 * (g * WQ + w0) + jr % 32);
-                f[g] = exp2_fast(e[0] - ref);
-                den += f[g] * e[1];
-            }
-            const int i = a.by_group.page(row), g0 = row - i * G;
-            if (i < tile_n) {
-                const float scale = slot >= 0 ? 1.f : den == 0.f ? 0.f : c.v_scale / den;
-                uint16_t* out = a.out + (x.t0 + tok0 + i) * a.out_stride + (h * G + g0) * kHeadDim;
-                float* po = slot >= 0 ? a.part_out + (static_cast<size_t>(slot) * kRowsM + row) * kHeadDim : nullptr;
-#pragma unroll
-                for (int d = 4 * part; d < kHeadDim; d += 4 * TR) {
-                    f32x4 y = {0.f, 0.f, 0.f, 0.f};
-#pragma unroll
-                    for (int g = 0; g < WK; ++g) {
-                        const f32x4 z = *reinterpret_cast<const f32x4*>(ol + (32 * (g * WQ + w0) + jr % 32) * kOutLd + d);
-#pragma unroll
-                        for (int e = 0; e < 4; ++e) y[e] = fmaf(z[e], f[g], y[e]);
-                    }
-#pragma unroll
-                    for (int e = 0; e < 4; ++e) y[e] *= scale;
-                    if (slot >= 0) {
-                        *reinterpret_cast<f32x4*>(po + d) = y;
-                    } else {
-                        const f16x2 lo = {static_cast<_Float16>(y[0]), static_cast<_Float16>(y[1])};
-                        const f16x2 hi = {static_cast<_Float16>(y[2]), static_cast<_Float16>(y[3])};
-                        *reinterpret_cast<u32x2*>(out + d) =
+                    for (int i = 0; i < 4; ++i) {
+                        const f16x2 lo = {static_cast<_Float16>(o[d][4 * i] * scale), static_cast<_Float16>(o[d][4 * i + 1] * scale)};
+                        const f16x2 hi = {static_cast<_Float16>(o[d][4 * i + 2] * scale), static_cast<_Float16>(o[d][4 * i + 3] * scale)};
+                        *reinterpret_cast<u32x2*>(out + 32 * d + 8 * i) =
                             u32x2{__builtin_bit_cast(uint32_t, lo), __builtin_bit_cast(uint32_t, hi)};
                     }
-                }
-                if (slot >= 0 && part == 0)
-                    *reinterpret_cast<f32x2*>(a.part_ml + 2 * (static_cast<size_t>(slot) * kRowsM + row)) = f32x2{ref == 0.f && top == -INFINITY ? -INFINITY : ref, den};
             }
+            if constexpr (WQ > 1) block_sync();   // the stage is free again
+            return;
+        }
+
+        // The streams joined through LDS.
+        float* const ol = reinterpret_cast<float*>(lds);
+        float* const ml = ol + kWaves * 32 * kOutLd;
+        __syncthreads();
+        float* mine = ol + (32 * wave + ql) * kOutLd;
+#pragma unroll
+        for (int d = 0; d < 4; ++d)
+#pragma unroll
+            for (int i = 0; i < 4; ++i)
+                *reinterpret_cast<f32x4*>(mine + 32 * d + 8 * i + 4 * hl) =
+                    f32x4{o[d][4 * i], o[d][4 * i + 1], o[d][4 * i + 2], o[d][4 * i + 3]};
+        if (hl == 0) *reinterpret_cast<f32x2*>(ml + 2 * (32 * wave + ql)) = f32x2{m, sum};
+        __syncthreads();
+        constexpr int TR = kBlock / kRowsM;   // threads of a row
+        const int row = tid / TR, part = tid % TR;
+        float top = -INFINITY, den = 0.f, f[WK];
+#pragma unroll
+        for (int g = 0; g < WK; ++g) top = fmaxf(top, ml[2 * (kRowsM * g + row)]);
+        const float ref = top == -INFINITY ? 0.f : top;
+#pragma unroll
+        for (int g = 0; g < WK; ++g) {
+            const float* e = ml + 2 * (kRowsM * g + row);
+            f[g] = exp2_fast(e[0] - ref);
+            den += f[g] * e[1];
+        }
+        const int i = a.by_group.page(row), g0 = row - i * G;
+        if (i < tile_n) {
+            const float scale = slot >= 0 ? 1.f : den == 0.f ? 0.f : c.v_scale / den;
+            uint16_t* out = a.out + (x.t0 + tok0 + i) * a.out_stride + (h * G + g0) * kHeadDim;
+            const size_t at = static_cast<size_t>(max(slot, 0)) * kRowsM + row;
+#pragma unroll
+            for (int n = 0; n < 32 / TR; ++n) {
+                const int d = 4 * (part + TR * n);
+                f32x4 y = {0.f, 0.f, 0.f, 0.f};
+#pragma unroll
+                for (int g = 0; g < WK; ++g) {
+                    const f32x4 z = *reinterpret_cast<const f32x4*>(ol + (kRowsM * g + row) * kOutLd + d);
+#pragma unroll
+                    for (int e = 0; e < 4; ++e) y[e] = fmaf(z[e], f[g], y[e]);
+                }
+                if (slot >= 0) {
+                    *reinterpret_cast<f32x4*>(a.part_out + at * kHeadDim + d) = y;
+                } else {
+                    const f16x2 lo = {static_cast<_Float16>(y[0] * scale), static_cast<_Float16>(y[1] * scale)};
+                    const f16x2 hi = {static_cast<_Float16>(y[2] * scale), static_cast<_Float16>(y[3] * scale)};
+                    *reinterpret_cast<u32x2*>(out + d) =
+                        u32x2{__builtin_bit_cast(uint32_t, lo), __builtin_bit_cast(uint32_t, hi)};
+                }
+            }
+            if (slot >= 0 && part == 0) *reinterpret_cast<f32x2*>(a.part_ml + 2 * at) = f32x2{top, den};
         }
         __syncthreads();   // the stage is free again
     }
 };
 
-template <int EB, bool BS, int RQ, int WQ, int WK>
-__global__ __launch_bounds__(kThreads) void tree_attention_kernel(const TreeAttention a) {
-    using T = TreeKernel<EB, BS, RQ, WQ, WK>;
+template <int EB, bool BS, int WQ, int WK, bool UNI>
+__global__ __launch_bounds__(64 * WQ * WK, 2) void tree_attention_kernel(const TreeAttention a) {
+    using T = TreeKernel<EB, BS, WQ, WK, UNI>;
     __shared__ __attribute__((aligned(16))) unsigned char lds[T::kLds];
     __shared__ Schedule sch;
     T::run(a, lds, sch);
 }
 
 // Rows whose item was split: their parts joined. A wave a row.
-__global__ __launch_bounds__(kThreads) void tree_merge_kernel(const TreeAttention a) {
+__global__ __launch_bounds__(64 * kMergeWaves) void tree_merge_kernel(const TreeAttention a) {
     const CachedTokens& c = a.c;
     const int lane = threadIdx.x & 63;
     const int wave = __builtin_amdgcn_readfirstlane(threadIdx.x >> 6);
-    const long id = static_cast<long>(blockIdx.x) * kWavesT + wave;
+    const long id = static_cast<long>(blockIdx.x) * kMergeWaves + wave;
     const int hq = c.hkv * a.group;
     const int t = static_cast<int>(id / hq), head = static_cast<int>(id - static_cast<long>(t) * hq);
     if (t >= c.n_tok) return;
@@ -582,15 +635,20 @@ __global__ __launch_bounds__(kThreads) void tree_merge_kernel(const TreeAttentio
     *reinterpret_cast<uint32_t*>(a.out + t * a.out_stride + head * kHeadDim + 2 * lane) = __builtin_bit_cast(uint32_t, r);
 }
 
+template <int EB, bool BS, bool UNI>
+void launch_u(const TreeAttention& a, hipStream_t s) {
+    const dim3 grid(a.grid);
+    switch (a.rows) {
+        case 32: hipLaunchKernelGGL((tree_attention_kernel<EB, BS, 1, 4, UNI>), grid, dim3(256), 0, s, a); break;
+        case 64: hipLaunchKernelGGL((tree_attention_kernel<EB, BS, 2, 2, UNI>), grid, dim3(256), 0, s, a); break;
+        case 128: hipLaunchKernelGGL((tree_attention_kernel<EB, BS, 4, 1, UNI>), grid, dim3(256), 0, s, a); break;
+        default: hipLaunchKernelGGL((tree_attention_kernel<EB, BS, 8, 1, UNI>), grid, dim3(512), 0, s, a); break;
+    }
+}
 template <int EB, bool BS>
 void launch_e(const TreeAttention& a, hipStream_t s) {
-    const dim3 grid(a.grid), block(kThreads);
-    switch (a.rows) {
-        case 32: hipLaunchKernelGGL((tree_attention_kernel<EB, BS, 1, 1, 4>), grid, block, 0, s, a); break;
-        case 64: hipLaunchKernelGGL((tree_attention_kernel<EB, BS, 2, 1, 4>), grid, block, 0, s, a); break;
-        case 128: hipLaunchKernelGGL((tree_attention_kernel<EB, BS, 2, 2, 2>), grid, block, 0, s, a); break;
-        default: hipLaunchKernelGGL((tree_attention_kernel<EB, BS, 2, 4, 1>), grid, block, 0, s, a); break;
-    }
+    if (a.c.page_size % 4 == 0) launch_u<EB, BS, true>(a, s);
+    else if constexpr (!BS) launch_u<EB, false, false>(a, s);
 }
 
 int device_cus() {
@@ -610,7 +668,7 @@ void tree_shape(int dtype, TreeAttention& a) {
     const long items = (static_cast<long>(a.c.n_tok) / a.tile_tokens + a.c.n_ent) * a.c.hkv;   // at most
     const int  cus = device_cus();
     a.split = items <= 16l * cus;
-    a.grid  = a.split ? cus * (a.rows <= 32 ? 2 : 1) : static_cast<int>(items);
+    a.grid  = a.split ? cus * (a.rows <= 128 ? 2 : 1) : static_cast<int>(items);
 }
 
 size_t tree_workspace(const TreeAttention& a) {
@@ -633,7 +691,7 @@ hipError_t launch_tree_attention(int dtype, const TreeAttention& a, hipStream_t 
     else launch_e<1, true>(a, s);
     if (a.split) {
         const long rows = static_cast<long>(a.c.n_tok) * a.c.hkv * a.group;
-        hipLaunchKernelGGL(tree_merge_kernel, dim3(static_cast<unsigned>((rows + kWavesT - 1) / kWavesT)), dim3(kThreads), 0, s, a);
+        hipLaunchKernelGGL(tree_merge_kernel, dim3(static_cast<unsigned>((rows + kMergeWaves - 1) / kMergeWaves)), dim3(64 * kMergeWaves), 0, s, a);
     }
     return hipGetLastError();
 }
