@@ -79,7 +79,8 @@ pa::TreeAttention tree_sizes(int dtype, const pa_cached_tokens* c, int hq) {
     a.c.n_ent = c->num_entries;
     a.c.hkv   = c->num_kv_heads;
     a.group   = hq / c->num_kv_heads;
-    a.by_group = pa::page_div(a.group);
+    a.by_page = pa::place_div(c->page_size);
+    a.by_group = pa::place_div(a.group);
     return a;
 }
 

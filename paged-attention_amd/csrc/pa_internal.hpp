@@ -118,6 +118,20 @@ inline PageDiv page_div(int page_size) {
     return {~(l - 1), static_cast<uint32_t>((1ull << (31 + l)) / P + 1)};
 }
 
+// tok / d for 0 <= tok < 2^31 without a branch on d: floor(2 tok * magic / 2^(32 + l)), with l and
+// magic as above (a power of two has l = log2 d and magic 2^31 + 1).
+struct PlaceDiv {
+    uint32_t magic;
+    int      shift;
+    __device__ __forceinline__ int of(int tok) const {
+        return static_cast<int>(__umulhi(2u * static_cast<uint32_t>(tok), magic) >> shift);
+    }
+};
+inline PlaceDiv place_div(int d) {
+    const int l = d <= 1 ? 0 : 32 - __builtin_clz(static_cast<uint32_t>(d) - 1);   // ceil(log2 d)
+    return {static_cast<uint32_t>((1ull << (31 + l)) / static_cast<uint32_t>(d) + 1), l};
+}
+
 // Block-scaled caches: tokens per block, the exponents that a scale may have, and
 // the largest code at the largest of them (240 * 2^8 = 61440; 448 * 2^8, and even
 // 256 * 2^8, would be past fp16, which the decode kernel widens to).
@@ -209,7 +223,7 @@ struct TreeAttention {
     const uint64_t* tree;      // [n_tok][words], or null: a chain
     int             words;
     int             group;     // query heads of a kv head
-    PageDiv         by_group;
+    PlaceDiv        by_page, by_group;
     float           score_scale;   // of q k into base-2 exponents
     // Set by tree_shape, with the workspace.
     int             rows, tile_tokens, split, grid;

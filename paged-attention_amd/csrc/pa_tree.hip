@@ -2,13 +2,12 @@
 // trees, chains, pieces of prompts.
 
 #include "pa_device.hpp"
+#include "pa_fp8.hpp"
 
 #include <algorithm>
 #include <climits>
 #include <cmath>
 #include <cstdint>
-#include <stdexcept>
-#include <string>
 #include <type_traits>
 
 namespace pa {
@@ -21,6 +20,7 @@ typedef short    s16x4  __attribute__((ext_vector_type(4)));
 constexpr int kSub     = 32;              // places of one MFMA step
 constexpr int kScan    = 256;             // entries that a block looks at together
 constexpr int kMergeWaves = 4;
+constexpr int kDesc    = 8;               // ints of a block's entry for the merge
 constexpr int kOutLd   = kHeadDim + 4;    // floats of a row in the joining of waves
 
 // A probability is kept as 2^(score - reference + kShift) in fp16, where the reference
@@ -66,6 +66,37 @@ __device__ __forceinline__ long entry_cost(const TreeAttention& a, const Entry& 
     return tiles * a.c.hkv * (a.split ? (x.start + x.n + step - 1) / step : 1);
 }
 
+// The kernel's arguments, read again where this is called: read once, at the kernel's start, the
+// seventy scalars would be held (and spilled) through everything.
+__device__ __forceinline__ TreeAttention arguments() {
+    using words = const __attribute__((address_space(4))) uint32_t*;
+    words p = (words)__builtin_amdgcn_kernarg_segment_ptr();
+    asm volatile("" : "+s"(p));
+    uint32_t w[sizeof(TreeAttention) / 4];
+#pragma unroll
+    for (size_t i = 0; i < sizeof(TreeAttention) / 4; ++i) w[i] = p[i];
+    TreeAttention a;
+    __builtin_memcpy(&a, w, sizeof a);
+    return a;
+}
+
+__device__ __forceinline__ int uniform(int x) { return __builtin_amdgcn_readfirstlane(x); }
+// A value that every lane has the same, as a scalar (what comes from LDS or a shuffle is
+// taken to differ, and then so is every loop that it bounds).
+__device__ __forceinline__ long uniform(long x) {
+    return static_cast<long>(static_cast<uint64_t>(static_cast<uint32_t>(__builtin_amdgcn_readfirstlane(static_cast<int>(x >> 32)))) << 32 |
+                             static_cast<uint32_t>(__builtin_amdgcn_readfirstlane(static_cast<int>(x))));
+}
+
+// a / b for 0 <= a < 2^52, b > 0, wave-uniform: through doubles (a 64-bit integer
+// division is 140 scalar instructions).
+__device__ __forceinline__ long divide(long a, long b) {
+    long q = static_cast<long>(static_cast<double>(a) / static_cast<double>(b));
+    const long r = a - q * b;
+    q += r >= b ? 1 : r < 0 ? -1 : 0;
+    return uniform(q);
+}
+
 struct Schedule {
     long pre[kScan + 1];   // units before each entry of the chunk
     long wave_sum[kScan / 64];
@@ -103,12 +134,13 @@ __device__ __forceinline__ long scan_chunk(const TreeAttention& a, Schedule& s, 
     if (mine) s.pre[tid + 1] = before + x;
     if (tid == 0) s.pre[0] = 0;
     __syncthreads();
-    return total;
+    return uniform(total);
 }
 
-// LDS chunk (16 bytes) of a row that holds its chunk ch: rows that a fragment read takes
-// together lie in different banks (K: 16 rows, one chunk; V: 4 rows, 4 chunks).
-__device__ __forceinline__ int swizzle(int row) { return ((row & 3) << 2) | ((row >> 2) & 3); }
+// Bytes of a staged row: 128 fp16 and 32 more, so that the rows that a fragment read takes
+// together (K: 8 rows, 16 bytes of each; V: 4 rows, 32 bytes) lie in different banks, and every
+// fragment at a constant distance from the lane's first.
+constexpr int kRowLds = 288;
 
 __device__ __forceinline__ void block_sync() {
     __builtin_amdgcn_fence(__ATOMIC_RELEASE, "workgroup", "local");
@@ -163,8 +195,10 @@ struct TreeKernel {
     static constexpr int kStep   = kPart * WK;
     static constexpr int NJ      = kPart / (4 * WQ);           // loads of 4 rows per wave, of K and of V
     static constexpr int kBufs   = WQ > 1 ? 2 : 1;
-    static constexpr int kTile   = kPart * 256;                // bytes of a step's rows in fp16
-    static constexpr int kBuf    = 2 * kTile + (BS ? 4 * kPart / 4 : 0);
+    static constexpr int kTile   = kPart * kRowLds;            // bytes of a step's rows in fp16
+    static constexpr int kScales = 2 * kTile;                  // in a buffer: K's scales, a float per 4 rows
+    static constexpr int kFlags  = kScales + kPart;            // whether a wave met a value that is not finite
+    static constexpr int kBuf    = kFlags + 16 * ((4 * WQ + 15) / 16);
     static constexpr int kStage  = WK * kBufs * kBuf;
     static constexpr int kJoin   = kWaves * 32 * (kOutLd * 4 + 8);
     static constexpr int kJoinOf = WK > 1 ? kJoin : 0;
@@ -181,9 +215,11 @@ struct TreeKernel {
         const int lb = nb % 8 == 0 ? (blockIdx.x % 8) * (nb / 8) + blockIdx.x / 8 : blockIdx.x;
         long total = 0, chunk = 0;
         for (int c0 = 0; c0 < a.c.n_ent; c0 += kScan) total += chunk = scan_chunk(a, sch, c0, kStep);
-        const long per = a.split ? max((total + nb - 1) / nb, 1l) : 1;
+        const long per = a.split ? max(divide(total + nb - 1, nb), 1l) : 1;
         long w = lb * per;
         const long w_end = min(w + per, total);
+        int32_t* const desc = a.desc + kDesc * lb;   // what the merge has to join from here on
+        if (a.split && threadIdx.x == 0) desc[0] = 1;
         if (w >= w_end) return;
         int  c0 = 0;
         long before = 0;
@@ -199,59 +235,65 @@ struct TreeKernel {
             if (tid < kScan && sch.pre[tid] <= w - before && w - before < sch.pre[tid + 1]) sch.hit = tid;
             __syncthreads();
             const int  hit = a.c.n_ent == 1 ? 0 : __builtin_amdgcn_readfirstlane(sch.hit);
-            const long at  = before + sch.pre[hit];
+            const long at  = before + uniform(sch.pre[hit]);
             __syncthreads();
-            const Entry x = entry_at(a.c, c0 + hit);
+            Entry x = entry_at(a.c, c0 + hit);
+            x.n = uniform(x.n);
             const int tiles = (x.n + a.tile_tokens - 1) / a.tile_tokens;
             const int steps = static_cast<int>((x.start + x.n + step - 1) / step);
             const int units = a.split ? steps : 1;
             const long local = w - at;
-            const long item  = local / units;
+            const long item  = divide(local, units);
             const int  u0    = static_cast<int>(local - item * units);
             const int  u1    = static_cast<int>(min(static_cast<long>(units), u0 + (w_end - w)));
-            const int  h     = static_cast<int>(item / tiles);
+            const int  h     = static_cast<int>(divide(item, tiles));
             const int  rt    = tiles - 1 - static_cast<int>(item - static_cast<long>(h) * tiles);
             const bool whole = u0 == 0 && u1 == units;
-            if (a.split && u0 == 0) {
-                // For the merge: where the item's parts lie.
-                const long b0 = w / per, b1 = (at + (item + 1) * units - 1) / per;
-                const int  n  = min(a.tile_tokens, x.n - rt * a.tile_tokens);
-                for (int i = threadIdx.x; i < n; i += kBlock) {
-                    int32_t* d = a.desc + 2 * (static_cast<size_t>(x.t0 + rt * a.tile_tokens + i) * a.c.hkv + h);
-                    d[0] = static_cast<int>(2 * b0 + (w == w_first ? 0 : 1));
-                    d[1] = static_cast<int>(b1 - b0 + 1);
-                }
+            if (u0 == 0 && u1 < units && threadIdx.x == 0) {   // the block's last item: its other parts are the next blocks' first
+                const int b1 = static_cast<int>(divide(at + (item + 1) * units - 1, per));
+                desc[1] = x.t0 + rt * a.tile_tokens;
+                desc[2] = min(a.tile_tokens, x.n - rt * a.tile_tokens);
+                desc[3] = h;
+                desc[4] = 2 * lb + (w == w_first ? 0 : 1);
+                desc[0] = b1 - lb + 1;
             }
             const int slot = whole ? -1 : 2 * lb + (w == w_first ? 0 : 1);
-            item_part(a, lds, x, h, rt, a.split ? u0 : 0, a.split ? u1 : steps, slot);
+            item_part(lds, x, h, rt, uniform(a.split ? u0 : 0), uniform(a.split ? u1 : steps), uniform(slot));
             w += u1 - u0;
         }
     }
 
-    static __device__ __forceinline__ void item_part(const TreeAttention& a, unsigned char* lds, const Entry& x, int h,
-                                                     int rt, int k0, int k1, int slot) {
+    static __device__ __forceinline__ void item_part(unsigned char* lds, const Entry& x, int h, int rt, int k0,
+                                                     int k1, int slot) {
+        const TreeAttention a = arguments();
         const CachedTokens& c = a.c;
         const int tid = threadIdx.x, lane = tid & 63;
         const int wave = __builtin_amdgcn_readfirstlane(tid >> 6), wq = wave % WQ, wk = wave / WQ;
         const int ql = lane & 31, hl = lane >> 5;
         const int G = a.group, P = c.page_size;
         const int tok0 = rt * a.tile_tokens;   // first token of the tile, within the entry
-        const int tile_n = min(a.tile_tokens, x.n - tok0);
-        const int end = x.start + (a.tree ? x.n : tok0 + tile_n);   // places from here on are not seen
-        k1 = min(k1, (end + kStep - 1) / kStep);
+        const int tile_n = uniform(min(a.tile_tokens, x.n - tok0));
+        const int end = uniform(x.start + (a.tree ? x.n : tok0 + tile_n));   // places from here on are not seen
+        k1 = uniform(min(k1, (end + kStep - 1) / kStep));
 
-        // Query fragments, and the lane's token.
+        // Query fragments, and the lane's token. (A negative scale turns the queries' signs.)
+        const float    score_scale = fabsf(a.score_scale);
+        const uint32_t flip = a.score_scale < 0.f ? 0x80008000u : 0u;
         f16x8 q[8];
-        const int my_row = 32 * wq + ql, my_i = a.by_group.page(my_row), my_g = my_row - my_i * G;
+        const int my_row = 32 * wq + ql, my_i = a.by_group.of(my_row), my_g = my_row - my_i * G;
         const bool row_ok = my_i < tile_n;
         const int  tok = row_ok ? tok0 + my_i : INT_MAX;
         {
             const uint16_t* p = a.q + (x.t0 + tok0 + (row_ok ? my_i : 0)) * a.q_stride + (h * G + (row_ok ? my_g : 0)) * kHeadDim + 8 * hl;
 #pragma unroll
-            for (int s = 0; s < 8; ++s) q[s] = __builtin_bit_cast(f16x8, *reinterpret_cast<const u32x4*>(p + 16 * s));
+            for (int s = 0; s < 8; ++s) {
+                u32x4 y = *reinterpret_cast<const u32x4*>(p + 16 * s);
+#pragma unroll
+                for (int e = 0; e < 4; ++e) y[e] ^= flip;
+                q[s] = __builtin_bit_cast(f16x8, y);
+            }
         }
-        // Places before this one are seen by every row of the wave.
-        const int open_end = x.start + (a.tree ? 0 : tok0 + a.by_group.page(32 * wq) + 1);
+        const int all_open = uniform(x.start + (a.tree ? 0 : tok0 + 1));   // places before this one are seen by every row
 
         f32x16 o[4];
         float  m = -INFINITY, l = 0.f;
@@ -273,12 +315,12 @@ struct TreeKernel {
         uint32_t live = 0;     // general pages: loads whose row holds a place
         auto lookup = [&](int k) {
             const int t = k * kStep + kPart * wk + RG * lane;
-            pg = lane < kPart / RG && t < end ? table[c.by_page.page(t)] : -1;
+            pg = lane < kPart / RG && t < end ? table[a.by_page.of(t)] : -1;
         };
         auto issue = [&](int k) {
             const int  t  = k * kStep + kPart * wk + RG * lane;
             const bool ok = pg >= 0 && pg < c.num_pages;
-            const int  s  = t - c.by_page.page(t) * P;
+            const int  s  = t - a.by_page.of(t) * P;
             const size_t off = ok ? pg * page_bytes + head_off + static_cast<size_t>(s) * kRowBytes<EB> : 0;
             const uint32_t lo = static_cast<uint32_t>(off), hi = static_cast<uint32_t>(off >> 32);
             const int rows = ok ? min(RG, end - t) : 0;
@@ -317,8 +359,12 @@ struct TreeKernel {
                               fp8x2_to_f16x2<false>(x[1], scale), fp8x2_to_f16x2<true>(x[1], scale)};
         };
         auto stage_at = [&](int buf) { return lds + (wk * kBufs + buf) * kBuf; };
-        auto store = [&](int buf) {
+        // A place that a row does not see must not reach it, whatever its value: 0 * infinity is
+        // NaN. So where rows see different places (masked), values that are not finite are staged as
+        // zeros, and add_odd adds them to the rows that see them.
+        auto store = [&](int buf, bool masked) {
             unsigned char* k = stage_at(buf);
+            bool odd = false;
 #pragma unroll
             for (int j = 0; j < NJ; ++j) {
                 const int r4 = wq + WQ * j, row = 4 * r4 + row0;
@@ -327,20 +373,59 @@ struct TreeKernel {
                     const uint32_t pair = __builtin_amdgcn_readlane(sc, r4 * 4 / RG);
                     vs = __builtin_bit_cast(float, (pair >> 8) << 23);
                     if (lane == 0)
-                        *reinterpret_cast<float*>(k + 2 * kTile + 4 * r4) = a.score_scale * __builtin_bit_cast(float, (pair & 0xff) << 23);
+                        *reinterpret_cast<float*>(k + kScales + 4 * r4) = score_scale * __builtin_bit_cast(float, (pair & 0xff) << 23);
                 }
                 u32x4 kx = widen(kr[j], 1.0f), vx = widen(vr[j], vs);
                 if (!UNI && !(live >> j & 1)) kx = vx = u32x4{0, 0, 0, 0};
-                const int at = row * 256 + ((ch ^ swizzle(row)) << 4);
+                const int at = row * kRowLds + 16 * ch;
                 *reinterpret_cast<u32x4*>(k + at) = kx;
+                if (masked) {
+#pragma unroll
+                    for (int e = 0; e < 4; ++e) {
+                        const uint32_t lo = (vx[e] & 0x7c00u) == 0x7c00u ? 0xffffu : 0u;
+                        const uint32_t hi = (vx[e] & 0x7c000000u) == 0x7c000000u ? 0xffff0000u : 0u;
+                        odd |= (lo | hi) != 0;
+                        vx[e] &= ~(lo | hi);
+                    }
+                }
                 *reinterpret_cast<u32x4*>(k + kTile + at) = vx;
             }
+            if (masked) {
+                const bool any = __builtin_amdgcn_ballot_w64(odd) != 0;
+                if (lane == 0) *reinterpret_cast<int*>(k + kFlags + 4 * wq) = any;
+            }
+        };
+        // (By way of memory: rare, and 64 sums indexed by constants would weigh on the loop's registers.)
+        auto add_odd = [&](int base, const uint32_t (&seen)[SUBS], f32x16 (&o)[4]) {
+            float sums[64];
+#pragma unroll
+            for (int n = 0; n < 64; ++n) sums[n] = o[n / 16][n % 16];
+#pragma unroll 1
+            for (int t = 0; t < kPart && base + t < end; ++t) {
+                const int i = a.by_page.of(base + t), page = load_uniform(table, i);
+                if (page < 0 || page >= c.num_pages) continue;
+                const unsigned char* v = static_cast<const unsigned char*>(c.v_cache) + page * page_bytes + head_off +
+                                         static_cast<size_t>(base + t - i * P) * kRowBytes<EB>;
+                uint32_t word = seen[0];
+#pragma unroll
+                for (int b = 1; b < SUBS; ++b) word = t >= kSub * b ? seen[b] : word;
+                if (!(word >> (t & 31) & 1)) continue;
+#pragma unroll 1
+                for (int n = 0; n < 64; ++n) {
+                    const int at = 8 * (n / 4) + 4 * hl + n % 4;
+                    float y;
+                    if constexpr (EB == 2) y = f16_bits_to_f32(reinterpret_cast<const uint16_t*>(v)[at]);
+                    else y = (v[at] & 0x7f) == 0x7f ? NAN : 0.f;
+                    if (!(fabsf(y) < INFINITY)) sums[n] += y;
+                }
+            }
+#pragma unroll
+            for (int n = 0; n < 64; ++n) o[n / 16][n % 16] = sums[n];
         };
 
         // Where this lane's fragments lie in the stage.
-        const int ka = ql * 256 + ((hl ^ swizzle(ql)) << 4);
-        const int vi = lane & 15, vg = (lane >> 4) & 1;
-        const int va = (4 * hl + (vi >> 2)) * 256 + ((((vi >> 2) << 2) | ((2 * vg + ((vi >> 1) & 1)) ^ hl)) << 4) + 8 * (vi & 1);
+        const int ka = ql * kRowLds + 16 * hl;
+        const int va = (4 * hl + ((lane & 15) >> 2)) * kRowLds + 32 * ((lane >> 4) & 1) + 8 * (lane & 3);
 
         auto step_of = [&](auto masked_c, int base, const unsigned char* ks) {
             constexpr bool MASK = decltype(masked_c)::value;
@@ -352,20 +437,18 @@ struct TreeKernel {
                 for (int i = 0; i < 16; ++i) s[b][i] = 0.f;
 #pragma unroll
                 for (int t = 0; t < 8; ++t) {
-                    const f16x8 kf = *reinterpret_cast<const f16x8*>(ks + (ka ^ (t << 5)) + b * kSub * 256);
+                    const f16x8 kf = *reinterpret_cast<const f16x8*>(ks + ka + 32 * t + b * kSub * kRowLds);
                     s[b] = __builtin_amdgcn_mfma_f32_32x32x16_f16(kf, q[t], s[b], 0, 0, 0);
                 }
             }
             uint32_t seen[SUBS];
             float top = -INFINITY;
-            const float one = a.score_scale;
 #pragma unroll
             for (int b = 0; b < SUBS; ++b) {
                 if constexpr (BS) {
-                    // Scores in base 2 (elsewhere the one scale goes into the exponent's argument).
 #pragma unroll
                     for (int i = 0; i < 4; ++i) {
-                        const float cs = *reinterpret_cast<const float*>(ks + 2 * kTile + 4 * (8 * b + 2 * i + hl));
+                        const float cs = *reinterpret_cast<const float*>(ks + kScales + 4 * (8 * b + 2 * i + hl));
 #pragma unroll
                         for (int e = 0; e < 4; ++e) s[b][4 * i + e] *= cs;
                     }
@@ -374,16 +457,21 @@ struct TreeKernel {
                     seen[b] = visible(a, x, tok, base + kSub * b - x.start);
                     const uint32_t mine = seen[b] >> (4 * hl);
 #pragma unroll
-                    for (int i = 0; i < 16; ++i)
-                        s[b][i] = mine >> (8 * (i / 4) + i % 4) & 1 ? (BS ? s[b][i] : s[b][i] * one) : -INFINITY;
-                } else if constexpr (!BS) {
-#pragma unroll
-                    for (int i = 0; i < 16; ++i) s[b][i] *= one;
+                    for (int i = 0; i < 16; ++i) {
+                        // (By bits: a comparison each would hold 16 lane masks at once.)
+                        const uint32_t all = __builtin_amdgcn_sbfe(mine, 8 * (i / 4) + i % 4, 1);
+                        const float    raw = s[b][i];
+                        const uint32_t y = __builtin_bit_cast(uint32_t, raw) & all;
+                        s[b][i] = __builtin_bit_cast(float, y | (~all & 0xff800000u));
+                    }
                 }
 #pragma unroll
                 for (int i = 0; i < 16; ++i) top = fmaxf(top, s[b][i]);
             }
-            top = max_halves(top);
+            // Block scales: scores in base 2 already; elsewhere the one scale (not below 0) goes into
+            // the exponent's argument.
+            const float one = BS ? 1.0f : score_scale;
+            top = max_halves(top) * one;
             if (__builtin_amdgcn_ballot_w64(top > m + kLag) != 0) {
                 const float now = fmaxf(m, top), ref = now == -INFINITY ? 0.f : now;
                 const float f = exp2_fast(m - ref);
@@ -400,80 +488,30 @@ struct TreeKernel {
             for (int b = 0; b < SUBS; ++b)
 #pragma unroll
                 for (int i = 0; i < 16; ++i) {
-                    const float e = exp2_fast(s[b][i] - ref);
+                    const float e = exp2_fast(BS ? s[b][i] - ref : fmaf(s[b][i], one, -ref));
                     l += e;
                     p[b][i / 8][i % 8] = static_cast<_Float16>(e);
                 }
             auto v_part = [&](int b, int d, int u, int w) {
-                const int at = (va ^ (d << 6) ^ (w << 5)) + (kSub * b + 16 * u + 8 * w) * 256;
+                const int at = va + 64 * d + (kSub * b + 16 * u + 8 * w) * kRowLds;
                 return __builtin_amdgcn_ds_read_tr16_b64_v4i16((__attribute__((address_space(3))) s16x4*)(vs + at));
             };
             auto v_frag = [&](int b, int d, int u) {
                 const s16x4 lo = v_part(b, d, u, 0), hi = v_part(b, d, u, 1);
                 return __builtin_bit_cast(f16x8, __builtin_shufflevector(lo, hi, 0, 1, 2, 3, 4, 5, 6, 7));
             };
-            if constexpr (!MASK) {
 #pragma unroll
-                for (int b = 0; b < SUBS; ++b)
+            for (int b = 0; b < SUBS; ++b)
 #pragma unroll
-                    for (int u = 0; u < 2; ++u)
+                for (int u = 0; u < 2; ++u)
 #pragma unroll
-                        for (int d = 0; d < 4; ++d)
-                            o[d] = __builtin_amdgcn_mfma_f32_32x32x16_f16(v_frag(b, d, u), p[b][u], o[d], 0, 0, 0);
-                return;
-            } else {
-                // A place that a row does not see must not reach it, whatever its value: 0 * infinity
-                // is NaN. Values that are not finite are taken as zeros, and then added as such to the
-                // rows that see them: how many of each sign a row sees comes from two more products.
-                uint32_t odd = 0;
+                    for (int d = 0; d < 4; ++d)
+                        o[d] = __builtin_amdgcn_mfma_f32_32x32x16_f16(v_frag(b, d, u), p[b][u], o[d], 0, 0, 0);
+            if constexpr (MASK) {
+                int odd = 0;
 #pragma unroll
-                for (int b = 0; b < SUBS; ++b)
-#pragma unroll
-                    for (int u = 0; u < 2; ++u)
-#pragma unroll
-                        for (int d = 0; d < 4; ++d) {
-                            f16x8 v = v_frag(b, d, u);
-                            const u32x4 w = __builtin_bit_cast(u32x4, v);
-                            bool bad = false;
-#pragma unroll
-                            for (int e = 0; e < 8; ++e) bad |= (w[e / 2] >> (16 * (e & 1)) & 0x7c00u) == 0x7c00u;
-                            if (__builtin_amdgcn_ballot_w64(bad) != 0) {
-                                odd |= 1u << (4 * b + d);
-#pragma unroll
-                                for (int e = 0; e < 8; ++e)
-                                    if ((w[e / 2] >> (16 * (e & 1)) & 0x7c00u) == 0x7c00u) v[e] = static_cast<_Float16>(0.f);
-                            }
-                            o[d] = __builtin_amdgcn_mfma_f32_32x32x16_f16(v, p[b][u], o[d], 0, 0, 0);
-                        }
-                if (odd == 0) return;
-#pragma unroll
-                for (int b = 0; b < SUBS; ++b)
-#pragma unroll
-                    for (int d = 0; d < 4; ++d) {
-                        if (!(odd >> (4 * b + d) & 1)) continue;
-                        const uint32_t mine = seen[b] >> (4 * hl);
-#pragma unroll 1
-                        for (int sign = 0; sign < 2; ++sign) {
-                            f32x16 n = {};
-#pragma unroll
-                            for (int u = 0; u < 2; ++u) {
-                                const u32x4 w = __builtin_bit_cast(u32x4, v_frag(b, d, u));
-                                f16x8 is, sees;
-#pragma unroll
-                                for (int e = 0; e < 8; ++e) {
-                                    const uint32_t y = w[e / 2] >> (16 * (e & 1)) & 0xffffu;
-                                    const bool hit = (y & 0x7fffu) > 0x7c00u || y == (sign ? 0xfc00u : 0x7c00u);
-                                    const int  i = 8 * u + e;
-                                    is[e]   = static_cast<_Float16>(hit ? 1.f : 0.f);
-                                    sees[e] = static_cast<_Float16>(mine >> (8 * (i / 4) + i % 4) & 1 ? 1.f : 0.f);
-                                }
-                                n = __builtin_amdgcn_mfma_f32_32x32x16_f16(is, sees, n, 0, 0, 0);
-                            }
-#pragma unroll
-                            for (int i = 0; i < 16; ++i)
-                                if (n[i] > 0.f) o[d][i] += sign ? -INFINITY : INFINITY;
-                        }
-                    }
+                for (int w = 0; w < WQ; ++w) odd |= *reinterpret_cast<const int*>(ks + kFlags + 4 * w);
+                if (__builtin_amdgcn_readfirstlane(odd)) add_odd(base, seen, o);
             }
         };
 
@@ -484,15 +522,15 @@ struct TreeKernel {
         }
         for (int k = k0; k < k1; ++k) {
             const int buf = kBufs == 2 ? (k - k0) & 1 : 0;
-            store(buf);
+            const int base = k * kStep + kPart * wk;
+            store(buf, base + kPart > all_open);
             if (k + 1 < k1) {
                 issue(k + 1);
                 if (k + 2 < k1) lookup(k + 2);
             }
             if constexpr (WQ > 1) block_sync();
             else wave_lds_sync();
-            const int base = k * kStep + kPart * wk;
-            if (base + kPart <= open_end) step_of(std::false_type{}, base, stage_at(buf));
+            if (base + kPart <= all_open) step_of(std::false_type{}, base, stage_at(buf));
             else if (base < end) step_of(std::true_type{}, base, stage_at(buf));
             if constexpr (WQ == 1) wave_lds_sync();
         }
@@ -552,7 +590,7 @@ struct TreeKernel {
             f[g] = exp2_fast(e[0] - ref);
             den += f[g] * e[1];
         }
-        const int i = a.by_group.page(row), g0 = row - i * G;
+        const int i = a.by_group.of(row), g0 = row - i * G;
         if (i < tile_n) {
             const float scale = slot >= 0 ? 1.f : den == 0.f ? 0.f : c.v_scale / den;
             uint16_t* out = a.out + (x.t0 + tok0 + i) * a.out_stride + (h * G + g0) * kHeadDim;
@@ -590,47 +628,40 @@ __global__ __launch_bounds__(64 * WQ * WK, 2) void tree_attention_kernel(const T
     T::run(a, lds, sch);
 }
 
-// Rows whose item was split: their parts joined. A wave a row.
-__global__ __launch_bounds__(64 * kMergeWaves) void tree_merge_kernel(const TreeAttention a) {
-    const CachedTokens& c = a.c;
+// The item that begins in block x and goes on in the next ones: its parts joined, a wave
+// a row. (At most one begins in a block and is not whole there: its last.)
+__global__ __launch_bounds__(64 * kMergeWaves) void tree_merge_kernel(const int32_t* __restrict__ desc, const TreeAttention a) {
     const int lane = threadIdx.x & 63;
-    const int wave = __builtin_amdgcn_readfirstlane(threadIdx.x >> 6);
-    const long id = static_cast<long>(blockIdx.x) * kMergeWaves + wave;
-    const int hq = c.hkv * a.group;
-    const int t = static_cast<int>(id / hq), head = static_cast<int>(id - static_cast<long>(t) * hq);
-    if (t >= c.n_tok) return;
-    // The token's entry: the last that begins at or before it.
-    int lo = 0;
-    for (int span = c.n_ent; span > 1;) {
-        const int step = (span + 63) / 64, i = lo + step * lane;
-        const bool le = i < lo + span && c.tok_begin[i] <= t;
-        const int at = max(__builtin_popcountll(__builtin_amdgcn_ballot_w64(le)) - 1, 0);
-        const int end = lo + span;
-        lo += step * at;
-        span = min(step, end - lo);
-    }
-    const Entry x = entry_at(c, lo);
-    if (t < x.t0 || t >= x.t0 + x.n) return;
-    const int h = head / a.group, g = head - h * a.group;
-    const int32_t* d = a.desc + 2 * (static_cast<size_t>(t) * c.hkv + h);
-    const int slot0 = d[0], n = d[1];
+    const int row  = blockIdx.y * kMergeWaves + __builtin_amdgcn_readfirstlane(threadIdx.x >> 6);
+    const int32_t* d = desc + kDesc * blockIdx.x;
+    const int n = load_uniform(d, 0);
     if (n <= 1) return;
-    const int row = (t - x.t0) % a.tile_tokens * a.group + g;
+    const int i = a.by_group.of(row), g = row - i * a.group;
+    if (i >= load_uniform(d, 2)) return;
+    const int t = load_uniform(d, 1) + i, head = load_uniform(d, 3) * a.group + g, slot0 = load_uniform(d, 4);
     f32x2 acc = {0.f, 0.f};
     float m = -INFINITY, den = 0.f;
-    for (int k = 0; k < n; ++k) {
-        const int    slot = k == 0 ? slot0 : 2 * (slot0 / 2 + k);
-        const size_t at = static_cast<size_t>(slot) * a.rows + row;
-        const f32x2  e = *reinterpret_cast<const f32x2*>(a.part_ml + 2 * at);
-        const f32x2  y = *reinterpret_cast<const f32x2*>(a.part_out + at * kHeadDim + 2 * lane);
-        const float now = fmaxf(m, e[0]), ref = now == -INFINITY ? 0.f : now;
-        const float f0 = exp2_fast(m - ref), f1 = exp2_fast(e[0] - ref);
-        acc[0] = acc[0] * f0 + y[0] * f1;
-        acc[1] = acc[1] * f0 + y[1] * f1;
-        den = den * f0 + e[1] * f1;
-        m = now;
+    for (int k0 = 0; k0 < n; k0 += 8) {
+        f32x2 e[8], y[8];
+#pragma unroll
+        for (int k = 0; k < 8; ++k) {
+            const int    slot = k0 + k == 0 ? slot0 : 2 * (slot0 / 2 + min(k0 + k, n - 1));
+            const size_t at = static_cast<size_t>(slot) * a.rows + row;
+            e[k] = *reinterpret_cast<const f32x2*>(a.part_ml + 2 * at);
+            y[k] = *reinterpret_cast<const f32x2*>(a.part_out + at * kHeadDim + 2 * lane);
+        }
+#pragma unroll
+        for (int k = 0; k < 8; ++k) {
+            if (k0 + k >= n) break;
+            const float now = fmaxf(m, e[k][0]), ref = now == -INFINITY ? 0.f : now;
+            const float f0 = exp2_fast(m - ref), f1 = exp2_fast(e[k][0] - ref);
+            acc[0] = acc[0] * f0 + y[k][0] * f1;
+            acc[1] = acc[1] * f0 + y[k][1] * f1;
+            den = den * f0 + e[k][1] * f1;
+            m = now;
+        }
     }
-    const float scale = den == 0.f ? 0.f : c.v_scale / den;
+    const float scale = den == 0.f ? 0.f : a.c.v_scale / den;
     const f16x2 r = {static_cast<_Float16>(acc[0] * scale), static_cast<_Float16>(acc[1] * scale)};
     *reinterpret_cast<uint32_t*>(a.out + t * a.out_stride + head * kHeadDim + 2 * lane) = __builtin_bit_cast(uint32_t, r);
 }
@@ -674,7 +705,7 @@ void tree_shape(int dtype, TreeAttention& a) {
 size_t tree_workspace(const TreeAttention& a) {
     if (!a.split) return 0;
     return static_cast<size_t>(2 * a.grid) * a.rows * (kHeadDim + 2) * sizeof(float) +
-           static_cast<size_t>(a.c.n_tok) * a.c.hkv * 2 * sizeof(int32_t);
+           static_cast<size_t>(a.grid) * kDesc * sizeof(int32_t);
 }
 
 void tree_place(TreeAttention& a, void* workspace) {
@@ -689,10 +720,8 @@ hipError_t launch_tree_attention(int dtype, const TreeAttention& a, hipStream_t 
     if (dtype == PA_KV_FP16) launch_e<2, false>(a, s);
     else if (dtype == PA_KV_FP8_E4M3) launch_e<1, false>(a, s);
     else launch_e<1, true>(a, s);
-    if (a.split) {
-        const long rows = static_cast<long>(a.c.n_tok) * a.c.hkv * a.group;
-        hipLaunchKernelGGL(tree_merge_kernel, dim3(static_cast<unsigned>((rows + kMergeWaves - 1) / kMergeWaves)), dim3(64 * kMergeWaves), 0, s, a);
-    }
+    if (a.split)
+        hipLaunchKernelGGL(tree_merge_kernel, dim3(a.grid, a.rows / kMergeWaves), dim3(64 * kMergeWaves), 0, s, a.desc, a);
     return hipGetLastError();
 }
 
