@@ -20,6 +20,7 @@ typedef short    s16x4  __attribute__((ext_vector_type(4)));
 constexpr int kSub     = 32;              // places of one MFMA step
 constexpr int kScan    = 256;             // entries that a block looks at together
 constexpr int kMergeWaves = 4;
+constexpr int kSchedMfma = 0x8, kSchedLds = 0x100;   // of sched_group_barrier
 constexpr int kDesc    = 8;               // ints of a block's entry for the merge
 constexpr int kOutLd   = kHeadDim + 4;    // floats of a row in the joining of waves
 
@@ -137,10 +138,10 @@ __device__ __forceinline__ long scan_chunk(const TreeAttention& a, Schedule& s, 
     return uniform(total);
 }
 
-// Bytes of a staged row: 128 fp16 and 32 more, so that the rows that a fragment read takes
-// together (K: 8 rows, 16 bytes of each; V: 4 rows, 32 bytes) lie in different banks, and every
-// fragment at a constant distance from the lane's first.
-constexpr int kRowLds = 288;
+// Bytes of a staged row: 128 fp16 and some more, so that the rows that a fragment read takes at
+// once lie in different banks (64 of 4 bytes: 16 rows of K, 16 bytes of each; 4 rows of V, 64
+// bytes of each), and every fragment at a constant distance from the lane's first.
+constexpr int kRowK = 256 + 16, kRowV = 256 + 64;
 
 __device__ __forceinline__ void block_sync() {
     __builtin_amdgcn_fence(__ATOMIC_RELEASE, "workgroup", "local");
@@ -195,8 +196,8 @@ struct TreeKernel {
     static constexpr int kStep   = kPart * WK;
     static constexpr int NJ      = kPart / (4 * WQ);           // loads of 4 rows per wave, of K and of V
     static constexpr int kBufs   = WQ > 1 ? 2 : 1;
-    static constexpr int kTile   = kPart * kRowLds;            // bytes of a step's rows in fp16
-    static constexpr int kScales = 2 * kTile;                  // in a buffer: K's scales, a float per 4 rows
+    static constexpr int kTileK  = kPart * kRowK, kTileV = kPart * kRowV;   // bytes of a step's rows
+    static constexpr int kScales = kTileK + kTileV;                 // in a buffer: K's scales, a float per 4 rows
     static constexpr int kFlags  = kScales + kPart;            // whether a wave met a value that is not finite
     static constexpr int kBuf    = kFlags + 16 * ((4 * WQ + 15) / 16);
     static constexpr int kStage  = WK * kBufs * kBuf;
@@ -362,7 +363,8 @@ struct TreeKernel {
         // A place that a row does not see must not reach it, whatever its value: 0 * infinity is
         // NaN. So where rows see different places (masked), values that are not finite are staged as
         // zeros, and add_odd adds them to the rows that see them.
-        auto store = [&](int buf, bool masked) {
+        auto store = [&](int buf, auto masked_c) {
+            constexpr bool masked = decltype(masked_c)::value;
             unsigned char* k = stage_at(buf);
             bool odd = false;
 #pragma unroll
@@ -377,9 +379,8 @@ struct TreeKernel {
                 }
                 u32x4 kx = widen(kr[j], 1.0f), vx = widen(vr[j], vs);
                 if (!UNI && !(live >> j & 1)) kx = vx = u32x4{0, 0, 0, 0};
-                const int at = row * kRowLds + 16 * ch;
-                *reinterpret_cast<u32x4*>(k + at) = kx;
-                if (masked) {
+                *reinterpret_cast<u32x4*>(k + row * kRowK + 16 * ch) = kx;
+                if constexpr (masked) {
 #pragma unroll
                     for (int e = 0; e < 4; ++e) {
                         const uint32_t lo = (vx[e] & 0x7c00u) == 0x7c00u ? 0xffffu : 0u;
@@ -388,9 +389,9 @@ struct TreeKernel {
                         vx[e] &= ~(lo | hi);
                     }
                 }
-                *reinterpret_cast<u32x4*>(k + kTile + at) = vx;
+                *reinterpret_cast<u32x4*>(k + kTileK + row * kRowV + 16 * ch) = vx;
             }
-            if (masked) {
+            if constexpr (masked) {
                 const bool any = __builtin_amdgcn_ballot_w64(odd) != 0;
                 if (lane == 0) *reinterpret_cast<int*>(k + kFlags + 4 * wq) = any;
             }
@@ -424,22 +425,48 @@ struct TreeKernel {
         };
 
         // Where this lane's fragments lie in the stage.
-        const int ka = ql * kRowLds + 16 * hl;
-        const int va = (4 * hl + ((lane & 15) >> 2)) * kRowLds + 32 * ((lane >> 4) & 1) + 8 * (lane & 3);
+        const int ka = ql * kRowK + 16 * hl;
+        const int va = (4 * hl + ((lane & 15) >> 2)) * kRowV + 32 * ((lane >> 4) & 1) + 8 * (lane & 3);
 
         auto step_of = [&](auto masked_c, int base, const unsigned char* ks) {
             constexpr bool MASK = decltype(masked_c)::value;
-            const unsigned char* vs = ks + kTile;
+            const unsigned char* vs = ks + kTileK;
+            auto k_frag = [&](int n) {   // of part n / 8, dims 16 (n % 8) ..
+                return *reinterpret_cast<const f16x8*>(ks + ka + 32 * (n % 8) + n / 8 * kSub * kRowK);
+            };
+            auto v_part = [&](int n, int w) {
+                const int at = va + 64 * (n % 4) + (16 * (n / 4) + 8 * w) * kRowV;
+                return __builtin_amdgcn_ds_read_tr16_b64_v4i16((__attribute__((address_space(3))) s16x4*)(vs + at));
+            };
+            auto v_frag = [&](int n) {   // of 16 places from 16 (n / 4) on, dims 32 (n % 4) ..
+                const s16x4 lo = v_part(n, 0), hi = v_part(n, 1);
+                return __builtin_bit_cast(f16x8, __builtin_shufflevector(lo, hi, 0, 1, 2, 3, 4, 5, 6, 7));
+            };
+            // Fragments are read eight products ahead; the first of V before the softmax.
             f32x16 s[SUBS];
+            f16x8  kf[8], vf[8];
 #pragma unroll
-            for (int b = 0; b < SUBS; ++b) {
+            for (int n = 0; n < 8; ++n) kf[n] = k_frag(n);
+#pragma unroll
+            for (int b = 0; b < SUBS; ++b)
 #pragma unroll
                 for (int i = 0; i < 16; ++i) s[b][i] = 0.f;
 #pragma unroll
-                for (int t = 0; t < 8; ++t) {
-                    const f16x8 kf = *reinterpret_cast<const f16x8*>(ks + ka + 32 * t + b * kSub * kRowLds);
-                    s[b] = __builtin_amdgcn_mfma_f32_32x32x16_f16(kf, q[t], s[b], 0, 0, 0);
-                }
+            for (int n = 0; n < 8 * SUBS; ++n) {
+                s[n / 8] = __builtin_amdgcn_mfma_f32_32x32x16_f16(kf[n % 8], q[n % 8], s[n / 8], 0, 0, 0);
+                if (n + 8 < 8 * SUBS) kf[n % 8] = k_frag(n + 8);
+                else vf[n % 8] = v_frag(n % 8);
+            }
+            __builtin_amdgcn_sched_group_barrier(kSchedLds, 8, 0);
+#pragma unroll
+            for (int n = 0; n < 8 * (SUBS - 1); ++n) {
+                __builtin_amdgcn_sched_group_barrier(kSchedMfma, 1, 0);
+                __builtin_amdgcn_sched_group_barrier(kSchedLds, 1, 0);
+            }
+#pragma unroll
+            for (int n = 0; n < 8; ++n) {
+                __builtin_amdgcn_sched_group_barrier(kSchedMfma, 1, 0);
+                __builtin_amdgcn_sched_group_barrier(kSchedLds, 2, 0);
             }
             uint32_t seen[SUBS];
             float top = -INFINITY;
@@ -492,21 +519,18 @@ struct TreeKernel {
                     l += e;
                     p[b][i / 8][i % 8] = static_cast<_Float16>(e);
                 }
-            auto v_part = [&](int b, int d, int u, int w) {
-                const int at = va + 64 * d + (kSub * b + 16 * u + 8 * w) * kRowLds;
-                return __builtin_amdgcn_ds_read_tr16_b64_v4i16((__attribute__((address_space(3))) s16x4*)(vs + at));
-            };
-            auto v_frag = [&](int b, int d, int u) {
-                const s16x4 lo = v_part(b, d, u, 0), hi = v_part(b, d, u, 1);
-                return __builtin_bit_cast(f16x8, __builtin_shufflevector(lo, hi, 0, 1, 2, 3, 4, 5, 6, 7));
-            };
 #pragma unroll
-            for (int b = 0; b < SUBS; ++b)
+            for (int n = 0; n < 8 * SUBS; ++n) {
+                o[n % 4] = __builtin_amdgcn_mfma_f32_32x32x16_f16(vf[n % 8], p[n / 8][n / 4 % 2], o[n % 4], 0, 0, 0);
+                if (n + 8 < 8 * SUBS) vf[n % 8] = v_frag(n + 8);
+            }
+            if constexpr (SUBS == 2) {
 #pragma unroll
-                for (int u = 0; u < 2; ++u)
-#pragma unroll
-                    for (int d = 0; d < 4; ++d)
-                        o[d] = __builtin_amdgcn_mfma_f32_32x32x16_f16(v_frag(b, d, u), p[b][u], o[d], 0, 0, 0);
+                for (int n = 0; n < 8; ++n) {
+                    __builtin_amdgcn_sched_group_barrier(kSchedMfma, 1, 1);
+                    __builtin_amdgcn_sched_group_barrier(kSchedLds, 2, 1);
+                }
+            }
             if constexpr (MASK) {
                 int odd = 0;
 #pragma unroll
@@ -520,20 +544,28 @@ struct TreeKernel {
             issue(k0);
             if (k0 + 1 < k1) lookup(k0 + 1);
         }
-        for (int k = k0; k < k1; ++k) {
-            const int buf = kBufs == 2 ? (k - k0) & 1 : 0;
-            const int base = k * kStep + kPart * wk;
-            store(buf, base + kPart > all_open);
-            if (k + 1 < k1) {
-                issue(k + 1);
-                if (k + 2 < k1) lookup(k + 2);
+        // Steps that every row sees whole, then those that rows see in part: two loops, so that the
+        // second's masks cost the first neither registers nor copies of the sums.
+        auto steps = [&](auto masked_c, int from, int to) {
+            constexpr bool MASK = decltype(masked_c)::value;
+#pragma unroll 1
+            for (int k = from; k < to; ++k) {
+                const int buf = kBufs == 2 ? (k - k0) & 1 : 0;
+                const int base = k * kStep + kPart * wk;
+                store(buf, masked_c);
+                if (k + 1 < k1) {
+                    issue(k + 1);
+                    if (k + 2 < k1) lookup(k + 2);
+                }
+                if constexpr (WQ > 1) block_sync();
+                else wave_lds_sync();
+                if (!MASK || base < end) step_of(masked_c, base, stage_at(buf));
+                if constexpr (WQ == 1) wave_lds_sync();
             }
-            if constexpr (WQ > 1) block_sync();
-            else wave_lds_sync();
-            if (base + kPart <= all_open) step_of(std::false_type{}, base, stage_at(buf));
-            else if (base < end) step_of(std::true_type{}, base, stage_at(buf));
-            if constexpr (WQ == 1) wave_lds_sync();
-        }
+        };
+        const int mid = uniform(max(k0, min(k1, all_open / kStep)));
+        steps(std::false_type{}, k0, mid);
+        steps(std::true_type{}, mid, k1);
 
         const float sum = add_halves(l);
         if constexpr (WK == 1) {
