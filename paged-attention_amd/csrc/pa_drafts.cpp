@@ -115,7 +115,7 @@ pa_status pa_tree_attention(int dtype, const pa_cached_tokens* c, const pa_head_
         if (c->num_pages == 0) throw std::invalid_argument("tree_attention: a cache of no pages");
         pa::tree_shape(dtype, a);
         const size_t need = pa::tree_workspace(a);
-        if (workspace_bytes < need || (need && (!workspace || !aligned(workspace, 16))))
+        if (workspace_bytes < need || !workspace || !aligned(workspace, 16))
             throw std::invalid_argument("tree_attention: the workspace must have " + std::to_string(need) +
                                         " bytes, 16-byte aligned");
         a.q           = r.in;
@@ -125,7 +125,7 @@ pa_status pa_tree_attention(int dtype, const pa_cached_tokens* c, const pa_head_
         a.tree        = tree;
         a.words       = tree_words;
         a.score_scale = sm_scale * a.c.k_scale * 1.44269504088896340736f;
-        if (need) pa::tree_place(a, workspace);
+        pa::tree_place(a, workspace);
         pa::hip_check(pa::launch_tree_attention(dtype, a, as_stream(stream)), "tree_attention kernel launch");
     });
 }

@@ -59,12 +59,17 @@ __device__ __forceinline__ Entry entry_of_lane(const CachedTokens& c, int e) {
     return x;
 }
 
-// Units of work of an entry and one kv head: tiles of rows, times the steps over the
-// places where items are split.
+// Steps over the places that the first j row tiles of an entry are given, of each kv head: for
+// a tree j times the steps over all of its places; for a chain, whose tile i ends at place
+// start + (i + 1) tile_tokens, the sum of these ends over the step, and one more a tile, which
+// covers what rounding up adds.
+__device__ __forceinline__ long steps_before(const TreeAttention& a, const Entry& x, int step, int j) {
+    if (a.tree) return static_cast<long>(j) * ((x.start + x.n + step - 1) / step);
+    return static_cast<long>(j) + (static_cast<long>(j) * x.start + static_cast<long>(j) * (j + 1) / 2 * a.tile_tokens) / step;
+}
+__device__ __forceinline__ int tiles_of(const TreeAttention& a, const Entry& x) { return (x.n + a.tile_tokens - 1) / a.tile_tokens; }
 __device__ __forceinline__ long entry_cost(const TreeAttention& a, const Entry& x, int step) {
-    if (x.n == 0) return 0;
-    const long tiles = (x.n + a.tile_tokens - 1) / a.tile_tokens;
-    return tiles * a.c.hkv * (a.split ? (x.start + x.n + step - 1) / step : 1);
+    return x.n == 0 ? 0 : steps_before(a, x, step, tiles_of(a, x)) * a.c.hkv;
 }
 
 // The kernel's arguments, read again where this is called: read once, at the kernel's start, the
@@ -210,17 +215,16 @@ struct TreeKernel {
     typedef uint32_t Raw __attribute__((ext_vector_type(EB == 2 ? 4 : 2)));
 
     static __device__ __forceinline__ void run(const TreeAttention& a, unsigned char* lds, Schedule& sch) {
-        const long step = kStep;
         // The block's share of the units, consecutive ones on one XCD (blocks go round the 8 XCDs).
         const int nb = gridDim.x;
         const int lb = nb % 8 == 0 ? (blockIdx.x % 8) * (nb / 8) + blockIdx.x / 8 : blockIdx.x;
         long total = 0, chunk = 0;
         for (int c0 = 0; c0 < a.c.n_ent; c0 += kScan) total += chunk = scan_chunk(a, sch, c0, kStep);
-        const long per = a.split ? max(divide(total + nb - 1, nb), 1l) : 1;
+        const long per = max(divide(total + nb - 1, nb), 1l);
         long w = lb * per;
         const long w_end = min(w + per, total);
         int32_t* const desc = a.desc + kDesc * lb;   // what the merge has to join from here on
-        if (a.split && threadIdx.x == 0) desc[0] = 1;
+        if (threadIdx.x == 0) desc[0] = 1;
         if (w >= w_end) return;
         int  c0 = 0;
         long before = 0;
@@ -240,18 +244,25 @@ struct TreeKernel {
             __syncthreads();
             Entry x = entry_at(a.c, c0 + hit);
             x.n = uniform(x.n);
-            const int tiles = (x.n + a.tile_tokens - 1) / a.tile_tokens;
-            const int steps = static_cast<int>((x.start + x.n + step - 1) / step);
-            const int units = a.split ? steps : 1;
+            const int  tiles = tiles_of(a, x);
+            const long head_steps = uniform(steps_before(a, x, kStep, tiles));
             const long local = w - at;
-            const long item  = divide(local, units);
-            const int  u0    = static_cast<int>(local - item * units);
+            const int  h     = static_cast<int>(divide(local, head_steps));
+            const long inner = local - h * head_steps;
+            int rt = 0;   // the last tile that begins at or before
+            for (int span = tiles; span > 1;) {
+                const int half = span / 2;
+                if (steps_before(a, x, kStep, rt + half) <= inner) rt += half;
+                span -= half;
+            }
+            rt = uniform(rt);
+            const long first = uniform(steps_before(a, x, kStep, rt));
+            const int  units = static_cast<int>(uniform(steps_before(a, x, kStep, rt + 1)) - first);
+            const int  u0    = static_cast<int>(inner - first);
             const int  u1    = static_cast<int>(min(static_cast<long>(units), u0 + (w_end - w)));
-            const int  h     = static_cast<int>(divide(item, tiles));
-            const int  rt    = tiles - 1 - static_cast<int>(item - static_cast<long>(h) * tiles);
             const bool whole = u0 == 0 && u1 == units;
             if (u0 == 0 && u1 < units && threadIdx.x == 0) {   // the block's last item: its other parts are the next blocks' first
-                const int b1 = static_cast<int>(divide(at + (item + 1) * units - 1, per));
+                const int b1 = static_cast<int>(divide(w + units - 1, per));
                 desc[1] = x.t0 + rt * a.tile_tokens;
                 desc[2] = min(a.tile_tokens, x.n - rt * a.tile_tokens);
                 desc[3] = h;
@@ -259,7 +270,7 @@ struct TreeKernel {
                 desc[0] = b1 - lb + 1;
             }
             const int slot = whole ? -1 : 2 * lb + (w == w_first ? 0 : 1);
-            item_part(lds, x, h, rt, uniform(a.split ? u0 : 0), uniform(a.split ? u1 : steps), uniform(slot));
+            item_part(lds, x, h, rt, uniform(u0), uniform(u1), uniform(slot));
             w += u1 - u0;
         }
     }
@@ -431,8 +442,8 @@ struct TreeKernel {
         auto step_of = [&](auto masked_c, int base, const unsigned char* ks) {
             constexpr bool MASK = decltype(masked_c)::value;
             const unsigned char* vs = ks + kTileK;
-            auto k_frag = [&](int n) {   // of part n / 8, dims 16 (n % 8) ..
-                return *reinterpret_cast<const f16x8*>(ks + ka + 32 * (n % 8) + n / 8 * kSub * kRowK);
+            auto k_frag = [&](int n) {   // of part n % SUBS, dims 16 (n / SUBS) .. (the parts' sums in turn)
+                return *reinterpret_cast<const f16x8*>(ks + ka + 32 * (n / SUBS) + n % SUBS * kSub * kRowK);
             };
             auto v_part = [&](int n, int w) {
                 const int at = va + 64 * (n % 4) + (16 * (n / 4) + 8 * w) * kRowV;
@@ -453,7 +464,7 @@ struct TreeKernel {
                 for (int i = 0; i < 16; ++i) s[b][i] = 0.f;
 #pragma unroll
             for (int n = 0; n < 8 * SUBS; ++n) {
-                s[n / 8] = __builtin_amdgcn_mfma_f32_32x32x16_f16(kf[n % 8], q[n % 8], s[n / 8], 0, 0, 0);
+                s[n % SUBS] = __builtin_amdgcn_mfma_f32_32x32x16_f16(kf[n % 8], q[n / SUBS], s[n % SUBS], 0, 0, 0);
                 if (n + 8 < 8 * SUBS) kf[n % 8] = k_frag(n + 8);
                 else vf[n % 8] = v_frag(n % 8);
             }
@@ -510,14 +521,19 @@ struct TreeKernel {
                 m = now;
             }
             const float ref = (m == -INFINITY ? 0.f : m) - kShift;
+            const f16x2 ones2 = {static_cast<_Float16>(1.f), static_cast<_Float16>(1.f)};
             f16x8 p[SUBS][2];
 #pragma unroll
             for (int b = 0; b < SUBS; ++b)
 #pragma unroll
-                for (int i = 0; i < 16; ++i) {
-                    const float e = exp2_fast(BS ? s[b][i] - ref : fmaf(s[b][i], one, -ref));
-                    l += e;
-                    p[b][i / 8][i % 8] = static_cast<_Float16>(e);
+                for (int i = 0; i < 16; i += 2) {
+                    const float e0 = exp2_fast(BS ? s[b][i] - ref : fmaf(s[b][i], one, -ref));
+                    const float e1 = exp2_fast(BS ? s[b][i + 1] - ref : fmaf(s[b][i + 1], one, -ref));
+                    // (Summed as they are rounded, two an instruction, in 32 bits.)
+                    const f16x2 e = {static_cast<_Float16>(e0), static_cast<_Float16>(e1)};
+                    l = __builtin_amdgcn_fdot2(e, ones2, l, false);
+                    p[b][i / 8][i % 8] = e[0];
+                    p[b][i / 8][i % 8 + 1] = e[1];
                 }
 #pragma unroll
             for (int n = 0; n < 8 * SUBS; ++n) {
@@ -728,14 +744,10 @@ void tree_shape(int dtype, TreeAttention& a) {
     const long per = (static_cast<long>(a.c.n_tok) * a.group + a.c.n_ent - 1) / std::max(a.c.n_ent, 1);   // rows of an entry
     a.rows        = per <= 32 && a.group <= 32 ? 32 : per <= 64 && a.group <= 64 ? 64 : per <= 128 ? 128 : 256;
     a.tile_tokens = a.rows / a.group;
-    const long items = (static_cast<long>(a.c.n_tok) / a.tile_tokens + a.c.n_ent) * a.c.hkv;   // at most
-    const int  cus = device_cus();
-    a.split = items <= 16l * cus;
-    a.grid  = a.split ? cus * (a.rows <= 128 ? 2 : 1) : static_cast<int>(items);
+    a.grid = device_cus() * (a.rows <= 128 ? 2 : 1);
 }
 
 size_t tree_workspace(const TreeAttention& a) {
-    if (!a.split) return 0;
     return static_cast<size_t>(2 * a.grid) * a.rows * (kHeadDim + 2) * sizeof(float) +
            static_cast<size_t>(a.grid) * kDesc * sizeof(int32_t);
 }
@@ -752,8 +764,7 @@ hipError_t launch_tree_attention(int dtype, const TreeAttention& a, hipStream_t 
     if (dtype == PA_KV_FP16) launch_e<2, false>(a, s);
     else if (dtype == PA_KV_FP8_E4M3) launch_e<1, false>(a, s);
     else launch_e<1, true>(a, s);
-    if (a.split)
-        hipLaunchKernelGGL(tree_merge_kernel, dim3(a.grid, a.rows / kMergeWaves), dim3(64 * kMergeWaves), 0, s, a.desc, a);
+    hipLaunchKernelGGL(tree_merge_kernel, dim3(a.grid, a.rows / kMergeWaves), dim3(64 * kMergeWaves), 0, s, a.desc, a);
     return hipGetLastError();
 }
 
