@@ -5,6 +5,7 @@
 #include "pa_fp8.hpp"
 
 #include <algorithm>
+#include <cfloat>
 #include <climits>
 #include <cmath>
 #include <cstdint>
@@ -29,6 +30,20 @@ constexpr int kOutLd   = kHeadDim + 4;    // floats of a row in the joining of w
 // to 2^-20 of the maximum (fp16 is subnormal below 2^-14).
 constexpr float kShift = 6.0f;
 constexpr float kLag   = 8.0f;
+
+// Accesses to global memory through pointers that come from memory (arguments() below): without
+// saying where they point, they count as LDS accesses, too, and out of order, and
+// every wait for a fragment then waits for all of them.
+template <class T>
+using Global = __attribute__((address_space(1))) T;
+template <class T>
+__device__ __forceinline__ T load_global(const void* p) {
+    return *(const Global<T>*)(p);
+}
+template <class T>
+__device__ __forceinline__ void store_global(void* p, T x) {
+    *(Global<T>*)(p) = x;
+}
 
 struct Entry {
     int t0, n, start, row;
@@ -178,11 +193,11 @@ __device__ __forceinline__ uint32_t visible(const TreeAttention& a, const Entry&
     uint32_t bits;
     if (j0 < 0) {
         bits = ones(-j0);
-        if (j0 > -32) bits |= static_cast<uint32_t>(row[0] << -j0);
+        if (j0 > -32) bits |= static_cast<uint32_t>(load_global<uint64_t>(row) << -j0);
     } else {
         const int w = j0 >> 6, sh = j0 & 63;
-        uint64_t v = w < a.words ? row[w] >> sh : 0;
-        if (sh > 32 && w + 1 < a.words) v |= row[w + 1] << (64 - sh);
+        uint64_t v = w < a.words ? load_global<uint64_t>(row + w) >> sh : 0;
+        if (sh > 32 && w + 1 < a.words) v |= load_global<uint64_t>(row + w + 1) << (64 - sh);
         bits = static_cast<uint32_t>(v);
     }
     return bits & ones(x.n - j0);
@@ -289,7 +304,7 @@ struct TreeKernel {
         k1 = uniform(min(k1, (end + kStep - 1) / kStep));
 
         // Query fragments, and the lane's token. (A negative scale turns the queries' signs.)
-        const float    score_scale = fabsf(a.score_scale);
+        const float    score_scale = fmaxf(fabsf(a.score_scale), FLT_MIN);   // (of 0, one that makes every score 0 but minus infinity)
         const uint32_t flip = a.score_scale < 0.f ? 0x80008000u : 0u;
         f16x8 q[8];
         const int my_row = 32 * wq + ql, my_i = a.by_group.of(my_row), my_g = my_row - my_i * G;
@@ -299,12 +314,13 @@ struct TreeKernel {
             const uint16_t* p = a.q + (x.t0 + tok0 + (row_ok ? my_i : 0)) * a.q_stride + (h * G + (row_ok ? my_g : 0)) * kHeadDim + 8 * hl;
 #pragma unroll
             for (int s = 0; s < 8; ++s) {
-                u32x4 y = *reinterpret_cast<const u32x4*>(p + 16 * s);
+                u32x4 y = load_global<u32x4>(p + 16 * s);
 #pragma unroll
                 for (int e = 0; e < 4; ++e) y[e] ^= flip;
                 q[s] = __builtin_bit_cast(f16x8, y);
             }
         }
+        const bool has_rows = 32 * wq < tile_n * G;   // else the wave only stages
         const int all_open = uniform(x.start + (a.tree ? 0 : tok0 + 1));   // places before this one are seen by every row
 
         f32x16 o[4];
@@ -327,7 +343,7 @@ struct TreeKernel {
         uint32_t live = 0;     // general pages: loads whose row holds a place
         auto lookup = [&](int k) {
             const int t = k * kStep + kPart * wk + RG * lane;
-            pg = lane < kPart / RG && t < end ? table[a.by_page.of(t)] : -1;
+            pg = lane < kPart / RG && t < end ? load_global<int32_t>(table + a.by_page.of(t)) : -1;
         };
         auto issue = [&](int k) {
             const int  t  = k * kStep + kPart * wk + RG * lane;
@@ -337,7 +353,7 @@ struct TreeKernel {
             const uint32_t lo = static_cast<uint32_t>(off), hi = static_cast<uint32_t>(off >> 32);
             const int rows = ok ? min(RG, end - t) : 0;
             if constexpr (BS)
-                sc = rows > 0 ? *reinterpret_cast<const uint16_t*>(c.scales + 2 * ((static_cast<size_t>(pg) * c.hkv + h) * nblk + (s >> bsh))) : 0;
+                sc = rows > 0 ? load_global<uint16_t>(c.scales + 2 * ((static_cast<size_t>(pg) * c.hkv + h) * nblk + (s >> bsh))) : 0;
             live = 0;
 #pragma unroll
             for (int j = 0; j < NJ; ++j) {
@@ -360,8 +376,8 @@ struct TreeKernel {
                     const size_t at = (static_cast<size_t>(static_cast<uint32_t>(__shfl(static_cast<int>(hi), from))) << 32 |
                                        static_cast<uint32_t>(__shfl(static_cast<int>(lo), from))) + ch * 8 * EB;
                     live |= __shfl(rows, from) > 0 ? 1u << j : 0u;
-                    kr[j] = *reinterpret_cast<const Raw*>(static_cast<const unsigned char*>(c.k_cache) + at);
-                    vr[j] = *reinterpret_cast<const Raw*>(static_cast<const unsigned char*>(c.v_cache) + at);
+                    kr[j] = load_global<Raw>(static_cast<const unsigned char*>(c.k_cache) + at);
+                    vr[j] = load_global<Raw>(static_cast<const unsigned char*>(c.v_cache) + at);
                 }
             }
         };
@@ -426,8 +442,8 @@ struct TreeKernel {
                 for (int n = 0; n < 64; ++n) {
                     const int at = 8 * (n / 4) + 4 * hl + n % 4;
                     float y;
-                    if constexpr (EB == 2) y = f16_bits_to_f32(reinterpret_cast<const uint16_t*>(v)[at]);
-                    else y = (v[at] & 0x7f) == 0x7f ? NAN : 0.f;
+                    if constexpr (EB == 2) y = f16_bits_to_f32(load_global<uint16_t>(v + 2 * at));
+                    else y = (load_global<uint8_t>(v + at) & 0x7f) == 0x7f ? NAN : 0.f;
                     if (!(fabsf(y) < INFINITY)) sums[n] += y;
                 }
             }
@@ -575,7 +591,7 @@ struct TreeKernel {
                 }
                 if constexpr (WQ > 1) block_sync();
                 else wave_lds_sync();
-                if (!MASK || base < end) step_of(masked_c, base, stage_at(buf));
+                if (has_rows && (!MASK || base < end)) step_of(masked_c, base, stage_at(buf));
                 if constexpr (WQ == 1) wave_lds_sync();
             }
         };
@@ -593,9 +609,8 @@ struct TreeKernel {
                 for (int d = 0; d < 4; ++d)
 #pragma unroll
                     for (int i = 0; i < 4; ++i)
-                        *reinterpret_cast<f32x4*>(po + 32 * d + 8 * i) =
-                            f32x4{o[d][4 * i], o[d][4 * i + 1], o[d][4 * i + 2], o[d][4 * i + 3]};
-                if (hl == 0) *reinterpret_cast<f32x2*>(a.part_ml + 2 * at) = f32x2{m, sum};
+                        store_global(po + 32 * d + 8 * i, f32x4{o[d][4 * i], o[d][4 * i + 1], o[d][4 * i + 2], o[d][4 * i + 3]});
+                if (hl == 0) store_global(a.part_ml + 2 * at, f32x2{m, sum});
             } else if (row_ok) {
                 const float scale = sum == 0.f ? 0.f : c.v_scale / sum;
                 uint16_t* out = a.out + (x.t0 + tok) * a.out_stride + (h * G + my_g) * kHeadDim + 4 * hl;
@@ -605,8 +620,7 @@ struct TreeKernel {
                     for (int i = 0; i < 4; ++i) {
                         const f16x2 lo = {static_cast<_Float16>(o[d][4 * i] * scale), static_cast<_Float16>(o[d][4 * i + 1] * scale)};
                         const f16x2 hi = {static_cast<_Float16>(o[d][4 * i + 2] * scale), static_cast<_Float16>(o[d][4 * i + 3] * scale)};
-                        *reinterpret_cast<u32x2*>(out + 32 * d + 8 * i) =
-                            u32x2{__builtin_bit_cast(uint32_t, lo), __builtin_bit_cast(uint32_t, hi)};
+                        store_global(out + 32 * d + 8 * i, u32x2{__builtin_bit_cast(uint32_t, lo), __builtin_bit_cast(uint32_t, hi)});
                     }
             }
             if constexpr (WQ > 1) block_sync();   // the stage is free again
@@ -654,15 +668,14 @@ struct TreeKernel {
                     for (int e = 0; e < 4; ++e) y[e] = fmaf(z[e], f[g], y[e]);
                 }
                 if (slot >= 0) {
-                    *reinterpret_cast<f32x4*>(a.part_out + at * kHeadDim + d) = y;
+                    store_global(a.part_out + at * kHeadDim + d, y);
                 } else {
                     const f16x2 lo = {static_cast<_Float16>(y[0] * scale), static_cast<_Float16>(y[1] * scale)};
                     const f16x2 hi = {static_cast<_Float16>(y[2] * scale), static_cast<_Float16>(y[3] * scale)};
-                    *reinterpret_cast<u32x2*>(out + d) =
-                        u32x2{__builtin_bit_cast(uint32_t, lo), __builtin_bit_cast(uint32_t, hi)};
+                    store_global(out + d, u32x2{__builtin_bit_cast(uint32_t, lo), __builtin_bit_cast(uint32_t, hi)});
                 }
             }
-            if (slot >= 0 && part == 0) *reinterpret_cast<f32x2*>(a.part_ml + 2 * at) = f32x2{top, den};
+            if (slot >= 0 && part == 0) store_global(a.part_ml + 2 * at, f32x2{top, den});
         }
         __syncthreads();   // the stage is free again
     }
