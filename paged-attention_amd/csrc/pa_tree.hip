@@ -212,7 +212,9 @@ struct TreeKernel {
     static constexpr int kBlock  = 64 * kWaves;
     static constexpr int kRowsM  = 32 * WQ;
     static constexpr int SUBS    = WQ >= 4 ? 2 : 1;            // 32-place parts of a stream's step
-    static constexpr int kPart   = kSub * SUBS;                // places of a stream's step
+    static constexpr int HALVES  = WQ == 8 && UNI ? 2 : 1;     // turns of that many parts between two barriers
+    static constexpr int kTurn   = kSub * SUBS;
+    static constexpr int kPart   = kTurn * HALVES;             // places of a stream's step
     static constexpr int kStep   = kPart * WK;
     static constexpr int NJ      = kPart / (4 * WQ);           // loads of 4 rows per wave, of K and of V
     static constexpr int kBufs   = WQ > 1 ? 2 : 1;
@@ -429,7 +431,7 @@ struct TreeKernel {
 #pragma unroll
             for (int n = 0; n < 64; ++n) sums[n] = o[n / 16][n % 16];
 #pragma unroll 1
-            for (int t = 0; t < kPart && base + t < end; ++t) {
+            for (int t = 0; t < kTurn && base + t < end; ++t) {
                 const int i = a.by_page.of(base + t), page = load_uniform(table, i);
                 if (page < 0 || page >= c.num_pages) continue;
                 const unsigned char* v = static_cast<const unsigned char*>(c.v_cache) + page * page_bytes + head_off +
@@ -455,9 +457,10 @@ struct TreeKernel {
         const int ka = ql * kRowK + 16 * hl;
         const int va = (4 * hl + ((lane & 15) >> 2)) * kRowV + 32 * ((lane >> 4) & 1) + 8 * (lane & 3);
 
-        auto step_of = [&](auto masked_c, int base, const unsigned char* ks) {
+        auto step_of = [&](auto masked_c, int base, const unsigned char* buf, int turn) {
             constexpr bool MASK = decltype(masked_c)::value;
-            const unsigned char* vs = ks + kTileK;
+            const unsigned char* ks = buf + turn * kTurn * kRowK;
+            const unsigned char* vs = buf + kTileK + turn * kTurn * kRowV;
             auto k_frag = [&](int n) {   // of part n % SUBS, dims 16 (n / SUBS) .. (the parts' sums in turn)
                 return *reinterpret_cast<const f16x8*>(ks + ka + 32 * (n / SUBS) + n % SUBS * kSub * kRowK);
             };
@@ -502,7 +505,7 @@ struct TreeKernel {
                 if constexpr (BS) {
 #pragma unroll
                     for (int i = 0; i < 4; ++i) {
-                        const float cs = *reinterpret_cast<const float*>(ks + kScales + 4 * (8 * b + 2 * i + hl));
+                        const float cs = *reinterpret_cast<const float*>(buf + kScales + kTurn * turn + 4 * (8 * b + 2 * i + hl));
 #pragma unroll
                         for (int e = 0; e < 4; ++e) s[b][4 * i + e] *= cs;
                     }
@@ -566,7 +569,7 @@ struct TreeKernel {
             if constexpr (MASK) {
                 int odd = 0;
 #pragma unroll
-                for (int w = 0; w < WQ; ++w) odd |= *reinterpret_cast<const int*>(ks + kFlags + 4 * w);
+                for (int w = 0; w < WQ; ++w) odd |= *reinterpret_cast<const int*>(buf + kFlags + 4 * w);
                 if (__builtin_amdgcn_readfirstlane(odd)) add_odd(base, seen, o);
             }
         };
@@ -591,7 +594,11 @@ struct TreeKernel {
                 }
                 if constexpr (WQ > 1) block_sync();
                 else wave_lds_sync();
-                if (has_rows && (!MASK || base < end)) step_of(masked_c, base, stage_at(buf));
+                if (has_rows) {
+#pragma unroll
+                    for (int t = 0; t < HALVES; ++t)
+                        if (!MASK || base + kTurn * t < end) step_of(masked_c, base + kTurn * t, stage_at(buf), t);
+                }
                 if constexpr (WQ == 1) wave_lds_sync();
             }
         };
