@@ -227,6 +227,7 @@ struct TreeAttention {
     float           score_scale;   // of q k into base-2 exponents
     // Set by tree_shape, with the workspace.
     int             rows, tile_tokens, grid;
+    PlaceDiv        by_tile;
     float*          part_out;  // [2 grid][rows][128]
     float*          part_ml;   // [2 grid][rows][2]
     int32_t*        desc;      // [n_tok][hkv][2]

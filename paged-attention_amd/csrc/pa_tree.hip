@@ -21,6 +21,7 @@ typedef short    s16x4  __attribute__((ext_vector_type(4)));
 constexpr int kSub     = 32;              // places of one MFMA step
 constexpr int kScan    = 256;             // entries that a block looks at together
 constexpr int kMergeWaves = 4;
+constexpr int kItemUnits  = 3;   // what a tile costs besides its steps, in steps
 constexpr int kSchedMfma = 0x8, kSchedLds = 0x100;   // of sched_group_barrier
 constexpr int kDesc    = 8;               // ints of a block's entry for the merge
 constexpr int kOutLd   = kHeadDim + 4;    // floats of a row in the joining of waves
@@ -74,15 +75,17 @@ __device__ __forceinline__ Entry entry_of_lane(const CachedTokens& c, int e) {
     return x;
 }
 
-// Steps over the places that the first j row tiles of an entry are given, of each kv head: for
-// a tree j times the steps over all of its places; for a chain, whose tile i ends at place
-// start + (i + 1) tile_tokens, the sum of these ends over the step, and one more a tile, which
-// covers what rounding up adds.
+// Units of work of the first j row tiles of an entry and one kv head: their steps over the places
+// that they are given, and kItemUnits each for what a tile costs besides (its queries, the first
+// rows' way through the page table, its output: 7 to 10 us, a step of 256 rows 3.5). For a tree j
+// times the steps over all of the entry's places; for a chain, whose tile i ends at place start +
+// (i + 1) tile_tokens, the sum of these ends over the step, and one more a tile, which covers what
+// rounding up adds.
 __device__ __forceinline__ long steps_before(const TreeAttention& a, const Entry& x, int step, int j) {
-    if (a.tree) return static_cast<long>(j) * ((x.start + x.n + step - 1) / step);
-    return static_cast<long>(j) + (static_cast<long>(j) * x.start + static_cast<long>(j) * (j + 1) / 2 * a.tile_tokens) / step;
+    if (a.tree) return static_cast<long>(j) * (kItemUnits + (x.start + x.n + step - 1) / step);
+    return static_cast<long>(j) * (kItemUnits + 1) + (static_cast<long>(j) * x.start + static_cast<long>(j) * (j + 1) / 2 * a.tile_tokens) / step;
 }
-__device__ __forceinline__ int tiles_of(const TreeAttention& a, const Entry& x) { return (x.n + a.tile_tokens - 1) / a.tile_tokens; }
+__device__ __forceinline__ int tiles_of(const TreeAttention& a, const Entry& x) { return a.by_tile.of(x.n + a.tile_tokens - 1); }
 __device__ __forceinline__ long entry_cost(const TreeAttention& a, const Entry& x, int step) {
     return x.n == 0 ? 0 : steps_before(a, x, step, tiles_of(a, x)) * a.c.hkv;
 }
@@ -109,9 +112,18 @@ __device__ __forceinline__ long uniform(long x) {
                              static_cast<uint32_t>(__builtin_amdgcn_readfirstlane(static_cast<int>(x))));
 }
 
-// a / b for 0 <= a < 2^52, b > 0, wave-uniform: through doubles (a 64-bit integer
-// division is 140 scalar instructions).
+// a / b for 0 <= a < 2^53, 0 < b, wave-uniform: in 32 bits where a is small (nearly always), else
+// through doubles (a 64-bit integer division is 140 scalar instructions). Either quotient is off
+// by one at most before it is put right.
 __device__ __forceinline__ long divide(long a, long b) {
+    if (a < (1 << 22)) {
+        if (b > a) return 0;
+        const int x = static_cast<int>(a), y = static_cast<int>(b);
+        int q = static_cast<int>(static_cast<float>(x) * __builtin_amdgcn_rcpf(static_cast<float>(y)));
+        const int r = x - q * y;
+        q += r >= y ? 1 : r < 0 ? -1 : 0;
+        return uniform(q);
+    }
     long q = static_cast<long>(static_cast<double>(a) / static_cast<double>(b));
     const long r = a - q * b;
     q += r >= b ? 1 : r < 0 ? -1 : 0;
@@ -127,15 +139,7 @@ struct Schedule {
 // The units of entries c0 .. c0 + 255 as a running sum in s.pre (by the block's first 256 threads).
 __device__ __forceinline__ long scan_chunk(const TreeAttention& a, Schedule& s, int c0, int step) {
     const int tid = threadIdx.x, lane = tid & 63, wave = tid >> 6;
-    if (a.c.n_ent == 1) {
-        const long one = entry_cost(a, entry_at(a.c, 0), step);
-        if (tid == 0) {
-            s.pre[0] = 0;
-            s.pre[1] = one;
-        }
-        __syncthreads();
-        return one;
-    }
+    if (a.c.n_ent == 1) return entry_cost(a, entry_at(a.c, 0), step);   // nothing to look for
     const bool mine = tid < kScan;
     long x = mine && c0 + tid < a.c.n_ent ? entry_cost(a, entry_of_lane(a.c, c0 + tid), step) : 0;
 #pragma unroll
@@ -224,8 +228,10 @@ struct TreeKernel {
     static constexpr int kBuf    = kFlags + 16 * ((4 * WQ + 15) / 16);
     static constexpr int kStage  = WK * kBufs * kBuf;
     static constexpr int kJoin   = kWaves * 32 * (kOutLd * 4 + 8);
-    static constexpr int kJoinOf = WK > 1 ? kJoin : 0;
-    static constexpr int kLds    = kStage > kJoinOf ? kStage : kJoinOf;
+    static constexpr int kLds    = kStage > kJoin ? kStage : kJoin;
+    // Loads bypass the caches where hardly any place is read twice: tiles that hold all of an entry's
+    // rows. (us with cached and with such loads: 16 over 32 x 8192 fp16 219 / 203, 4096 over 4096 451 / 511.)
+    static constexpr int kAux    = WQ < 8 ? 2 : 0;
     static constexpr int RG      = UNI ? 4 : 1;                // rows that a lane looks up
     static_assert(kPart / RG <= 64 && NJ >= 1);
 
@@ -246,19 +252,22 @@ struct TreeKernel {
         int  c0 = 0;
         long before = 0;
         if (a.c.n_ent > kScan) chunk = scan_chunk(a, sch, 0, kStep);
-        const long w_first = w;
         while (w < w_end) {
             while (w >= before + chunk) {
                 before += chunk;
                 c0 += kScan;
                 chunk = scan_chunk(a, sch, c0, kStep);
             }
-            const int tid = threadIdx.x;
-            if (tid < kScan && sch.pre[tid] <= w - before && w - before < sch.pre[tid + 1]) sch.hit = tid;
-            __syncthreads();
-            const int  hit = a.c.n_ent == 1 ? 0 : __builtin_amdgcn_readfirstlane(sch.hit);
-            const long at  = before + uniform(sch.pre[hit]);
-            __syncthreads();
+            int  hit = 0;
+            long at  = 0;
+            if (a.c.n_ent > 1) {
+                const int tid = threadIdx.x;
+                if (tid < kScan && sch.pre[tid] <= w - before && w - before < sch.pre[tid + 1]) sch.hit = tid;
+                __syncthreads();
+                hit = __builtin_amdgcn_readfirstlane(sch.hit);
+                at  = before + uniform(sch.pre[hit]);
+                __syncthreads();
+            }
             Entry x = entry_at(a.c, c0 + hit);
             x.n = uniform(x.n);
             const int  tiles = tiles_of(a, x);
@@ -277,17 +286,18 @@ struct TreeKernel {
             const int  units = static_cast<int>(uniform(steps_before(a, x, kStep, rt + 1)) - first);
             const int  u0    = static_cast<int>(inner - first);
             const int  u1    = static_cast<int>(min(static_cast<long>(units), u0 + (w_end - w)));
-            const bool whole = u0 == 0 && u1 == units;
-            if (u0 == 0 && u1 < units && threadIdx.x == 0) {   // the block's last item: its other parts are the next blocks' first
-                const int b1 = static_cast<int>(divide(w + units - 1, per));
-                desc[1] = x.t0 + rt * a.tile_tokens;
-                desc[2] = min(a.tile_tokens, x.n - rt * a.tile_tokens);
-                desc[3] = h;
-                desc[4] = 2 * lb + (w == w_first ? 0 : 1);
-                desc[0] = b1 - lb + 1;
+            // Its first kItemUnits are no steps: a share that ends among them leaves the tile to the next block.
+            if (u1 > kItemUnits) {
+                const bool begins = u0 <= kItemUnits, ends = u1 == units;
+                if (begins && !ends && threadIdx.x == 0) {   // the block's last tile: its other parts are the next blocks' first
+                    desc[1] = x.t0 + rt * a.tile_tokens;
+                    desc[2] = min(a.tile_tokens, x.n - rt * a.tile_tokens);
+                    desc[3] = h;
+                    desc[0] = static_cast<int>(divide(w - u0 + units - 1, per)) - lb + 1;
+                }
+                item_part(lds, x, h, rt, uniform(max(u0, kItemUnits) - kItemUnits), uniform(u1 - kItemUnits),
+                          uniform(begins && ends ? -1 : 2 * lb + (begins ? 1 : 0)));
             }
-            const int slot = whole ? -1 : 2 * lb + (w == w_first ? 0 : 1);
-            item_part(lds, x, h, rt, uniform(u0), uniform(u1), uniform(slot));
             w += u1 - u0;
         }
     }
@@ -305,23 +315,6 @@ struct TreeKernel {
         const int end = uniform(x.start + (a.tree ? x.n : tok0 + tile_n));   // places from here on are not seen
         k1 = uniform(min(k1, (end + kStep - 1) / kStep));
 
-        // Query fragments, and the lane's token. (A negative scale turns the queries' signs.)
-        const float    score_scale = fmaxf(fabsf(a.score_scale), FLT_MIN);   // (of 0, one that makes every score 0 but minus infinity)
-        const uint32_t flip = a.score_scale < 0.f ? 0x80008000u : 0u;
-        f16x8 q[8];
-        const int my_row = 32 * wq + ql, my_i = a.by_group.of(my_row), my_g = my_row - my_i * G;
-        const bool row_ok = my_i < tile_n;
-        const int  tok = row_ok ? tok0 + my_i : INT_MAX;
-        {
-            const uint16_t* p = a.q + (x.t0 + tok0 + (row_ok ? my_i : 0)) * a.q_stride + (h * G + (row_ok ? my_g : 0)) * kHeadDim + 8 * hl;
-#pragma unroll
-            for (int s = 0; s < 8; ++s) {
-                u32x4 y = load_global<u32x4>(p + 16 * s);
-#pragma unroll
-                for (int e = 0; e < 4; ++e) y[e] ^= flip;
-                q[s] = __builtin_bit_cast(f16x8, y);
-            }
-        }
         const bool has_rows = 32 * wq < tile_n * G;   // else the wave only stages
         const int all_open = uniform(x.start + (a.tree ? 0 : tok0 + 1));   // places before this one are seen by every row
 
@@ -347,6 +340,23 @@ struct TreeKernel {
             const int t = k * kStep + kPart * wk + RG * lane;
             pg = lane < kPart / RG && t < end ? load_global<int32_t>(table + a.by_page.of(t)) : -1;
         };
+        if (k0 < k1) lookup(k0);   // (before the queries' loads, which come back in order)
+
+        // The tile's queries, 16 lanes a row, on their way to LDS (loaded as fragments, each load would
+        // touch 32 lines: 4 us an item with 8 waves). A negative scale turns their signs.
+        const float    score_scale = fmaxf(fabsf(a.score_scale), FLT_MIN);   // (of 0, one that makes every score 0 but minus infinity)
+        const uint32_t flip = a.score_scale < 0.f ? 0x80008000u : 0u;
+        constexpr int NQ = kRowsM * 16 / kBlock;
+        f16x8 q[8];
+        u32x4 qr[NQ];
+#pragma unroll
+        for (int j = 0; j < NQ; ++j) {
+            const int row = (tid >> 4) + j * (kBlock / 16), i = a.by_group.of(row), g = row - i * G;
+            const bool ok = i < tile_n;
+            qr[j] = load_global<u32x4>(a.q + (x.t0 + tok0 + (ok ? i : 0)) * a.q_stride + (h * G + (ok ? g : 0)) * kHeadDim + 8 * (tid & 15));
+        }
+        const int my_row = 32 * wq + ql, my_i = a.by_group.of(my_row);
+        const int tok = my_i < tile_n ? tok0 + my_i : INT_MAX;
         auto issue = [&](int k) {
             const int  t  = k * kStep + kPart * wk + RG * lane;
             const bool ok = pg >= 0 && pg < c.num_pages;
@@ -367,11 +377,11 @@ struct TreeKernel {
                     const __amdgpu_buffer_rsrc_t kb = buffer_rsrc(static_cast<const unsigned char*>(c.k_cache) + at, bytes);
                     const __amdgpu_buffer_rsrc_t vb = buffer_rsrc(static_cast<const unsigned char*>(c.v_cache) + at, bytes);
                     if constexpr (EB == 2) {
-                        kr[j] = __builtin_bit_cast(Raw, __builtin_amdgcn_raw_buffer_load_b128(kb, 16 * lane, 0, 0));
-                        vr[j] = __builtin_bit_cast(Raw, __builtin_amdgcn_raw_buffer_load_b128(vb, 16 * lane, 0, 0));
+                        kr[j] = __builtin_bit_cast(Raw, __builtin_amdgcn_raw_buffer_load_b128(kb, 16 * lane, 0, kAux));
+                        vr[j] = __builtin_bit_cast(Raw, __builtin_amdgcn_raw_buffer_load_b128(vb, 16 * lane, 0, kAux));
                     } else {
-                        kr[j] = __builtin_bit_cast(Raw, __builtin_amdgcn_raw_buffer_load_b64(kb, 8 * lane, 0, 0));
-                        vr[j] = __builtin_bit_cast(Raw, __builtin_amdgcn_raw_buffer_load_b64(vb, 8 * lane, 0, 0));
+                        kr[j] = __builtin_bit_cast(Raw, __builtin_amdgcn_raw_buffer_load_b64(kb, 8 * lane, 0, kAux));
+                        vr[j] = __builtin_bit_cast(Raw, __builtin_amdgcn_raw_buffer_load_b64(vb, 8 * lane, 0, kAux));
                     }
                 } else {
                     const int from = 4 * r4 + row0;
@@ -575,10 +585,21 @@ struct TreeKernel {
         };
 
         if (k0 < k1) {
-            lookup(k0);
             issue(k0);
             if (k0 + 1 < k1) lookup(k0 + 1);
         }
+        // (At the end of the stage, which the first step does not write where streams have two buffers.)
+        unsigned char* const qs = lds + kStage - kRowsM * kRowK;
+#pragma unroll
+        for (int j = 0; j < NQ; ++j) {
+#pragma unroll
+            for (int e = 0; e < 4; ++e) qr[j][e] ^= flip;
+            *reinterpret_cast<u32x4*>(qs + ((tid >> 4) + j * (kBlock / 16)) * kRowK + 16 * (tid & 15)) = qr[j];
+        }
+        block_sync();
+#pragma unroll
+        for (int s = 0; s < 8; ++s) q[s] = *reinterpret_cast<const f16x8*>(qs + my_row * kRowK + 32 * s + 16 * hl);
+        if constexpr (kBufs == 1) block_sync();
         // Steps that every row sees whole, then those that rows see in part: two loops, so that the
         // second's masks cost the first neither registers nor copies of the sums.
         auto steps = [&](auto masked_c, int from, int to) {
@@ -608,27 +629,42 @@ struct TreeKernel {
 
         const float sum = add_halves(l);
         if constexpr (WK == 1) {
-            // The wave has its rows' whole sums: from the registers.
+            // The wave has its rows' whole sums. They go through LDS, so that a store takes whole rows.
+            block_sync();   // no wave reads the stage any more
+            unsigned char* const mine = lds + wave * 32 * kOutLd * 4;
             if (slot >= 0) {
-                const size_t at = static_cast<size_t>(slot) * kRowsM + my_row;
-                float* po = a.part_out + at * kHeadDim + 4 * hl;
+                const size_t at = static_cast<size_t>(slot) * kRowsM + 32 * wq;
 #pragma unroll
                 for (int d = 0; d < 4; ++d)
 #pragma unroll
                     for (int i = 0; i < 4; ++i)
-                        store_global(po + 32 * d + 8 * i, f32x4{o[d][4 * i], o[d][4 * i + 1], o[d][4 * i + 2], o[d][4 * i + 3]});
-                if (hl == 0) store_global(a.part_ml + 2 * at, f32x2{m, sum});
-            } else if (row_ok) {
+                        *reinterpret_cast<f32x4*>(mine + 4 * (ql * kOutLd + 32 * d + 8 * i + 4 * hl)) =
+                            f32x4{o[d][4 * i], o[d][4 * i + 1], o[d][4 * i + 2], o[d][4 * i + 3]};
+                wave_lds_sync();
+                if (hl == 0) store_global(a.part_ml + 2 * (at + ql), f32x2{m, sum});
+#pragma unroll 4
+                for (int r = 0; r < 32; r += 2)
+                    store_global(a.part_out + (at + r + hl) * kHeadDim + 4 * ql,
+                                 *reinterpret_cast<const f32x4*>(mine + 4 * ((r + hl) * kOutLd + 4 * ql)));
+            } else if (has_rows) {
                 const float scale = sum == 0.f ? 0.f : c.v_scale / sum;
-                uint16_t* out = a.out + (x.t0 + tok) * a.out_stride + (h * G + my_g) * kHeadDim + 4 * hl;
 #pragma unroll
                 for (int d = 0; d < 4; ++d)
 #pragma unroll
                     for (int i = 0; i < 4; ++i) {
                         const f16x2 lo = {static_cast<_Float16>(o[d][4 * i] * scale), static_cast<_Float16>(o[d][4 * i + 1] * scale)};
                         const f16x2 hi = {static_cast<_Float16>(o[d][4 * i + 2] * scale), static_cast<_Float16>(o[d][4 * i + 3] * scale)};
-                        store_global(out + 32 * d + 8 * i, u32x2{__builtin_bit_cast(uint32_t, lo), __builtin_bit_cast(uint32_t, hi)});
+                        *reinterpret_cast<u32x2*>(mine + ql * kRowK + 64 * d + 16 * i + 8 * hl) =
+                            u32x2{__builtin_bit_cast(uint32_t, lo), __builtin_bit_cast(uint32_t, hi)};
                     }
+                wave_lds_sync();
+#pragma unroll 4
+                for (int r = lane >> 4; r < 32; r += 4) {
+                    const int i = a.by_group.of(32 * wq + r), g = 32 * wq + r - i * G;
+                    if (i < tile_n)
+                        store_global(a.out + (x.t0 + tok0 + i) * a.out_stride + (h * G + g) * kHeadDim + 8 * (lane & 15),
+                                     *reinterpret_cast<const u32x4*>(mine + r * kRowK + 16 * (lane & 15)));
+                }
             }
             if constexpr (WQ > 1) block_sync();   // the stage is free again
             return;
@@ -651,7 +687,8 @@ struct TreeKernel {
         const int row = tid / TR, part = tid % TR;
         float top = -INFINITY, den = 0.f, f[WK];
 #pragma unroll
-        for (int g = 0; g < WK; ++g) top = fmaxf(top, ml[2 * (kRowsM * g + row)]);
+        for (int g = 0; g < WK; ++g)
+            top = fmaxf(top, ml[2 * (kRowsM * g + row)]);
         const float ref = top == -INFINITY ? 0.f : top;
 #pragma unroll
         for (int g = 0; g < WK; ++g) {
@@ -696,52 +733,83 @@ __global__ __launch_bounds__(64 * WQ * WK, 2) void tree_attention_kernel(const T
     T::run(a, lds, sch);
 }
 
-// The item that begins in block x and goes on in the next ones: its parts joined, a wave
-// a row. (At most one begins in a block and is not whole there: its last.)
+// A row's n parts joined by a wave, 32 lanes a part's 128 sums: two parts are taken at once, 2 U are on
+// their way.
+template <int U>
+__device__ __forceinline__ void merge_row(const TreeAttention& a, int n, int block, int row, int t, int head) {
+    const int lane = threadIdx.x & 63, half = lane >> 5, d4 = 4 * (lane & 31);
+    f32x4 acc = {0.f, 0.f, 0.f, 0.f};
+    float m = -INFINITY, den = 0.f;
+    for (int k0 = half; k0 < n; k0 += 2 * U) {
+        f32x2 e[U];
+        f32x4 y[U];
+#pragma unroll
+        for (int k = 0; k < U; ++k) {
+            const int    part = min(k0 + 2 * k, n - 1);
+            const size_t at = static_cast<size_t>(2 * (block + part) + (part == 0)) * a.rows + row;
+            e[k] = *reinterpret_cast<const f32x2*>(a.part_ml + 2 * at);
+            y[k] = *reinterpret_cast<const f32x4*>(a.part_out + at * kHeadDim + d4);
+        }
+#pragma unroll
+        for (int k = 0; k < U; ++k) {
+            const bool  mine = k0 + 2 * k < n;
+            const float lse = mine ? e[k][0] : -INFINITY, now = fmaxf(m, lse), ref = now == -INFINITY ? 0.f : now;
+            const float f0 = exp2_fast(m - ref), f1 = exp2_fast(lse - ref);
+#pragma unroll
+            for (int c = 0; c < 4; ++c) acc[c] = acc[c] * f0 + (mine ? y[k][c] : 0.f) * f1;
+            den = den * f0 + (mine ? e[k][1] : 0.f) * f1;
+            m = now;
+        }
+    }
+    // The two halves' parts together. (NaN stays: a part's own, where it has one.)
+    const float m2 = __shfl_xor(m, 32), now = fmaxf(m, m2), ref = now == -INFINITY ? 0.f : now;
+    const float f0 = exp2_fast(m - ref), f1 = exp2_fast(m2 - ref);
+    den = den * f0 + __shfl_xor(den, 32) * f1;
+#pragma unroll
+    for (int c = 0; c < 4; ++c) acc[c] = acc[c] * f0 + __shfl_xor(acc[c], 32) * f1;
+    const float scale = den == 0.f ? 0.f : a.c.v_scale / den;
+    const f16x2 lo = {static_cast<_Float16>(acc[0] * scale), static_cast<_Float16>(acc[1] * scale)};
+    const f16x2 hi = {static_cast<_Float16>(acc[2] * scale), static_cast<_Float16>(acc[3] * scale)};
+    if (half == 0)
+        *reinterpret_cast<u32x2*>(a.out + t * a.out_stride + head * kHeadDim + d4) =
+            u32x2{__builtin_bit_cast(uint32_t, lo), __builtin_bit_cast(uint32_t, hi)};
+}
+
+// The tile that begins in block x and goes on in the next ones. (At most one begins in a block and
+// is not whole there, its last: slot 1 of the block holds it; slot 0 the block's part of one that
+// began before.)
 __global__ __launch_bounds__(64 * kMergeWaves) void tree_merge_kernel(const int32_t* __restrict__ desc, const TreeAttention a) {
-    const int lane = threadIdx.x & 63;
-    const int row  = blockIdx.y * kMergeWaves + __builtin_amdgcn_readfirstlane(threadIdx.x >> 6);
-    const int32_t* d = desc + kDesc * blockIdx.x;
+    const int row = blockIdx.y * kMergeWaves + __builtin_amdgcn_readfirstlane(threadIdx.x >> 6);
+    const int block = blockIdx.x;
+    const int32_t* d = desc + kDesc * block;
     const int n = load_uniform(d, 0);
     if (n <= 1) return;
     const int i = a.by_group.of(row), g = row - i * a.group;
     if (i >= load_uniform(d, 2)) return;
-    const int t = load_uniform(d, 1) + i, head = load_uniform(d, 3) * a.group + g, slot0 = load_uniform(d, 4);
-    f32x2 acc = {0.f, 0.f};
-    float m = -INFINITY, den = 0.f;
-    for (int k0 = 0; k0 < n; k0 += 8) {
-        f32x2 e[8], y[8];
-#pragma unroll
-        for (int k = 0; k < 8; ++k) {
-            const int    slot = k0 + k == 0 ? slot0 : 2 * (slot0 / 2 + min(k0 + k, n - 1));
-            const size_t at = static_cast<size_t>(slot) * a.rows + row;
-            e[k] = *reinterpret_cast<const f32x2*>(a.part_ml + 2 * at);
-            y[k] = *reinterpret_cast<const f32x2*>(a.part_out + at * kHeadDim + 2 * lane);
-        }
-#pragma unroll
-        for (int k = 0; k < 8; ++k) {
-            if (k0 + k >= n) break;
-            const float now = fmaxf(m, e[k][0]), ref = now == -INFINITY ? 0.f : now;
-            const float f0 = exp2_fast(m - ref), f1 = exp2_fast(e[k][0] - ref);
-            acc[0] = acc[0] * f0 + y[k][0] * f1;
-            acc[1] = acc[1] * f0 + y[k][1] * f1;
-            den = den * f0 + e[k][1] * f1;
-            m = now;
-        }
-    }
-    const float scale = den == 0.f ? 0.f : a.c.v_scale / den;
-    const f16x2 r = {static_cast<_Float16>(acc[0] * scale), static_cast<_Float16>(acc[1] * scale)};
-    *reinterpret_cast<uint32_t*>(a.out + t * a.out_stride + head * kHeadDim + 2 * lane) = __builtin_bit_cast(uint32_t, r);
+    const int t = load_uniform(d, 1) + i, head = load_uniform(d, 3) * a.group + g;
+    if (n <= 2) merge_row<1>(a, n, block, row, t, head);
+    else if (n <= 4) merge_row<2>(a, n, block, row, t, head);
+    else merge_row<8>(a, n, block, row, t, head);
 }
 
+// Waves of rows and of places of a block for tiles of that many rows. fp16: one block of 8 waves
+// on a CU; FP8, whose steps are half as many bytes: two of 4 up to 128 rows. us with 4 and with 8
+// waves, 32 x 8192 fp16, 4, 8, 16 and 32 tokens each: 212 / 200, 217 / 197, 203 / 180, 247 / 230;
+// 64 x 8192 FP8, 8 tokens: 195 / 206, block scales, 32 tokens: 374 / 389.
+constexpr bool small_blocks(int eb, int rows) { return eb == 1 && rows <= 128; }
+
+template <int EB, bool BS, bool UNI, int ROWS>
+void launch_r(const TreeAttention& a, hipStream_t s) {
+    constexpr int WQ = ROWS / 32, WK = (small_blocks(EB, ROWS) ? 4 : 8) / WQ;
+    hipLaunchKernelGGL((tree_attention_kernel<EB, BS, WQ, WK, UNI>), dim3(a.grid), dim3(64 * WQ * WK), 0, s, a);
+}
 template <int EB, bool BS, bool UNI>
 void launch_u(const TreeAttention& a, hipStream_t s) {
-    const dim3 grid(a.grid);
     switch (a.rows) {
-        case 32: hipLaunchKernelGGL((tree_attention_kernel<EB, BS, 1, 4, UNI>), grid, dim3(256), 0, s, a); break;
-        case 64: hipLaunchKernelGGL((tree_attention_kernel<EB, BS, 2, 2, UNI>), grid, dim3(256), 0, s, a); break;
-        case 128: hipLaunchKernelGGL((tree_attention_kernel<EB, BS, 4, 1, UNI>), grid, dim3(256), 0, s, a); break;
-        default: hipLaunchKernelGGL((tree_attention_kernel<EB, BS, 8, 1, UNI>), grid, dim3(512), 0, s, a); break;
+        case 32: launch_r<EB, BS, UNI, 32>(a, s); break;
+        case 64: launch_r<EB, BS, UNI, 64>(a, s); break;
+        case 128: launch_r<EB, BS, UNI, 128>(a, s); break;
+        default: launch_r<EB, BS, UNI, 256>(a, s); break;
     }
 }
 template <int EB, bool BS>
@@ -760,11 +828,11 @@ int device_cus() {
 }  // namespace
 
 void tree_shape(int dtype, TreeAttention& a) {
-    (void)dtype;
     const long per = (static_cast<long>(a.c.n_tok) * a.group + a.c.n_ent - 1) / std::max(a.c.n_ent, 1);   // rows of an entry
     a.rows        = per <= 32 && a.group <= 32 ? 32 : per <= 64 && a.group <= 64 ? 64 : per <= 128 ? 128 : 256;
     a.tile_tokens = a.rows / a.group;
-    a.grid = device_cus() * (a.rows <= 128 ? 2 : 1);
+    a.by_tile     = place_div(a.tile_tokens);
+    a.grid = device_cus() * (small_blocks(dtype == PA_KV_FP16 ? 2 : 1, a.rows) ? 2 : 1);
 }
 
 size_t tree_workspace(const TreeAttention& a) {
