@@ -223,8 +223,7 @@ struct TreeKernel {
     static constexpr int NJ      = kPart / (4 * WQ);           // loads of 4 rows per wave, of K and of V
     static constexpr int kBufs   = WQ > 1 ? 2 : 1;
     static constexpr int kTileK  = kPart * kRowK, kTileV = kPart * kRowV;   // bytes of a step's rows
-    static constexpr int kScales = kTileK + kTileV;                 // in a buffer: K's scales, a float per 4 rows
-    static constexpr int kFlags  = kScales + kPart;            // whether a wave met a value that is not finite
+    static constexpr int kFlags  = kTileK + kTileV;            // in a buffer: whether a wave met a value that is not finite
     static constexpr int kBuf    = kFlags + 16 * ((4 * WQ + 15) / 16);
     static constexpr int kStage  = WK * kBufs * kBuf;
     static constexpr int kJoin   = kWaves * 32 * (kOutLd * 4 + 8);
@@ -409,14 +408,13 @@ struct TreeKernel {
 #pragma unroll
             for (int j = 0; j < NJ; ++j) {
                 const int r4 = wq + WQ * j, row = 4 * r4 + row0;
-                float vs = 1.0f;
-                if constexpr (BS) {
+                float ks = 1.0f, vs = 1.0f;
+                if constexpr (BS) {   // (the conversion takes the scale along)
                     const uint32_t pair = __builtin_amdgcn_readlane(sc, r4 * 4 / RG);
+                    ks = __builtin_bit_cast(float, (pair & 0xff) << 23);
                     vs = __builtin_bit_cast(float, (pair >> 8) << 23);
-                    if (lane == 0)
-                        *reinterpret_cast<float*>(k + kScales + 4 * r4) = score_scale * __builtin_bit_cast(float, (pair & 0xff) << 23);
                 }
-                u32x4 kx = widen(kr[j], 1.0f), vx = widen(vr[j], vs);
+                u32x4 kx = widen(kr[j], ks), vx = widen(vr[j], vs);
                 if (!UNI && !(live >> j & 1)) kx = vx = u32x4{0, 0, 0, 0};
                 *reinterpret_cast<u32x4*>(k + row * kRowK + 16 * ch) = kx;
                 if constexpr (masked) {
@@ -512,14 +510,6 @@ struct TreeKernel {
             float top = -INFINITY;
 #pragma unroll
             for (int b = 0; b < SUBS; ++b) {
-                if constexpr (BS) {
-#pragma unroll
-                    for (int i = 0; i < 4; ++i) {
-                        const float cs = *reinterpret_cast<const float*>(buf + kScales + kTurn * turn + 4 * (8 * b + 2 * i + hl));
-#pragma unroll
-                        for (int e = 0; e < 4; ++e) s[b][4 * i + e] *= cs;
-                    }
-                }
                 if constexpr (MASK) {
                     seen[b] = visible(a, x, tok, base + kSub * b - x.start);
                     const uint32_t mine = seen[b] >> (4 * hl);
@@ -535,10 +525,7 @@ struct TreeKernel {
 #pragma unroll
                 for (int i = 0; i < 16; ++i) top = fmaxf(top, s[b][i]);
             }
-            // Block scales: scores in base 2 already; elsewhere the one scale (not below 0) goes into
-            // the exponent's argument.
-            const float one = BS ? 1.0f : score_scale;
-            top = max_halves(top) * one;
+            top = max_halves(top) * score_scale;   // (which is not below 0)
             if (__builtin_amdgcn_ballot_w64(top > m + kLag) != 0) {
                 const float now = fmaxf(m, top), ref = now == -INFINITY ? 0.f : now;
                 const float f = exp2_fast(m - ref);
@@ -556,8 +543,8 @@ struct TreeKernel {
             for (int b = 0; b < SUBS; ++b)
 #pragma unroll
                 for (int i = 0; i < 16; i += 2) {
-                    const float e0 = exp2_fast(BS ? s[b][i] - ref : fmaf(s[b][i], one, -ref));
-                    const float e1 = exp2_fast(BS ? s[b][i + 1] - ref : fmaf(s[b][i + 1], one, -ref));
+                    const float e0 = exp2_fast(fmaf(s[b][i], score_scale, -ref));
+                    const float e1 = exp2_fast(fmaf(s[b][i + 1], score_scale, -ref));
                     // (Summed as they are rounded, two an instruction, in 32 bits.)
                     const f16x2 e = {static_cast<_Float16>(e0), static_cast<_Float16>(e1)};
                     l = __builtin_amdgcn_fdot2(e, ones2, l, false);
@@ -588,7 +575,7 @@ struct TreeKernel {
             issue(k0);
             if (k0 + 1 < k1) lookup(k0 + 1);
         }
-        // (At the end of the stage, which the first step does not write where streams have two buffers.)
+        // (At the end of the stage: in the last buffer where they fit there, which the first step does not write.)
         unsigned char* const qs = lds + kStage - kRowsM * kRowK;
 #pragma unroll
         for (int j = 0; j < NQ; ++j) {
@@ -599,7 +586,7 @@ struct TreeKernel {
         block_sync();
 #pragma unroll
         for (int s = 0; s < 8; ++s) q[s] = *reinterpret_cast<const f16x8*>(qs + my_row * kRowK + 32 * s + 16 * hl);
-        if constexpr (kBufs == 1) block_sync();
+        if constexpr (kBufs == 1 || kRowsM * kRowK > kBuf) block_sync();
         // Steps that every row sees whole, then those that rows see in part: two loops, so that the
         // second's masks cost the first neither registers nor copies of the sums.
         auto steps = [&](auto masked_c, int from, int to) {
