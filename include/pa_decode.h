@@ -386,12 +386,14 @@ typedef struct pa_cached_tokens {
  * matrix instructions, sums and the softmax in 32 bits, probabilities rounded to fp16 for
  * the second product, one rounding at the end. A token that sees nothing (no earlier
  * place, no bit) gets zeros. What lies in a place reaches only the tokens that see it,
- * infinities and NaN among the entry's own tokens included.
+ * infinities and NaN among the entry's own tokens included. Values of a block-scaled cache are
+ * taken as fp16: exact from 2^-14 up, within 2^-25 below, infinite past 65504 (which no append
+ * here writes).
  * q: head rows (no weight) of num_kv_heads * (1 to 32) heads, query heads h * group ..
  * (h + 1) * group - 1 reading kv head h; out may be the rows themselves. Tokens of no entry,
  * and of one whose start is below 0, whose row is out of range or whose places pass the
- * table's row or 2^31 - 130, are left out: their `out` stays as it was. Pages out of range (num_pages) read as
- * rows of zeros.
+ * table's row or 2^31 - 257, are left out: their `out` stays as it was. Pages out of range
+ * (num_pages) read as rows of zeros.
  * workspace: pa_tree_attention_workspace bytes (may be 0) for these sizes on this device,
  * 16-byte aligned, of any content and without meaning after the call; calls that may run at
  * the same time have one each. */
@@ -401,7 +403,8 @@ pa_status pa_tree_attention(int dtype, const pa_cached_tokens* c, const pa_head_
 
 /* Rows as numbers: token t's kv head h to k_out + t * k_stride + h * 128 (elements of
  * `type`), its value row to v_out likewise (either may be NULL; 16-byte aligned, strides
- * multiples of 8 below 2^26, rows that do not overlap). code * scale in 32 bits, rounded once. Tokens of no entry
+ * multiples of 8 below 2^26, rows that do not overlap). code * scale in 32 bits, rounded
+ * once. Tokens of no entry
  * and those whose place, row or page is out of range keep what their output held. */
 typedef enum pa_value_type {
     PA_VALUE_FP16 = 0,
@@ -413,11 +416,12 @@ pa_status pa_read_cache(int dtype, const pa_cached_tokens* c, int type, void* k_
 
 /* Of the tokens at the places start_pos[e], start_pos[e] + 1, ... of a sequence those
  * with the numbers kept[e][0] < kept[e][1] < ... < kept[e][counts[e] - 1] move to the
- * places start_pos[e], start_pos[e] + 1, ... (token kept[e][j] to start_pos[e] + j), in place. kept:
- * device, [num_entries][width] int32; counts: device, [num_entries] (at most width are
- * taken, none if negative). Each sequence once a call; num_tokens and tok_begin are not used. Rows past
- * the last kept one keep their bytes. A row whose number is below its index, or whose
- * places or pages are out of range, is left out.
+ * places start_pos[e], start_pos[e] + 1, ... (token kept[e][j] to start_pos[e] + j), in
+ * place. kept: device, [num_entries][width] int32; counts: device, [num_entries] (at most
+ * width are taken, none if negative). Each sequence once a call; num_tokens and tok_begin are
+ * not used. Rows past the last kept one keep their bytes. A row whose number is below its
+ * index, or whose places or pages are out of range, is left out. num_entries * num_kv_heads
+ * is 2^25 at most.
  * Block-scaled caches: a block (of places) that no row moves into keeps its bytes and scale.
  * Any other gets the smallest scale that holds its kept rows, as an append would choose; if it
  * begins before start_pos[e], not below the scale that it has, and its earlier rows are

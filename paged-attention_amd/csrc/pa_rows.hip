@@ -71,42 +71,44 @@ __device__ __forceinline__ void store_values(void* out, size_t at, const float (
     }
 }
 
+constexpr int kMaxReadBlocks = 1 << 22;   // (a launch holds fewer than 2^32 threads)
+
 // A wave a token: its rows of every kv head, K's then V's.
 template <int EB, bool BS, int OUT>
 __global__ __launch_bounds__(64 * kWavesR) void read_cache_kernel(const ReadCache a) {
     const CachedTokens& c = a.c;
     const int lane = threadIdx.x & 63, ch = lane % kLanesR, r = lane / kLanesR;
-    const int t = blockIdx.x * kWavesR + __builtin_amdgcn_readfirstlane(threadIdx.x >> 6);
-    if (t >= c.n_tok) return;
-    const int e = __builtin_amdgcn_readfirstlane(entry_of_token(c, t));
-    const int t0 = load_uniform(c.tok_begin, e), t1 = load_uniform(c.tok_begin, e + 1), st = load_uniform(c.start, e);
-    if (t < t0 || t >= t1 || st < 0 || st > INT_MAX - (t - t0)) return;
-    const int pos  = st + (t - t0);
-    const int page = page_at(c, c.slot_ids ? load_uniform(c.slot_ids, e) : e, pos);
-    if (page < 0) return;
-    const int P = c.page_size, slot = pos - c.by_page.page(pos) * P;
-    const int sh = BS ? (P % 16 == 0 ? 4 : 3) : 0;
-    for (int h = r; h < c.hkv; h += kRowsR) {
-        const size_t off = kv_row_offset<EB>(page, h, slot, P, c.hkv) + ch * 8 * EB;
-        uint32_t sc = 0;
-        if constexpr (BS)
-            sc = *reinterpret_cast<const uint16_t*>(c.scales + 2 * ((static_cast<size_t>(page) * c.hkv + h) * (P >> sh) + (slot >> sh)));
+    const int P = c.page_size, sh = BS ? (P % 16 == 0 ? 4 : 3) : 0;
+    for (int t = blockIdx.x * kWavesR + __builtin_amdgcn_readfirstlane(threadIdx.x >> 6); t < c.n_tok; t += gridDim.x * kWavesR) {
+        const int e = __builtin_amdgcn_readfirstlane(entry_of_token(c, t));
+        const int t0 = load_uniform(c.tok_begin, e), t1 = load_uniform(c.tok_begin, e + 1), st = load_uniform(c.start, e);
+        if (t < t0 || t >= t1 || st < 0 || st > INT_MAX - (t - t0)) continue;
+        const int pos  = st + (t - t0);
+        const int page = page_at(c, c.slot_ids ? load_uniform(c.slot_ids, e) : e, pos);
+        if (page < 0) continue;
+        const int slot = pos - c.by_page.page(pos) * P;
+        for (int h = r; h < c.hkv; h += kRowsR) {
+            const size_t off = kv_row_offset<EB>(page, h, slot, P, c.hkv) + ch * 8 * EB;
+            uint32_t sc = 0;
+            if constexpr (BS)
+                sc = *reinterpret_cast<const uint16_t*>(c.scales + 2 * ((static_cast<size_t>(page) * c.hkv + h) * (P >> sh) + (slot >> sh)));
 #pragma unroll
-        for (int v = 0; v < 2; ++v) {
-            void* out = v ? a.v_out : a.k_out;
-            if (!out) continue;
-            const unsigned char* p = static_cast<const unsigned char*>(v ? c.v_cache : c.k_cache) + off;
-            float y[8];
-            f16x8 x;
-            if constexpr (EB == 2) x = *reinterpret_cast<const f16x8*>(p);
-            else {
-                const u32x2 b = *reinterpret_cast<const u32x2*>(p);
-                x = fp8x8_to_f16x8(b[0], b[1]);
+            for (int v = 0; v < 2; ++v) {
+                void* out = v ? a.v_out : a.k_out;
+                if (!out) continue;
+                const unsigned char* p = static_cast<const unsigned char*>(v ? c.v_cache : c.k_cache) + off;
+                float y[8];
+                f16x8 x;
+                if constexpr (EB == 2) x = *reinterpret_cast<const f16x8*>(p);
+                else {
+                    const u32x2 b = *reinterpret_cast<const u32x2*>(p);
+                    x = fp8x8_to_f16x8(b[0], b[1]);
+                }
+                const float f = EB == 2 ? 1.f : (v ? c.v_scale : c.k_scale) * (BS ? exp2_byte(v ? sc >> 8 : sc & 0xff) : 1.f);
+#pragma unroll
+                for (int i = 0; i < 8; ++i) y[i] = EB == 2 ? static_cast<float>(x[i]) : static_cast<float>(x[i]) * f;
+                store_values<OUT>(out, t * (v ? a.v_stride : a.k_stride) + h * kHeadDim + ch * 8, y);
             }
-            const float f = EB == 2 ? 1.f : (v ? c.v_scale : c.k_scale) * (BS ? exp2_byte(v ? sc >> 8 : sc & 0xff) : 1.f);
-#pragma unroll
-            for (int i = 0; i < 8; ++i) y[i] = EB == 2 ? static_cast<float>(x[i]) : static_cast<float>(x[i]) * f;
-            store_values<OUT>(out, t * (v ? a.v_stride : a.k_stride) + h * kHeadDim + ch * 8, y);
         }
     }
 }
@@ -245,7 +247,7 @@ __global__ __launch_bounds__(64) void keep_blocks_kernel(const KeepRows a) {
 
 template <int EB, bool BS>
 void launch_read(int out_type, const ReadCache& a, hipStream_t s) {
-    const dim3 grid((a.c.n_tok + kWavesR - 1) / kWavesR), block(64 * kWavesR);
+    const dim3 grid(std::min((a.c.n_tok + kWavesR - 1) / kWavesR, kMaxReadBlocks)), block(64 * kWavesR);
     if (out_type == PA_VALUE_FP32) hipLaunchKernelGGL((read_cache_kernel<EB, BS, PA_VALUE_FP32>), grid, block, 0, s, a);
     else if (out_type == PA_VALUE_BF16) hipLaunchKernelGGL((read_cache_kernel<EB, BS, PA_VALUE_BF16>), grid, block, 0, s, a);
     else hipLaunchKernelGGL((read_cache_kernel<EB, BS, PA_VALUE_FP16>), grid, block, 0, s, a);

@@ -22,6 +22,7 @@ constexpr int kSub     = 32;              // places of one MFMA step
 constexpr int kScan    = 256;             // entries that a block looks at together
 constexpr int kMergeWaves = 4;
 constexpr int kItemUnits  = 3;   // what a tile costs besides its steps, in steps
+constexpr long kMaxUnits  = 1l << 52;   // more than entries that lie behind one another can have (2^51): others are left out
 constexpr int kSchedMfma = 0x8, kSchedLds = 0x100;   // of sched_group_barrier
 constexpr int kDesc    = 8;               // ints of a block's entry for the merge
 constexpr int kOutLd   = kHeadDim + 4;    // floats of a row in the joining of waves
@@ -241,7 +242,8 @@ struct TreeKernel {
         const int nb = gridDim.x;
         const int lb = nb % 8 == 0 ? (blockIdx.x % 8) * (nb / 8) + blockIdx.x / 8 : blockIdx.x;
         long total = 0, chunk = 0;
-        for (int c0 = 0; c0 < a.c.n_ent; c0 += kScan) total += chunk = scan_chunk(a, sch, c0, kStep);
+        for (int c0 = 0; c0 < a.c.n_ent && total <= kMaxUnits; c0 += kScan) total += chunk = scan_chunk(a, sch, c0, kStep);
+        if (total > kMaxUnits) total = 0;
         const long per = max(divide(total + nb - 1, nb), 1l);
         long w = lb * per;
         const long w_end = min(w + per, total);
