@@ -16,6 +16,7 @@ namespace {
 
 typedef float    f32x16 __attribute__((ext_vector_type(16)));
 typedef float    f32x2  __attribute__((ext_vector_type(2)));
+typedef uint16_t u16x2  __attribute__((ext_vector_type(2)));
 typedef short    s16x4  __attribute__((ext_vector_type(4)));
 
 constexpr int kSub     = 32;              // places of one MFMA step
@@ -406,7 +407,7 @@ struct TreeKernel {
         auto store = [&](int buf, auto masked_c) {
             constexpr bool masked = decltype(masked_c)::value;
             unsigned char* k = stage_at(buf);
-            bool odd = false;
+            u16x2 largest = {0, 0};
 #pragma unroll
             for (int j = 0; j < NJ; ++j) {
                 const int r4 = wq + WQ * j, row = 4 * r4 + row0;
@@ -421,18 +422,26 @@ struct TreeKernel {
                 *reinterpret_cast<u32x4*>(k + row * kRowK + 16 * ch) = kx;
                 if constexpr (masked) {
 #pragma unroll
-                    for (int e = 0; e < 4; ++e) {
-                        const uint32_t lo = (vx[e] & 0x7c00u) == 0x7c00u ? 0xffffu : 0u;
-                        const uint32_t hi = (vx[e] & 0x7c000000u) == 0x7c000000u ? 0xffff0000u : 0u;
-                        odd |= (lo | hi) != 0;
-                        vx[e] &= ~(lo | hi);
-                    }
+                    for (int e = 0; e < 4; ++e) largest = __builtin_elementwise_max(largest, __builtin_bit_cast(u16x2, vx[e] & 0x7fff7fffu));
                 }
                 *reinterpret_cast<u32x4*>(k + kTileK + row * kRowV + 16 * ch) = vx;
             }
             if constexpr (masked) {
-                const bool any = __builtin_amdgcn_ballot_w64(odd) != 0;
+                const bool any = __builtin_amdgcn_ballot_w64(largest[0] >= 0x7c00 || largest[1] >= 0x7c00) != 0;
                 if (lane == 0) *reinterpret_cast<int*>(k + kFlags + 4 * wq) = any;
+                if (any) {
+#pragma unroll 1
+                    for (int j = 0; j < NJ; ++j) {   // (a lane's own values, again)
+                        u32x4* const at = reinterpret_cast<u32x4*>(k + kTileK + (4 * (wq + WQ * j) + row0) * kRowV + 16 * ch);
+                        u32x4 vx = *at;
+#pragma unroll
+                        for (int e = 0; e < 4; ++e) {
+                            if ((vx[e] & 0x7c00u) == 0x7c00u) vx[e] &= 0xffff0000u;
+                            if ((vx[e] & 0x7c000000u) == 0x7c000000u) vx[e] &= 0xffffu;
+                        }
+                        *at = vx;
+                    }
+                }
             }
         };
         // (By way of memory: rare, and 64 sums indexed by constants would weigh on the loop's registers.)
