@@ -206,38 +206,42 @@ __device__ __forceinline__ u32x2 recode(u32x2 was, float (&y)[8], int k) {
     return now;
 }
 
-// Block by block of the places that the accepted rows come to.
-__global__ __launch_bounds__(64) void keep_blocks_kernel(const KeepRows a) {
+constexpr int kWavesB = 2;
+
+// Blocks of the places that the accepted rows come to, kWavesB at a time, a wave each: all are read
+// before any is written. (A row comes from its own block or a later one, so what is read next has not
+// been written.)
+__global__ __launch_bounds__(64 * kWavesB) void keep_blocks_kernel(const KeepRows a) {
     const CachedTokens& c = a.c;
     const int lane = threadIdx.x & 63, ch = lane % kLanesR, r = lane / kLanesR;
+    const int wave = __builtin_amdgcn_readfirstlane(threadIdx.x >> 6);
     const int e = blockIdx.x / c.hkv, h = blockIdx.x - e * c.hkv, v = blockIdx.y;
     unsigned char* pool = static_cast<unsigned char*>(v ? c.v_cache : c.k_cache);
     const int n = min(load_uniform(a.counts, e), a.width), st = load_uniform(c.start, e);
     const int row = c.slot_ids ? load_uniform(c.slot_ids, e) : e;
     if (st < 0 || n <= 0 || st > INT_MAX - 32 - n) return;
-    const int P = c.page_size, sh = P % 16 == 0 ? 4 : 3, B = 1 << sh, nb = P >> sh;
+    const int P = c.page_size, sh = P % 16 == 0 ? 4 : 3, B = 1 << sh, nb = P >> sh, last = (st + n - 1) >> sh;
     const int32_t* kept = a.kept + static_cast<size_t>(e) * a.width;
     auto scale_at = [&](int page, int slot) {
         return c.scales + 2 * ((static_cast<size_t>(page) * c.hkv + h) * nb + (slot >> sh)) + v;
     };
-    for (int b = st >> sh; b <= (st + n - 1) >> sh; ++b) {
+    for (int b0 = st >> sh; b0 <= last; b0 += kWavesB) {
         // Lane group r holds the block's places r, r + 4, ...
-        const int page = page_at(c, row, b * B);
-        if (page < 0) continue;
-        const int slot0 = b * B - c.by_page.page(b * B) * P;
+        const int b = b0 + wave, page = b <= last ? page_at(c, row, b * B) : -1;
+        const int slot0 = page < 0 ? 0 : b * B - c.by_page.page(b * B) * P;
         u32x2 was[4];
-        int   from[4];     // 0: not in the path, 1: stays in its place, 2: moves in
+        int   from[4];     // 0: not in the path, 1: stays in its place, 2: moves in, 3: lies before the path
         float y[4][8], amax = 0.f;
         bool  moved = false;
-        uint8_t* const sc = scale_at(page, slot0);
-        const int old = *sc;
+        uint8_t* const sc = scale_at(max(page, 0), slot0);
+        const int old = page < 0 ? 0 : *sc;
 #pragma unroll
         for (int i = 0; i < 4; ++i) {
             const int s = kRowsR * i + r, j = b * B + s - st;
             from[i] = 0;
             was[i] = u32x2{0, 0};
             float f = 0.f;
-            if (s < B && j < n) {
+            if (page >= 0 && s < B && j < n) {
                 const int k = j < 0 ? j : kept[j];
                 const int pos = st + k;
                 const int ps = j >= 0 && (k < j || k > INT_MAX - st) ? -1 : k == j ? page : page_at(c, row, pos);
@@ -256,6 +260,7 @@ __global__ __launch_bounds__(64) void keep_blocks_kernel(const KeepRows a) {
                 if (from[i] == 1 || from[i] == 2) amax = fmaxf(amax, fabsf(y[i][d]));
             }
         }
+        __syncthreads();
         if (__builtin_amdgcn_ballot_w64(moved) == 0) continue;
         int k = __builtin_amdgcn_readfirstlane(block_exponent(wave_max64(amax)));
         if (b * B < st) k = max(k, old - 127);
@@ -265,7 +270,6 @@ __global__ __launch_bounds__(64) void keep_blocks_kernel(const KeepRows a) {
             *reinterpret_cast<u32x2*>(pool + kv_row_offset<1>(page, h, slot0 + kRowsR * i + r, P, c.hkv) + ch * 8) = recode(was[i], y[i], k);
         }
         if (lane == 0) *sc = static_cast<uint8_t>(k + 127);
-        asm volatile("" ::: "memory");
     }
 }
 
@@ -290,10 +294,10 @@ hipError_t launch_read_cache(int dtype, int out_type, const ReadCache& a, hipStr
 
 hipError_t launch_keep_rows(int dtype, const KeepRows& a, hipStream_t s) {
     check_kv_dtype(dtype);
-    const dim3 grid(a.c.n_ent * a.c.hkv, 2), one(grid.x), block(64);
-    if (dtype == PA_KV_FP16) hipLaunchKernelGGL((keep_rows_kernel<2>), one, block, 0, s, a);
-    else if (dtype == PA_KV_FP8_E4M3) hipLaunchKernelGGL((keep_rows_kernel<1>), one, block, 0, s, a);
-    else hipLaunchKernelGGL(keep_blocks_kernel, grid, block, 0, s, a);
+    const dim3 grid(a.c.n_ent * a.c.hkv, 2), both(a.c.n_ent * a.c.hkv), block(64);
+    if (dtype == PA_KV_FP16) hipLaunchKernelGGL((keep_rows_kernel<2>), both, block, 0, s, a);
+    else if (dtype == PA_KV_FP8_E4M3) hipLaunchKernelGGL((keep_rows_kernel<1>), both, block, 0, s, a);
+    else hipLaunchKernelGGL(keep_blocks_kernel, grid, dim3(64 * kWavesB), 0, s, a);
     return hipGetLastError();
 }
 
