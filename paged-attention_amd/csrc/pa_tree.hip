@@ -1,5 +1,36 @@
 // gfx950 attention of several new tokens per sequence over a paged cache: drafted
-// trees, chains, pieces of prompts.
+// trees, chains, pieces of prompts. (No counterpart in the reference.)
+//
+//   tree_attention_kernel   the work, in equal shares
+//   tree_merge_kernel       tiles that shares cut apart, joined
+//
+// out_i = sum_p exp(s_ip - m_i) v_p / sum_p exp(s_ip - m_i), s_ip = sm_scale q_i k_p, over the
+// places p that token i sees: one pass with a running m_i, sums in 32 bits.
+//
+// Rows and tiles. The query heads of a kv head and the tokens of an entry are rows of one
+// product, token by token, so a place is read once for all of them: tiles of 64, 128 or 256
+// rows, 32 a wave. A tile walks its places in steps of 64 to 128 (kStep). Waves of one tile share
+// a stream of places (WQ of them); WK streams take a part of every step each and are joined at the end.
+//
+// Shares. Lengths are device data, so the host cannot lay out the work: every block adds up the
+// entries' costs and takes one of gridDim.x equal shares of (entry, kv head, tile, step), in that
+// order. A share cuts at most two tiles, whose sums go to the workspace (two slots a block). One
+// token over 131072 places and a prompt of 4096 go through the same code.
+//
+// Products. S^T = K Q^T with v_mfma_f32_32x32x16_f16: a lane holds 16 places of one row, so the
+// softmax needs one exchange between the wave's halves, and P^T is the second product's operand
+// as it lies. O^T = V^T P^T, V's fragments read transposed from LDS (ds_read_b64_tr_b16). K and V
+// go through registers into LDS as fp16: FP8 is widened once for all of the tile's rows, a block's
+// scale along with it, and places that are not there become zeros. Two buffers, loads a whole
+// step ahead.
+//
+// What bounds it (one MI355X): trees of few rows, memory (4 tokens over 32 x 8192, fp16: 170 us,
+// 6.3 TB/s; 16: 176); tiles of 128 rows and more, two pipes: 32 places by 32 rows are 16 MFMAs of
+// 32 cycles and, per lane, 16 exponentials, maxima, sums and roundings besides the staging. The
+// matrix pipe is busy 46% of the time, the vector pipe 42%, and no order of the code that was tried
+// laid one over the other (4096 tokens after 4096: 445 us, 925 TFLOP/s, a large library product 1242;
+// 32 over 64 x 8192, block scales: 350). Small calls: the instructions of a tile's prologue and end,
+// and the merge's launch (8 tokens over 200: 11 us, 4 of them the merge's).
 
 #include "pa_device.hpp"
 #include "pa_fp8.hpp"
@@ -223,11 +254,10 @@ struct TreeKernel {
     static constexpr int kPart   = kTurn * HALVES;             // places of a stream's step
     static constexpr int kStep   = kPart * WK;
     static constexpr int NJ      = kPart / (4 * WQ);           // loads of 4 rows per wave, of K and of V
-    static constexpr int kBufs   = WQ > 1 ? 2 : 1;
     static constexpr int kTileK  = kPart * kRowK, kTileV = kPart * kRowV;   // bytes of a step's rows
     static constexpr int kFlags  = kTileK + kTileV;            // in a buffer: whether a wave met a value that is not finite
     static constexpr int kBuf    = kFlags + 16 * ((4 * WQ + 15) / 16);
-    static constexpr int kStage  = WK * kBufs * kBuf;
+    static constexpr int kStage  = WK * 2 * kBuf;
     static constexpr int kJoin   = kWaves * 32 * (kOutLd * 4 + 8);
     static constexpr int kLds    = kStage > kJoin ? kStage : kJoin;
     // Loads bypass the caches where hardly any place is read twice: tiles that hold all of an entry's
@@ -400,7 +430,7 @@ struct TreeKernel {
             else return u32x4{fp8x2_to_f16x2<false>(x[0], scale), fp8x2_to_f16x2<true>(x[0], scale),
                               fp8x2_to_f16x2<false>(x[1], scale), fp8x2_to_f16x2<true>(x[1], scale)};
         };
-        auto stage_at = [&](int buf) { return lds + (wk * kBufs + buf) * kBuf; };
+        auto stage_at = [&](int buf) { return lds + (2 * wk + buf) * kBuf; };
         // A place that a row does not see must not reach it, whatever its value: 0 * infinity is
         // NaN. So where rows see different places (masked), values that are not finite are staged as
         // zeros, and add_odd adds them to the rows that see them.
@@ -597,28 +627,26 @@ struct TreeKernel {
         block_sync();
 #pragma unroll
         for (int s = 0; s < 8; ++s) q[s] = *reinterpret_cast<const f16x8*>(qs + my_row * kRowK + 32 * s + 16 * hl);
-        if constexpr (kBufs == 1 || kRowsM * kRowK > kBuf) block_sync();
+        if constexpr (kRowsM * kRowK > kBuf) block_sync();
         // Steps that every row sees whole, then those that rows see in part: two loops, so that the
         // second's masks cost the first neither registers nor copies of the sums.
         auto steps = [&](auto masked_c, int from, int to) {
             constexpr bool MASK = decltype(masked_c)::value;
 #pragma unroll 1
             for (int k = from; k < to; ++k) {
-                const int buf = kBufs == 2 ? (k - k0) & 1 : 0;
+                const int buf = (k - k0) & 1;
                 const int base = k * kStep + kPart * wk;
                 store(buf, masked_c);
                 if (k + 1 < k1) {
                     issue(k + 1);
                     if (k + 2 < k1) lookup(k + 2);
                 }
-                if constexpr (WQ > 1) block_sync();
-                else wave_lds_sync();
+                block_sync();
                 if (has_rows) {
 #pragma unroll
                     for (int t = 0; t < HALVES; ++t)
                         if (!MASK || base + kTurn * t < end) step_of(masked_c, base + kTurn * t, stage_at(buf), t);
                 }
-                if constexpr (WQ == 1) wave_lds_sync();
             }
         };
         const int mid = uniform(max(k0, min(k1, all_open / kStep)));
@@ -664,7 +692,7 @@ struct TreeKernel {
                                      *reinterpret_cast<const u32x4*>(mine + r * kRowK + 16 * (lane & 15)));
                 }
             }
-            if constexpr (WQ > 1) block_sync();   // the stage is free again
+            block_sync();   // the stage is free again
             return;
         }
 
@@ -790,10 +818,10 @@ __global__ __launch_bounds__(64 * kMergeWaves) void tree_merge_kernel(const int3
     else merge_row<8>(a, n, block, row, t, head);
 }
 
-// Waves of rows and of places of a block for tiles of that many rows. fp16: one block of 8 waves
-// on a CU; FP8, whose steps are half as many bytes: two of 4 up to 128 rows. us with 4 and with 8
-// waves, 32 x 8192 fp16, 4, 8, 16 and 32 tokens each: 212 / 200, 217 / 197, 203 / 180, 247 / 230;
-// 64 x 8192 FP8, 8 tokens: 195 / 206, block scales, 32 tokens: 374 / 389.
+// Blocks on a CU. fp16: one of 8 waves; FP8, whose steps are half as many bytes: two of 4 waves
+// up to 128 rows. us with two of 4 and with one of 8: fp16, 32 x 8192, 4 and 32 tokens 175 / 171 and
+// 232 / 219, 37 ragged sequences, 8 tokens 45.5 / 41.6; FP8, 64 x 8192, 8 tokens 200 / 212, 37 ragged
+// 36.4 / 38.1; block scales, 64 x 8192, 32 tokens 348 / 362.
 constexpr bool small_blocks(int eb, int rows) { return eb == 1 && rows <= 128; }
 
 template <int EB, bool BS, bool UNI, int ROWS>
@@ -804,7 +832,6 @@ void launch_r(const TreeAttention& a, hipStream_t s) {
 template <int EB, bool BS, bool UNI>
 void launch_u(const TreeAttention& a, hipStream_t s) {
     switch (a.rows) {
-        case 32: launch_r<EB, BS, UNI, 32>(a, s); break;
         case 64: launch_r<EB, BS, UNI, 64>(a, s); break;
         case 128: launch_r<EB, BS, UNI, 128>(a, s); break;
         default: launch_r<EB, BS, UNI, 256>(a, s); break;
@@ -825,9 +852,14 @@ int device_cus() {
 
 }  // namespace
 
+// Rows of a tile: those of an average entry, if no more than 256. us with 64, 128 and 256: fp16,
+// 32 x 8192, 16 tokens of 4 heads a kv head (64 rows) 171 / 192 / 222, 32 tokens (128) 344 / 224 / 246;
+// FP8, 1 x 131072, 64 tokens (256) 244 / 192 / 169; 4096 tokens after 4096 785 / 597 / 447. (Tiles of
+// 32 rows, every wave a stream of its own, lost to 64: 4 tokens over 32 x 8192 197 / 170, 8 over
+// 1 x 200 17.2 / 11.1; FP8 64 x 8192, 8 tokens, block scales 197 / 203.)
 void tree_shape(int dtype, TreeAttention& a) {
     const long per = (static_cast<long>(a.c.n_tok) * a.group + a.c.n_ent - 1) / std::max(a.c.n_ent, 1);   // rows of an entry
-    a.rows        = per <= 32 && a.group <= 32 ? 32 : per <= 64 && a.group <= 64 ? 64 : per <= 128 ? 128 : 256;
+    a.rows        = per <= 64 ? 64 : per <= 128 ? 128 : 256;
     a.tile_tokens = a.rows / a.group;
     a.by_tile     = place_div(a.tile_tokens);
     a.grid = device_cus() * (small_blocks(dtype == PA_KV_FP16 ? 2 : 1, a.rows) ? 2 : 1);
