@@ -114,6 +114,8 @@ pa_status pa_tree_attention(int dtype, const pa_cached_tokens* c, const pa_head_
         if (c->num_entries == 0) throw std::invalid_argument("tree_attention: tokens of no entry");
         a.c = cached_tokens("tree_attention", dtype, c, true);
         if (c->num_pages == 0) throw std::invalid_argument("tree_attention: a cache of no pages");
+        a.score_scale = sm_scale * a.c.k_scale * 1.44269504088896340736f;
+        if (!std::isfinite(a.score_scale)) throw std::invalid_argument("tree_attention: sm_scale * k_scale must be finite");
         pa::tree_shape(dtype, a);
         const size_t need = pa::tree_workspace(a);
         if (workspace_bytes < need || !workspace || !aligned(workspace, 16))
@@ -125,7 +127,6 @@ pa_status pa_tree_attention(int dtype, const pa_cached_tokens* c, const pa_head_
         a.out_stride  = r.out_stride;
         a.tree        = tree;
         a.words       = tree_words;
-        a.score_scale = sm_scale * a.c.k_scale * 1.44269504088896340736f;
         pa::tree_place(a, workspace);
         pa::hip_check(pa::launch_tree_attention(dtype, a, as_stream(stream)), "tree_attention kernel launch");
     });

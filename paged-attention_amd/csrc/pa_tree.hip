@@ -288,6 +288,7 @@ struct TreeKernel {
             while (w >= before + chunk) {
                 before += chunk;
                 c0 += kScan;
+                if (c0 >= a.c.n_ent) return;   // (the entries were changed under the call, here and below)
                 chunk = scan_chunk(a, sch, c0, kStep);
             }
             int  hit = 0;
@@ -296,17 +297,19 @@ struct TreeKernel {
                 const int tid = threadIdx.x;
                 if (tid < kScan && sch.pre[tid] <= w - before && w - before < sch.pre[tid + 1]) sch.hit = tid;
                 __syncthreads();
-                hit = __builtin_amdgcn_readfirstlane(sch.hit);
+                hit = min(max(__builtin_amdgcn_readfirstlane(sch.hit), 0), min(kScan, a.c.n_ent - c0) - 1);
                 at  = before + uniform(sch.pre[hit]);
                 __syncthreads();
             }
             Entry x = entry_at(a.c, c0 + hit);
             x.n = uniform(x.n);
+            if (x.n == 0) return;
             const int  tiles = tiles_of(a, x);
             const long head_steps = uniform(steps_before(a, x, kStep, tiles));
             const long local = w - at;
             const int  h     = static_cast<int>(divide(local, head_steps));
             const long inner = local - h * head_steps;
+            if (h < 0 || h >= a.c.hkv || inner < 0) return;
             int rt = 0;   // the last tile that begins at or before
             for (int span = tiles; span > 1;) {
                 const int half = span / 2;
@@ -318,6 +321,7 @@ struct TreeKernel {
             const int  units = static_cast<int>(uniform(steps_before(a, x, kStep, rt + 1)) - first);
             const int  u0    = static_cast<int>(inner - first);
             const int  u1    = static_cast<int>(min(static_cast<long>(units), u0 + (w_end - w)));
+            if (u1 <= u0) return;
             // Its first kItemUnits are no steps: a share that ends among them leaves the tile to the next block.
             if (u1 > kItemUnits) {
                 const bool begins = u0 <= kItemUnits, ends = u1 == units;
@@ -483,8 +487,13 @@ struct TreeKernel {
             for (int t = 0; t < kTurn && base + t < end; ++t) {
                 const int i = a.by_page.of(base + t), page = load_uniform(table, i);
                 if (page < 0 || page >= c.num_pages) continue;
+                const int slot = base + t - i * P;
                 const unsigned char* v = static_cast<const unsigned char*>(c.v_cache) + page * page_bytes + head_off +
-                                         static_cast<size_t>(base + t - i * P) * kRowBytes<EB>;
+                                         static_cast<size_t>(slot) * kRowBytes<EB>;
+                float vs = 1.0f;
+                if constexpr (BS)
+                    vs = __builtin_bit_cast(float, static_cast<uint32_t>(load_global<uint8_t>(
+                             c.scales + 2 * ((static_cast<size_t>(page) * c.hkv + h) * nblk + (slot >> bsh)) + 1)) << 23);
                 uint32_t word = seen[0];
 #pragma unroll
                 for (int b = 1; b < SUBS; ++b) word = t >= kSub * b ? seen[b] : word;
@@ -494,7 +503,7 @@ struct TreeKernel {
                     const int at = 8 * (n / 4) + 4 * hl + n % 4;
                     float y;
                     if constexpr (EB == 2) y = f16_bits_to_f32(load_global<uint16_t>(v + 2 * at));
-                    else y = (load_global<uint8_t>(v + at) & 0x7f) == 0x7f ? NAN : 0.f;
+                    else y = f16_bits_to_f32(fp8x2_to_f16x2<false>(load_global<uint8_t>(v + at), vs) & 0xffffu);
                     if (!(fabsf(y) < INFINITY)) sums[n] += y;
                 }
             }
@@ -809,7 +818,7 @@ __global__ __launch_bounds__(64 * kMergeWaves) void tree_merge_kernel(const int3
     const int row = blockIdx.x * kMergeWaves + __builtin_amdgcn_readfirstlane(threadIdx.x >> 6);
     const int block = blockIdx.y;
     const int32_t* d = desc + kDesc * block;
-    const int n = load_uniform(d, 0);
+    const int n = min(load_uniform(d, 0), static_cast<int>(gridDim.y) - block);
     if (n <= 1) return;
     const int i = a.by_group.of(row), g = row - i * a.group;
     if (i >= load_uniform(d, 2)) return;

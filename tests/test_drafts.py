@@ -97,6 +97,7 @@ def test_attention_refuses_trees_scales_and_entries():
     assert attend(tree=A + 4, words=1) == BAD and "aligned" in message()
     for bad in (float("nan"), float("inf")):
         assert attend(scale=bad) == BAD and "sm_scale" in message()
+    assert attend(dtype=pa_amd.FP8_E4M3, scale=1e38, k_scale=1e5) == BAD and "k_scale must be finite" in message()
     assert attend(tok_begin=None) == BAD and "null" in message()
     assert attend(num_entries=0) == BAD and "no entry" in message()
     assert attend(num_pages=0) == BAD and "pages" in message()

@@ -235,6 +235,23 @@ def test_one_query_for_all_and_one_that_is_not_a_number():
     assert torch.equal(bad, out)
 
 
+@pytest.mark.parametrize("chain", [False, True])
+def test_values_past_fp16_in_block_scales(chain):
+    """A code and scale that no append writes, 448 * 2^8: infinite for the tokens that see it, nothing to the others."""
+    cache, start, n = Cache("block", 16, 2, 1, 4, seed=8), 32, 12
+    page = cache.table[0, start // 16]
+    cache.scales[page, :, 0, 1] = 135
+    cache.kv[1][page] = 0x38                       # ones, 256 with the scale
+    cache.kv[1][page, :, 7, 3], cache.kv[1][page, :, 7, 90] = 0x7e, 0xfe
+    tree = [(1 << i) | (1 << 7 if i == 9 else 0) for i in range(n)]
+    out, _ = run_attention(cache, [(start, n)], 8, None if chain else [tree])
+    see = seen_of(start, n, None if chain else tree)[:, start + 7]
+    got = out.float().cpu().numpy()
+    assert (got[see][:, :, 3] == np.inf).all() and (got[see][:, :, 90] == -np.inf).all() and see.any() and not see.all()
+    got[np.ix_(see, range(8), [3, 90])] = 0
+    assert np.isfinite(got).all()
+
+
 def test_no_tokens():
     cache = Cache("block", 16, 2, 2, 4, seed=9)
     k, v, table, scales = cache.device()
