@@ -25,12 +25,14 @@
 // step ahead.
 //
 // What bounds it (one MI355X): trees of few rows, memory (4 tokens over 32 x 8192, fp16: 170 us,
-// 6.3 TB/s; 16: 176); tiles of 128 rows and more, two pipes: 32 places by 32 rows are 16 MFMAs of
-// 32 cycles and, per lane, 16 exponentials, maxima, sums and roundings besides the staging. The
-// matrix pipe is busy 46% of the time, the vector pipe 42%, and no order of the code that was tried
-// laid one over the other (4096 tokens after 4096: 445 us, 925 TFLOP/s, a large library product 1242;
-// 32 over 64 x 8192, block scales: 350). Small calls: the instructions of a tile's prologue and end,
-// and the merge's launch (8 tokens over 200: 11 us, 4 of them the merge's).
+// 6.3 TB/s; 16: 176); tiles of 128 rows and more, three pipes: 32 places by 32 rows are 16 MFMAs of
+// 32 cycles, per lane 16 exponentials, maxima, sums and roundings besides the staging, and 16 KB out
+// of LDS, which a wave reads for its 32 rows alone. The matrix pipe is busy 46% of the time, the
+// vector pipe 42%, LDS about half, and no order of the code that was tried laid them wholly over
+// each other (4096 tokens after 4096: 445 us, 925 TFLOP/s, a large library product 1242; 32 over
+// 64 x 8192, block scales: 350). Twice the rows a wave, half the reads, does not fit the registers
+// (705 us, 130 spilled). Small calls: the instructions of a tile's prologue and end, and the
+// merge's launch (8 tokens over 200: 11 us, 3 of them the merge's).
 
 #include "pa_device.hpp"
 #include "pa_fp8.hpp"
@@ -52,7 +54,7 @@ typedef short    s16x4  __attribute__((ext_vector_type(4)));
 
 constexpr int kSub     = 32;              // places of one MFMA step
 constexpr int kScan    = 256;             // entries that a block looks at together
-constexpr int kMergeWaves = 4;
+constexpr int kMergeWaves = 4, kMergeRows = 2 * kMergeWaves;
 constexpr int kItemUnits  = 3;   // what a tile costs besides its steps, in steps
 constexpr long kMaxUnits  = 1l << 52;   // more than entries that lie behind one another can have (2^51): others are left out
 constexpr int kSchedMfma = 0x8, kSchedLds = 0x100;   // of sched_group_barrier
@@ -768,26 +770,25 @@ __global__ __launch_bounds__(64 * WQ * WK, 2) void tree_attention_kernel(const T
     T::run(a, lds, sch);
 }
 
-// A row's n parts joined by a wave, 32 lanes a part's 128 sums: two parts are taken at once, 2 U are on
-// their way.
+// A row's n parts joined by half a wave, a lane four sums; U parts are on their way.
 template <int U>
 __device__ __forceinline__ void merge_row(const TreeAttention& a, int n, int block, int row, int t, int head) {
-    const int lane = threadIdx.x & 63, half = lane >> 5, d4 = 4 * (lane & 31);
+    const int d4 = 4 * (threadIdx.x & 31);
     f32x4 acc = {0.f, 0.f, 0.f, 0.f};
     float m = -INFINITY, den = 0.f;
-    for (int k0 = half; k0 < n; k0 += 2 * U) {
+    for (int k0 = 0; k0 < n; k0 += U) {
         f32x2 e[U];
         f32x4 y[U];
 #pragma unroll
         for (int k = 0; k < U; ++k) {
-            const int    part = min(k0 + 2 * k, n - 1);
+            const int    part = min(k0 + k, n - 1);
             const size_t at = static_cast<size_t>(2 * (block + part) + (part == 0)) * a.rows + row;
             e[k] = *reinterpret_cast<const f32x2*>(a.part_ml + 2 * at);
             y[k] = *reinterpret_cast<const f32x4*>(a.part_out + at * kHeadDim + d4);
         }
 #pragma unroll
         for (int k = 0; k < U; ++k) {
-            const bool  mine = k0 + 2 * k < n;
+            const bool  mine = k0 + k < n;
             const float lse = mine ? e[k][0] : -INFINITY, now = fmaxf(m, lse), ref = now == -INFINITY ? 0.f : now;
             const float f0 = exp2_fast(m - ref), f1 = exp2_fast(lse - ref);
 #pragma unroll
@@ -796,18 +797,11 @@ __device__ __forceinline__ void merge_row(const TreeAttention& a, int n, int blo
             m = now;
         }
     }
-    // The two halves' parts together. (NaN stays: a part's own, where it has one.)
-    const float m2 = __shfl_xor(m, 32), now = fmaxf(m, m2), ref = now == -INFINITY ? 0.f : now;
-    const float f0 = exp2_fast(m - ref), f1 = exp2_fast(m2 - ref);
-    den = den * f0 + __shfl_xor(den, 32) * f1;
-#pragma unroll
-    for (int c = 0; c < 4; ++c) acc[c] = acc[c] * f0 + __shfl_xor(acc[c], 32) * f1;
     const float scale = den == 0.f ? 0.f : a.c.v_scale / den;
     const f16x2 lo = {static_cast<_Float16>(acc[0] * scale), static_cast<_Float16>(acc[1] * scale)};
     const f16x2 hi = {static_cast<_Float16>(acc[2] * scale), static_cast<_Float16>(acc[3] * scale)};
-    if (half == 0)
-        *reinterpret_cast<u32x2*>(a.out + t * a.out_stride + head * kHeadDim + d4) =
-            u32x2{__builtin_bit_cast(uint32_t, lo), __builtin_bit_cast(uint32_t, hi)};
+    *reinterpret_cast<u32x2*>(a.out + t * a.out_stride + head * kHeadDim + d4) =
+        u32x2{__builtin_bit_cast(uint32_t, lo), __builtin_bit_cast(uint32_t, hi)};
 }
 
 // The tile that begins in block x and goes on in the next ones. (At most one begins in a block and
@@ -815,7 +809,7 @@ __device__ __forceinline__ void merge_row(const TreeAttention& a, int n, int blo
 // began before.) A tile's rows go round the XCDs: with blocks x in a row of the grid, tiles that begin
 // in every 32nd block were all joined on one of the eight (64 tokens over 1 x 131072: 22 us).
 __global__ __launch_bounds__(64 * kMergeWaves) void tree_merge_kernel(const int32_t* __restrict__ desc, const TreeAttention a) {
-    const int row = blockIdx.x * kMergeWaves + __builtin_amdgcn_readfirstlane(threadIdx.x >> 6);
+    const int row = blockIdx.x * kMergeRows + (threadIdx.x >> 5);
     const int block = blockIdx.y;
     const int32_t* d = desc + kDesc * block;
     const int n = min(load_uniform(d, 0), static_cast<int>(gridDim.y) - block);
@@ -823,8 +817,8 @@ __global__ __launch_bounds__(64 * kMergeWaves) void tree_merge_kernel(const int3
     const int i = a.by_group.of(row), g = row - i * a.group;
     if (i >= load_uniform(d, 2)) return;
     const int t = load_uniform(d, 1) + i, head = load_uniform(d, 3) * a.group + g;
-    if (n <= 2) merge_row<1>(a, n, block, row, t, head);
-    else if (n <= 4) merge_row<2>(a, n, block, row, t, head);
+    if (n <= 2) merge_row<2>(a, n, block, row, t, head);
+    else if (n <= 4) merge_row<4>(a, n, block, row, t, head);
     else merge_row<8>(a, n, block, row, t, head);
 }
 
@@ -892,7 +886,7 @@ hipError_t launch_tree_attention(int dtype, const TreeAttention& a, hipStream_t 
     if (dtype == PA_KV_FP16) launch_e<2, false>(a, s);
     else if (dtype == PA_KV_FP8_E4M3) launch_e<1, false>(a, s);
     else launch_e<1, true>(a, s);
-    hipLaunchKernelGGL(tree_merge_kernel, dim3(a.rows / kMergeWaves, a.grid), dim3(64 * kMergeWaves), 0, s, a.desc, a);
+    hipLaunchKernelGGL(tree_merge_kernel, dim3(a.rows / kMergeRows, a.grid), dim3(64 * kMergeWaves), 0, s, a.desc, a);
     return hipGetLastError();
 }
 
