@@ -29,8 +29,8 @@
 // 32 cycles, per lane 16 exponentials, maxima, sums and roundings besides the staging, and 16 KB out
 // of LDS, which a wave reads for its 32 rows alone. The matrix pipe is busy 46% of the time, the
 // vector pipe 42%, LDS about half, and no order of the code that was tried laid them wholly over
-// each other (4096 tokens after 4096: 445 us, 925 TFLOP/s, a large library product 1242; 32 over
-// 64 x 8192, block scales: 350). Twice the rows a wave, half the reads, does not fit the registers
+// each other (4096 tokens after 4096: 440 to 465 us, 890 to 935 TFLOP/s, a large library product
+// 1242; 32 over 64 x 8192, block scales: 345 to 363). Twice the rows a wave, half the reads, does not fit the registers
 // (705 us, 130 spilled). Small calls: the instructions of a tile's prologue and end, and the
 // merge's launch (8 tokens over 200: 11 us, 3 of them the merge's).
 
@@ -325,7 +325,6 @@ struct TreeKernel {
             const int  units = static_cast<int>(uniform(steps_before(a, x, kStep, rt + 1)) - first);
             const int  u0    = static_cast<int>(inner - first);
             const int  u1    = static_cast<int>(min(static_cast<long>(units), u0 + (w_end - w)));
-            if (u1 <= u0) return;
             // Its first kItemUnits are no steps: a share that ends among them leaves the tile to the next block.
             if (u1 > kItemUnits) {
                 const bool begins = u0 <= kItemUnits, ends = u1 == units;
@@ -338,7 +337,7 @@ struct TreeKernel {
                 item_part(lds, x, h, rt, uniform(max(u0, kItemUnits) - kItemUnits), uniform(u1 - kItemUnits),
                           uniform(begins && ends ? -1 : 2 * lb + (begins ? 1 : 0)));
             }
-            w += u1 - u0;
+            w += max(u1 - u0, 1);   // (1 as above; a return here slows the long loops by 3%)
         }
     }
 
