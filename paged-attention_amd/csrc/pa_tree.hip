@@ -21,8 +21,9 @@
 // softmax needs one exchange between the wave's halves, and P^T is the second product's operand
 // as it lies. O^T = V^T P^T, V's fragments read transposed from LDS (ds_read_b64_tr_b16). K and V
 // go through registers into LDS as fp16: FP8 is widened once for all of the tile's rows, a block's
-// scale along with it, and places that are not there become zeros. Two buffers, loads a whole
-// step ahead.
+// scale of V along with it (within 2^-25, as the decode has it), and places that are not there become
+// zeros. K's goes into its scores in 32 bits (345 / 357 us for 32 tokens over 64 x 8192 with K scaled
+// in fp16 and so, but fp16 has no keys below 2^-24). Two buffers, loads a whole step ahead.
 //
 // What bounds it (one MI355X): trees of few rows, memory (4 tokens over 32 x 8192, fp16: 170 us,
 // 6.3 TB/s; 16: 176); tiles of 128 rows and more, three pipes: 32 places by 32 rows are 16 MFMAs of
@@ -374,6 +375,7 @@ struct TreeKernel {
         int      pg = -1;
         Raw      kr[NJ], vr[NJ];
         uint32_t sc = 0;       // the lane's rows' scale pair
+        float    k_sc = 0.f;   // of the step in the stage: the scale of K's scores, into base-2 exponents
         uint32_t live = 0;     // general pages: loads whose row holds a place
         auto lookup = [&](int k) {
             const int t = k * kStep + kPart * wk + RG * lane;
@@ -445,16 +447,15 @@ struct TreeKernel {
             constexpr bool masked = decltype(masked_c)::value;
             unsigned char* k = stage_at(buf);
             u16x2 largest = {0, 0};
+            // (In 32 bits: under its smallest scales K is below what fp16 holds, at its largest past it. Within the
+            // positive normal numbers, so that minus infinity stays what it is and 0 stays 0.)
+            if constexpr (BS) k_sc = fminf(fmaxf(score_scale * __builtin_bit_cast(float, (sc & 0xff) << 23), FLT_MIN), FLT_MAX);
 #pragma unroll
             for (int j = 0; j < NJ; ++j) {
                 const int r4 = wq + WQ * j, row = 4 * r4 + row0;
-                float ks = 1.0f, vs = 1.0f;
-                if constexpr (BS) {   // (the conversion takes the scale along)
-                    const uint32_t pair = __builtin_amdgcn_readlane(sc, r4 * 4 / RG);
-                    ks = __builtin_bit_cast(float, (pair & 0xff) << 23);
-                    vs = __builtin_bit_cast(float, (pair >> 8) << 23);
-                }
-                u32x4 kx = widen(kr[j], ks), vx = widen(vr[j], vs);
+                float vs = 1.0f;   // (the conversion takes V's scale along)
+                if constexpr (BS) vs = __builtin_bit_cast(float, __builtin_amdgcn_readlane(sc, r4 * 4 / RG) >> 8 << 23);
+                u32x4 kx = widen(kr[j], 1.0f), vx = widen(vr[j], vs);
                 if (!UNI && !(live >> j & 1)) kx = vx = u32x4{0, 0, 0, 0};
                 *reinterpret_cast<u32x4*>(k + row * kRowK + 16 * ch) = kx;
                 if constexpr (masked) {
@@ -560,9 +561,11 @@ struct TreeKernel {
                 __builtin_amdgcn_sched_group_barrier(kSchedLds, 2, 0);
             }
             uint32_t seen[SUBS];
-            float top = -INFINITY;
+            float top = -INFINITY, cs[SUBS][4];   // scales of scores: a block has 8 places or 16
 #pragma unroll
             for (int b = 0; b < SUBS; ++b) {
+#pragma unroll
+                for (int i = 0; i < 4; ++i) cs[b][i] = BS ? readlane_f(k_sc, (kTurn * turn + kSub * b + 8 * i) / RG) : score_scale;
                 if constexpr (MASK) {
                     seen[b] = visible(a, x, tok, base + kSub * b - x.start);
                     const uint32_t mine = seen[b] >> (4 * hl);
@@ -575,10 +578,17 @@ struct TreeKernel {
                         s[b][i] = __builtin_bit_cast(float, y | (~all & 0xff800000u));
                     }
                 }
+                if constexpr (BS) {   // (scales are above 0)
 #pragma unroll
-                for (int i = 0; i < 16; ++i) top = fmaxf(top, s[b][i]);
+                    for (int i = 0; i < 16; i += 4)
+                        top = fmaxf(top, fmaxf(fmaxf(s[b][i], s[b][i + 1]), fmaxf(s[b][i + 2], s[b][i + 3])) * cs[b][i / 4]);
+                } else {
+#pragma unroll
+                    for (int i = 0; i < 16; ++i) top = fmaxf(top, s[b][i]);
+                }
             }
-            top = max_halves(top) * score_scale;   // (which is not below 0)
+            top = max_halves(top);
+            if constexpr (!BS) top *= score_scale;   // (which is not below 0)
             if (__builtin_amdgcn_ballot_w64(top > m + kLag) != 0) {
                 const float now = fmaxf(m, top), ref = now == -INFINITY ? 0.f : now;
                 const float f = exp2_fast(m - ref);
@@ -596,8 +606,8 @@ struct TreeKernel {
             for (int b = 0; b < SUBS; ++b)
 #pragma unroll
                 for (int i = 0; i < 16; i += 2) {
-                    const float e0 = exp2_fast(fmaf(s[b][i], score_scale, -ref));
-                    const float e1 = exp2_fast(fmaf(s[b][i + 1], score_scale, -ref));
+                    const float e0 = exp2_fast(fmaf(s[b][i], cs[b][i / 4], -ref));
+                    const float e1 = exp2_fast(fmaf(s[b][i + 1], cs[b][i / 4], -ref));
                     // (Summed as they are rounded, two an instruction, in 32 bits.)
                     const f16x2 e = {static_cast<_Float16>(e0), static_cast<_Float16>(e1)};
                     l = __builtin_amdgcn_fdot2(e, ones2, l, false);

@@ -1,0 +1,81 @@
+"""GPU tests of the numbers that attention of drafted tokens and rows read back stand for, where they are very small or
+very large."""
+
+from __future__ import annotations
+
+import numpy as np
+import pytest
+import torch
+
+import pa_amd
+from drafts import D, Cache, attention, random_tree
+from test_gpu_drafts import begins, check_attention, cols_for, ints, run_attention
+
+pytestmark = [pytest.mark.gpu, pytest.mark.usefixtures("gpu_device")]
+
+
+# Exponents of K's and V's scales (of 448 2^k, V's largest is an fp16 value up to k = 7), and a softmax scale at which
+# scores are of order one.
+RANGES = {"smallest": ((-32, -26), (-32, -20), 2.0 ** 20), "largest": ((3, 9), (0, 8), 2.0 ** -15),
+          "all": ((-32, 9), (-32, 8), 2.0 ** -14)}
+
+
+@pytest.mark.parametrize("page", [16, 24])
+@pytest.mark.parametrize("which", list(RANGES))
+@pytest.mark.parametrize("entries,chain", [([(0, 3), (70, 9)], False), ([(200, 40)], True), ([(3000, 100)], False)])
+def test_block_scales_over_their_range(which, entries, chain, page):
+    """K's scales multiply scores in 32 bits; V's rows are fp16, within 2^-25 below 2^-14."""
+    (k0, k1), (v0, v1), scale = RANGES[which]
+    cache = Cache("block", page, 2, len(entries), cols_for(entries, page), seed=page)
+    r = np.random.default_rng(page)
+    shape = cache.scales.shape[:-1]
+    cache.scales[..., 0] = r.integers(127 + k0, 127 + k1, shape)
+    cache.scales[..., 1] = r.integers(127 + v0, 127 + v1, shape)
+    if which != "smallest":   # keys past fp16, 448 * 2^8
+        cache.kv[0].reshape(-1)[::4001] = 0x7e
+        cache.scales[::3, ..., 0] = 135
+    trees = None if chain else [random_tree(np.random.default_rng(i), n) for i, (_, n) in enumerate(entries)]
+    out, q = run_attention(cache, entries, 8, trees, sm_scale=scale)
+    check_attention(cache, entries, 8, trees, out, q, scale=scale)
+
+
+def test_decode_and_attention_agree_on_small_keys():
+    """One token over keys near 2^-30, as the decode has it."""
+    hq, hkv, page, lens = 8, 2, 16, [300, 77]
+    cache = Cache("block", page, hkv, 2, cols_for([(n, 0) for n in lens], page), seed=1)
+    cache.scales[..., 0] = np.random.default_rng(0).integers(92 + 3, 92 + 8, cache.scales.shape[:-1])
+    k, v, table, scales = cache.device()
+    q = torch.from_numpy((np.random.default_rng(1).standard_normal((2, hq, D)) * 6e4 / 5).astype(np.float16)).cuda()
+    q_scale = 2.0 ** 7 * D ** 0.5                     # (the decode's softmax scale is 1 / sqrt(128): k_scale takes the rest)
+    dec = pa_amd.Decoder(hq, hkv, D, page, True, block_scales=True)
+    dec.plan(torch.tensor(lens, dtype=torch.int32))
+    one = dec.run(q, k, v, table, ints(lens), q_scale, 1.0, kv_scales=scales)
+    same = pa_amd.tree_attention(q, k, v, table, begins([1, 1]), ints(n - 1 for n in lens), k_scale=q_scale, kv_scales=scales)
+    for e, n in enumerate(lens):
+        K, V = (cache.rows(j, e, 0, n) for j in range(2))
+        ref, tol = attention(q[e:e + 1].double().cpu().numpy(), K, V, np.ones((1, n), bool), q_scale / D ** 0.5)
+        for got in (one, same):
+            assert (np.abs(got[e].double().cpu().numpy() - ref[0]) <= tol[0]).all(), e
+
+
+@pytest.mark.parametrize("kind", ["fp16", "fp8"])
+@pytest.mark.parametrize("low", [-14.5, -17.5])
+def test_tails(kind, low):
+    """A place of score 0 and 99999 of `low`: probabilities that are subnormal in fp16 and a twentieth of the sum."""
+    n = 100_000
+    cache = Cache(kind, 16, 1, 1, n // 16, seed=3, k_scale=2.0 ** -6, v_scale=2.0 ** -8)
+    if kind == "fp16":
+        cache.kv[0][:] = 0
+        cache.kv[0][..., 0] = low / 16
+        cache.kv[1] = np.abs(cache.kv[1])
+    else:
+        cache.kv[0][:] = 0
+        cache.kv[0][..., 0] = {-14.5: 0xe7, -17.5: 0xe9}[low]      # -60 and -72, 2^-6 of which times 16 is near `low`
+        cache.kv[1] &= 0x7f
+    page = cache.table[0, 0]
+    cache.kv[0][page, :, 0, 0] = 0
+    cache.kv[1][page, :, 0] = 0
+    q = np.zeros((1, 2, D), np.float16)
+    q[..., 0] = 16.0
+    out, _ = run_attention(cache, [(n - 1, 1)], 2, None, q=q, sm_scale=1.0)
+    check_attention(cache, [(n - 1, 1)], 2, None, out, q, scale=1.0)
