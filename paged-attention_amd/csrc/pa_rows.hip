@@ -122,10 +122,11 @@ __global__ __launch_bounds__(64 * kWavesR) void read_cache_kernel(const ReadCach
                 f16x8 y16;
                 if constexpr (EB == 2) y16 = __builtin_bit_cast(f16x8, x[i][v]);
                 else y16 = fp8x8_to_f16x8(x[i][v][0], x[i][v][1]);
-                const float f = EB == 2 ? 1.f : (v ? c.v_scale : c.k_scale) * (BS ? exp2_byte(v ? sc[i] >> 8 : sc[i] & 0xff) : 1.f);
+                // (A code times its block's scale is exact; the scales' product might not be, or past fp32.)
+                const float f = BS ? exp2_byte(v ? sc[i] >> 8 : sc[i] & 0xff) : 1.f, g = v ? c.v_scale : c.k_scale;
                 float y[8];
 #pragma unroll
-                for (int d = 0; d < 8; ++d) y[d] = EB == 2 ? static_cast<float>(y16[d]) : static_cast<float>(y16[d]) * f;
+                for (int d = 0; d < 8; ++d) y[d] = EB == 2 ? static_cast<float>(y16[d]) : static_cast<float>(y16[d]) * f * g;
                 store_values<OUT>(out, t * (v ? a.v_stride : a.k_stride) + h * kHeadDim + ch * 8, y);
             }
         }

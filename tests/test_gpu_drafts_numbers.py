@@ -79,3 +79,24 @@ def test_tails(kind, low):
     q[..., 0] = 16.0
     out, _ = run_attention(cache, [(n - 1, 1)], 2, None, q=q, sm_scale=1.0)
     check_attention(cache, [(n - 1, 1)], 2, None, out, q, scale=1.0)
+
+
+@pytest.mark.parametrize("scale", [2.0 ** 120, 2.0 ** -100, 1.7e38, 3e-38])
+def test_read_cache_of_large_and_small_scales(scale):
+    """code * scale in 32 bits, rounded once: a block's scale times the cache's may be past fp32 where its codes'
+    values are not."""
+    cache = Cache("block", 16, 2, 1, 4, seed=2)
+    r = np.random.default_rng(3)
+    shape = cache.scales.shape
+    cache.scales = np.where(r.random(shape) < 0.5, 135, 95).astype(np.uint8)
+    cache.kv = [r.integers(0, 256, x.shape).astype(np.uint8) for x in cache.kv]
+    for x in cache.kv:
+        x[..., ::3] &= 0x87                          # zeros and subnormals among them
+    k, v, table, scales = cache.device()
+    got = pa_amd.read_cache(k, v, table, begins([64]), ints([0]), 64, dtype=torch.float32, k_scale=scale, v_scale=scale,
+                            kv_scales=scales)
+    for j in range(2):
+        x = cache.rows(j, 0, 0, 64)
+        with np.errstate(over="ignore", invalid="ignore"):
+            want = x.astype(np.float32) * np.float32(scale)
+        np.testing.assert_array_equal(got[j].cpu().numpy(), want)
