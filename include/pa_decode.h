@@ -421,7 +421,7 @@ pa_status pa_read_cache(int dtype, const pa_cached_tokens* c, int type, void* k_
  * width are taken, none if negative). Each sequence once a call; num_tokens and tok_begin are
  * not used. Rows past the last kept one keep their bytes. A row whose number is below its
  * index, or whose places or pages are out of range, is left out. num_entries * num_kv_heads
- * is 2^25 at most.
+ * is 2^25 at most, below 2^25 with block scales.
  * Block-scaled caches: a block (of places) that no row moves into keeps its bytes and scale.
  * Any other gets the smallest scale that holds its kept rows, as an append would choose; if it
  * begins before start_pos[e], not below the scale that it has, and its earlier rows are

@@ -18,7 +18,7 @@ bool aligned(const void* p, size_t n) { return reinterpret_cast<uintptr_t>(p) % 
 // Sizes that the kernels index in 32 bits.
 constexpr int kMaxKvHeads = 1 << 14;
 constexpr int kMaxEntries = 1 << 20;
-constexpr int kMaxKeepWaves = 1 << 25;   // (a launch holds fewer than 2^32 threads)
+constexpr int kMaxKeepItems = 1 << 25;   // entries times kv heads
 
 // Sizes of a call, checked (no pointer is looked at).
 void check_sizes(const char* what, int dtype, const pa_cached_tokens* c) {
@@ -169,8 +169,10 @@ pa_status pa_keep_rows(int dtype, const pa_cached_tokens* c, const int32_t* kept
         check_sizes("keep_rows", dtype, c);
         if (width < 0) throw std::invalid_argument("keep_rows: negative width");
         if (c->num_entries == 0 || width == 0) return;
-        if (static_cast<long long>(c->num_entries) * c->num_kv_heads > kMaxKeepWaves)
-            throw std::length_error("keep_rows: entries * kv heads exceeds 2^25");
+        // (Block-scaled caches: 2^25 items would be 2^32 threads, one more than a launch holds.)
+        const int most = std::min<long long>(kMaxKeepItems, UINT32_MAX / pa::keep_threads(dtype));
+        if (static_cast<long long>(c->num_entries) * c->num_kv_heads > most)
+            throw std::length_error("keep_rows: entries * kv heads exceeds " + std::string(most < kMaxKeepItems ? "2^25 - 1" : "2^25"));
         if (!kept || !counts) throw std::invalid_argument("keep_rows: null pointer");
         pa::KeepRows a{};
         a.c      = cached_tokens("keep_rows", dtype, c, false);

@@ -253,6 +253,7 @@ struct KeepRows {
     int            width;
     const int32_t* counts;
 };
+int        keep_threads(int dtype);   // of an entry and kv head
 hipError_t launch_keep_rows(int dtype, const KeepRows& a, hipStream_t s);
 // Stores one zero.
 hipError_t launch_zero_int(int32_t* p, hipStream_t s);

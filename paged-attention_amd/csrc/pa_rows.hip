@@ -298,12 +298,14 @@ hipError_t launch_read_cache(int dtype, int out_type, const ReadCache& a, hipStr
     return hipGetLastError();
 }
 
+int keep_threads(int dtype) { return dtype == PA_KV_FP8_E4M3_BLOCK ? 64 * kWavesB : 64; }
+
 hipError_t launch_keep_rows(int dtype, const KeepRows& a, hipStream_t s) {
     check_kv_dtype(dtype);
-    const dim3 grid(a.c.n_ent * a.c.hkv, 2), both(a.c.n_ent * a.c.hkv), block(64);
+    const dim3 grid(a.c.n_ent * a.c.hkv, 2), both(a.c.n_ent * a.c.hkv), block(keep_threads(dtype));
     if (dtype == PA_KV_FP16) hipLaunchKernelGGL((keep_rows_kernel<2>), both, block, 0, s, a);
     else if (dtype == PA_KV_FP8_E4M3) hipLaunchKernelGGL((keep_rows_kernel<1>), both, block, 0, s, a);
-    else hipLaunchKernelGGL(keep_blocks_kernel, grid, dim3(64 * kWavesB), 0, s, a);
+    else hipLaunchKernelGGL(keep_blocks_kernel, grid, block, 0, s, a);
     return hipGetLastError();
 }
 
