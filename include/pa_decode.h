@@ -390,7 +390,8 @@ typedef struct pa_cached_tokens {
  * multiply scores in 32 bits; the rows of V are taken as fp16, exact from 2^-14 up, within 2^-25
  * below, infinite past 65504 (which no append here writes).
  * q: head rows (no weight) of num_kv_heads * (1 to 32) heads, query heads h * group ..
- * (h + 1) * group - 1 reading kv head h; out may be the rows themselves. Tokens of no entry,
+ * (h + 1) * group - 1 reading kv head h; out may be the rows themselves, and shares no byte with
+ * the pools, scales, table, entries or tree (refused; the workspace likewise). Tokens of no entry,
  * and of one whose start is below 0, whose row is out of range or whose places pass the
  * table's row or 2^31 - 257, are left out: their `out` stays as it was. Pages out of range
  * (num_pages) read as rows of zeros.
@@ -403,9 +404,8 @@ pa_status pa_tree_attention(int dtype, const pa_cached_tokens* c, const pa_head_
 
 /* Rows as numbers: token t's kv head h to k_out + t * k_stride + h * 128 (elements of
  * `type`), its value row to v_out likewise (either may be NULL; 16-byte aligned, strides
- * multiples of 8 below 2^26, rows that do not overlap). code * scale in 32 bits, rounded
- * once. Tokens of no entry
- * and those whose place, row or page is out of range keep what their output held. */
+ * multiples of 8 below 2^26, rows that do not overlap, nor anything that the call reads). code *
+ * scale in 32 bits, rounded once. Tokens of no entry and those whose place, row or page is out of range keep what their output held. */
 typedef enum pa_value_type {
     PA_VALUE_FP16 = 0,
     PA_VALUE_BF16 = 1,

@@ -44,17 +44,17 @@ int64_t floor_div(int64_t a, int64_t b) { return a / b - (a % b < 0); }   // b >
 // lie between each other and do not.) Rows of one stride: whether a row's distance
 // from some row of the other, which moves by that stride, falls inside it; else
 // row by row, which only rows of different strides that lie among each other need.
+bool hits(const Rows& b, int64_t from, int64_t bytes, int64_t first, int64_t last) {   // any of b's rows first .. last
+    if (b.step == 0) return from < b.base + b.bytes && b.base < from + bytes;
+    const int64_t lo = std::max(first, floor_div(from - b.base - b.bytes, b.step) + 1);
+    return lo <= last && b.base + lo * b.step < from + bytes;
+}
 bool meet(const Rows& a, const Rows& b, int n) {
     const int64_t last = n - 1;
     if (a.base >= b.base + last * b.step + b.bytes || b.base >= a.base + last * a.step + a.bytes) return false;
-    auto hits = [&](int64_t from, int64_t bytes, int64_t first, int64_t steps) {   // of b's rows first .. steps
-        if (b.step == 0) return from < b.base + b.bytes && b.base < from + bytes;
-        const int64_t lo = std::max(first, floor_div(from - b.base - b.bytes, b.step) + 1);
-        return lo <= steps && b.base + lo * b.step < from + bytes;
-    };
-    if (a.step == b.step) return hits(a.base, a.bytes, -last, last);
+    if (a.step == b.step) return hits(b, a.base, a.bytes, -last, last);
     for (int64_t i = 0; i <= last; ++i)
-        if (hits(a.base + i * a.step, a.bytes, 0, last)) return true;
+        if (hits(b, a.base + i * a.step, a.bytes, 0, last)) return true;
     return false;
 }
 
@@ -123,6 +123,11 @@ bool rows_overlap(const void* a, int64_t a_stride, const void* b, int64_t b_stri
     const Rows x{static_cast<int64_t>(reinterpret_cast<uintptr_t>(a)), elem * a_stride, elem * row};
     const Rows y{static_cast<int64_t>(reinterpret_cast<uintptr_t>(b)), elem * b_stride, elem * row};
     return meet(x, y, n);
+}
+
+bool rows_touch(const void* a, int64_t a_stride, int64_t row, int elem, int n, const void* p, size_t bytes) {
+    const Rows x{static_cast<int64_t>(reinterpret_cast<uintptr_t>(a)), elem * a_stride, elem * row};
+    return n > 0 && p && bytes && hits(x, static_cast<int64_t>(reinterpret_cast<uintptr_t>(p)), static_cast<int64_t>(bytes), 0, n - 1);
 }
 
 void check_page_bytes(const char* what, int dtype, int page_size, int kv_heads) {

@@ -5,6 +5,7 @@
 #include "pa_host.hpp"
 
 #include <algorithm>
+#include <array>
 #include <climits>
 #include <cmath>
 #include <string>
@@ -68,6 +69,26 @@ pa::CachedTokens cached_tokens(const char* what, int dtype, const pa_cached_toke
     return t;
 }
 
+struct Bytes {
+    const void* p;
+    size_t      n;
+};
+// What a call over cached tokens reads of its cache, table and entries.
+std::array<Bytes, 7> reads_of(int dtype, const pa::CachedTokens& c) {
+    const size_t rows = static_cast<size_t>(c.num_pages) * c.hkv * c.page_size;   // of a pool
+    const size_t pool = rows * pa::kHeadDim * (dtype == PA_KV_FP16 ? 2 : 1);
+    const size_t scales = c.scales ? 2 * rows / pa::block_tokens(c.page_size) : 0, ents = 4 * static_cast<size_t>(c.n_ent);
+    return {{{c.k_cache, pool}, {c.v_cache, pool}, {c.scales, scales},
+             {c.table, 4 * static_cast<size_t>(c.table_rows) * c.table_stride},
+             {c.tok_begin, ents + 4}, {c.start, ents}, {c.slot_ids, ents}}};
+}
+// Refuses output rows that lie in what the call reads: other tokens' results would change under it.
+void check_apart(const char* what, int dtype, const pa::CachedTokens& c, const void* out, int64_t stride, int64_t row, int elem) {
+    for (const Bytes& b : reads_of(dtype, c))
+        if (rows_touch(out, stride, row, elem, c.n_tok, b.p, b.n))
+            throw std::invalid_argument(std::string(what) + ": an output overlaps the cache or another operand");
+}
+
 // The launch of an attention over c with hq query heads, its sizes checked.
 pa::TreeAttention tree_sizes(int dtype, const pa_cached_tokens* c, int hq) {
     check_sizes("tree_attention", dtype, c);
@@ -116,11 +137,21 @@ pa_status pa_tree_attention(int dtype, const pa_cached_tokens* c, const pa_head_
         if (c->num_pages == 0) throw std::invalid_argument("tree_attention: a cache of no pages");
         a.score_scale = sm_scale * a.c.k_scale * 1.44269504088896340736f;
         if (!std::isfinite(a.score_scale)) throw std::invalid_argument("tree_attention: sm_scale * k_scale must be finite");
+        const int64_t row = static_cast<int64_t>(q->heads) * pa::kHeadDim;
+        const Bytes   bits{tree, tree ? 8 * static_cast<size_t>(c->num_tokens) * tree_words : 0};
+        check_apart("tree_attention", dtype, a.c, r.out, r.out_stride, row, 2);
+        if (rows_touch(r.out, r.out_stride, row, 2, c->num_tokens, bits.p, bits.n))
+            throw std::invalid_argument("tree_attention: the output overlaps the tree");
         pa::tree_shape(dtype, a);
         const size_t need = pa::tree_workspace(a);
         if (workspace_bytes < need || !workspace || !aligned(workspace, 16))
             throw std::invalid_argument("tree_attention: the workspace must have " + std::to_string(need) +
                                         " bytes, 16-byte aligned");
+        bool apart = !rows_touch(r.in, r.in_stride, row, 2, c->num_tokens, workspace, need) &&
+                     !rows_touch(r.out, r.out_stride, row, 2, c->num_tokens, workspace, need);
+        for (const Bytes& b : reads_of(dtype, a.c)) apart = apart && !rows_touch(workspace, 0, static_cast<int64_t>(need), 1, 1, b.p, b.n);
+        if (!apart || rows_touch(workspace, 0, static_cast<int64_t>(need), 1, 1, bits.p, bits.n))
+            throw std::invalid_argument("tree_attention: the workspace overlaps an operand");
         a.q           = r.in;
         a.q_stride    = r.in_stride;
         a.out         = r.out;
@@ -155,6 +186,8 @@ pa_status pa_read_cache(int dtype, const pa_cached_tokens* c, int type, void* k_
         if (c->num_entries == 0) throw std::invalid_argument("read_cache: tokens of no entry");
         pa::ReadCache a{};
         a.c        = cached_tokens("read_cache", dtype, c, true);
+        for (const Out& o : {Out{k_out, k_stride}, Out{v_out, v_stride}})
+            if (o.p) check_apart("read_cache", dtype, a.c, o.p, o.stride, row, type == PA_VALUE_FP32 ? 4 : 2);
         a.k_out    = k_out;
         a.k_stride = static_cast<long>(k_stride);
         a.v_out    = v_out;

@@ -242,6 +242,8 @@ void check_outputs(const char* what, const pa::HeadRows& q, const pa::HeadRows& 
                    int64_t v_stride, int n);
 // Whether any of n rows of `row` elements of `elem` bytes at a shares a byte with one at b.
 bool rows_overlap(const void* a, int64_t a_stride, const void* b, int64_t b_stride, int64_t row, int elem, int n);
+// Whether any of them shares a byte with p .. p + bytes - 1 (none where p is null).
+bool rows_touch(const void* a, int64_t a_stride, int64_t row, int elem, int n, const void* p, size_t bytes);
 void check_page_bytes(const char* what, int dtype, int page_size, int kv_heads);
 
 // ---- page pool (pa_pool.cpp)
