@@ -94,7 +94,7 @@ pa::TreeAttention tree_sizes(int dtype, const pa_cached_tokens* c, int hq) {
     check_sizes("tree_attention", dtype, c);
     if (hq <= 0 || hq % c->num_kv_heads != 0 || hq / c->num_kv_heads > 32)
         throw std::invalid_argument("tree_attention: the query heads must be 1 to 32 times the kv heads");
-    if (static_cast<long long>(c->num_tokens) * hq * 16 > INT_MAX)
+    if (static_cast<long long>(c->num_tokens) * hq > pa::kMaxTreeRows)
         throw std::length_error("tree_attention: tokens * heads * 16 exceeds INT_MAX");
     pa::TreeAttention a{};
     a.c.n_tok = c->num_tokens;

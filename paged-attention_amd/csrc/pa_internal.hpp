@@ -7,6 +7,7 @@
 
 #include <hip/hip_runtime.h>
 
+#include <climits>
 #include <cstdint>
 #include <stdexcept>
 #include <string>
@@ -213,6 +214,8 @@ struct CachedTokens {
     float          k_scale, v_scale;
     PageDiv        by_page;
 };
+// Tokens times query heads of an attention, at most (its rows are indexed in 32 bits, 8 dims at a time).
+constexpr long kMaxTreeRows = INT_MAX / (kHeadDim / 8);
 // Attention of those tokens over their sequences.
 struct TreeAttention {
     CachedTokens    c;

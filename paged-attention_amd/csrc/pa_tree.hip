@@ -57,7 +57,13 @@ constexpr int kSub     = 32;              // places of one MFMA step
 constexpr int kScan    = 256;             // entries that a block looks at together
 constexpr int kMergeWaves = 4, kMergeRows = 2 * kMergeWaves;
 constexpr int kItemUnits  = 3;   // what a tile costs besides its steps, in steps
-constexpr long kMaxUnits  = 1l << 52;   // more than entries that lie behind one another can have (2^51): others are left out
+constexpr int kMinStep    = 64;  // places of a step, at least
+// Entries with more units than this are left out, all of them (divide() takes less than 2^53). Entries
+// that lie behind one another have fewer: at most kMaxTreeRows tiles, as a tile and kv head has a row of
+// its own at least, and a tile kItemUnits, its steps over 2^31 places at most, one for rounding and, in
+// a chain, one more.
+constexpr long kMaxUnits  = (1l << 53) - (1l << 20);
+static_assert(kMaxTreeRows * (kItemUnits + 2 + (1l << 31) / kMinStep) <= kMaxUnits);
 constexpr int kSchedMfma = 0x8, kSchedLds = 0x100;   // of sched_group_barrier
 constexpr int kDesc    = 8;               // ints of a block's entry for the merge
 constexpr int kOutLd   = kHeadDim + 4;    // floats of a row in the joining of waves
@@ -269,7 +275,7 @@ struct TreeKernel {
     // rows. (us with cached and with such loads: 16 over 32 x 8192 fp16 219 / 203, 4096 over 4096 451 / 511.)
     static constexpr int kAux    = WQ < 8 ? 2 : 0;
     static constexpr int RG      = UNI ? 4 : 1;                // rows that a lane looks up
-    static_assert(kPart / RG <= 64 && NJ >= 1);
+    static_assert(kPart / RG <= 64 && NJ >= 1 && kStep >= kMinStep);
 
     typedef uint32_t Raw __attribute__((ext_vector_type(EB == 2 ? 4 : 2)));
 
