@@ -386,7 +386,8 @@ typedef struct pa_cached_tokens {
  * matrix instructions, sums and the softmax in 32 bits, probabilities rounded to fp16 for
  * the second product, one rounding at the end. A token that sees nothing (no earlier
  * place, no bit) gets zeros. What lies in a place reaches only the tokens that see it,
- * infinities and NaN among the entry's own tokens included. Block-scaled caches: K's scales
+ * infinities and NaN among the entry's own tokens included; those of value rows reach each
+ * of them, of whatever weight: where a dim has some, their sum is its result. Block-scaled caches: K's scales
  * multiply scores in 32 bits; the rows of V are taken as fp16, exact from 2^-14 up, within 2^-25
  * below, infinite past 65504 (which no append here writes).
  * q: head rows (no weight) of num_kv_heads * (1 to 32) heads, query heads h * group ..

@@ -228,6 +228,7 @@ struct TreeAttention {
     int             group;     // query heads of a kv head
     PlaceDiv        by_page, by_group;
     float           score_scale;   // of q k into base-2 exponents
+    int             elem, step;    // set by the launch: bytes of a cached value, places of a step
     // Set by tree_shape, with the workspace.
     int             rows, tile_tokens, grid;
     PlaceDiv        by_tile;
@@ -239,7 +240,7 @@ struct TreeAttention {
 void   tree_shape(int dtype, TreeAttention& a);
 size_t tree_workspace(const TreeAttention& a);
 void   tree_place(TreeAttention& a, void* workspace);
-hipError_t launch_tree_attention(int dtype, const TreeAttention& a, hipStream_t s);
+hipError_t launch_tree_attention(int dtype, TreeAttention a, hipStream_t s);
 // Rows of the caches into k_out / v_out (one may be null); out_type: pa_value_type.
 struct ReadCache {
     CachedTokens c;

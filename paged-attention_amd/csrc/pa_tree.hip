@@ -206,6 +206,75 @@ __device__ __forceinline__ long scan_chunk(const TreeAttention& a, Schedule& s, 
     return uniform(total);
 }
 
+// A part of a share: units u0 .. u1 - 1 of a tile's `units` (more than kItemUnits at least), the first of them unit w of the call.
+struct Share {
+    Entry x;
+    int   h, rt, u0, u1, units;
+    long  w, per;
+};
+
+// f(share) for what block lb of nb has to do, in order. (All threads of a block of 256 at least.)
+template <class F>
+__device__ __forceinline__ void walk(const TreeAttention& a, Schedule& sch, int nb, int lb, int step, F&& f) {
+    long total = 0, chunk = 0;
+    for (int c0 = 0; c0 < a.c.n_ent && total <= kMaxUnits; c0 += kScan) total += chunk = scan_chunk(a, sch, c0, step);
+    if (total > kMaxUnits) total = 0;
+    const long per = max(divide(total + nb - 1, nb), 1l);
+    long w = lb * per;
+    const long w_end = min(w + per, total);
+    if (w >= w_end) return;
+    int  c0 = 0;
+    long before = 0;
+    if (a.c.n_ent > kScan) chunk = scan_chunk(a, sch, 0, step);
+    while (w < w_end) {
+        while (w >= before + chunk) {
+            before += chunk;
+            c0 += kScan;
+            if (c0 >= a.c.n_ent) return;   // (the entries were changed under the call, here and below)
+            chunk = scan_chunk(a, sch, c0, step);
+        }
+        int  hit = 0;
+        long at  = 0;
+        if (a.c.n_ent > 1) {
+            const int tid = threadIdx.x;
+            if (tid < kScan && sch.pre[tid] <= w - before && w - before < sch.pre[tid + 1]) sch.hit = tid;
+            __syncthreads();
+            hit = min(max(__builtin_amdgcn_readfirstlane(sch.hit), 0), min(kScan, a.c.n_ent - c0) - 1);
+            at  = before + uniform(sch.pre[hit]);
+            __syncthreads();
+        }
+        Share s;
+        s.x   = entry_at(a.c, c0 + hit);
+        s.x.n = uniform(s.x.n);
+        if (s.x.n == 0) return;
+        const int  tiles = tiles_of(a, s.x);
+        const long head_steps = uniform(steps_before(a, s.x, step, tiles));
+        const long local = w - at;
+        s.h = static_cast<int>(divide(local, head_steps));
+        const long inner = local - s.h * head_steps;
+        if (s.h < 0 || s.h >= a.c.hkv || inner < 0) return;
+        int rt = 0;   // the last tile that begins at or before
+        for (int span = tiles; span > 1;) {
+            const int half = span / 2;
+            if (steps_before(a, s.x, step, rt + half) <= inner) rt += half;
+            span -= half;
+        }
+        s.rt = uniform(rt);
+        const long first = uniform(steps_before(a, s.x, step, s.rt));
+        s.units = static_cast<int>(uniform(steps_before(a, s.x, step, s.rt + 1)) - first);
+        s.u0 = static_cast<int>(inner - first);
+        s.u1 = static_cast<int>(min(static_cast<long>(s.units), s.u0 + (w_end - w)));
+        s.w  = w;
+        s.per = per;
+        // A tile's first kItemUnits are no steps: a share that ends among them leaves the tile to the next block.
+        if (s.u1 > kItemUnits) f(s);
+        w += max(s.u1 - s.u0, 1);   // (1 as above; a return here slows the long loops by 3%)
+    }
+}
+
+// Whether wave w of block lb met values that are not finite.
+__device__ __forceinline__ uint8_t* odd_flag(int32_t* desc, int lb, int w) { return reinterpret_cast<uint8_t*>(desc + kDesc * lb + 4) + w; }
+
 // Bytes of a staged row: 128 fp16 and some more, so that the rows that a fragment read takes at
 // once lie in different banks (64 of 4 bytes: 16 rows of K, 16 bytes of each; 4 rows of V, 64
 // bytes of each), and every fragment at a constant distance from the lane's first.
@@ -266,8 +335,7 @@ struct TreeKernel {
     static constexpr int kStep   = kPart * WK;
     static constexpr int NJ      = kPart / (4 * WQ);           // loads of 4 rows per wave, of K and of V
     static constexpr int kTileK  = kPart * kRowK, kTileV = kPart * kRowV;   // bytes of a step's rows
-    static constexpr int kFlags  = kTileK + kTileV;            // in a buffer: whether a wave met a value that is not finite
-    static constexpr int kBuf    = kFlags + 16 * ((4 * WQ + 15) / 16);
+    static constexpr int kBuf    = kTileK + kTileV;
     static constexpr int kStage  = WK * 2 * kBuf;
     static constexpr int kJoin   = kWaves * 32 * (kOutLd * 4 + 8);
     static constexpr int kLds    = kStage > kJoin ? kStage : kJoin;
@@ -283,73 +351,26 @@ struct TreeKernel {
         // The block's share of the units, consecutive ones on one XCD (blocks go round the 8 XCDs).
         const int nb = gridDim.x;
         const int lb = nb % 8 == 0 ? (blockIdx.x % 8) * (nb / 8) + blockIdx.x / 8 : blockIdx.x;
-        long total = 0, chunk = 0;
-        for (int c0 = 0; c0 < a.c.n_ent && total <= kMaxUnits; c0 += kScan) total += chunk = scan_chunk(a, sch, c0, kStep);
-        if (total > kMaxUnits) total = 0;
-        const long per = max(divide(total + nb - 1, nb), 1l);
-        long w = lb * per;
-        const long w_end = min(w + per, total);
-        int32_t* const desc = a.desc + kDesc * lb;   // what the merge has to join from here on
+        int32_t* const desc = a.desc + kDesc * lb;   // what the merge has to do from here on
         if (threadIdx.x == 0) desc[0] = 1;
-        if (w >= w_end) return;
-        int  c0 = 0;
-        long before = 0;
-        if (a.c.n_ent > kScan) chunk = scan_chunk(a, sch, 0, kStep);
-        while (w < w_end) {
-            while (w >= before + chunk) {
-                before += chunk;
-                c0 += kScan;
-                if (c0 >= a.c.n_ent) return;   // (the entries were changed under the call, here and below)
-                chunk = scan_chunk(a, sch, c0, kStep);
+        if (threadIdx.x % 64 == 0)
+            for (int w = threadIdx.x / 64; w < 8; w += kWaves) store_global<uint8_t>(odd_flag(a.desc, lb, w), 0);
+        walk(a, sch, nb, lb, kStep, [&](const Share& s) __attribute__((always_inline)) {
+            const Entry& x = s.x;
+            const bool begins = s.u0 <= kItemUnits, ends = s.u1 == s.units;
+            if (begins && !ends && threadIdx.x == 0) {   // the block's last tile: its other parts are the next blocks' first
+                desc[1] = x.t0 + s.rt * a.tile_tokens;
+                desc[2] = min(a.tile_tokens, x.n - s.rt * a.tile_tokens);
+                desc[3] = s.h;
+                desc[0] = static_cast<int>(divide(s.w - s.u0 + s.units - 1, s.per)) - lb + 1;
             }
-            int  hit = 0;
-            long at  = 0;
-            if (a.c.n_ent > 1) {
-                const int tid = threadIdx.x;
-                if (tid < kScan && sch.pre[tid] <= w - before && w - before < sch.pre[tid + 1]) sch.hit = tid;
-                __syncthreads();
-                hit = min(max(__builtin_amdgcn_readfirstlane(sch.hit), 0), min(kScan, a.c.n_ent - c0) - 1);
-                at  = before + uniform(sch.pre[hit]);
-                __syncthreads();
-            }
-            Entry x = entry_at(a.c, c0 + hit);
-            x.n = uniform(x.n);
-            if (x.n == 0) return;
-            const int  tiles = tiles_of(a, x);
-            const long head_steps = uniform(steps_before(a, x, kStep, tiles));
-            const long local = w - at;
-            const int  h     = static_cast<int>(divide(local, head_steps));
-            const long inner = local - h * head_steps;
-            if (h < 0 || h >= a.c.hkv || inner < 0) return;
-            int rt = 0;   // the last tile that begins at or before
-            for (int span = tiles; span > 1;) {
-                const int half = span / 2;
-                if (steps_before(a, x, kStep, rt + half) <= inner) rt += half;
-                span -= half;
-            }
-            rt = uniform(rt);
-            const long first = uniform(steps_before(a, x, kStep, rt));
-            const int  units = static_cast<int>(uniform(steps_before(a, x, kStep, rt + 1)) - first);
-            const int  u0    = static_cast<int>(inner - first);
-            const int  u1    = static_cast<int>(min(static_cast<long>(units), u0 + (w_end - w)));
-            // Its first kItemUnits are no steps: a share that ends among them leaves the tile to the next block.
-            if (u1 > kItemUnits) {
-                const bool begins = u0 <= kItemUnits, ends = u1 == units;
-                if (begins && !ends && threadIdx.x == 0) {   // the block's last tile: its other parts are the next blocks' first
-                    desc[1] = x.t0 + rt * a.tile_tokens;
-                    desc[2] = min(a.tile_tokens, x.n - rt * a.tile_tokens);
-                    desc[3] = h;
-                    desc[0] = static_cast<int>(divide(w - u0 + units - 1, per)) - lb + 1;
-                }
-                item_part(lds, x, h, rt, uniform(max(u0, kItemUnits) - kItemUnits), uniform(u1 - kItemUnits),
-                          uniform(begins && ends ? -1 : 2 * lb + (begins ? 1 : 0)));
-            }
-            w += max(u1 - u0, 1);   // (1 as above; a return here slows the long loops by 3%)
-        }
+            item_part(lds, x, s.h, s.rt, uniform(max(s.u0, kItemUnits) - kItemUnits), uniform(s.u1 - kItemUnits),
+                      uniform(begins && ends ? -1 : 2 * lb + (begins ? 1 : 0)), lb);
+        });
     }
 
     static __device__ __forceinline__ void item_part(unsigned char* lds, const Entry& x, int h, int rt, int k0,
-                                                     int k1, int slot) {
+                                                     int k1, int slot, int lb) {
         const TreeAttention a = arguments();
         const CachedTokens& c = a.c;
         const int tid = threadIdx.x, lane = tid & 63;
@@ -448,7 +469,10 @@ struct TreeKernel {
         auto stage_at = [&](int buf) { return lds + (2 * wk + buf) * kBuf; };
         // A place that a row does not see must not reach it, whatever its value: 0 * infinity is
         // NaN. So where rows see different places (masked), values that are not finite are staged as
-        // zeros, and add_odd adds them to the rows that see them.
+        // zeros; the merge has them at the end (odd_tile).
+        auto tell = [&] {
+            if (lane == 0) store_global<uint8_t>(odd_flag(arguments().desc, lb, wave), 1);
+        };
         auto store = [&](int buf, auto masked_c) {
             constexpr bool masked = decltype(masked_c)::value;
             unsigned char* k = stage_at(buf);
@@ -472,8 +496,8 @@ struct TreeKernel {
             }
             if constexpr (masked) {
                 const bool any = __builtin_amdgcn_ballot_w64(largest[0] >= 0x7c00 || largest[1] >= 0x7c00) != 0;
-                if (lane == 0) *reinterpret_cast<int*>(k + kFlags + 4 * wq) = any;
                 if (any) {
+                    tell();
 #pragma unroll 1
                     for (int j = 0; j < NJ; ++j) {   // (a lane's own values, again)
                         u32x4* const at = reinterpret_cast<u32x4*>(k + kTileK + (4 * (wq + WQ * j) + row0) * kRowV + 16 * ch);
@@ -488,45 +512,17 @@ struct TreeKernel {
                 }
             }
         };
-        // (By way of memory: rare, and 64 sums indexed by constants would weigh on the loop's registers.)
-        auto add_odd = [&](int base, const uint32_t (&seen)[SUBS], f32x16 (&o)[4]) {
-            float sums[64];
-#pragma unroll
-            for (int n = 0; n < 64; ++n) sums[n] = o[n / 16][n % 16];
-#pragma unroll 1
-            for (int t = 0; t < kTurn && base + t < end; ++t) {
-                const int i = a.by_page.of(base + t), page = load_uniform(table, i);
-                if (page < 0 || page >= c.num_pages) continue;
-                const int slot = base + t - i * P;
-                const unsigned char* v = static_cast<const unsigned char*>(c.v_cache) + page * page_bytes + head_off +
-                                         static_cast<size_t>(slot) * kRowBytes<EB>;
-                float vs = 1.0f;
-                if constexpr (BS)
-                    vs = __builtin_bit_cast(float, static_cast<uint32_t>(load_global<uint8_t>(
-                             c.scales + 2 * ((static_cast<size_t>(page) * c.hkv + h) * nblk + (slot >> bsh)) + 1)) << 23);
-                uint32_t word = seen[0];
-#pragma unroll
-                for (int b = 1; b < SUBS; ++b) word = t >= kSub * b ? seen[b] : word;
-                if (!(word >> (t & 31) & 1)) continue;
-#pragma unroll 1
-                for (int n = 0; n < 64; ++n) {
-                    const int at = 8 * (n / 4) + 4 * hl + n % 4;
-                    float y;
-                    if constexpr (EB == 2) y = f16_bits_to_f32(load_global<uint16_t>(v + 2 * at));
-                    else y = f16_bits_to_f32(fp8x2_to_f16x2<false>(load_global<uint8_t>(v + at), vs) & 0xffffu);
-                    if (!(fabsf(y) < INFINITY)) sums[n] += y;
-                }
-            }
-#pragma unroll
-            for (int n = 0; n < 64; ++n) o[n / 16][n % 16] = sums[n];
-        };
-
-        // Where this lane's fragments lie in the stage.
-        const int ka = ql * kRowK + 16 * hl;
+        // Where this lane's fragments of V lie in the stage.
         const int va = (4 * hl + ((lane & 15) >> 2)) * kRowV + 32 * ((lane >> 4) & 1) + 8 * (lane & 3);
 
         auto step_of = [&](auto masked_c, int base, const unsigned char* buf, int turn) {
             constexpr bool MASK = decltype(masked_c)::value;
+            // And of K, worked out in every step: held, it would be spilled, and a wait for a spilled
+            // register is one for the loads of the next step, too (1% of a chain of 4096).
+            unsigned all = ~0u;
+            asm volatile("" : "+s"(all));
+            const int self = __builtin_amdgcn_mbcnt_hi(all, __builtin_amdgcn_mbcnt_lo(all, 0));
+            const int ka = (self & 31) * kRowK + 16 * (self >> 5);
             const unsigned char* ks = buf + turn * kTurn * kRowK;
             const unsigned char* vs = buf + kTileK + turn * kTurn * kRowV;
             auto k_frag = [&](int n) {   // of part n % SUBS, dims 16 (n / SUBS) .. (the parts' sums in turn)
@@ -586,8 +582,12 @@ struct TreeKernel {
                 }
                 if constexpr (BS) {   // (scales are above 0)
 #pragma unroll
-                    for (int i = 0; i < 16; i += 4)
-                        top = fmaxf(top, fmaxf(fmaxf(s[b][i], s[b][i + 1]), fmaxf(s[b][i + 2], s[b][i + 3])) * cs[b][i / 4]);
+                    for (int i = 0; i < 16; i += 4) {
+                        float t = -INFINITY;   // (from the values alone, two would be made canonical first)
+#pragma unroll
+                        for (int e = 0; e < 4; ++e) t = fmaxf(t, s[b][i + e]);
+                        top = fmaxf(top, t * cs[b][i / 4]);
+                    }
                 } else {
 #pragma unroll
                     for (int i = 0; i < 16; ++i) top = fmaxf(top, s[b][i]);
@@ -631,12 +631,6 @@ struct TreeKernel {
                     __builtin_amdgcn_sched_group_barrier(kSchedMfma, 1, 1);
                     __builtin_amdgcn_sched_group_barrier(kSchedLds, 2, 1);
                 }
-            }
-            if constexpr (MASK) {
-                int odd = 0;
-#pragma unroll
-                for (int w = 0; w < WQ; ++w) odd |= *reinterpret_cast<const int*>(buf + kFlags + 4 * w);
-                if (__builtin_amdgcn_readfirstlane(odd)) add_odd(base, seen, o);
             }
         };
 
@@ -684,6 +678,13 @@ struct TreeKernel {
         const float sum = add_halves(l);
         if constexpr (WK == 1) {
             // The wave has its rows' whole sums. They go through LDS, so that a store takes whole rows.
+            float zero[4] = {0.f, 0.f, 0.f, 0.f};
+#pragma unroll
+            for (int i = 0; i < 16; ++i)
+#pragma unroll
+                for (int d = 0; d < 4; ++d) zero[d] = fmaf(o[d][i], 0.f, zero[d]);
+            // (NaN is not 0. Sums that are not finite, of rows whose softmax is, come of values in steps without masks.)
+            if (__builtin_amdgcn_ballot_w64((zero[0] + zero[1]) + (zero[2] + zero[3]) != 0.f && sum == sum) != 0) tell();
             block_sync();   // no wave reads the stage any more
             unsigned char* const mine = lds + wave * 32 * kOutLd * 4;
             if (slot >= 0) {
@@ -751,6 +752,7 @@ struct TreeKernel {
             den += f[g] * e[1];
         }
         const int i = a.by_group.of(row), g0 = row - i * G;
+        float zero = 0.f;
         if (i < tile_n) {
             const float scale = slot >= 0 ? 1.f : den == 0.f ? 0.f : c.v_scale / den;
             uint16_t* out = a.out + (x.t0 + tok0 + i) * a.out_stride + (h * G + g0) * kHeadDim;
@@ -765,6 +767,7 @@ struct TreeKernel {
 #pragma unroll
                     for (int e = 0; e < 4; ++e) y[e] = fmaf(z[e], f[g], y[e]);
                 }
+                zero = fmaf(y[0], 0.f, fmaf(y[1], 0.f, fmaf(y[2], 0.f, fmaf(y[3], 0.f, zero))));
                 if (slot >= 0) {
                     store_global(a.part_out + at * kHeadDim + d, y);
                 } else {
@@ -775,6 +778,7 @@ struct TreeKernel {
             }
             if (slot >= 0 && part == 0) store_global(a.part_ml + 2 * at, f32x2{top, den});
         }
+        if (__builtin_amdgcn_ballot_w64(zero != 0.f && den == den) != 0) tell();   // (as above)
         __syncthreads();   // the stage is free again
     }
 };
@@ -821,22 +825,122 @@ __device__ __forceinline__ void merge_row(const TreeAttention& a, int n, int blo
         u32x2{__builtin_bit_cast(uint32_t, lo), __builtin_bit_cast(uint32_t, hi)};
 }
 
+// Values that are not finite into a tile's result, kMergeRows rows of it, half a wave each: a token that sees
+// one has it in that dim, of whatever weight. (A weight that is 0 in fp16, or in 32 bits, makes NaN of an
+// infinity, and whether it is 0 goes by how the places fall into steps and parts.) A row whose softmax is not a
+// number is NaN in the dims that hold none, and stays as it is. Rare: the tiles of blocks that met some come
+// here (an infinity at a place that all see: 16 tokens over 32 x 8192 168 -> 507 us, 4096 after 4096 3.7 ms). In the
+// attention kernel this took registers from its loops (168 -> 185 to 203 us without any).
+__device__ __forceinline__ void odd_tile(const TreeAttention& a, uint32_t* words, const Entry& x, int h, int rt) {
+    const CachedTokens& c = a.c;
+    constexpr int kWords = 4 * kMergeWaves;   // of 32 places, looked at together
+    constexpr int kOddLoads = 4;              // (more of them would take registers from the joining)
+    const int tid = threadIdx.x, lane = tid & 63, wave = tid >> 6;
+    const int P = c.page_size, bsh = P % 16 == 0 ? 4 : 3, eb = a.elem;
+    const int tok0 = rt * a.tile_tokens, tile_n = min(a.tile_tokens, x.n - tok0);
+    const int row = blockIdx.x * kMergeRows + (tid >> 5), i = a.by_group.of(row), g = row - i * a.group, d4 = 4 * (tid & 31);
+    if (static_cast<int>(blockIdx.x) * kMergeRows >= tile_n * a.group) return;
+    const int tok = i < tile_n ? tok0 + i : INT_MAX;
+    const int end = x.start + (a.tree ? x.n : tok0 + tile_n);
+    const int32_t* table = c.table + static_cast<size_t>(x.row) * c.table_stride;
+    // Place t's row of V; null where there is none.
+    auto v_row = [&](int t, float& scale) {
+        const int n = t < end ? a.by_page.of(t) : 0, page = t < end ? table[n] : -1, s = t - n * P;
+        scale = 1.0f;
+        if (page < 0 || page >= c.num_pages) return static_cast<const unsigned char*>(nullptr);
+        const size_t at = (static_cast<size_t>(page) * c.hkv + h) * P + s;
+        if (c.scales) scale = __builtin_bit_cast(float, static_cast<uint32_t>(c.scales[2 * (at >> bsh) + 1]) << 23);
+        return static_cast<const unsigned char*>(c.v_cache) + at * (kHeadDim * eb);
+    };
+    auto value = [&](const unsigned char* p, int d, float scale) {
+        return f16_bits_to_f32(eb == 2 ? reinterpret_cast<const uint16_t*>(p)[d] : fp8x2_to_f16x2<false>(p[d], scale) & 0xffffu);
+    };
+    float sums[4] = {0.f, 0.f, 0.f, 0.f};
+    for (int base = 0; base < end; base += 32 * kWords) {
+        __syncthreads();
+#pragma unroll 1
+        for (int w = wave; w < kWords; w += kMergeWaves) {
+            uint32_t odd = 0;
+#pragma unroll 1
+            for (int j0 = 0; j0 < 32; j0 += 4 * kOddLoads) {   // 16 lanes a row
+                const unsigned char* p[kOddLoads];
+                float scale[kOddLoads];
+                u32x4 v[kOddLoads];
+#pragma unroll
+                for (int j = 0; j < kOddLoads; ++j) p[j] = v_row(base + 32 * w + j0 + 4 * j + (lane >> 4), scale[j]);
+#pragma unroll
+                for (int j = 0; j < kOddLoads; ++j) {
+                    v[j] = u32x4{0, 0, 0, 0};
+                    if (p[j] && eb == 2) v[j] = reinterpret_cast<const u32x4*>(p[j])[lane & 15];
+                    if (p[j] && eb == 1) {
+                        const u32x2 y = reinterpret_cast<const u32x2*>(p[j])[lane & 15];
+                        v[j][0] = y[0], v[j][1] = y[1];
+                    }
+                }
+#pragma unroll
+                for (int j = 0; j < kOddLoads; ++j) {
+                    if (eb == 1)
+                        v[j] = u32x4{fp8x2_to_f16x2<false>(v[j][0], scale[j]), fp8x2_to_f16x2<true>(v[j][0], scale[j]),
+                                     fp8x2_to_f16x2<false>(v[j][1], scale[j]), fp8x2_to_f16x2<true>(v[j][1], scale[j])};
+                    bool any = false;
+#pragma unroll
+                    for (int e = 0; e < 4; ++e) any |= (v[j][e] & 0x7c00u) == 0x7c00u || (v[j][e] & 0x7c000000u) == 0x7c000000u;
+                    const uint64_t lanes = __builtin_amdgcn_ballot_w64(any);
+#pragma unroll
+                    for (int r = 0; r < 4; ++r) odd |= (lanes >> (16 * r) & 0xffff) != 0 ? 1u << (j0 + 4 * j + r) : 0u;
+                }
+            }
+            if (lane == 0) words[w] = odd;
+        }
+        __syncthreads();
+        for (int w = 0; w < kWords; ++w) {
+            if (words[w] == 0) continue;
+            for (uint32_t mine = words[w] & visible(a, x, tok, base + 32 * w - x.start); mine != 0; mine &= mine - 1) {
+                float scale;
+                const unsigned char* p = v_row(base + 32 * w + __builtin_ctz(mine), scale);
+                for (int e = 0; e < 4; ++e) {
+                    const float y = value(p, d4 + e, scale);
+                    if (!__builtin_isfinite(y)) sums[e] += y;
+                }
+            }
+        }
+    }
+    if (tok == INT_MAX) return;
+    _Float16* const out = reinterpret_cast<_Float16*>(a.out) + (x.t0 + tok) * a.out_stride + (h * a.group + g) * kHeadDim + d4;
+    bool nan = false;
+    for (int e = 0; e < 4; ++e) nan |= sums[e] == 0.f && out[e] != out[e];
+    if (__builtin_amdgcn_ballot_w64(nan) >> (tid & 32) & 0xffffffffu) return;
+    for (int e = 0; e < 4; ++e)
+        if (!(sums[e] == 0.f)) out[e] = static_cast<_Float16>(sums[e] * c.v_scale);
+}
+
 // The tile that begins in block x and goes on in the next ones. (At most one begins in a block and
 // is not whole there, its last: slot 1 of the block holds it; slot 0 the block's part of one that
 // began before.) A tile's rows go round the XCDs: with blocks x in a row of the grid, tiles that begin
 // in every 32nd block were all joined on one of the eight (64 tokens over 1 x 131072: 22 us).
-__global__ __launch_bounds__(64 * kMergeWaves) void tree_merge_kernel(const int32_t* __restrict__ desc, const TreeAttention a) {
+// And values that are not finite, in the tiles that begin in block x.
+__global__ __launch_bounds__(64 * kMergeWaves, 6) void tree_merge_kernel(const int32_t* __restrict__ desc, const TreeAttention a) {
     const int row = blockIdx.x * kMergeRows + (threadIdx.x >> 5);
-    const int block = blockIdx.y;
+    const int block = blockIdx.y, blocks = gridDim.y;
     const int32_t* d = desc + kDesc * block;
-    const int n = min(load_uniform(d, 0), static_cast<int>(gridDim.y) - block);
-    if (n <= 1) return;
-    const int i = a.by_group.of(row), g = row - i * a.group;
-    if (i >= load_uniform(d, 2)) return;
-    const int t = load_uniform(d, 1) + i, head = load_uniform(d, 3) * a.group + g;
-    if (n <= 2) merge_row<2>(a, n, block, row, t, head);
-    else if (n <= 4) merge_row<4>(a, n, block, row, t, head);
-    else merge_row<8>(a, n, block, row, t, head);
+    const int n = min(load_uniform(d, 0), blocks - block);
+    uint32_t odd = load_uniform(d, 4) | load_uniform(d, 5);
+    if (n > 1) {
+        for (int k = 1 + static_cast<int>(threadIdx.x & 63); k < n; k += 64) odd |= d[kDesc * k + 4] | d[kDesc * k + 5];
+        const int i = a.by_group.of(row), g = row - i * a.group;
+        if (i < load_uniform(d, 2)) {
+            const int t = load_uniform(d, 1) + i, head = load_uniform(d, 3) * a.group + g;
+            if (n <= 2) merge_row<2>(a, n, block, row, t, head);
+            else if (n <= 4) merge_row<4>(a, n, block, row, t, head);
+            else merge_row<8>(a, n, block, row, t, head);
+        }
+    }
+    if (__builtin_amdgcn_ballot_w64(odd != 0) == 0) return;
+    __shared__ Schedule sch;
+    __shared__ uint32_t words[4 * kMergeWaves];
+    walk(a, sch, blocks, block, a.step, [&](const Share& s) {
+        if (s.u0 <= kItemUnits) odd_tile(a, words, s.x, s.h, s.rt);
+    });
 }
 
 // Blocks on a CU. fp16: one of 8 waves; FP8, whose steps are half as many bytes: two of 4 waves
@@ -846,12 +950,14 @@ __global__ __launch_bounds__(64 * kMergeWaves) void tree_merge_kernel(const int3
 constexpr bool small_blocks(int eb, int rows) { return eb == 1 && rows <= 128; }
 
 template <int EB, bool BS, bool UNI, int ROWS>
-void launch_r(const TreeAttention& a, hipStream_t s) {
+void launch_r(TreeAttention& a, hipStream_t s) {
     constexpr int WQ = ROWS / 32, WK = (small_blocks(EB, ROWS) ? 4 : 8) / WQ;
+    a.elem = EB;
+    a.step = TreeKernel<EB, BS, WQ, WK, UNI>::kStep;
     hipLaunchKernelGGL((tree_attention_kernel<EB, BS, WQ, WK, UNI>), dim3(a.grid), dim3(64 * WQ * WK), 0, s, a);
 }
 template <int EB, bool BS, bool UNI>
-void launch_u(const TreeAttention& a, hipStream_t s) {
+void launch_u(TreeAttention& a, hipStream_t s) {
     switch (a.rows) {
         case 64: launch_r<EB, BS, UNI, 64>(a, s); break;
         case 128: launch_r<EB, BS, UNI, 128>(a, s); break;
@@ -859,7 +965,7 @@ void launch_u(const TreeAttention& a, hipStream_t s) {
     }
 }
 template <int EB, bool BS>
-void launch_e(const TreeAttention& a, hipStream_t s) {
+void launch_e(TreeAttention& a, hipStream_t s) {
     if (a.c.page_size % 4 == 0) launch_u<EB, BS, true>(a, s);
     else if constexpr (!BS) launch_u<EB, false, false>(a, s);
 }
@@ -898,7 +1004,7 @@ void tree_place(TreeAttention& a, void* workspace) {
     a.desc     = reinterpret_cast<int32_t*>(a.part_ml + 2 * rows);
 }
 
-hipError_t launch_tree_attention(int dtype, const TreeAttention& a, hipStream_t s) {
+hipError_t launch_tree_attention(int dtype, TreeAttention a, hipStream_t s) {
     check_kv_dtype(dtype);
     if (dtype == PA_KV_FP16) launch_e<2, false>(a, s);
     else if (dtype == PA_KV_FP8_E4M3) launch_e<1, false>(a, s);
