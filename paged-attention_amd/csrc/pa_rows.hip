@@ -225,16 +225,17 @@ __global__ __launch_bounds__(64 * kWavesB) void keep_blocks_kernel(const KeepRow
     unsigned char* pool = static_cast<unsigned char*>(v ? c.v_cache : c.k_cache);
     const int n = min(load_uniform(a.counts, e), a.width), st = load_uniform(c.start, e);
     const int row = c.slot_ids ? load_uniform(c.slot_ids, e) : e;
-    if (st < 0 || n <= 0 || st > INT_MAX - 32 - n) return;
-    const int P = c.page_size, sh = P % 16 == 0 ? 4 : 3, B = 1 << sh, nb = P >> sh, last = (st + n - 1) >> sh;
+    if (st < 0 || n <= 0) return;
+    const int P = c.page_size, sh = P % 16 == 0 ? 4 : 3, B = 1 << sh, nb = P >> sh;
+    const int last = (n - 1 > INT_MAX - st ? INT_MAX : st + n - 1) >> sh;
     const int32_t* kept = a.kept + static_cast<size_t>(e) * a.width;
     auto scale_at = [&](int page, int slot) {
         return c.scales + 2 * ((static_cast<size_t>(page) * c.hkv + h) * nb + (slot >> sh)) + v;
     };
     for (int b0 = st >> sh; b0 <= last; b0 += kWavesB) {
         // Lane group r holds the block's places r, r + 4, ...
-        const int b = b0 + wave, page = b <= last ? page_at(c, row, b * B) : -1;
-        const int slot0 = page < 0 ? 0 : b * B - c.by_page.page(b * B) * P;
+        const int b = b0 + wave, at = b <= last ? b * B : -1, page = page_at(c, row, at);   // (none before place 0)
+        const int slot0 = page < 0 ? 0 : at - c.by_page.page(at) * P;
         u32x2 was[4];
         int   from[4];     // 0: not in the path, 1: stays in its place, 2: moves in, 3: lies before the path
         float y[4][8], amax = 0.f;
@@ -243,7 +244,7 @@ __global__ __launch_bounds__(64 * kWavesB) void keep_blocks_kernel(const KeepRow
         const int old = page < 0 ? 0 : *sc;
 #pragma unroll
         for (int i = 0; i < 4; ++i) {
-            const int s = kRowsR * i + r, j = b * B + s - st;
+            const int s = kRowsR * i + r, j = max(at, 0) + s - st;
             from[i] = 0;
             was[i] = u32x2{0, 0};
             float f = 0.f;
@@ -269,7 +270,7 @@ __global__ __launch_bounds__(64 * kWavesB) void keep_blocks_kernel(const KeepRow
         __syncthreads();
         if (__builtin_amdgcn_ballot_w64(moved) == 0) continue;
         int k = __builtin_amdgcn_readfirstlane(block_exponent(wave_max64(amax)));
-        if (b * B < st) k = max(k, old - 127);
+        if (at < st) k = max(k, old - 127);
 #pragma unroll
         for (int i = 0; i < 4; ++i) {
             if (from[i] == 0 || (from[i] == 3 && k <= old - 127)) continue;

@@ -74,6 +74,23 @@ def test_rows_at_the_last_places(kind):
     assert (out[5:] == 7).all()
 
 
+@pytest.mark.parametrize("kind", ["fp16", "fp8", "block"])
+@pytest.mark.parametrize("start", [2 ** 31 - 10, 2 ** 31 - 36])
+def test_rows_kept_to_the_last_place(kind, start):
+    """The last places of all, and numbers that would lie behind them."""
+    page = 2 ** 16
+    cache = Cache(kind, page, 2, 1, 1, seed=4, spare=0)
+    k, v, _, scales = cache.device()
+    table = torch.zeros((1, 2 ** 15), dtype=torch.int32, device="cuda")
+    pa_amd.keep_rows(k, v, table, ints([1, 3, 9, 12, 30, 40, 2 ** 31 - 1]).view(1, 7), ints([7]), ints([start]), kv_scales=scales)
+    here = start % page
+    drafts.keep(cache, [(0, here, [j for j in (1, 3, 9, 12, 30) if here + j < page])])
+    for x, want in zip((k, v), cache.kv):
+        np.testing.assert_array_equal(x.cpu().numpy().view(np.uint8), want.view(np.uint8))
+    if scales is not None:
+        np.testing.assert_array_equal(scales.cpu().numpy(), cache.scales)
+
+
 @pytest.mark.parametrize("n,words", [(100, 1), (129, 2), (3, 5), (64, 1), (64, 3), (200, 4)])
 def test_tree_rows_with_fewer_or_more_bits(n, words):
     """Tokens past a row's bits are not seen; bits past the entry's tokens name none."""
