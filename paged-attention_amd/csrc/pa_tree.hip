@@ -25,15 +25,15 @@
 // zeros. K's goes into its scores in 32 bits (345 / 357 us for 32 tokens over 64 x 8192 with K scaled
 // in fp16 and so, but fp16 has no keys below 2^-24). Two buffers, loads a whole step ahead.
 //
-// What bounds it (one MI355X): trees of few rows, memory (4 tokens over 32 x 8192, fp16: 170 us,
-// 6.3 TB/s; 16: 176); tiles of 128 rows and more, three pipes: 32 places by 32 rows are 16 MFMAs of
+// What bounds it (one MI355X): trees of few rows, memory (1 token over 32 x 8192, fp16: 170 us,
+// 6.3 TB/s; 16: 168); tiles of 128 rows and more, three pipes: 32 places by 32 rows are 16 MFMAs of
 // 32 cycles, per lane 16 exponentials, maxima, sums and roundings besides the staging, and 16 KB out
-// of LDS, which a wave reads for its 32 rows alone. The matrix pipe is busy 46% of the time, the
-// vector pipe 42%, LDS about half, and no order of the code that was tried laid them wholly over
-// each other (4096 tokens after 4096: 440 to 465 us, 890 to 935 TFLOP/s, a large library product
-// 1242; 32 over 64 x 8192, block scales: 345 to 363). Twice the rows a wave, half the reads, does not fit the registers
-// (705 us, 130 spilled). Small calls: the instructions of a tile's prologue and end, and the
-// merge's launch (8 tokens over 200: 11 us, 3 of them the merge's).
+// of LDS, which a wave reads for its 32 rows alone (45% of its time at 128 bytes a cycle; its counter
+// says 29%). The matrix pipe is busy 45% of the time, the vector pipe 43%, and no order of the code that was
+// tried laid them wholly over each other (4096 tokens after 4096: 458 to 474 us, 870 to 900 TFLOP/s, a large
+// library product 1232; 32 over 64 x 8192, block scales: 357 to 371). Twice the rows a wave, half the
+// reads, does not fit the registers (705 us, 130 spilled). Small calls: the instructions of a tile's
+// prologue and end, and the merge's launch (8 tokens over 200: 11 us, 3 of them the merge's).
 
 #include "pa_device.hpp"
 #include "pa_fp8.hpp"
@@ -339,8 +339,9 @@ struct TreeKernel {
     static constexpr int kStage  = WK * 2 * kBuf;
     static constexpr int kJoin   = kWaves * 32 * (kOutLd * 4 + 8);
     static constexpr int kLds    = kStage > kJoin ? kStage : kJoin;
-    // Loads bypass the caches where hardly any place is read twice: tiles that hold all of an entry's
-    // rows. (us with cached and with such loads: 16 over 32 x 8192 fp16 219 / 203, 4096 over 4096 451 / 511.)
+    // Loads bypass the caches where hardly any place is read twice: tiles of 64 and 128 rows, which hold all of an
+    // average entry's. (us with cached and with such loads: 16 over 32 x 8192 fp16 219 / 203, 4096 over 4096 451 / 511.
+    // An entry of many tiles beside short ones that make the call's tiles small has its places read past the caches, too.)
     static constexpr int kAux    = WQ < 8 ? 2 : 0;
     static constexpr int RG      = UNI ? 4 : 1;                // rows that a lane looks up
     static_assert(kPart / RG <= 64 && NJ >= 1 && kStep >= kMinStep);
@@ -828,11 +829,13 @@ __device__ __forceinline__ void merge_row(const TreeAttention& a, int n, int blo
 // Values that are not finite into a tile's result, kMergeRows rows of it, half a wave each: a token that sees
 // one has it in that dim, of whatever weight. (A weight that is 0 in fp16, or in 32 bits, makes NaN of an
 // infinity, and whether it is 0 goes by how the places fall into steps and parts.) A row whose softmax is not a
-// number is NaN in the dims that hold none, and stays as it is. Rare: the tiles of blocks that met some come
-// here (an infinity at a place that all see: 16 tokens over 32 x 8192 168 -> 507 us, 4096 after 4096 3.7 ms). In the
-// attention kernel this took registers from its loops (168 -> 185 to 203 us without any).
-__device__ __forceinline__ void odd_tile(const TreeAttention& a, uint32_t* words, const Entry& x, int h, int rt) {
+// number is NaN in the dims that hold none, and stays as it is. Rare: only the parts of blocks that met some
+// are looked through (one at a place that all see: 16 tokens over 32 x 8192 168 -> 449 us, 64 over 1 x 131072 165 -> 351,
+// 4096 after 4096 3.5 ms). In the attention kernel this took registers from its loops (168 -> 185 to 203 us without any).
+__device__ __forceinline__ void odd_tile(const TreeAttention& a, uint32_t* words, const Share& tile, int block) {
     const CachedTokens& c = a.c;
+    const Entry& x = tile.x;
+    const int h = tile.h, rt = tile.rt;
     constexpr int kWords = 4 * kMergeWaves;   // of 32 places, looked at together
     constexpr int kOddLoads = 4;              // (more of them would take registers from the joining)
     const int tid = threadIdx.x, lane = tid & 63, wave = tid >> 6;
@@ -843,10 +846,12 @@ __device__ __forceinline__ void odd_tile(const TreeAttention& a, uint32_t* words
     const int tok = i < tile_n ? tok0 + i : INT_MAX;
     const int end = x.start + (a.tree ? x.n : tok0 + tile_n);
     const int32_t* table = c.table + static_cast<size_t>(x.row) * c.table_stride;
-    // Place t's row of V; null where there is none.
-    auto v_row = [&](int t, float& scale) {
-        const int n = t < end ? a.by_page.of(t) : 0, page = t < end ? table[n] : -1, s = t - n * P;
+    int hi = 0;   // of the part that is looked through: places from here on are not its
+    // Place t's row of V; null where there is none. (t may be past 2^31, hi is not.)
+    auto v_row = [&](uint32_t t, float& scale) {
         scale = 1.0f;
+        if (t >= static_cast<uint32_t>(hi)) return static_cast<const unsigned char*>(nullptr);
+        const int n = a.by_page.of(static_cast<int>(t)), page = table[n], s = static_cast<int>(t) - n * P;
         if (page < 0 || page >= c.num_pages) return static_cast<const unsigned char*>(nullptr);
         const size_t at = (static_cast<size_t>(page) * c.hkv + h) * P + s;
         if (c.scales) scale = __builtin_bit_cast(float, static_cast<uint32_t>(c.scales[2 * (at >> bsh) + 1]) << 23);
@@ -856,7 +861,7 @@ __device__ __forceinline__ void odd_tile(const TreeAttention& a, uint32_t* words
         return f16_bits_to_f32(eb == 2 ? reinterpret_cast<const uint16_t*>(p)[d] : fp8x2_to_f16x2<false>(p[d], scale) & 0xffffu);
     };
     float sums[4] = {0.f, 0.f, 0.f, 0.f};
-    for (int base = 0; base < end; base += 32 * kWords) {
+    auto look = [&](uint32_t base) {
         __syncthreads();
 #pragma unroll 1
         for (int w = wave; w < kWords; w += kMergeWaves) {
@@ -895,7 +900,7 @@ __device__ __forceinline__ void odd_tile(const TreeAttention& a, uint32_t* words
         __syncthreads();
         for (int w = 0; w < kWords; ++w) {
             if (words[w] == 0) continue;
-            for (uint32_t mine = words[w] & visible(a, x, tok, base + 32 * w - x.start); mine != 0; mine &= mine - 1) {
+            for (uint32_t mine = words[w] & visible(a, x, tok, static_cast<int>(base + 32 * w) - x.start); mine != 0; mine &= mine - 1) {
                 float scale;
                 const unsigned char* p = v_row(base + 32 * w + __builtin_ctz(mine), scale);
                 for (int e = 0; e < 4; ++e) {
@@ -904,6 +909,18 @@ __device__ __forceinline__ void odd_tile(const TreeAttention& a, uint32_t* words
                 }
             }
         }
+    };
+    // The tile's parts are its units in this block and the next ones.
+    const long unit0 = tile.w - tile.u0;
+    const int  parts = min(static_cast<int>(divide(unit0 + tile.units - 1, tile.per)) + 1, static_cast<int>(gridDim.y)) - block;
+    for (int k = 0; k < parts; ++k) {
+        const int32_t* d = a.desc + kDesc * (block + k);
+        if ((load_uniform(d, 4) | load_uniform(d, 5)) == 0) continue;
+        const long u0 = max((block + k) * tile.per - unit0, static_cast<long>(kItemUnits));
+        const long u1 = min((block + k + 1) * tile.per - unit0, static_cast<long>(tile.units));
+        const uint32_t lo = static_cast<uint32_t>(uniform((u0 - kItemUnits) * a.step));
+        hi = max(static_cast<int>(uniform(min((u1 - kItemUnits) * a.step, static_cast<long>(end)))), 0);
+        for (uint32_t at = lo; at < static_cast<uint32_t>(hi); at += 32 * kWords) look(at);
     }
     if (tok == INT_MAX) return;
     _Float16* const out = reinterpret_cast<_Float16*>(a.out) + (x.t0 + tok) * a.out_stride + (h * a.group + g) * kHeadDim + d4;
@@ -939,7 +956,7 @@ __global__ __launch_bounds__(64 * kMergeWaves, 6) void tree_merge_kernel(const i
     __shared__ Schedule sch;
     __shared__ uint32_t words[4 * kMergeWaves];
     walk(a, sch, blocks, block, a.step, [&](const Share& s) {
-        if (s.u0 <= kItemUnits) odd_tile(a, words, s.x, s.h, s.rt);
+        if (s.u0 <= kItemUnits) odd_tile(a, words, s, block);
     });
 }
 

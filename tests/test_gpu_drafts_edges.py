@@ -52,6 +52,24 @@ def test_the_last_places():
             assert (np.abs(got[i, h] - p @ V) <= tol).all(), (i, h, np.abs(got[i, h] - p @ V).max())
 
 
+def test_values_that_are_not_finite_at_the_last_places():
+    """The same table: one that all tokens see, one that the second token brings."""
+    page, n, hq = 2 ** 16, 3, 2
+    cache = Cache("fp8", page, 1, 1, 2, seed=3, spare=0)
+    own = int(cache.table[0, 1])
+    cache.kv[1][own, 0, LAST % page - 9, 5] = 0x7f
+    cache.kv[1][own, 0, LAST % page - 2, 9] = 0xff
+    k, v, _, _ = cache.device()
+    table = torch.full((1, 2 ** 15), int(cache.table[0, 0]), dtype=torch.int32, device="cuda")
+    table[0, -1] = own
+    q = torch.randn((n, hq, D), device="cuda", generator=torch.Generator(device="cuda").manual_seed(1)).half()
+    got = pa_amd.tree_attention(q, k, v, table, begins([n]), ints([LAST - n]), **cache.kw(None)).cpu().numpy()
+    want = np.zeros((n, hq, D), bool)
+    want[:, :, 5] = want[1:, :, 9] = True
+    np.testing.assert_array_equal(np.isnan(got), want)
+    assert np.isfinite(got[~want]).all()
+
+
 @pytest.mark.parametrize("kind", ["fp16", "block"])
 def test_rows_at_the_last_places(kind):
     """Rows read and kept at the end of 2^31 places."""
