@@ -369,7 +369,7 @@ typedef struct pa_cached_tokens {
     const int32_t*  block_table;    /* [num_table_rows][block_table_stride] */
     int32_t         block_table_stride;
     int32_t         num_table_rows;
-    int32_t         num_pages;
+    int32_t         num_pages;      /* that each pool holds */
     int32_t         page_size;
     int32_t         num_kv_heads;
     float           k_scale;        /* FP8: a stored code c stands for c * scale (times its block's, */
@@ -406,7 +406,8 @@ pa_status pa_tree_attention(int dtype, const pa_cached_tokens* c, const pa_head_
 /* Rows as numbers: token t's kv head h to k_out + t * k_stride + h * 128 (elements of
  * `type`), its value row to v_out likewise (either may be NULL; 16-byte aligned, strides
  * multiples of 8 below 2^26, rows that do not overlap, nor anything that the call reads). code *
- * scale in 32 bits, rounded once. Tokens of no entry and those whose place, row or page is out of range keep what their output held. */
+ * scale in 32 bits, rounded once. Tokens of no entry and those whose place, row or page is out of
+ * range keep what their output held. */
 typedef enum pa_value_type {
     PA_VALUE_FP16 = 0,
     PA_VALUE_BF16 = 1,

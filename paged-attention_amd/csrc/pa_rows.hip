@@ -8,9 +8,12 @@
 // (No counterparts in the reference.)
 //
 // read_cache is bound by memory: a code in, its value (code times scale, in 32 bits, rounded once)
-// out. 8 x 8192 places, block scales, into fp16: 61 us, 6.6 TB/s; 37 ragged sequences, FP8, 44 us.
-// The keeping kernels move some rows of each sequence and are bound by their chains of loads
-// (counts, numbers, pages, rows): 64 sequences 3.7 us, 512 7.8; block scales 6.2.
+// out. 8 x 8192 places, block scales, into fp16: 74 us, 5.5 TB/s (the kernel over inputs that the last
+// pass left in the caches: 59); 37 ragged sequences, FP8, 57 us (42). Of one kv head, 48 lanes of a
+// wave have no row: 21 us for an eighth of the bytes. The keeping kernels move some rows of each sequence:
+// a chain of loads (counts, numbers, pages, rows), and what its waves, one an entry and head, add. The kernels
+// alone, 6 rows kept in 64 / 512 sequences: fp16 4.1 / 5.8 us, FP8 3.7 / 4.9, block scales 6.0 / 15; 16 rows: 5.1 / 9.4,
+// 4.9 / 7.0, 6.2 / 20.
 
 #include "pa_device.hpp"
 #include "pa_fp8.hpp"
@@ -56,7 +59,8 @@ __device__ __forceinline__ int page_at(const CachedTokens& c, int row, int pos) 
 
 // (Streaming stores: outputs are the larger part of the traffic, and cached they push rows that are
 // still to be read out of the caches. us with cached and with streaming stores: 8 x 8192 places,
-// block scales, 84 / 61; 37 ragged sequences, FP8, 57 / 44.)
+// block scales, 84 / 61 on one input again and again, 84 / 74 on inputs in turn; 37 ragged sequences, FP8, 54 / 44 and
+// 63 / 57.)
 template <int OUT>
 __device__ __forceinline__ void store_values(void* out, size_t at, const float (&y)[8]) {
     if constexpr (OUT == PA_VALUE_FP32) {
