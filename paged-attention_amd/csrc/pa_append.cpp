@@ -127,7 +127,8 @@ bool rows_overlap(const void* a, int64_t a_stride, const void* b, int64_t b_stri
 
 bool rows_touch(const void* a, int64_t a_stride, int64_t row, int elem, int n, const void* p, size_t bytes) {
     const Rows x{static_cast<int64_t>(reinterpret_cast<uintptr_t>(a)), elem * a_stride, elem * row};
-    return n > 0 && p && bytes && hits(x, static_cast<int64_t>(reinterpret_cast<uintptr_t>(p)), static_cast<int64_t>(bytes), 0, n - 1);
+    const int64_t size = static_cast<int64_t>(std::min(bytes, size_t{1} << 60));   // (a table's claimed size may pass 2^63)
+    return n > 0 && p && bytes && hits(x, static_cast<int64_t>(reinterpret_cast<uintptr_t>(p)), size, 0, n - 1);
 }
 
 void check_page_bytes(const char* what, int dtype, int page_size, int kv_heads) {

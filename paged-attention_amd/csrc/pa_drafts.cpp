@@ -79,7 +79,7 @@ std::array<Bytes, 7> reads_of(int dtype, const pa::CachedTokens& c) {
     const size_t pool = rows * pa::kHeadDim * (dtype == PA_KV_FP16 ? 2 : 1);
     const size_t scales = c.scales ? 2 * rows / pa::block_tokens(c.page_size) : 0, ents = 4 * static_cast<size_t>(c.n_ent);
     return {{{c.k_cache, pool}, {c.v_cache, pool}, {c.scales, scales},
-             {c.table, 4 * static_cast<size_t>(c.table_rows) * c.table_stride},
+             {c.table, std::min(static_cast<size_t>(c.table_rows) * c.table_stride, size_t{1} << 58) * 4},
              {c.tok_begin, ents + 4}, {c.start, ents}, {c.slot_ids, ents}}};
 }
 // Refuses output rows that lie in what the call reads: other tokens' results would change under it.

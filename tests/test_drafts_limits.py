@@ -40,4 +40,7 @@ def test_only_what_a_pool_holds_is_its():
     for at, kw in ((end - 16, dict(type=0)), (V - 3 * 4096 - 4080, dict(type=2)), (V + (1 << 18) - 16, dict(dtype=pa_amd.FP16))):
         assert read(k=at, v=FAR, **kw, **PLACES) == BAD and "overlaps the cache" in message(), message()
     assert attend(dtype=pa_amd.FP16, q=rows(in_=FAR, out=V + (1 << 18) - 16), **PLACES) == BAD and "overlaps the cache" in message()
+    # A table that is said to have 2^62 entries reaches over everything behind it.
+    huge = {**PLACES, "num_table_rows": 2**31 - 1, "block_table_stride": 2**31 - 1}
+    assert attend(q=rows(in_=FAR, out=FAR + (1 << 19)), **huge) == BAD and "overlaps the cache" in message()
     assert attend(q=rows(in_=FAR + (1 << 19), out=FAR), tree=FAR + 4 * ROW - 8, words=1, **PLACES) == BAD and "tree" in message()
