@@ -234,7 +234,7 @@ struct TreeAttention {
     PlaceDiv        by_tile;
     float*          part_out;  // [2 grid][rows][128]
     float*          part_ml;   // [2 grid][rows][2]
-    int32_t*        desc;      // [grid][8], the tile that a block begins and others end
+    int32_t*        desc;      // [grid][8], the tile that a block begins and others end, whether it met values that are not finite
 };
 // Chooses the launch from the call's sizes (host only, but for the device's CU count).
 void   tree_shape(int dtype, TreeAttention& a);

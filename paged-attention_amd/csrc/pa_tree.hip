@@ -2,7 +2,7 @@
 // trees, chains, pieces of prompts. (No counterpart in the reference.)
 //
 //   tree_attention_kernel   the work, in equal shares
-//   tree_merge_kernel       tiles that shares cut apart, joined
+//   tree_merge_kernel       tiles that shares cut apart, joined; values that are not finite
 //
 // out_i = sum_p exp(s_ip - m_i) v_p / sum_p exp(s_ip - m_i), s_ip = sm_scale q_i k_p, over the
 // places p that token i sees: one pass with a running m_i, sums in 32 bits.
@@ -65,7 +65,7 @@ constexpr int kMinStep    = 64;  // places of a step, at least
 constexpr long kMaxUnits  = (1l << 53) - (1l << 20);
 static_assert(kMaxTreeRows * (kItemUnits + 2 + (1l << 31) / kMinStep) <= kMaxUnits);
 constexpr int kSchedMfma = 0x8, kSchedLds = 0x100;   // of sched_group_barrier
-constexpr int kDesc    = 8;               // ints of a block's entry for the merge
+constexpr int kDesc    = 8;               // ints of a block's entry for the merge: parts, first token, tokens, kv head, 8 bytes of odd_flag
 constexpr int kOutLd   = kHeadDim + 4;    // floats of a row in the joining of waves
 
 // A probability is kept as 2^(score - reference + kShift) in fp16, where the reference
